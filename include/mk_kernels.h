@@ -577,6 +577,80 @@ int mk_sdpa_bwd(void* stream, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int6
                 void* dv, int64_t dv_bs, int64_t dv_hs, int64_t dv_ss,
                 float scale, int causal, void* workspace);
 
+/* ========================================================================
+ * Eight-bit serving.  No counterpart in the reference: products whose operands
+ * are rows of whole numbers of 8 bits with an fp32 scale each (half the bytes of
+ * bf16 and twice its matrix rate), what makes such rows, and the choice of
+ * the next token.  They stand beside mk_gemm, mk_add_layernorm, mk_convert and
+ * mk_row_argmax.  Rows are `ld_*` elements apart (inputs: any pitch >= 0,
+ * outputs: at least their columns), their elements contiguous; pointers need
+ * the alignment of their elements, and rows on 16-byte boundaries are fastest.
+ * Rows that end before their pitch are left as they are past their end.
+ * ====================================================================== */
+
+/* Residual add, RMS norm and rounding to 8 bits in one pass over rows of `cols`:
+ *   s = x + residual        (fp32 add, one RNE rounding to io_type, stored to sum)
+ *   y = s / sqrt(mean(s^2) + eps) * gamma
+ *   scale = max |y| / 127,  q = y / scale rounded to the nearest whole number
+ * io_type in {MK_BF16, MK_F16, MK_F32} for x, residual, gamma and sum.  residual
+ * NULL: s = x and sum is not written (sum may be x or residual, at its pitch);
+ * gamma NULL: 1.  The mean is summed in 64 bits.  A row with max |s gamma| below
+ * 2^-119 gets scale 0 and zeros.  A row with a NaN or an infinity in s gamma gets
+ * scale NaN and zeros, so that every product with it is NaN. */
+int mk_add_rmsnorm_int8(void* stream, int io_type, int64_t rows, int64_t cols, const void* x, int64_t ld_x,
+                        const void* residual, int64_t ld_residual, const void* gamma, float eps, void* sum,
+                        int64_t ld_sum, int8_t* q, int64_t ld_q, float* scale);
+
+/* Rows to 8 bits: scale = max |y| / 127, q = y / scale rounded, with y = x or
+ * (gelu != 0) gelu_tanh(x) in fp32: an attention output, an MLP's hidden rows, or
+ * weights with a scale for each output channel.  Zeros, NaN and infinities as
+ * above (for y). */
+int mk_quantize_rows(void* stream, int io_type, int64_t rows, int64_t cols, const void* x, int64_t ld_x, int gelu,
+                     int8_t* q, int64_t ld_q, float* scale);
+
+/* The values that rows of 8 bits stand for: y = q * scale, one rounding to
+ * out_type in {MK_BF16, MK_F16, MK_F32}. */
+int mk_dequantize_rows(void* stream, int out_type, int64_t rows, int64_t cols, const int8_t* q, int64_t ld_q,
+                       const float* scale, void* y, int64_t ld_y);
+
+/* C[m][n] = (sum_k A[m][k] B[k][n]) * a_scale[m] * b_scale[n]  (+ bias[n]) (then ReLU)
+ * for 8-bit A and B, k contiguous in both: A element (m, k) at A + m*a_ms + k, B
+ * element (k, n) at B + n*b_ns + k (weights stored by output channel).  The sum is
+ * exact (32 bits; K <= 131071, MK_ERR_UNSUPPORTED past that); it is scaled in
+ * fp32, a_scale first, and rounded once to c_type in {MK_F32, MK_BF16, MK_F16}.
+ * a_scale [M] and b_scale [N] are fp32.  epilogue and bias as mk_gemm's (0 none,
+ * 1 + bias, 2 + bias then max(., 0), 5 / 6 as 1 / 2 with an fp32 bias).  K = 0 is a
+ * sum of 0. */
+int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int64_t K, const int8_t* A, int64_t a_ms,
+                 const float* a_scale, const int8_t* B, int64_t b_ns, const float* b_scale, void* C, int64_t c_ms,
+                 const void* bias, int epilogue);
+
+/* The next token of each row of logits, drawn with the caller's random numbers
+ * u[rows] in [0, 1):
+ *   w_i = exp((x_i - max x) / temperature)
+ *   tokens are ranked by x, larger first, ties by lower index
+ *   top_k: the first top_k ranks are kept (<= 0: all)
+ *   top_p: of those, a rank is kept while the weights of the ranks before it sum to
+ *          less than top_p times the sum over all of them (>= 1: all; the first
+ *          rank always)
+ *   min_p: of those, the tokens with w_i >= min_p (above 1: taken as 1)
+ *   token  = the lowest index i such that the kept weights of indices 0 .. i sum to
+ *            more than u times all kept weights
+ *   logprob = log(w_token / sum of kept weights), fp32 (logprobs may be NULL)
+ * temperature 0 takes the largest logit, the lowest index among equals, whatever
+ * the other limits say.  Sums are exact sums of weights rounded to whole multiples
+ * of 2^-s, s >= 41 (46 for 50257 tokens).  temperature, top_k, top_p and min_p: a
+ * device array of one value a row, or NULL and the value `*_all` for every row.
+ * -inf logits are never drawn.  A row that holds a NaN or +inf, or nothing above
+ * -inf, and a row whose u, temperature, top_p or min_p is NaN or whose temperature
+ * is negative or infinite gets token -1 and logprob NaN.  u outside [0, 1) takes
+ * the first or the last kept token.  io_type in {MK_BF16, MK_F16, MK_F32};
+ * index_type in {MK_S32, MK_S64}; at most 2097152 tokens and 2^22 - 1 rows. */
+int mk_sample_rows(void* stream, int io_type, int64_t rows, int64_t vocab, const void* logits, int64_t ld_logits,
+                   const float* u, const float* temperature, float temperature_all, const int32_t* top_k,
+                   int top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                   int index_type, void* tokens, float* logprobs);
+
 #ifdef __cplusplus
 }
 #endif

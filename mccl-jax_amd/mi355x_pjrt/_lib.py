@@ -100,6 +100,11 @@ SIGNATURES = {
     "mk_sdpa_bwd": (_I, [_P, _I64, _I64, _I64, _I64, _I64]
                     + [_P, _I64, _I64, _I64] * 5 + [_P]
                     + [_P, _I64, _I64, _I64] * 3 + [_F, _I, _P]),
+    "mk_add_rmsnorm_int8": (_I, [_P, _I, _I64, _I64, _P, _I64, _P, _I64, _P, _F, _P, _I64, _P, _I64, _P]),
+    "mk_quantize_rows": (_I, [_P, _I, _I64, _I64, _P, _I64, _I, _P, _I64, _P]),
+    "mk_dequantize_rows": (_I, [_P, _I, _I64, _I64, _P, _I64, _P, _P, _I64]),
+    "mk_gemm_int8": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _P, _I]),
+    "mk_sample_rows": (_I, [_P, _I, _I64, _I64, _P, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _I, _P, _P]),
 }
 
 _kernels = None

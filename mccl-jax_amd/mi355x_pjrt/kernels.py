@@ -661,3 +661,189 @@ def sdpa_bwd(q, k, v, o, dout, lse, scale, causal=True, dq=None, dk=None, dv=Non
     rc = lib().mk_sdpa_bwd(*args)
     _check(rc, "mk_sdpa_bwd")
     return dq, dk, dv
+
+
+# ------------------------------------------------------------------ eight-bit serving
+_ROW_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _take(what, t, name, dtypes, shape):
+    """An operand of the shape and a type asked for, on the current device, elements of a row contiguous."""
+    if not t.is_cuda or t.get_device() != _device():
+        raise ValueError(f"{what}: {name} is not on the current device")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what}: {name} has dtype {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, {shape} is asked for")
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: {name} is not contiguous along its last dimension")
+
+
+def _new(shape, dtype, device, stream):
+    """An output, from the memory of the stream that writes it."""
+    if stream is None or not isinstance(stream, torch.cuda.Stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _new_int8_rows(rows, cols, device, stream):
+    """Rows of 8 bits that start on 16-byte boundaries, as gemm_int8's fastest kernels take them."""
+    pitch = (cols + 15) // 16 * 16
+    q = _new((rows, pitch), torch.int8, device, stream)
+    return q if pitch == cols else q[:, :cols]
+
+
+def _own_rows(what, t, name):
+    """Rows to be written do not overlap."""
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what}: rows of {name} overlap")
+
+
+def _int8_outputs(what, x, q, scale, stream):
+    rows, cols = x.shape
+    if q is None:
+        q = _new_int8_rows(rows, cols, x.device, stream)
+    else:
+        _take(what, q, "q", (torch.int8,), (rows, cols))
+        _own_rows(what, q, "q")
+    if scale is None:
+        scale = _new((rows,), torch.float32, x.device, stream)
+    else:
+        _take(what, scale, "scale", (torch.float32,), (rows,))
+    return q, scale
+
+
+def add_rmsnorm_int8(x, residual=None, gamma=None, eps=1e-6, sum_out=None, q=None, scale=None, stream=None):
+    """(q, scale, sum) of [rows, cols] x: sum = x + residual (x itself where
+    residual is None), and 8-bit rows q with one fp32 scale each that stand for
+    y = sum / sqrt(mean(sum^2) + eps) * gamma, the operand of gemm_int8
+    (mk_add_rmsnorm_int8).  Any row pitch; sum_out may be x or residual."""
+    what = "add_rmsnorm_int8"
+    if x.dim() != 2:
+        raise ValueError(f"{what}: x must be 2-D")
+    shape = (rows, cols) = tuple(x.shape)
+    _take(what, x, "x", _ROW_TYPES, shape)
+    total = x
+    if residual is not None:
+        _take(what, residual, "residual", (x.dtype,), shape)
+        if sum_out is None:
+            total = _new(shape, x.dtype, x.device, stream)
+        else:
+            total = sum_out
+            _take(what, total, "sum_out", (x.dtype,), shape)
+            _own_rows(what, total, "sum_out")
+    elif sum_out is not None:
+        raise ValueError(f"{what}: sum_out without a residual")
+    if gamma is not None:
+        _take(what, gamma, "gamma", (x.dtype,), (cols,))
+    q, scale = _int8_outputs(what, x, q, scale, stream)
+    rc = lib().mk_add_rmsnorm_int8(_stream(stream), mk_dtype(x.dtype), rows, cols, x.data_ptr(), x.stride(0),
+                                   _ptr(residual), 0 if residual is None else residual.stride(0), _ptr(gamma),
+                                   float(eps), None if residual is None else total.data_ptr(), total.stride(0),
+                                   q.data_ptr(), q.stride(0), scale.data_ptr())
+    _check(rc, "mk_add_rmsnorm_int8")
+    return q, scale, total
+
+
+def quantize_rows(x, gelu=False, q=None, scale=None, stream=None):
+    """(q, scale): the rows of a 2-D x, or (gelu) of gelu_tanh(x), as 8-bit
+    rows with one fp32 scale each, max |y| / 127 (mk_quantize_rows).  For
+    weights x is [out, in] and the product takes q.t()."""
+    what = "quantize_rows"
+    if x.dim() != 2:
+        raise ValueError(f"{what}: x must be 2-D")
+    _take(what, x, "x", _ROW_TYPES, tuple(x.shape))
+    q, scale = _int8_outputs(what, x, q, scale, stream)
+    rc = lib().mk_quantize_rows(_stream(stream), mk_dtype(x.dtype), x.shape[0], x.shape[1], x.data_ptr(), x.stride(0),
+                                int(bool(gelu)), q.data_ptr(), q.stride(0), scale.data_ptr())
+    _check(rc, "mk_quantize_rows")
+    return q, scale
+
+
+def dequantize_rows(q, scale, dtype=torch.bfloat16, out=None, stream=None):
+    """The values q * scale that 8-bit rows stand for, in `dtype`."""
+    what = "dequantize_rows"
+    if q.dim() != 2:
+        raise ValueError(f"{what}: q must be 2-D")
+    shape = tuple(q.shape)
+    _take(what, q, "q", (torch.int8,), shape)
+    _take(what, scale, "scale", (torch.float32,), shape[:1])
+    if out is None:
+        out = _new(shape, dtype, q.device, stream)
+    _take(what, out, "out", (dtype,) if dtype in _ROW_TYPES else (), shape)
+    _own_rows(what, out, "out")
+    rc = lib().mk_dequantize_rows(_stream(stream), mk_dtype(dtype), shape[0], shape[1], q.data_ptr(), q.stride(0),
+                                  scale.data_ptr(), out.data_ptr(), out.stride(0))
+    _check(rc, "mk_dequantize_rows")
+    return out
+
+
+def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16, bias=None, relu=False, out=None, stream=None):
+    """C = (a @ b) * a_scale[:, None] * b_scale (+ bias)(ReLU) for int8 a
+    [M, K] and b [K, N], k contiguous in both: a as quantize_rows and
+    add_rmsnorm_int8 give it, b the transposed view of weights stored by output
+    channel (quantize_rows(w)[0].t()).  a_scale [M], b_scale [N] fp32; the sum
+    over k is exact (mk_gemm_int8)."""
+    what = "gemm_int8"
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[0]:
+        raise ValueError(f"{what}: a [M, K] and b [K, N] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
+    (M, Kd), N = a.shape, b.shape[1]
+    w = b.t()
+    _take(what, a, "a", (torch.int8,), (M, Kd))
+    _take(what, w, "b, transposed,", (torch.int8,), (N, Kd))
+    _take(what, a_scale, "a_scale", (torch.float32,), (M,))
+    _take(what, b_scale, "b_scale", (torch.float32,), (N,))
+    if out is None:
+        out = _new((M, N), out_dtype, a.device, stream)
+    _take(what, out, "out", (out_dtype,) if out_dtype in _ROW_TYPES else (), (M, N))
+    _own_rows(what, out, "out")
+    epi = 0
+    if bias is not None:
+        _take(what, bias, "bias", (out_dtype, torch.float32), (N,))
+        epi = (2 if relu else 1) | (4 if bias.dtype != out_dtype else 0)
+    elif relu:
+        raise ValueError(f"{what}: relu goes with a bias")
+    rc = lib().mk_gemm_int8(_stream(stream), mk_dtype(out_dtype), M, N, Kd, a.data_ptr(), a.stride(0),
+                            a_scale.data_ptr(), w.data_ptr(), w.stride(0), b_scale.data_ptr(), out.data_ptr(),
+                            out.stride(0), _ptr(bias), epi)
+    _check(rc, "mk_gemm_int8")
+    return out
+
+
+def _per_row(what, v, name, dtype, rows, off):
+    """(pointer, value) of a parameter that is a number for all rows or a tensor of one for each."""
+    if isinstance(v, torch.Tensor):
+        _take(what, v, name, (dtype,), (rows,))
+        return v.data_ptr(), off
+    return None, off if v is None else v
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, index_dtype=torch.int32,
+                with_logprob=True, stream=None):
+    """(token, logprob) of each row of [rows, vocab] logits, drawn with the
+    random numbers u [rows] (fp32, in [0, 1)): softmax(logits / temperature)
+    limited to the top_k largest, then to the fewest of those that hold top_p of
+    their weight, then to those with at least min_p of the largest one's
+    (mk_sample_rows has the exact terms).  Each limit is a number, None, or a
+    tensor of one value a row (top_k int32, the others fp32).  temperature 0 is
+    row_argmax.  A row without a valid choice gives token -1 and logprob NaN."""
+    what = "sample_rows"
+    if logits.dim() != 2:
+        raise ValueError(f"{what}: logits must be 2-D")
+    rows, vocab = logits.shape
+    _take(what, logits, "logits", _ROW_TYPES, (rows, vocab))
+    _take(what, u, "u", (torch.float32,), (rows,))
+    if index_dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: index_dtype must be int32 or int64")
+    t, t_all = _per_row(what, temperature, "temperature", torch.float32, rows, 1.0)
+    k, k_all = _per_row(what, top_k, "top_k", torch.int32, rows, 0)
+    p, p_all = _per_row(what, top_p, "top_p", torch.float32, rows, 1.0)
+    m, m_all = _per_row(what, min_p, "min_p", torch.float32, rows, 0.0)
+    token = _new((rows,), index_dtype, logits.device, stream)
+    logprob = _new((rows,), torch.float32, logits.device, stream) if with_logprob else None
+    rc = lib().mk_sample_rows(_stream(stream), mk_dtype(logits.dtype), rows, vocab, logits.data_ptr(),
+                              logits.stride(0), u.data_ptr(), t, float(t_all), k, min(int(k_all), 2 ** 31 - 1), p,
+                              float(p_all), m, float(m_all), mk_dtype(index_dtype), token.data_ptr(), _ptr(logprob))
+    _check(rc, "mk_sample_rows")
+    return token, logprob
