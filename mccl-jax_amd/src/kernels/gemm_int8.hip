@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace mk {
 namespace {
@@ -31,6 +32,7 @@ struct Int8Gemm {
   int64_t lda, ldb, ldc;
   int tiles_m, tiles_n;
   int c_type, epilogue;
+  int stream_c;  // C goes past the caches
 };
 
 // one value of C from its sum
@@ -41,9 +43,391 @@ __device__ inline float finish(const Int8Gemm& p, int sum, float sa, int64_t n) 
   return v;
 }
 
-// 16 bytes from any address
-struct __attribute__((packed, aligned(1))) Any16 { u32x4_t v; };
+// 16 bytes from any address, one instruction on gfx950
+struct __attribute__((packed, aligned(1))) Any16 { i32x4_t v; };
+__device__ inline i32x4_t load16(const int8_t* p) { return reinterpret_cast<const Any16*>(p)->v; }
+// bytes 0 .. n - 1 of 16, zeros past them
+__device__ inline i32x4_t load16_upto(const int8_t* p, int64_t n) {
+  if (n >= 16) return load16(p);
+  uint8_t b[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) b[e] = e < n ? uint8_t(p[e]) : uint8_t(0);
+  return __builtin_bit_cast(i32x4_t, b);
+}
 
+// ---------------------------------------------------------------- few rows
+// At most 64 rows: reading B (the weights) once is the work.  A workgroup has 16 VN
+// columns and all rows; its NW waves take k in steps of 128 bytes round-robin,
+// kD steps ahead in registers, and their sums meet in LDS (whole numbers: in any
+// order).  Nothing is staged.  A lane (c, g) of v_mfma_i32_16x16x64_i8 loads 32
+// consecutive bytes of row c at k = 32 g, so that 4 lanes take a whole line of a
+// row, and they are the operands of two MFMAs: which k an MFMA's slots mean is
+// free as long as A and B agree.  Rows need no alignment.
+constexpr int kStep = 128;
+
+template <int VN, int MT, int NW, int kD>
+__global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm p) {
+  constexpr int NT = 16 * VN;
+  __shared__ __attribute__((aligned(16))) int red[NW][16][NT + 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int64_t n0 = int64_t(blockIdx.x) * NT;
+  // rows past the operands' repeat the last and are not stored
+  const int8_t *ap[MT], *bp[VN];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) ap[m] = p.A + std::min<int64_t>(16 * m + c, p.M - 1) * p.lda + 32 * g;
+#pragma unroll
+  for (int j = 0; j < VN; ++j) bp[j] = p.B + std::min<int64_t>(n0 + 16 * j + c, p.N - 1) * p.ldb + 32 * g;
+  struct Step {
+    i32x4_t a[MT][2], b[VN][2];
+  };
+  auto load = [&](Step& s, int64_t step) __attribute__((always_inline)) {
+    const int64_t k = step * kStep;
+#pragma unroll
+    for (int j = 0; j < VN; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s.b[j][h] = load16(bp[j] + k + 16 * h);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s.a[m][h] = load16(ap[m] + k + 16 * h);
+  };
+  i32x4_t acc[MT][VN] = {};
+  auto multiply = [&](const Step& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < VN; ++j)
+          acc[m][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.b[j][h], s.a[m][h], acc[m][j], 0, 0, 0);
+  };
+  // the loop's loads are unconditional: with a branch around them the compiler
+  // waits for every load at the loop's head
+  const int64_t full = p.K / kStep, n = full > wave ? (full - wave + NW - 1) / NW : 0;
+  Step s[kD];
+  auto fetch = [&](int d, int64_t i) __attribute__((always_inline)) { load(s[d], wave + NW * i); };
+  if (n >= kD) {
+    int64_t i = 0;
+#pragma unroll
+    for (int d = 0; d < kD; ++d) fetch(d, d);
+    for (; i + 2 * kD <= n; i += kD) {
+#pragma unroll
+      for (int d = 0; d < kD; ++d) {
+        multiply(s[d]);
+        fetch(d, i + kD + d);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kD; ++d) {
+      multiply(s[d]);
+      if (i + kD + d < n) fetch(d, i + kD + d);
+    }
+#pragma unroll
+    for (int d = 0; d < kD; ++d)
+      if (i + kD + d < n) multiply(s[d]);
+  } else {
+#pragma unroll
+    for (int d = 0; d < kD - 1; ++d)
+      if (d < n) fetch(d, d);
+#pragma unroll
+    for (int d = 0; d < kD - 1; ++d)
+      if (d < n) multiply(s[d]);
+  }
+  if (p.K % kStep != 0 && full % NW == wave) {  // the last, shorter step: zeros past K
+    const int64_t k = full * kStep, left = p.K - k - 32 * g;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < VN; ++j) s[0].b[j][h] = load16_upto(bp[j] + k + 16 * h, left - 16 * h);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s[0].a[m][h] = load16_upto(ap[m] + k + 16 * h, left - 16 * h);
+    }
+    multiply(s[0]);
+  }
+  // acc[m][j] reg r of lane (c, g): row 16 m + c, column 16 j + 4 g + r
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (m > 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < VN; ++j) *reinterpret_cast<i32x4_t*>(&red[wave][c][16 * j + 4 * g]) = acc[m][j];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * NT; e += 64 * NW) {
+      const int row = e / NT, col = e % NT;
+      int sum = red[0][row][col];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) sum += red[w][row][col];
+      const int64_t mrow = 16 * m + row, nc = n0 + col;
+      if (mrow < p.M && nc < p.N)
+        store_from_f32(p.C, mrow * p.ldc + nc, p.c_type, finish(p, sum, p.a_scale[mrow], nc));
+    }
+  }
+}
+
+template <int VN, int MT>
+void launch_rows(hipStream_t s, const Int8Gemm& a) {
+  // sixteen waves where the steps in flight and the sums fit 128 registers, else eight
+  constexpr int kWords = 8 * (VN + MT), kSums = 4 * VN * MT;
+  constexpr int NW = 2 * kWords + kSums <= 72 ? 16 : 8;
+  constexpr int kFit = ((NW == 16 ? 72 : 192) - kSums) / kWords, kD = kFit > 4 ? 4 : kFit;
+  static_assert(kD >= 2, "two steps in flight");
+  const int64_t tiles = (a.N + 16 * VN - 1) / (16 * VN);
+  hipLaunchKernelGGL((gemm_int8_rows_kernel<VN, MT, NW, kD>), dim3(unsigned(tiles)), dim3(64 * NW), 0, s, a);
+}
+
+template <int VN>
+void launch_rows(hipStream_t s, const Int8Gemm& a) {
+  if (a.M <= 16) launch_rows<VN, 1>(s, a);
+  else if (a.M <= 32) launch_rows<VN, 2>(s, a);
+  else launch_rows<VN, 4>(s, a);
+}
+
+// ---------------------------------------------------------------- tiles
+// Rows on the 16-byte grid.  Workgroup tile TM x TN, k in tiles of 128 bytes,
+// WGM x WGN waves of 32 x 32 blocks.  Operand tiles go straight into LDS
+// (buffer_load ... lds, attn_common.h) in two stages: the copies of the next
+// k tile are issued while this one is multiplied, one barrier a tile.  An LDS row is
+// 128 bytes, its 16-byte chunk c at position c ^ ((row >> 1) & 7), so that the
+// 16 rows a ds_read_b128 takes at one chunk lie on 16 different bank groups.
+// Chunks past M, N or K are loaded from an out-of-range offset, which reads
+// zeros.  Where K is no multiple of 16 the last chunk of a row is loaded whole
+// (16 aligned bytes, so on the row's last page) and, A's bytes past K are
+// cleared as they are read from LDS: what B holds there is multiplied by zero.
+//
+// Tile order: workgroups are dealt round-robin to the 8 XCDs, each with its own
+// L2; workgroup i takes tile (i % 8) (tiles / 8) + i / 8 of an order that walks
+// groups of 4 tile rows column by column, so that an XCD's tiles are a compact block.
+constexpr int kBK = 128, kStages = 2;
+constexpr int kGroupM = 4;
+constexpr int kInvalid = int(0x80000000u);  // buffer offset past every accepted range
+
+// The copies one wave makes of an operand tile of W * kC * 8 rows: copy c is 1 KB,
+// 8 rows, lane l of it writes chunk position l % 8 of row l / 8.
+template <int kC, int W>
+struct Copies {
+  uint32_t off[kC];
+  int32_t k[kC];
+  __device__ inline Copies(int wave, int lane, int64_t r0, int64_t rows, int64_t ld) {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int row = 8 * (wave + W * c) + lane / 8;
+      k[c] = 16 * ((lane % 8) ^ ((row >> 1) & 7));
+      off[c] = r0 + row < rows ? uint32_t((r0 + row) * ld + k[c]) : uint32_t(kInvalid);
+    }
+  }
+  // offset for the k tile at k0, or one that reads zeros once the chunk lies past K
+  __device__ inline int at(int c, int k0, int64_t K) const {
+    return off[c] != uint32_t(kInvalid) && k[c] + k0 < K ? int(off[c] + uint32_t(k0)) : kInvalid;
+  }
+};
+
+// MFMA operand for rows rb .. rb + 31 and k 32 ks .. 32 ks + 31 of a tile
+__device__ inline i32x4_t read_operand(const int8_t* t, int rb, int ks, int lane) {
+  const int row = rb + (lane & 31), ch = (2 * ks + (lane >> 5)) ^ ((row >> 1) & 7);
+  return *reinterpret_cast<const i32x4_t*>(t + row * kBK + 16 * ch);
+}
+
+// the first n (any whole number) of 16 bytes, zeros for the others
+__device__ inline i32x4_t first_bytes(i32x4_t v, int n) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int b = n - 4 * q;
+    v[q] &= b >= 4 ? -1 : b <= 0 ? 0 : (1 << (8 * b)) - 1;
+  }
+  return v;
+}
+
+template <int N>
+__device__ inline void wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+template <int TM_, int TN_, int WGM_, int WGN_>
+struct Shape {
+  static constexpr int TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_;
+};
+
+typedef uint32_t u32x4_by4_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// C's tile through LDS in passes of as many rows as the operand stages hold:
+// a lane writes 4 consecutive columns at a time, chunk c of staging row r at
+// position c ^ (r & 15) (rows of 8 chunks: c ^ ((r >> 1) & 7)), and the workgroup stores runs of 16 bytes (of whole
+// rows; they need no alignment past an element's).
+template <int CT, bool STREAM, int TM, int TN, int kW, int kWM, int kWN, int kI, int kJ>
+__device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm& p, const i32x16_t (&acc)[kI][kJ],
+                                                                 int8_t* stage, const float* sa, const float* sb,
+                                                                 const float* bias, int64_t m0, int64_t n0, int wm,
+                                                                 int wn, int lane) {
+  constexpr int kSz = CT == MK_F32 ? 4 : 2, kPer = 16 / kSz, kCpr = TN / kPer, kThreads = 64 * kW;
+  constexpr int kRoom = kStages * kBK * (TM + TN), kFit = kRoom / (TN * kSz) / kWM * kWM;
+  constexpr int kRP = kFit >= TM ? TM : TM % kFit == 0 ? kFit : kWM;  // rows a pass
+  static_assert(kRP > 0 && TM % kRP == 0 && kRP % kWM == 0 && kCpr % 8 == 0, "passes of whole wave rows");
+  static_assert(kRP * kCpr % kThreads == 0, "chunks split evenly over the threads");
+  using out_t = std::conditional_t<CT == MK_F32, u32x4_by4_t, u32x4_by2_t>;
+  auto pos = [](int row, int cn) { return kCpr % 16 == 0 ? cn ^ (row & 15) : cn ^ ((row >> 1) & 7); };
+  const int c = lane & 31, g = lane >> 5;
+  char* C = static_cast<char*>(p.C);
+#pragma unroll
+  for (int pass = 0; pass < TM / kRP; ++pass) {
+    if (pass > 0) lds_barrier();
+    if (wm * kWM >= pass * kRP && wm * kWM < (pass + 1) * kRP) {
+#pragma unroll
+      for (int a = 0; a < kI; ++a) {
+        const int ml = wm * kWM + 32 * a + c, row = ml - pass * kRP;
+        const float s = sa[ml];
+#pragma unroll
+        for (int b = 0; b < kJ; ++b)
+#pragma unroll
+          for (int rg = 0; rg < 4; ++rg) {
+            const int nl = wn * kWN + 32 * b + 8 * rg + 4 * g;
+            float v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              v[q] = float(acc[a][b][4 * rg + q]) * s * sb[nl + q];
+              if ((p.epilogue & 3) != 0) v[q] += bias[nl + q];
+              if ((p.epilogue & 3) == 2) v[q] = v[q] < 0.f ? 0.f : v[q];
+            }
+            int8_t* to = stage + row * TN * kSz + 16 * pos(row, nl / kPer) + nl % kPer * kSz;
+            if constexpr (CT == MK_F32) {
+              *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
+            } else {
+              uint16_t h[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) h[q] = CT == MK_BF16 ? f32_to_bf16(v[q]) : f32_to_f16(v[q]);
+              __builtin_memcpy(to, h, 8);
+            }
+          }
+      }
+    }
+    lds_barrier();
+#pragma unroll 2
+    for (int it = 0; it < kRP * kCpr / kThreads; ++it) {
+      const int e = it * kThreads + int(threadIdx.x);
+      const int row = e / kCpr, cn = e % kCpr;
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + row * TN * kSz + 16 * pos(row, cn));
+      const int64_t m = m0 + pass * kRP + row, n = n0 + cn * kPer;
+      if (m >= p.M || n >= p.N) continue;
+      char* to = C + kSz * (m * p.ldc + n);
+      if (n + kPer <= p.N) {
+        if constexpr (STREAM) __builtin_nontemporal_store(out_t(v), reinterpret_cast<out_t*>(to));
+        else *reinterpret_cast<out_t*>(to) = v;
+      } else {  // the chunk that straddles N
+#pragma unroll
+        for (int q = 0; q < kPer; ++q)
+          if (n + q < p.N) {
+            if constexpr (CT == MK_F32) reinterpret_cast<uint32_t*>(to)[q] = v[q];
+            else reinterpret_cast<uint16_t*>(to)[q] = uint16_t(v[q / 2] >> (16 * (q & 1)));
+          }
+      }
+    }
+  }
+}
+
+template <class Sh, int CT, bool RAGGED>
+__global__ __launch_bounds__(64 * Sh::WGM * Sh::WGN, 1) void gemm_int8_tiled_kernel(const Int8Gemm p) {
+  constexpr int TM = Sh::TM, TN = Sh::TN, WGN = Sh::WGN, kW = Sh::WGM * WGN;
+  constexpr int kWM = TM / Sh::WGM, kWN = TN / WGN, kI = kWM / 32, kJ = kWN / 32;
+  constexpr int kCa = TM / 8 / kW, kCb = TN / 8 / kW, kNC = kCa + kCb;
+  static_assert(kI * 32 * Sh::WGM == TM && kJ * 32 * WGN == TN, "wave blocks tile the workgroup tile");
+  static_assert(kCa * kW * 8 == TM && kCb * kW * 8 == TN, "copies split evenly over the waves");
+  __shared__ __attribute__((aligned(1024))) int8_t lds[kStages * kBK * (TM + TN)];
+  __shared__ float sa[TM], sb[TN], bias[TN];
+  int8_t (*As)[TM * kBK] = reinterpret_cast<int8_t (*)[TM * kBK]>(lds);
+  int8_t (*Bs)[TN * kBK] = reinterpret_cast<int8_t (*)[TN * kBK]>(lds + kStages * TM * kBK);
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WGN, wn = wave % WGN;
+  const uint32_t nt = gridDim.x, per = nt / 8, i = blockIdx.x;
+  const uint32_t t = i < 8 * per ? (i % 8) * per + i / 8 : i;
+  const uint32_t group = t / (kGroupM * uint32_t(p.tiles_n)), first_m = group * kGroupM;
+  const uint32_t gm = min(uint32_t(kGroupM), uint32_t(p.tiles_m) - first_m);
+  const uint32_t w_in = t - group * kGroupM * uint32_t(p.tiles_n);
+  const int64_t m0 = int64_t(first_m + w_in % gm) * TM, n0 = int64_t(w_in / gm) * TN;
+  // the last row's last chunk whole: to the next multiple of 16 bytes
+  const i32x4_t ra = tile_desc(p.A, uint32_t(((p.M - 1) * p.lda + p.K + 15) & ~int64_t(15)));
+  const i32x4_t rb = tile_desc(p.B, uint32_t(((p.N - 1) * p.ldb + p.K + 15) & ~int64_t(15)));
+  const Copies<kCa, kW> ca(wave, lane, m0, p.M, p.lda);
+  const Copies<kCb, kW> cb(wave, lane, n0, p.N, p.ldb);
+  const int K = int(p.K);
+  auto issue = [&](int kt, int stage, int lo, int hi) __attribute__((always_inline)) {
+    const int k0 = kBK * kt;
+#pragma unroll
+    for (int c = 0; c < kNC; ++c) {
+      if (c < lo || c >= hi) continue;
+      const uint32_t to = c < kCa ? lds_addr(&As[stage][(wave + kW * c) * 1024])
+                                  : lds_addr(&Bs[stage][(wave + kW * (c - kCa)) * 1024]);
+      if (k0 + kBK <= K)
+        copy_to_lds_so(c < kCa ? ra : rb, to, int(c < kCa ? ca.off[c < kCa ? c : 0] : cb.off[c < kCa ? 0 : c - kCa]),
+                       uint32_t(k0));
+      else
+        copy_to_lds(c < kCa ? ra : rb, to, c < kCa ? ca.at(c < kCa ? c : 0, k0, K) : cb.at(c < kCa ? 0 : c - kCa, k0, K));
+    }
+  };
+  i32x16_t acc[kI][kJ] = {};
+  const int nk = (K + kBK - 1) / kBK;
+  issue(0, 0, 0, kNC);
+  // the scales and the bias of the tile, for the end (after the first copies, so
+  // that these go first)
+  for (int e = threadIdx.x; e < TM; e += 64 * kW) sa[e] = m0 + e < p.M ? p.a_scale[m0 + e] : 0.f;
+  for (int e = threadIdx.x; e < TN; e += 64 * kW) {
+    sb[e] = n0 + e < p.N ? p.b_scale[n0 + e] : 0.f;
+    if ((p.epilogue & 3) != 0)
+      bias[e] = n0 + e < p.N ? load_as_f32(p.bias, n0 + e, (p.epilogue & 4) ? int(MK_F32) : CT) : 0.f;
+  }
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_vm<0>();
+    lds_barrier();
+    const bool more = kt + 1 < nk, last = RAGGED && !more;
+    const int8_t *at = As[kt % 2], *bt = Bs[kt % 2];
+#pragma unroll
+    for (int ks = 0; ks < kBK / 32; ++ks) {
+      i32x4_t af[kI], bf[kJ];
+#pragma unroll
+      for (int a = 0; a < kI; ++a) af[a] = read_operand(at, wm * kWM + 32 * a, ks, lane);
+#pragma unroll
+      for (int b = 0; b < kJ; ++b) bf[b] = read_operand(bt, wn * kWN + 32 * b, ks, lane);
+      if (more && ks < 2) issue(kt + 1, (kt + 1) % 2, ks * kNC / 2, (ks + 1) * kNC / 2);
+      if (RAGGED && last) {
+#pragma unroll
+        for (int a = 0; a < kI; ++a) af[a] = first_bytes(af[a], K - kBK * kt - 32 * ks - 16 * (lane >> 5));
+      }
+#pragma unroll
+      for (int a = 0; a < kI; ++a)
+#pragma unroll
+        for (int b = 0; b < kJ; ++b)
+          acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[b], af[a], acc[a][b], 0, 0, 0);
+    }
+  }
+  lds_barrier();  // every wave is done with the operand stages before they hold C
+  if (p.stream_c) store_tile<CT, true, TM, TN, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
+  else store_tile<CT, false, TM, TN, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
+}
+
+template <class Sh>
+void launch_tiled(hipStream_t s, Int8Gemm a) {
+  a.tiles_m = int((a.M + Sh::TM - 1) / Sh::TM);
+  a.tiles_n = int((a.N + Sh::TN - 1) / Sh::TN);
+  const dim3 g{unsigned(int64_t(a.tiles_m) * a.tiles_n)}, b{unsigned(64 * Sh::WGM * Sh::WGN)};
+  auto go = [&](auto ct) {
+    constexpr int CT = decltype(ct)::value;
+    if (a.K % 16 != 0) hipLaunchKernelGGL((gemm_int8_tiled_kernel<Sh, CT, true>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((gemm_int8_tiled_kernel<Sh, CT, false>), g, b, 0, s, a);
+  };
+  if (a.c_type == MK_BF16) go(Int<MK_BF16>{});
+  else if (a.c_type == MK_F16) go(Int<MK_F16>{});
+  else go(Int<MK_F32>{});
+}
+
+// rows on the 16-byte grid that do not overlap, below the 2^31 bytes of a buffer's offsets
+bool on_grid(const int8_t* p, int64_t rows, int64_t K, int64_t ld) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld >= K &&
+         (rows - 1) * ld + K + 16 < (int64_t(1) << 31);
+}
+
+// ---------------------------------------------------------------- any operands
 // Any shape, pitch and alignment: 64 x 64 tiles, 4 waves of 32 x 32, k 64 deep
 // through registers and LDS.
 __global__ __launch_bounds__(256) void gemm_int8_any_kernel(const Int8Gemm p) {
@@ -58,22 +442,12 @@ __global__ __launch_bounds__(256) void gemm_int8_any_kernel(const Int8Gemm p) {
                           p.B + std::min<int64_t>(n0 + row, p.N - 1) * p.ldb + at};
   i32x16_t acc = {};
   for (int64_t k0 = 0; k0 < p.K; k0 += BK) {
-    u32x4_t v[2];
+    i32x4_t v[2];
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int64_t left = p.K - k0 - at;
-      if (left >= 16) {
-        v[o] = reinterpret_cast<const Any16*>(src[o] + k0)->v;
-      } else {
-        uint8_t b[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) b[e] = e < left ? uint8_t(src[o][k0 + e]) : 0;
-        __builtin_memcpy(&v[o], b, 16);
-      }
-    }
+    for (int o = 0; o < 2; ++o) v[o] = load16_upto(src[o] + k0, p.K - k0 - at);
     __syncthreads();
 #pragma unroll
-    for (int o = 0; o < 2; ++o) *reinterpret_cast<u32x4_t*>(&lds[o][row * kPitch + at]) = v[o];
+    for (int o = 0; o < 2; ++o) *reinterpret_cast<i32x4_t*>(&lds[o][row * kPitch + at]) = v[o];
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < BK / 32; ++ks) {
@@ -121,8 +495,22 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
       (epi != 0 && reinterpret_cast<uintptr_t>(bias) % ((epilogue & 4) ? 4 : dtype_bytes(c_type))))
     return fail(MK_ERR_INVALID, at + "an operand is not aligned to its elements");
   Int8Gemm a{A, B, a_scale, b_scale, C, bias, M, N, K, a_ms, b_ns, c_ms, int((M + 63) / 64), int((N + 63) / 64),
-             c_type, epilogue};
-  hipLaunchKernelGGL(gemm_int8_any_kernel, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n)), dim3(256), 0,
-                     as_stream(stream), a);
+             c_type, epilogue, 0};
+  hipStream_t s = as_stream(stream);
+  if (M <= 64) {
+    // 64 columns per workgroup where that fills the chip's 256 CUs, else fewer
+    if (N >= 64 * 192) launch_rows<4>(s, a);
+    else if (N >= 32 * 192) launch_rows<2>(s, a);
+    else launch_rows<1>(s, a);
+    return check_launch("mk_gemm_int8");
+  }
+  if (K > 0 && N > 1 && on_grid(A, M, K, a_ms) && on_grid(B, N, K, b_ns)) {
+    a.stream_c = M * N * dtype_bytes(c_type) >= int64_t(192) << 20;
+    if (M >= 256 && N >= 256) launch_tiled<Shape<256, 256, 2, 4>>(s, a);
+    else if (M >= 128 && N >= 128) launch_tiled<Shape<128, 128, 4, 2>>(s, a);
+    else launch_tiled<Shape<64, 64, 2, 2>>(s, a);
+    return check_launch("mk_gemm_int8");
+  }
+  hipLaunchKernelGGL(gemm_int8_any_kernel, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n)), dim3(256), 0, s, a);
   return check_launch("mk_gemm_int8");
 }
