@@ -664,85 +664,132 @@ def sdpa_bwd(q, k, v, o, dout, lse, scale, causal=True, dq=None, dk=None, dv=Non
 
 
 # ------------------------------------------------------------------ eight-bit serving
-_ROW_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+# The smallest of these calls are this layer's time too: operands are looked at
+# once by _fits, and what is wrong with one is worked out only for the error
+# (a norm of 1 x 768 with its residual: HOST_BEFORE -> HOST_AFTER us a call).
+_ROW_TYPES = {torch.bfloat16: MK["BF16"], torch.float16: MK["F16"], torch.float32: MK["F32"]}
 
 
-def _take(what, t, name, dtypes, shape):
-    """An operand of the shape and a type asked for, on the current device, elements of a row contiguous."""
-    if not t.is_cuda or t.get_device() != _device():
+def _here(what, t, name):
+    """The device of a call's operand, which is the current one."""
+    dev = t.get_device()
+    if dev < 0 or dev != _device():
         raise ValueError(f"{what}: {name} is not on the current device")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{what}: {name} has dtype {t.dtype}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, {shape} is asked for")
-    if shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}: {name} is not contiguous along its last dimension")
+    return dev
 
 
-def _new(shape, dtype, device, stream):
-    """An output, from the memory of the stream that writes it."""
+def _fits(t, dtype, shape, dev):
+    """Whether an operand has the type and shape asked for, on that device, the elements of a row contiguous."""
+    return t.dtype is dtype and t.shape == shape and t.get_device() == dev and (shape[-1] <= 1 or t.stride()[-1] == 1)
+
+
+def _refuse(what, name, t, dtypes, shape, dev):
+    """The ValueError of an operand that does not fit."""
+    if t.get_device() != dev:
+        why = "is not on the current device"
+    elif t.dtype not in dtypes:
+        why = f"has dtype {t.dtype}"
+    elif t.shape != shape:
+        why = f"has shape {tuple(t.shape)}, {tuple(shape)} is asked for"
+    else:
+        why = "is not contiguous along its last dimension, or its rows overlap"
+    raise ValueError(f"{what}: {name} {why}")
+
+
+def _operand(what, name, t, dtype, shape, dev):
+    if not _fits(t, dtype, shape, dev):
+        _refuse(what, name, t, (dtype,), shape, dev)
+
+
+def _result(what, name, t, dtype, shape, dev):
+    """A 2-D operand to be written: its rows do not overlap either."""
+    if not _fits(t, dtype, shape, dev) or (shape[0] > 1 and t.stride()[0] < shape[1]):
+        _refuse(what, name, t, (dtype,), shape, dev)
+
+
+def _rows(what, x, name="x"):
+    """(type, shape, row pitch, device) of a 2-D operand that gives a call its shape and type."""
+    dev, t = _here(what, x, name), _ROW_TYPES.get(x.dtype)
+    if x.dim() != 2:
+        raise ValueError(f"{what}: {name} must be 2-D")
+    shape, st = x.shape, x.stride()
+    if t is None or (st[1] != 1 and shape[1] > 1):
+        _refuse(what, name, x, _ROW_TYPES, shape, dev)
+    return t, shape, st[0], dev
+
+
+def _handle(what, stream, dev):
+    if stream is None:
+        return _raw_stream(dev)
+    if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
+        raise ValueError(f"{what}: the stream is another device's")
+    return stream.cuda_stream
+
+
+def _new(like, stream, dtype, *shape):
+    """An output on like's device, from the memory of the stream that writes it."""
     if stream is None or not isinstance(stream, torch.cuda.Stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(*shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(*shape, dtype=dtype)
 
 
-def _new_int8_rows(rows, cols, device, stream):
-    """Rows of 8 bits that start on 16-byte boundaries, as gemm_int8's fastest kernels take them."""
-    pitch = (cols + 15) // 16 * 16
-    q = _new((rows, pitch), torch.int8, device, stream)
-    return q if pitch == cols else q[:, :cols]
+def _new_like(x, stream, dtype):
+    """An output of the shape of rows x, which is dense."""
+    if stream is None or not isinstance(stream, torch.cuda.Stream):
+        return torch.empty_like(x, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(x, dtype=dtype)
 
 
-def _own_rows(what, t, name):
-    """Rows to be written do not overlap."""
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{what}: rows of {name} overlap")
-
-
-def _int8_outputs(what, x, q, scale, stream):
-    rows, cols = x.shape
+def _int8_outputs(what, x, shape, ld, q, scale, dev, stream):
+    """q, its row pitch and scale: a new q has its rows on 16-byte boundaries, which gemm_int8 multiplies fastest."""
+    rows, cols = shape
     if q is None:
-        q = _new_int8_rows(rows, cols, x.device, stream)
+        pitch = (cols + 15) // 16 * 16
+        if pitch == cols == ld:
+            q = _new_like(x, stream, torch.int8)
+        else:
+            q = _new(x, stream, torch.int8, rows, pitch)
+            if pitch != cols:
+                q = q[:, :cols]
     else:
-        _take(what, q, "q", (torch.int8,), (rows, cols))
-        _own_rows(what, q, "q")
+        _result(what, "q", q, torch.int8, shape, dev)
+        pitch = q.stride()[0]
     if scale is None:
-        scale = _new((rows,), torch.float32, x.device, stream)
+        scale = _new(x, stream, torch.float32, rows)
     else:
-        _take(what, scale, "scale", (torch.float32,), (rows,))
-    return q, scale
+        _operand(what, "scale", scale, torch.float32, shape[:1], dev)
+    return q, pitch, scale
 
 
 def add_rmsnorm_int8(x, residual=None, gamma=None, eps=1e-6, sum_out=None, q=None, scale=None, stream=None):
     """(q, scale, sum) of [rows, cols] x: sum = x + residual (x itself where
     residual is None), and 8-bit rows q with one fp32 scale each that stand for
     y = sum / sqrt(mean(sum^2) + eps) * gamma, the operand of gemm_int8
-    (mk_add_rmsnorm_int8).  Any row pitch; sum_out may be x or residual."""
+    (mk_add_rmsnorm_int8).  Any row pitch; sum_out may be x or residual.
+    Outputs that are not given come from the memory of `stream`."""
     what = "add_rmsnorm_int8"
-    if x.dim() != 2:
-        raise ValueError(f"{what}: x must be 2-D")
-    shape = (rows, cols) = tuple(x.shape)
-    _take(what, x, "x", _ROW_TYPES, shape)
-    total = x
+    t, shape, ld, dev = _rows(what, x)
+    total, r_ptr, r_ld, s_ptr, s_ld = x, None, 0, None, 0
     if residual is not None:
-        _take(what, residual, "residual", (x.dtype,), shape)
+        _operand(what, "residual", residual, x.dtype, shape, dev)
         if sum_out is None:
-            total = _new(shape, x.dtype, x.device, stream)
+            total = _new_like(x, stream, x.dtype) if ld == shape[1] else _new(x, stream, x.dtype, *shape)
         else:
             total = sum_out
-            _take(what, total, "sum_out", (x.dtype,), shape)
-            _own_rows(what, total, "sum_out")
+            _result(what, "sum_out", total, x.dtype, shape, dev)
+        r_ptr, r_ld, s_ptr, s_ld = residual.data_ptr(), residual.stride()[0], total.data_ptr(), total.stride()[0]
     elif sum_out is not None:
         raise ValueError(f"{what}: sum_out without a residual")
     if gamma is not None:
-        _take(what, gamma, "gamma", (x.dtype,), (cols,))
-    q, scale = _int8_outputs(what, x, q, scale, stream)
-    rc = lib().mk_add_rmsnorm_int8(_stream(stream), mk_dtype(x.dtype), rows, cols, x.data_ptr(), x.stride(0),
-                                   _ptr(residual), 0 if residual is None else residual.stride(0), _ptr(gamma),
-                                   float(eps), None if residual is None else total.data_ptr(), total.stride(0),
-                                   q.data_ptr(), q.stride(0), scale.data_ptr())
-    _check(rc, "mk_add_rmsnorm_int8")
+        _operand(what, "gamma", gamma, x.dtype, shape[1:], dev)
+    q, pitch, scale = _int8_outputs(what, x, shape, ld, q, scale, dev, stream)
+    rc = lib().mk_add_rmsnorm_int8(_handle(what, stream, dev), t, shape[0], shape[1], x.data_ptr(), ld, r_ptr, r_ld,
+                                   None if gamma is None else gamma.data_ptr(), eps, s_ptr, s_ld, q.data_ptr(), pitch,
+                                   scale.data_ptr())
+    if rc:
+        _check(rc, "mk_add_rmsnorm_int8")
     return q, scale, total
 
 
@@ -751,31 +798,34 @@ def quantize_rows(x, gelu=False, q=None, scale=None, stream=None):
     rows with one fp32 scale each, max |y| / 127 (mk_quantize_rows).  For
     weights x is [out, in] and the product takes q.t()."""
     what = "quantize_rows"
-    if x.dim() != 2:
-        raise ValueError(f"{what}: x must be 2-D")
-    _take(what, x, "x", _ROW_TYPES, tuple(x.shape))
-    q, scale = _int8_outputs(what, x, q, scale, stream)
-    rc = lib().mk_quantize_rows(_stream(stream), mk_dtype(x.dtype), x.shape[0], x.shape[1], x.data_ptr(), x.stride(0),
-                                int(bool(gelu)), q.data_ptr(), q.stride(0), scale.data_ptr())
-    _check(rc, "mk_quantize_rows")
+    t, shape, ld, dev = _rows(what, x)
+    q, pitch, scale = _int8_outputs(what, x, shape, ld, q, scale, dev, stream)
+    rc = lib().mk_quantize_rows(_handle(what, stream, dev), t, shape[0], shape[1], x.data_ptr(), ld, 1 if gelu else 0,
+                                q.data_ptr(), pitch, scale.data_ptr())
+    if rc:
+        _check(rc, "mk_quantize_rows")
     return q, scale
 
 
 def dequantize_rows(q, scale, dtype=torch.bfloat16, out=None, stream=None):
     """The values q * scale that 8-bit rows stand for, in `dtype`."""
-    what = "dequantize_rows"
+    what, t = "dequantize_rows", _ROW_TYPES.get(dtype)
+    dev = _here(what, q, "q")
+    if t is None:
+        raise ValueError(f"{what}: no rows of {dtype}")
     if q.dim() != 2:
         raise ValueError(f"{what}: q must be 2-D")
-    shape = tuple(q.shape)
-    _take(what, q, "q", (torch.int8,), shape)
-    _take(what, scale, "scale", (torch.float32,), shape[:1])
+    shape = q.shape
+    _operand(what, "q", q, torch.int8, shape, dev)
+    _operand(what, "scale", scale, torch.float32, shape[:1], dev)
     if out is None:
-        out = _new(shape, dtype, q.device, stream)
-    _take(what, out, "out", (dtype,) if dtype in _ROW_TYPES else (), shape)
-    _own_rows(what, out, "out")
-    rc = lib().mk_dequantize_rows(_stream(stream), mk_dtype(dtype), shape[0], shape[1], q.data_ptr(), q.stride(0),
-                                  scale.data_ptr(), out.data_ptr(), out.stride(0))
-    _check(rc, "mk_dequantize_rows")
+        out = _new_like(q, stream, dtype) if q.stride()[0] == shape[1] else _new(q, stream, dtype, *shape)
+    else:
+        _result(what, "out", out, dtype, shape, dev)
+    rc = lib().mk_dequantize_rows(_handle(what, stream, dev), t, shape[0], shape[1], q.data_ptr(), q.stride()[0],
+                                  scale.data_ptr(), out.data_ptr(), out.stride()[0])
+    if rc:
+        _check(rc, "mk_dequantize_rows")
     return out
 
 
@@ -785,38 +835,41 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16, bias=None, relu=
     add_rmsnorm_int8 give it, b the transposed view of weights stored by output
     channel (quantize_rows(w)[0].t()).  a_scale [M], b_scale [N] fp32; the sum
     over k is exact (mk_gemm_int8)."""
-    what = "gemm_int8"
+    what, t = "gemm_int8", _ROW_TYPES.get(out_dtype)
+    dev = _here(what, a, "a")
+    if t is None:
+        raise ValueError(f"{what}: no results in {out_dtype}")
     if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[0]:
         raise ValueError(f"{what}: a [M, K] and b [K, N] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
-    (M, Kd), N = a.shape, b.shape[1]
-    w = b.t()
-    _take(what, a, "a", (torch.int8,), (M, Kd))
-    _take(what, w, "b, transposed,", (torch.int8,), (N, Kd))
-    _take(what, a_scale, "a_scale", (torch.float32,), (M,))
-    _take(what, b_scale, "b_scale", (torch.float32,), (N,))
+    shape_a, sb = a.shape, b.stride()
+    M, Kd = shape_a
+    N = b.shape[1]
+    _operand(what, "a", a, torch.int8, shape_a, dev)
+    if b.dtype is not torch.int8 or b.get_device() != dev or (sb[0] != 1 and Kd > 1):
+        _refuse(what, "b, transposed,", b.t(), (torch.int8,), (N, Kd), dev)
+    _operand(what, "a_scale", a_scale, torch.float32, (M,), dev)
+    _operand(what, "b_scale", b_scale, torch.float32, (N,), dev)
     if out is None:
-        out = _new((M, N), out_dtype, a.device, stream)
-    _take(what, out, "out", (out_dtype,) if out_dtype in _ROW_TYPES else (), (M, N))
-    _own_rows(what, out, "out")
-    epi = 0
+        out = _new(a, stream, out_dtype, M, N)
+        ld = N
+    else:
+        _result(what, "out", out, out_dtype, (M, N), dev)
+        ld = out.stride()[0]
+    epi, bias_ptr = 0, None
     if bias is not None:
-        _take(what, bias, "bias", (out_dtype, torch.float32), (N,))
-        epi = (2 if relu else 1) | (4 if bias.dtype != out_dtype else 0)
+        epi = 2 if relu else 1
+        if not _fits(bias, out_dtype, (N,), dev):
+            if not _fits(bias, torch.float32, (N,), dev):
+                _refuse(what, "bias", bias, (out_dtype, torch.float32), (N,), dev)
+            epi |= 4  # an fp32 bias added before the narrowing store
+        bias_ptr = bias.data_ptr()
     elif relu:
         raise ValueError(f"{what}: relu goes with a bias")
-    rc = lib().mk_gemm_int8(_stream(stream), mk_dtype(out_dtype), M, N, Kd, a.data_ptr(), a.stride(0),
-                            a_scale.data_ptr(), w.data_ptr(), w.stride(0), b_scale.data_ptr(), out.data_ptr(),
-                            out.stride(0), _ptr(bias), epi)
-    _check(rc, "mk_gemm_int8")
+    rc = lib().mk_gemm_int8(_handle(what, stream, dev), t, M, N, Kd, a.data_ptr(), a.stride()[0], a_scale.data_ptr(),
+                            b.data_ptr(), sb[1], b_scale.data_ptr(), out.data_ptr(), ld, bias_ptr, epi)
+    if rc:
+        _check(rc, "mk_gemm_int8")
     return out
-
-
-def _per_row(what, v, name, dtype, rows, off):
-    """(pointer, value) of a parameter that is a number for all rows or a tensor of one for each."""
-    if isinstance(v, torch.Tensor):
-        _take(what, v, name, (dtype,), (rows,))
-        return v.data_ptr(), off
-    return None, off if v is None else v
 
 
 def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, index_dtype=torch.int32,
@@ -829,21 +882,39 @@ def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, 
     tensor of one value a row (top_k int32, the others fp32).  temperature 0 is
     row_argmax.  A row without a valid choice gives token -1 and logprob NaN."""
     what = "sample_rows"
-    if logits.dim() != 2:
-        raise ValueError(f"{what}: logits must be 2-D")
-    rows, vocab = logits.shape
-    _take(what, logits, "logits", _ROW_TYPES, (rows, vocab))
-    _take(what, u, "u", (torch.float32,), (rows,))
-    if index_dtype not in (torch.int32, torch.int64):
+    mk, shape, ld, dev = _rows(what, logits, "logits")
+    per_row = shape[:1]
+    _operand(what, "u", u, torch.float32, per_row, dev)
+    if index_dtype is not torch.int32 and index_dtype is not torch.int64:
         raise ValueError(f"{what}: index_dtype must be int32 or int64")
-    t, t_all = _per_row(what, temperature, "temperature", torch.float32, rows, 1.0)
-    k, k_all = _per_row(what, top_k, "top_k", torch.int32, rows, 0)
-    p, p_all = _per_row(what, top_p, "top_p", torch.float32, rows, 1.0)
-    m, m_all = _per_row(what, min_p, "min_p", torch.float32, rows, 0.0)
-    token = _new((rows,), index_dtype, logits.device, stream)
-    logprob = _new((rows,), torch.float32, logits.device, stream) if with_logprob else None
-    rc = lib().mk_sample_rows(_stream(stream), mk_dtype(logits.dtype), rows, vocab, logits.data_ptr(),
-                              logits.stride(0), u.data_ptr(), t, float(t_all), k, min(int(k_all), 2 ** 31 - 1), p,
-                              float(p_all), m, float(m_all), mk_dtype(index_dtype), token.data_ptr(), _ptr(logprob))
-    _check(rc, "mk_sample_rows")
+    # a number for all rows, or the address of one value a row
+    t = k = p = m = None
+    t_all, k_all, p_all, m_all = 1.0, 0, 1.0, 0.0
+    if isinstance(temperature, torch.Tensor):
+        _operand(what, "temperature", temperature, torch.float32, per_row, dev)
+        t = temperature.data_ptr()
+    elif temperature is not None:
+        t_all = temperature
+    if isinstance(top_k, torch.Tensor):
+        _operand(what, "top_k", top_k, torch.int32, per_row, dev)
+        k = top_k.data_ptr()
+    elif top_k is not None:
+        k_all = max(0, min(int(top_k), 2 ** 31 - 1))
+    if isinstance(top_p, torch.Tensor):
+        _operand(what, "top_p", top_p, torch.float32, per_row, dev)
+        p = top_p.data_ptr()
+    elif top_p is not None:
+        p_all = top_p
+    if isinstance(min_p, torch.Tensor):
+        _operand(what, "min_p", min_p, torch.float32, per_row, dev)
+        m = min_p.data_ptr()
+    elif min_p is not None:
+        m_all = min_p
+    token = _new(logits, stream, index_dtype, shape[0])
+    logprob = _new(logits, stream, torch.float32, shape[0]) if with_logprob else None
+    rc = lib().mk_sample_rows(_handle(what, stream, dev), mk, shape[0], shape[1], logits.data_ptr(), ld, u.data_ptr(), t,
+                              t_all, k, k_all, p, p_all, m, m_all, _TORCH_TO_MK[index_dtype], token.data_ptr(),
+                              _ptr(logprob))
+    if rc:
+        _check(rc, "mk_sample_rows")
     return token, logprob
