@@ -12,13 +12,25 @@
 // counts (top-k) or of weights (top-p) over x's bits, taken as a whole number
 // that orders as x does.
 //
-// Weights are whole numbers: w 2^s rounded, from an exponential in 64 bits, s
-// such that a row's sum stays below 2^63 (47 bits for 50257 tokens).  Their sums
-// are exact, whatever order the atomics take, and a token is the one that sums
-// in 64 bits give but for u within about 2^-40 of a border.
+// Weights are whole numbers: w 2^s, with 2^z to 2^-33 of itself in 64 bits, s
+// such that a row's sum stays below 2^63 (46 bits for 50257 tokens).  Their sums
+// are exact, whatever order the atomics take, so a result is the same on every
+// run, and errors of single weights cancel in them: for 50257 tokens a token is
+// the one that real numbers give but for about one u in a million.
 //
-// A workgroup has a row.  Bound: a few passes over the row, from L2 after the
-// first, at what one CU takes in.
+// A workgroup has a row and reads it two or three times (from L2 after the first):
+//   for the largest value, which also is the whole of a greedy choice;
+//   top-k: the k-th largest of the lanes' own maxima is below the row's k-th
+//   largest value, so what is at or above it holds the first k and is seldom much
+//   more: a second pass puts those tokens into a list in LDS;
+//   top-p alone: a second pass for the weights, a third for the list of the
+//   tokens of the first digit's cut and above;
+//   no cut: a second pass for the weights of each 512 tokens.
+// What remains happens on the list (16384 tokens; rows whose list is longer are
+// read again), then one wave finds the token in its 512.  Bound: one CU's work on
+// a row: barriers and LDS where there is a top-k, else an exponential in 64 bits
+// for each token.  Loops are kept short on purpose: unrolled over a row that
+// stayed in registers they ran slower, waiting for instructions (SLOWER).
 #include "mk_common.h"
 
 #include <algorithm>
@@ -31,7 +43,10 @@ constexpr int kThreads = 1024, kWaves = kThreads / kWave;
 constexpr int kBins = 4096;                 // 12 bits: a level of the histogram
 constexpr int kLane = 8;                    // elements a lane takes at once
 constexpr int kChunk = kLane * kWave;       // elements a wave takes at once
+constexpr int kList = 16384;                // tokens of the list
 constexpr int64_t kMaxVocab = int64_t(kBins) * kChunk;
+
+constexpr double kLowZ = -16.0;             // log2 of the weights that level 0 of top-p sums without digits
 
 typedef unsigned long long u64;
 
@@ -49,14 +64,16 @@ struct SampleArgs {
 };
 
 // An element type's values as whole numbers that order as they do, -0 as +0.
-// Finite values and infinities are at least 1.
+// No number and no infinity is 0: that stands for a place past the row's end.
 template <typename T> struct Order;
 template <> struct Order<float> {
   static constexpr int kLevels = 3;
   static constexpr int kShift[3] = {20, 10, 0}, kBits[3] = {12, 10, 10};
+  static __device__ inline float none() { return __builtin_bit_cast(float, 0xffffffffu); }
   static __device__ inline float value(float v) { return v; }
   static __device__ inline uint32_t key(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.f);
+    uint32_t b = __builtin_bit_cast(uint32_t, v);
+    b = b == 0x80000000u ? 0u : b;
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
   }
   static __device__ inline float of_key(uint32_t k) {
@@ -72,6 +89,7 @@ __device__ inline uint16_t of_key16(uint32_t k) { return uint16_t(k ^ (k >> 15 ?
 template <> struct Order<uint16_t> {
   static constexpr int kLevels = 2;
   static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4};
+  static __device__ inline uint16_t none() { return 0xffffu; }
   static __device__ inline float value(uint16_t v) { return bf16_to_f32(v); }
   static __device__ inline uint32_t key(uint16_t v) { return key16(v); }
   static __device__ inline float of_key(uint32_t k) { return bf16_to_f32(of_key16(k)); }
@@ -79,6 +97,7 @@ template <> struct Order<uint16_t> {
 template <> struct Order<F16> {
   static constexpr int kLevels = 2;
   static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4};
+  static __device__ inline F16 none() { return F16{0xffffu}; }
   static __device__ inline float value(F16 v) { return f16_to_f32(v.bits); }
   static __device__ inline uint32_t key(F16 v) { return key16(v.bits); }
   static __device__ inline float of_key(uint32_t k) { return f16_to_f32(of_key16(k)); }
@@ -87,13 +106,16 @@ template <> struct Order<F16> {
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Run { T v[kLane]; };
 
 struct Shared {
-  u64 mass[kBins];      // a level's weights by digit; then the chunks' weights
+  u64 mass[kBins];        // a level's weights by digit; then the chunks' weights
   uint32_t count[kBins];  // a level's counts by digit; then the chunks' ties
+  uint32_t key[kList];    // the list: keys, and the chunks they are from
+  uint16_t chunk[kList];
   u64 wave_sum[kWaves];
-  uint32_t top, bad;
+  u64 top, low;
+  uint32_t bad, n;
   // what the one thread that found a place leaves for the others
   int found;
-  u64 before, total;
+  u64 before;
   uint32_t ties_before;
 };
 
@@ -121,59 +143,156 @@ __device__ inline u64 scan(u64 v, Shared& sh, u64& total) {
   return before + s - v;
 }
 
+// sum over 16 lanes, in each of them (as wave_sum_dpp's first steps)
+template <int CTRL>
+__device__ inline u64 dpp_u64(u64 v) {
+  const uint32_t lo = uint32_t(__builtin_amdgcn_mov_dpp(int(uint32_t(v)), CTRL, 0xF, 0xF, false));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_mov_dpp(int(uint32_t(v >> 32)), CTRL, 0xF, 0xF, false));
+  return (u64(hi) << 32) | lo;
+}
+__device__ inline u64 row_sum(u64 v) {
+  v += dpp_u64<0xB1>(v);
+  v += dpp_u64<0x4E>(v);
+  v += dpp_u64<0x141>(v);
+  v += dpp_u64<0x140>(v);
+  return v;
+}
+// v of all lanes added to *to
+__device__ inline void add_all(u64* to, u64 v) {
+  v = row_sum(v);
+  if (threadIdx.x % 16 == 0 && v) atomicAdd(to, v);
+}
+
 template <typename T>
 struct Row {
   using O = Order<T>;
   const T* x;
   int64_t V;
   double top, per;  // the largest value; log2(e) / temperature
-  double least;     // min-p
   int shift;
   uint32_t cut;     // kept: keys above cut, and the first `ties` equal to it
   u64 ties;
+  int listed;       // tokens in the list, -1: there is none
+  bool whole;       // the list holds everything that is kept
 
-  // weight of a value, 2^shift for the largest
-  __device__ inline u64 weight(float v) const {
-    const double z = (double(v) - top) * per;
-    if (!(z > -double(shift) - 2.0)) return 0;  // rounds to 0 (z may be -inf)
-    const double w = exp2(z);
-    if (w < least) return 0;
-    // 2^52 + n holds the whole number n in its low bits
-    return __builtin_bit_cast(u64, ldexp(w, shift) + 0x1p52) & ((u64(1) << 52) - 1);
+  // log2 of a weight, at least -64 (weights below 2^-52 are 0)
+  __device__ inline double log2_weight(float v) const { return max((double(v) - top) * per, -64.0); }
+  // The weight, 2^shift for the largest.  2^z = 2^n 2^f, n the nearest whole number
+  // (1.5 2^52 + n holds it in its low bits); 2^f is the polynomial through it at 8
+  // Chebyshev points of [-1/2, 1/2], its constant made 1, 2^-33 of itself off;
+  // 2^52 + w holds the rounded weight in its low bits.
+  __device__ inline u64 weight_of(double z) const {
+    const double t = z + 0x1.8p52, f = z - (t - 0x1.8p52);
+    const int n = int(uint32_t(__builtin_bit_cast(u64, t)));
+    double e = 1.5303699001378845e-05;
+    e = fma(e, f, 0.00015469729140704658);
+    e = fma(e, f, 0.0013333478480888061);
+    e = fma(e, f, 0.0096180256135980358);
+    e = fma(e, f, 0.055504109063177154);
+    e = fma(e, f, 0.24022651213495422);
+    e = fma(e, f, 0.69314718055683411);
+    e = fma(e, f, 1.0);
+    return __builtin_bit_cast(u64, ldexp(e, shift + n) + 0x1p52) & ((u64(1) << 52) - 1);
   }
-  // f(index, element) over the row, kLane consecutive elements per lane
-  template <class F>
-  __device__ inline void each(F f) const {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    for (int64_t c = wave; c * kChunk < V; c += kWaves) {
-      const int64_t i = c * kChunk + lane * kLane;
-      chunk(c, i, f);
-    }
-  }
-  template <class F>
-  __device__ inline void chunk(int64_t c, int64_t i, F f) const {
-    if (i + kLane <= V) {
-      const Run<T> r = *reinterpret_cast<const Run<T>*>(x + i);
+  __device__ inline u64 weight(float v) const { return weight_of(log2_weight(v)); }
+
+  // The elements at i .. i + kLane - 1.  Where the row ends among or before them
+  // they are the row's last kLane, with none() for those before i: which of its
+  // chunk's elements a lane holds is all that counts.
+  __device__ inline Run<T> load(int64_t i) const {
+    Run<T> r;
+    if (V >= kLane) {
+      const int64_t from = min(i, V - kLane);
+      r = *reinterpret_cast<const Run<T>*>(x + from);
+      if (from < i) {
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) f(c, i + e, r.v[e]);
+        for (int e = 0; e < kLane; ++e) r.v[e] = from + e < i ? O::none() : r.v[e];
+      }
     } else {
-      for (int64_t k = i; k < V; ++k) f(c, k, x[k]);
+      for (int e = 0; e < kLane; ++e) r.v[e] = i + e < V ? x[i + e] : O::none();
     }
+    return r;
+  }
+  static __device__ inline int lane() { return threadIdx.x & (kWave - 1); }
+  static __device__ inline int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); }
+
+  // f(chunk, its kLane elements of this lane) over the row, kAhead chunks loaded ahead
+  template <int kAhead, class F>
+  __device__ inline void each(F f) const {
+    const int chunks = int((V + kChunk - 1) / kChunk);
+    auto at = [&](int c) { return load(int64_t(c) * kChunk + lane() * kLane); };
+    Run<T> next[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) next[a] = at(wave() + kWaves * a);
+#pragma unroll 1
+    for (int c = wave(); c < chunks; c += kAhead * kWaves) {
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const Run<T> r = next[a];
+        next[a] = at(c + kWaves * (a + kAhead));
+        if (c + kWaves * a < chunks) f(c + kWaves * a, r);
+      }
+    }
+  }
+  // f(chunk, key) over the list, or over the row
+  template <class F>
+  __device__ inline void over(const Shared& sh, F f) const {
+    if (listed >= 0) {
+#pragma unroll 1
+      for (int e = threadIdx.x; e < listed; e += kThreads) f(int(sh.chunk[e]), sh.key[e]);
+    } else {
+      each<1>([&](int c, const Run<T>& r) {
+#pragma unroll
+        for (int e = 0; e < kLane; ++e) f(c, O::key(r.v[e]));
+      });
+    }
+  }
+  // The list of the tokens whose key, without its low `by` bits, is at least (or
+  // ONLY: just) `least`; whether they fit.
+  template <bool ONLY>
+  __device__ inline bool make_list(Shared& sh, int by, uint32_t least) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    each<3>([&](int c, const Run<T>& r) {
+      uint32_t mine = 0;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) {
+        const uint32_t key = O::key(r.v[e]);
+        mine |= uint32_t(key != 0 && (ONLY ? (key >> by) == least : (key >> by) >= least)) << e;
+      }
+      if (mine) {
+        uint32_t at = atomicAdd(&sh.n, uint32_t(__popc(mine)));
+        if (at <= uint32_t(kList - kLane)) {
+#pragma unroll
+          for (int e = 0; e < kLane; ++e)
+            if (mine >> e & 1) {
+              sh.key[at] = O::key(r.v[e]);
+              sh.chunk[at] = uint16_t(c);
+              ++at;
+            }
+        }
+      }
+    });
+    __syncthreads();
+    listed = sh.n <= uint32_t(kList - kLane) ? int(sh.n) : -1;
+    return listed >= 0;
   }
 
   // The digit of a level in which the running sum from the largest digit down
-  // reaches `target`: sh.found, and sh.before, the sum above it.  The total of
-  // the level is returned first to `aim`, which says what the target is.
+  // (`above` before the level) reaches aim(sum of all): left in sh.found, and the
+  // sum above it in sh.before.  No digit where it takes sh.low as well: sh.found -1.
   template <bool MASS, class Aim>
-  __device__ inline void place(Shared& sh, int bits, u64 above, Aim aim) {
+  __device__ inline void place(Shared& sh, int bits, u64 above, Aim aim) const {
     const int bins = 1 << bits, per_thread = bins > kThreads ? bins / kThreads : 1;
-    u64 own = 0;
     const int first = bins - 1 - int(threadIdx.x) * per_thread;
+    if (threadIdx.x == 0) sh.found = -1;
+    u64 own = 0;
     for (int k = 0; k < per_thread; ++k)
       if (first - k >= 0) own += MASS ? sh.mass[first - k] : u64(sh.count[first - k]);
     u64 total;
     u64 before = above + scan(own, sh, total);
-    const u64 target = aim(above + total);
+    const u64 target = aim(above + total + (MASS ? sh.low : 0));
     if (before < target && target <= before + own) {
       for (int k = 0; k < per_thread; ++k) {
         const u64 n = MASS ? sh.mass[first - k] : u64(sh.count[first - k]);
@@ -187,6 +306,16 @@ struct Row {
     }
     __syncthreads();
   }
+  template <bool MASS>
+  __device__ inline void clear(Shared& sh, int n) const {
+    __syncthreads();
+    if (MASS && threadIdx.x == 0) sh.low = 0;
+    for (int b = threadIdx.x; b < n; b += kThreads) {
+      if (MASS) sh.mass[b] = 0;
+      else sh.count[b] = 0;
+    }
+    __syncthreads();
+  }
 
   // Moves the cut to where the kept counts (or weights) from the largest value
   // down reach aim(their total), and keeps as many ties there as that takes.
@@ -195,35 +324,56 @@ struct Row {
     uint32_t prefix = 0;
     u64 above = 0, target = 0;
     const u64 tie_weight = MASS && cut != 0 ? weight(O::of_key(cut)) : 0;
+#pragma unroll
     for (int level = 0; level < O::kLevels; ++level) {
-      const int shift_by = O::kShift[level], bits = O::kBits[level];
+      const int by = O::kShift[level], bits = O::kBits[level];
       const uint32_t mask = (1u << bits) - 1;
-      __syncthreads();
-      for (int b = threadIdx.x; b <= int(mask); b += kThreads) {
-        if (MASS) sh.mass[b] = 0;
-        else sh.count[b] = 0;
-      }
-      __syncthreads();
-      each([&](int64_t, int64_t, T v) {
-        const uint32_t key = O::key(v);
-        if (level > 0 && (key >> (shift_by + bits)) != prefix) return;
-        if (MASS) {
-          if (key > cut)
-            if (const u64 w = weight(O::value(v))) atomicAdd(&sh.mass[(key >> shift_by) & mask], w);
+      // The weights of the first level: a weight below 2^floor_z is seldom part of a
+      // cut, and goes without its digit into one sum, unless the cut turns out to
+      // need it.
+      double floor_z = MASS && level == 0 && listed < 0 ? kLowZ : -64.0;
+      for (;;) {
+        clear<MASS>(sh, int(mask) + 1);
+        if (MASS && level == 0 && listed < 0) {
+          u64 low = 0;
+          each<1>([&](int, const Run<T>& r) {
+#pragma unroll
+            for (int e = 0; e < kLane; ++e) {
+              const uint32_t key = O::key(r.v[e]);
+              if (key <= cut) continue;
+              const double z = log2_weight(O::value(r.v[e]));
+              const u64 w = weight_of(z);
+              if (z > floor_z) atomicAdd(&sh.mass[(key >> by) & mask], w);
+              else low += w;
+            }
+          });
+          add_all(&sh.low, low);
         } else {
-          atomicAdd(&sh.count[(key >> shift_by) & mask], 1u);
+          over(sh, [&](int, uint32_t key) {
+            if (key <= (MASS ? cut : 0u) || (level > 0 && (key >> (by + bits)) != prefix)) return;
+            if (MASS) atomicAdd(&sh.mass[(key >> by) & mask], weight(O::of_key(key)));
+            else atomicAdd(&sh.count[(key >> by) & mask], 1u);
+          });
         }
-      });
-      if (MASS && cut != 0 && threadIdx.x == 0 && (level == 0 || (cut >> (shift_by + bits)) == prefix))
-        atomicAdd(&sh.mass[(cut >> shift_by) & mask], ties * tie_weight);
-      __syncthreads();
-      place<MASS>(sh, bits, above, [&](u64 total) {
-        if (level == 0) target = aim(total);
-        return target;
-      });
+        if (MASS && cut != 0 && threadIdx.x == 0 && (level == 0 || (cut >> (by + bits)) == prefix))
+          atomicAdd(&sh.mass[(cut >> by) & mask], ties * tie_weight);
+        __syncthreads();
+        place<MASS>(sh, bits, above, [&](u64 total) {
+          if (level == 0) target = aim(total);
+          return target;
+        });
+        if (sh.found >= 0 || floor_z <= -64.0) break;
+        floor_z = -64.0;
+      }
       prefix = (prefix << bits) | uint32_t(sh.found);
       above = sh.before;
+      // the other digits on the tokens of this one, with those above where they fit
+      if (level == 0 && listed < 0) {
+        whole = make_list<false>(sh, by, prefix);
+        if (!whole) make_list<true>(sh, by, prefix);
+      }
     }
+    if (!whole) listed = -1;
     u64 need = target - above;
     if (MASS) {
       const u64 w = weight(O::of_key(prefix));
@@ -244,6 +394,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   r.x = static_cast<const T*>(p.x) + row * p.ld;
   r.V = p.V;
   r.shift = p.shift;
+  r.listed = -1;
+  r.whole = false;
   const float u = p.u[row];
   float t = p.temperature ? p.temperature[row] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
@@ -251,26 +403,32 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   int64_t k = p.top_k ? p.top_k[row] : p.top_k_all;
   bool bad = !(t >= 0.f) || t == INFINITY || top_p != top_p || min_p != min_p || u != u;
 
-  // the largest value, and whether there is a NaN
+  // The largest value, of this lane's and of all, with the first chunk that holds
+  // it; and whether there are more NaN than the places past the row's end.
   if (threadIdx.x == 0) sh.top = 0, sh.bad = 0;
   __syncthreads();
-  uint32_t top = 0, nan = 0;
-  r.each([&](int64_t, int64_t, T v) {
-    const float f = O::value(v);
-    nan |= f != f;
-    top = max(top, O::key(v));
-  });
+  uint32_t mine = 0, nan = 0;
+  int mine_at = 0;
+  r.template each<3>([&](int c, const Run<T>& v) {
+    const int64_t past = int64_t(c) * kChunk + (lane + 1) * kLane - p.V;
+    nan -= past > 0 ? uint32_t(min(past, int64_t(kLane))) : 0u;
+    uint32_t m = 0;
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    top = max(top, uint32_t(__shfl_xor(int(top), m, kWave)));
-    nan |= uint32_t(__shfl_xor(int(nan), m, kWave));
-  }
-  if (lane == 0) {
-    atomicMax(&sh.top, top);
-    atomicOr(&sh.bad, nan);
-  }
+    for (int e = 0; e < kLane; ++e) {
+      const float f = O::value(v.v[e]);
+      nan += f != f;
+      m = max(m, O::key(v.v[e]));
+    }
+    if (m > mine) mine = m, mine_at = c;
+  });
+  u64 best = (u64(mine) << 32) | uint32_t(~mine_at);
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) best = max(best, u64(__shfl_xor(best, m, kWave)));
+  if (lane == 0) atomicMax(&sh.top, best);
+  if (nan) sh.bad = 1;
   __syncthreads();
-  const float largest = O::of_key(sh.top);
+  const uint32_t top_key = uint32_t(sh.top >> 32);
+  const float largest = O::of_key(top_key);
   bad = bad || sh.bad || largest == INFINITY || largest == -INFINITY;
   if (bad) {  // the whole workgroup
     if (threadIdx.x == 0) {
@@ -280,106 +438,138 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     }
     return;
   }
-  const bool greedy = t == 0.f;
-  if (greedy) t = 1.f, k = 1;
+  if (t == 0.f) t = 1.f, k = 1;  // (one token is kept whatever the others say)
   r.top = largest;
   r.per = 1.4426950408889634 / double(t);
-  r.least = greedy ? 0.0 : min(double(min_p), 1.0);
   r.cut = 0;
   r.ties = 0;
+  u64 total, rest;
+  int chunk;
+  uint32_t ties_before;
+  // min-p as a weight
+  const u64 least = u64(ceil(ldexp(max(0.0, min(double(min_p), 1.0)), p.shift)));
+  u64 tie_weight;
   if (k == 1) {
-    r.cut = sh.top;
+    r.cut = top_key;
     r.ties = 1;
-  } else if (k > 0 && k < p.V) {
-    r.template select<false>(sh, [&](u64) { return u64(k); });
-  }
-  if (!greedy && top_p < 1.f && k != 1) {
-    // top-p counts what top-k kept, before min-p
-    const double least = r.least;
-    r.least = 0.0;
-    r.template select<true>(sh, [&](u64 total) {
-      const double aim = ceil(double(top_p) * double(total));
-      return aim >= 1.0 ? min(u64(aim), total) : u64(1);
-    });
-    r.least = least;
-  }
-
-  // weights and ties of each chunk
-  const u64 tie_weight = r.cut != 0 ? r.weight(O::of_key(r.cut)) : 0;
-  const int chunks = int((p.V + kChunk - 1) / kChunk);
-  __syncthreads();
-  for (int b = threadIdx.x; b < chunks; b += kThreads) sh.mass[b] = 0, sh.count[b] = 0;
-  __syncthreads();
-  r.each([&](int64_t c, int64_t, T v) {
-    const uint32_t key = O::key(v);
-    if (key > r.cut) {
-      if (const u64 w = r.weight(O::value(v))) atomicAdd(&sh.mass[c], w);
-    } else if (key == r.cut) {
-      atomicAdd(&sh.count[c], 1u);
-    }
-  });
-  __syncthreads();
-  // chunks in order: the ties that each still keeps, then the weights before it
-  const int each = (chunks + kThreads - 1) / kThreads, first = int(threadIdx.x) * each;
-  u64 own_ties = 0;
-  for (int b = first; b < min(first + each, chunks); ++b) own_ties += sh.count[b];
-  u64 all;
-  u64 ties_before = scan(own_ties, sh, all);
-  u64 own = 0, seen = ties_before;
-  for (int b = first; b < min(first + each, chunks); ++b) {
-    const u64 left = r.ties > seen ? r.ties - seen : 0;
-    own += sh.mass[b] + min(left, u64(sh.count[b])) * tie_weight;
-    seen += sh.count[b];
-  }
-  u64 total;
-  u64 before = scan(own, sh, total);
-  // the first token whose sum exceeds u total: whole numbers exceed its floor
-  const double aim = floor(double(u) * double(total));
-  const u64 goal = aim > 0.0 ? min(u64(min(aim, 0x1p63)), total - 1) : 0;
-  if (before <= goal && goal < before + own) {
-    seen = ties_before;
-    for (int b = first; b < min(first + each, chunks); ++b) {
-      const u64 left = r.ties > seen ? r.ties - seen : 0;
-      const u64 n = sh.mass[b] + min(left, u64(sh.count[b])) * tie_weight;
-      if (goal < before + n) {
-        sh.found = b;
-        sh.before = goal - before;
-        sh.ties_before = uint32_t(min(seen, u64(0xffffffffu)));
-        break;
+    tie_weight = total = u64(1) << p.shift;
+    rest = 0;
+    chunk = int(~uint32_t(sh.top));
+    ties_before = 0;
+  } else {
+    if (k > 0 && k < p.V) {
+      // a lane's maximum is at or above L for at least k lanes: so is the row's
+      // k-th largest value.  L is the lower end of a digit.
+      const int lanes = int(min((p.V + kLane - 1) / kLane, int64_t(kThreads)));  // that hold anything
+      if (k <= lanes / 2) {
+        constexpr int by = O::kShift[0], bits = O::kBits[0];
+        r.template clear<false>(sh, 1 << bits);
+        if (mine) atomicAdd(&sh.count[mine >> by], 1u);
+        __syncthreads();
+        r.template place<false>(sh, bits, 0, [&](u64) { return u64(k); });
+        r.whole = r.template make_list<false>(sh, by, uint32_t(sh.found));
       }
-      before += n;
+      r.template select<false>(sh, [&](u64) { return u64(k); });
+    }
+    if (top_p < 1.f)  // of what top-k kept, before min-p
+      r.template select<true>(sh, [&](u64 all) {
+        const double aim = ceil(double(top_p) * double(all));
+        return aim >= 1.0 ? min(u64(aim), all) : u64(1);
+      });
+    // weights and ties of each chunk
+    tie_weight = r.cut != 0 ? r.weight(O::of_key(r.cut)) : 0;
+    if (tie_weight < least) tie_weight = 0;
+    const int chunks = int((p.V + kChunk - 1) / kChunk);
+    r.template clear<true>(sh, chunks);
+    r.template clear<false>(sh, chunks);
+    if (r.listed >= 0) {
+      r.over(sh, [&](int c, uint32_t key) {
+        if (key > r.cut) {
+          const u64 w = r.weight(O::of_key(key));
+          if (w >= least) atomicAdd(&sh.mass[c], w);
+        } else if (key == r.cut) {
+          atomicAdd(&sh.count[c], 1u);
+        }
+      });
+    } else {
+      r.template each<1>([&](int c, const Run<T>& v) {
+        u64 own = 0;
+        uint32_t ties = 0;
+#pragma unroll
+        for (int e = 0; e < kLane; ++e) {
+          const uint32_t key = O::key(v.v[e]);
+          const u64 w = r.weight(O::value(v.v[e]));
+          own += key > r.cut && w >= least ? w : 0;
+          ties += key == r.cut && key != 0;
+        }
+        add_all(&sh.mass[c], own);
+        if (ties) atomicAdd(&sh.count[c], ties);
+      });
+    }
+    __syncthreads();
+    // chunks in order: the ties that each still keeps, then the weights before it
+    const int each = (chunks + kThreads - 1) / kThreads, first = int(threadIdx.x) * each;
+    u64 own_ties = 0, all;
+    for (int b = first; b < min(first + each, chunks); ++b) own_ties += sh.count[b];
+    const u64 before_ties = r.cut != 0 ? scan(own_ties, sh, all) : 0;
+    u64 own = 0, seen = before_ties;
+    auto kept = [&](int b) {  // a chunk's weight, `seen` ties before it
+      const u64 left = r.ties > seen ? r.ties - seen : 0;
+      return sh.mass[b] + min(left, u64(sh.count[b])) * tie_weight;
+    };
+    for (int b = first; b < min(first + each, chunks); ++b) {
+      own += kept(b);
       seen += sh.count[b];
     }
+    u64 before = scan(own, sh, total);
+    // the first token whose sum exceeds u total: whole numbers exceed its floor
+    const double aim = floor(double(u) * double(total));
+    const u64 goal = aim > 0.0 ? min(u64(min(aim, 0x1p63)), total - 1) : 0;
+    if (before <= goal && goal < before + own) {
+      seen = before_ties;
+      for (int b = first; b < min(first + each, chunks); ++b) {
+        const u64 n = kept(b);
+        if (goal < before + n) {
+          sh.found = b;
+          sh.before = goal - before;
+          sh.ties_before = uint32_t(seen);
+          break;
+        }
+        before += n;
+        seen += sh.count[b];
+      }
+    }
+    __syncthreads();
+    rest = sh.before;
+    chunk = sh.found;
+    ties_before = sh.ties_before;
   }
-  __syncthreads();
   if (threadIdx.x >= kWave) return;
 
   // within the chunk, one wave
-  const u64 rest = sh.before;
-  const int64_t i0 = int64_t(sh.found) * kChunk + lane * kLane;
+  const int64_t i0 = int64_t(chunk) * kChunk + lane * kLane;
   T v[kLane];
-  uint32_t mine = 0;
+  uint32_t equal = 0;
 #pragma unroll
   for (int e = 0; e < kLane; ++e) {
     v[e] = r.x[min(i0 + e, p.V - 1)];
-    mine += i0 + e < p.V && O::key(v[e]) == r.cut;
+    equal += i0 + e < p.V && O::key(v[e]) == r.cut;
   }
-  uint32_t tie = mine;
+  uint32_t tie = equal;
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
     const uint32_t o = uint32_t(__shfl_up(int(tie), d, kWave));
     if (lane >= d) tie += o;
   }
-  tie += sh.ties_before - mine;  // ties before this lane's elements
+  tie += ties_before - equal;  // ties before this lane's elements
   u64 w[kLane], sum = 0;
 #pragma unroll
   for (int e = 0; e < kLane; ++e) {
     const uint32_t key = O::key(v[e]);
-    w[e] = 0;
-    if (i0 + e < p.V) {
-      if (key > r.cut) w[e] = r.weight(O::value(v[e]));
-      else if (key == r.cut && u64(tie++) < r.ties) w[e] = tie_weight;
-    }
+    w[e] = r.weight(O::value(v[e]));
+    w[e] = key > r.cut && w[e] >= least ? w[e] : 0;
+    if (key == r.cut) w[e] = u64(tie++) < r.ties ? tie_weight : 0;
+    if (i0 + e >= p.V) w[e] = 0;
     sum += w[e];
   }
   u64 upto = sum;
@@ -390,20 +580,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   }
   u64 at = upto - sum;
   if (at <= rest && rest < upto) {
-    bool done = false;
+    int e_at = kLane;
+    float x_at = 0.f;
 #pragma unroll
     for (int e = 0; e < kLane; ++e) {
       at += w[e];
-      if (!done && rest < at) {
-        done = true;
-        if (p.index_type == MK_S64) static_cast<int64_t*>(p.token)[row] = i0 + e;
-        else static_cast<int32_t*>(p.token)[row] = int32_t(i0 + e);
-        if (p.logprob) {
-          const double z = (double(O::value(v[e])) - r.top) / double(t);
-          p.logprob[row] = float(z - log(ldexp(double(total), -r.shift)));
-        }
-      }
+      if (e_at == kLane && rest < at) e_at = e, x_at = O::value(v[e]);
     }
+    if (p.index_type == MK_S64) static_cast<int64_t*>(p.token)[row] = i0 + e_at;
+    else static_cast<int32_t*>(p.token)[row] = int32_t(i0 + e_at);
+    if (p.logprob)
+      p.logprob[row] = float((double(x_at) - r.top) / double(t) - log(ldexp(double(total), -p.shift)));
   }
 }
 
@@ -442,8 +629,8 @@ extern "C" int mk_sample_rows(void* stream, int io_type, int64_t rows, int64_t v
   while ((int64_t(1) << bits) < vocab) ++bits;
   const SampleArgs a{logits, rows, vocab, ld_logits, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all,
                      min_p_all, top_k_all, index_type, tokens, logprobs, std::min(51, 62 - bits)};
-  const dim3 g{unsigned(rows)}, b{kThreads};
   hipStream_t s = as_stream(stream);
+  const dim3 g{unsigned(rows)}, b{kThreads};
   if (io_type == MK_BF16) hipLaunchKernelGGL((sample_kernel<uint16_t>), g, b, 0, s, a);
   else if (io_type == MK_F16) hipLaunchKernelGGL((sample_kernel<F16>), g, b, 0, s, a);
   else hipLaunchKernelGGL((sample_kernel<float>), g, b, 0, s, a);
