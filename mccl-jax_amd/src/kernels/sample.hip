@@ -26,7 +26,7 @@
 //   top-p alone: a second pass for the weights, a third for the list of the
 //   tokens of the first digit's cut and above;
 //   no cut: a second pass for the weights of each 512 tokens.
-// What remains happens on the list (16384 tokens; rows whose list is longer are
+// What remains happens on the list (12288 tokens; rows whose list is longer are
 // read again), then one wave finds the token in its 512.  Bound: one CU's work on
 // a row: barriers and LDS where there is a top-k, else an exponential in 64 bits
 // for each token.  Loops are kept short on purpose: unrolled over a row that
@@ -43,7 +43,8 @@ constexpr int kThreads = 1024, kWaves = kThreads / kWave;
 constexpr int kBins = 4096;                 // 12 bits: a level of the histogram
 constexpr int kLane = 8;                    // elements a lane takes at once
 constexpr int kChunk = kLane * kWave;       // elements a wave takes at once
-constexpr int kList = 16384;                // tokens of the list
+constexpr int kList = 12288;                // tokens of the list
+constexpr int kFew = 256;                   // ... of one that is ranked by comparing each with each
 constexpr int64_t kMaxVocab = int64_t(kBins) * kChunk;
 
 constexpr double kLowZ = -16.0;             // log2 of the weights that level 0 of top-p sums without digits
@@ -69,6 +70,7 @@ template <typename T> struct Order;
 template <> struct Order<float> {
   static constexpr int kLevels = 3;
   static constexpr int kShift[3] = {20, 10, 0}, kBits[3] = {12, 10, 10};
+  static constexpr int kFine = 17;  // 64 steps from a power of two to the next
   static __device__ inline float none() { return __builtin_bit_cast(float, 0xffffffffu); }
   static __device__ inline float value(float v) { return v; }
   static __device__ inline uint32_t key(float v) {
@@ -88,7 +90,7 @@ __device__ inline uint32_t key16(uint32_t b) {
 __device__ inline uint16_t of_key16(uint32_t k) { return uint16_t(k ^ (k >> 15 ? 0x8000u : 0xffffu)); }
 template <> struct Order<uint16_t> {
   static constexpr int kLevels = 2;
-  static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4};
+  static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4}, kFine = 1;
   static __device__ inline uint16_t none() { return 0xffffu; }
   static __device__ inline float value(uint16_t v) { return bf16_to_f32(v); }
   static __device__ inline uint32_t key(uint16_t v) { return key16(v); }
@@ -96,7 +98,7 @@ template <> struct Order<uint16_t> {
 };
 template <> struct Order<F16> {
   static constexpr int kLevels = 2;
-  static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4};
+  static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4}, kFine = 4;
   static __device__ inline F16 none() { return F16{0xffffu}; }
   static __device__ inline float value(F16 v) { return f16_to_f32(v.bits); }
   static __device__ inline uint32_t key(F16 v) { return key16(v.bits); }
@@ -105,12 +107,23 @@ template <> struct Order<F16> {
 
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Run { T v[kLane]; };
 
+// A list of at most 256 tokens, in the two orders that count.
+struct Few {
+  u64 weight[kFew];           // by rank
+  uint32_t rank[4][kFew], place[4][kFew];  // partial counts of the tokens before one
+  uint32_t rank_at[kFew], index_at[kFew];  // by place in the vocabulary
+};
+
 struct Shared {
-  u64 mass[kBins];        // a level's weights by digit; then the chunks' weights
-  uint32_t count[kBins];  // a level's counts by digit; then the chunks' ties
-  uint32_t key[kList];    // the list: keys, and the chunks they are from
-  uint16_t chunk[kList];
-  u64 wave_sum[kWaves];
+  union {
+    struct {
+      u64 mass[kBins];        // a level's weights by digit; then the chunks' weights
+      uint32_t count[kBins];  // a level's counts by digit; then the chunks' ties
+    };
+    Few few;
+  };
+  uint32_t key[kList], index[kList];  // the list
+  u64 wave_sum[2][kWaves];
   u64 top, low;
   uint32_t bad, n;
   // what the one thread that found a place leaves for the others
@@ -119,42 +132,56 @@ struct Shared {
   uint32_t ties_before;
 };
 
-__device__ inline u64 shfl_up(u64 v, int d) { return __shfl_up(v, d, kWave); }
+// v of the lane that a DPP control word names, 0 where there is none
+template <int CTRL, int ROWS = 0xF>
+__device__ inline uint32_t dpp(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS = 0xF>
+__device__ inline u64 dpp(u64 v) {
+  return (u64(dpp<CTRL, ROWS>(uint32_t(v >> 32))) << 32) | dpp<CTRL, ROWS>(uint32_t(v));
+}
+// sum of v over the lanes up to and with this one: within rows of 16 (row_shr 1, 2,
+// 4, 8), then the last lane of a row to the next row and of two rows to the next two
+template <typename V>
+__device__ inline V upto(V v) {
+  v += dpp<0x111>(v);
+  v += dpp<0x112>(v);
+  v += dpp<0x114>(v);
+  v += dpp<0x118>(v);
+  v += dpp<0x142, 0xA>(v);
+  v += dpp<0x143, 0xC>(v);
+  return v;
+}
+__device__ inline u64 last_lane(u64 v) {
+  return (u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), 63))) << 32) |
+         uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), 63));
+}
 
-// sum of v over the threads before this one (and all of them, in total)
-__device__ inline u64 scan(u64 v, Shared& sh, u64& total) {
+// Sum of v over the threads before this one (and all of them, in total), one
+// barrier.  Two scans in a row take different `turn`s.
+__device__ inline u64 scan(u64 v, Shared& sh, int turn, u64& total) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  u64 s = v;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const u64 o = shfl_up(s, d);
-    if (lane >= d) s += o;
-  }
-  __syncthreads();
-  if (lane == kWave - 1) sh.wave_sum[wave] = s;
+  const u64 s = upto(v);
+  if (lane == kWave - 1) sh.wave_sum[turn][wave] = s;
   __syncthreads();
   u64 before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    if (w == wave) before = all;
-    all += sh.wave_sum[w];
+    const u64 n = sh.wave_sum[turn][w];
+    before += w < wave ? n : 0;
+    all += n;
   }
   total = all;
   return before + s - v;
 }
 
-// sum over 16 lanes, in each of them (as wave_sum_dpp's first steps)
-template <int CTRL>
-__device__ inline u64 dpp_u64(u64 v) {
-  const uint32_t lo = uint32_t(__builtin_amdgcn_mov_dpp(int(uint32_t(v)), CTRL, 0xF, 0xF, false));
-  const uint32_t hi = uint32_t(__builtin_amdgcn_mov_dpp(int(uint32_t(v >> 32)), CTRL, 0xF, 0xF, false));
-  return (u64(hi) << 32) | lo;
-}
+// sum over 16 lanes, in each of them: quad_perm [1,0,3,2] and [2,3,0,1], half_mirror, mirror
 __device__ inline u64 row_sum(u64 v) {
-  v += dpp_u64<0xB1>(v);
-  v += dpp_u64<0x4E>(v);
-  v += dpp_u64<0x141>(v);
-  v += dpp_u64<0x140>(v);
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  v += dpp<0x140>(v);
   return v;
 }
 // v of all lanes added to *to
@@ -167,13 +194,14 @@ template <typename T>
 struct Row {
   using O = Order<T>;
   const T* x;
-  int64_t V;
+  int V;
   double top, per;  // the largest value; log2(e) / temperature
   int shift;
   uint32_t cut;     // kept: keys above cut, and the first `ties` equal to it
   u64 ties;
   int listed;       // tokens in the list, -1: there is none
   bool whole;       // the list holds everything that is kept
+  u64 few_target;   // the weight that a short list is cut at, where it is known
 
   // log2 of a weight, at least -64 (weights below 2^-52 are 0)
   __device__ inline double log2_weight(float v) const { return max((double(v) - top) * per, -64.0); }
@@ -181,7 +209,8 @@ struct Row {
   // (1.5 2^52 + n holds it in its low bits); 2^f is the polynomial through it at 8
   // Chebyshev points of [-1/2, 1/2], its constant made 1, 2^-33 of itself off;
   // 2^52 + w holds the rounded weight in its low bits.
-  __device__ inline u64 weight_of(double z) const {
+  static constexpr u64 kRaw = u64(0x433) << 52;  // the bits of 2^52, which raw_weight is above its weight
+  __device__ inline u64 raw_weight(double z) const {
     const double t = z + 0x1.8p52, f = z - (t - 0x1.8p52);
     const int n = int(uint32_t(__builtin_bit_cast(u64, t)));
     double e = 1.5303699001378845e-05;
@@ -192,17 +221,20 @@ struct Row {
     e = fma(e, f, 0.24022651213495422);
     e = fma(e, f, 0.69314718055683411);
     e = fma(e, f, 1.0);
-    return __builtin_bit_cast(u64, ldexp(e, shift + n) + 0x1p52) & ((u64(1) << 52) - 1);
+    return __builtin_bit_cast(u64, ldexp(e, shift + n) + 0x1p52);
   }
+  __device__ inline u64 weight_of(double z) const { return raw_weight(z) - kRaw; }
   __device__ inline u64 weight(float v) const { return weight_of(log2_weight(v)); }
 
+  // where load(i) takes its elements from
+  __device__ inline int start(int i) const { return V >= kLane ? min(i, V - kLane) : i; }
   // The elements at i .. i + kLane - 1.  Where the row ends among or before them
   // they are the row's last kLane, with none() for those before i: which of its
   // chunk's elements a lane holds is all that counts.
-  __device__ inline Run<T> load(int64_t i) const {
+  __device__ inline Run<T> load(int i) const {
     Run<T> r;
     if (V >= kLane) {
-      const int64_t from = min(i, V - kLane);
+      const int from = start(i);
       r = *reinterpret_cast<const Run<T>*>(x + from);
       if (from < i) {
 #pragma unroll
@@ -219,8 +251,8 @@ struct Row {
   // f(chunk, its kLane elements of this lane) over the row, kAhead chunks loaded ahead
   template <int kAhead, class F>
   __device__ inline void each(F f) const {
-    const int chunks = int((V + kChunk - 1) / kChunk);
-    auto at = [&](int c) { return load(int64_t(c) * kChunk + lane() * kLane); };
+    const int chunks = (V + kChunk - 1) / kChunk;
+    auto at = [&](int c) { return load(c * kChunk + lane() * kLane); };
     Run<T> next[kAhead];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) next[a] = at(wave() + kWaves * a);
@@ -239,7 +271,7 @@ struct Row {
   __device__ inline void over(const Shared& sh, F f) const {
     if (listed >= 0) {
 #pragma unroll 1
-      for (int e = threadIdx.x; e < listed; e += kThreads) f(int(sh.chunk[e]), sh.key[e]);
+      for (int e = threadIdx.x; e < listed; e += kThreads) f(int(sh.index[e] / kChunk), sh.key[e]);
     } else {
       each<1>([&](int c, const Run<T>& r) {
 #pragma unroll
@@ -247,28 +279,25 @@ struct Row {
       });
     }
   }
-  // The list of the tokens whose key, without its low `by` bits, is at least (or
-  // ONLY: just) `least`; whether they fit.
-  template <bool ONLY>
-  __device__ inline bool make_list(Shared& sh, int by, uint32_t least) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.n = 0;
-    __syncthreads();
+  // The list of the tokens with first - key (over 2^by) at most `most`; whether
+  // they fit.  sh.n is 0 before it.
+  __device__ inline bool make_list(Shared& sh, uint32_t first, int by, uint32_t most) {
     each<3>([&](int c, const Run<T>& r) {
       uint32_t mine = 0;
 #pragma unroll
       for (int e = 0; e < kLane; ++e) {
         const uint32_t key = O::key(r.v[e]);
-        mine |= uint32_t(key != 0 && (ONLY ? (key >> by) == least : (key >> by) >= least)) << e;
+        mine |= uint32_t(key != 0 && ((first - key) >> by) <= most) << e;
       }
       if (mine) {
         uint32_t at = atomicAdd(&sh.n, uint32_t(__popc(mine)));
         if (at <= uint32_t(kList - kLane)) {
+          const uint32_t i = uint32_t(start(c * kChunk + lane() * kLane));
 #pragma unroll
           for (int e = 0; e < kLane; ++e)
             if (mine >> e & 1) {
               sh.key[at] = O::key(r.v[e]);
-              sh.chunk[at] = uint16_t(c);
+              sh.index[at] = i + e;
               ++at;
             }
         }
@@ -281,17 +310,17 @@ struct Row {
 
   // The digit of a level in which the running sum from the largest digit down
   // (`above` before the level) reaches aim(sum of all): left in sh.found, and the
-  // sum above it in sh.before.  No digit where it takes sh.low as well: sh.found -1.
+  // sum above it in sh.before.  No digit where it takes sh.low as well: sh.found -1
+  // as before the call.
   template <bool MASS, class Aim>
-  __device__ inline void place(Shared& sh, int bits, u64 above, Aim aim) const {
+  __device__ inline void place(Shared& sh, int bits, u64 above, int turn, Aim aim) const {
     const int bins = 1 << bits, per_thread = bins > kThreads ? bins / kThreads : 1;
     const int first = bins - 1 - int(threadIdx.x) * per_thread;
-    if (threadIdx.x == 0) sh.found = -1;
     u64 own = 0;
     for (int k = 0; k < per_thread; ++k)
       if (first - k >= 0) own += MASS ? sh.mass[first - k] : u64(sh.count[first - k]);
     u64 total;
-    u64 before = above + scan(own, sh, total);
+    u64 before = above + scan(own, sh, turn, total);
     const u64 target = aim(above + total + (MASS ? sh.low : 0));
     if (before < target && target <= before + own) {
       for (int k = 0; k < per_thread; ++k) {
@@ -306,10 +335,11 @@ struct Row {
     }
     __syncthreads();
   }
+  // an empty level (and list), behind a barrier
   template <bool MASS>
   __device__ inline void clear(Shared& sh, int n) const {
     __syncthreads();
-    if (MASS && threadIdx.x == 0) sh.low = 0;
+    if (threadIdx.x == 0) sh.low = 0, sh.found = -1;
     for (int b = threadIdx.x; b < n; b += kThreads) {
       if (MASS) sh.mass[b] = 0;
       else sh.count[b] = 0;
@@ -324,25 +354,25 @@ struct Row {
     uint32_t prefix = 0;
     u64 above = 0, target = 0;
     const u64 tie_weight = MASS && cut != 0 ? weight(O::of_key(cut)) : 0;
-#pragma unroll
+#pragma unroll 1
     for (int level = 0; level < O::kLevels; ++level) {
       const int by = O::kShift[level], bits = O::kBits[level];
       const uint32_t mask = (1u << bits) - 1;
       // The weights of the first level: a weight below 2^floor_z is seldom part of a
       // cut, and goes without its digit into one sum, unless the cut turns out to
       // need it.
-      double floor_z = MASS && level == 0 && listed < 0 ? kLowZ : -64.0;
+      const bool all = MASS && level == 0 && listed < 0;
+      double floor_z = all ? kLowZ : -64.0;
       for (;;) {
         clear<MASS>(sh, int(mask) + 1);
-        if (MASS && level == 0 && listed < 0) {
+        if (all) {
           u64 low = 0;
           each<1>([&](int, const Run<T>& r) {
 #pragma unroll
             for (int e = 0; e < kLane; ++e) {
               const uint32_t key = O::key(r.v[e]);
-              if (key <= cut) continue;
               const double z = log2_weight(O::value(r.v[e]));
-              const u64 w = weight_of(z);
+              const u64 w = key > cut ? weight_of(z) : 0;
               if (z > floor_z) atomicAdd(&sh.mass[(key >> by) & mask], w);
               else low += w;
             }
@@ -358,7 +388,7 @@ struct Row {
         if (MASS && cut != 0 && threadIdx.x == 0 && (level == 0 || (cut >> (by + bits)) == prefix))
           atomicAdd(&sh.mass[(cut >> by) & mask], ties * tie_weight);
         __syncthreads();
-        place<MASS>(sh, bits, above, [&](u64 total) {
+        place<MASS>(sh, bits, above, level & 1, [&](u64 total) {
           if (level == 0) target = aim(total);
           return target;
         });
@@ -369,8 +399,18 @@ struct Row {
       above = sh.before;
       // the other digits on the tokens of this one, with those above where they fit
       if (level == 0 && listed < 0) {
-        whole = make_list<false>(sh, by, prefix);
-        if (!whole) make_list<true>(sh, by, prefix);
+        const uint32_t least = prefix << by, width = (1u << by) - 1;
+        for (int only = 0; only < 2 && listed < 0; ++only) {
+          __syncthreads();
+          if (threadIdx.x == 0) sh.n = 0;
+          __syncthreads();
+          const uint32_t first = only ? least + width : 0xffffffffu;
+          whole = make_list(sh, first, 0, first - least) && !only;
+        }
+        if (MASS && whole && listed <= kFew) {
+          few_target = target;
+          return;
+        }
       }
     }
     if (!whole) listed = -1;
@@ -385,6 +425,96 @@ struct Row {
 };
 
 template <typename T>
+__device__ inline void put(const SampleArgs& p, const Row<T>& r, int64_t row, float t, int i, float x, u64 total) {
+  if (p.index_type == MK_S64) static_cast<int64_t*>(p.token)[row] = i;
+  else static_cast<int32_t*>(p.token)[row] = i;
+  if (p.logprob)
+    p.logprob[row] = float((double(x) - r.top) / double(t) - log(ldexp(double(total), -p.shift)));
+}
+
+// The first sum that exceeds u times the total exceeds this: whole numbers
+// exceed the product's floor.
+__device__ inline u64 goal_of(float u, u64 total) {
+  const double aim = floor(double(u) * double(total));
+  return aim > 0.0 ? min(u64(min(aim, 0x1p63)), total - 1) : 0;
+}
+// The weight that a cut by top-p reaches: a rank is kept while less than this is
+// before it.
+__device__ inline u64 cut_of(float top_p, u64 all) {
+  const double aim = ceil(double(top_p) * double(all));
+  return aim >= 1.0 ? min(u64(aim), all) : u64(1);
+}
+
+// The token of a list of at most kFew that holds all that is kept: the first k
+// ranks of it, cut at few_target or by top-p, and by min-p.  Four threads compare a
+// token with a quarter of the others each; then one wave sums in both orders.
+template <typename T>
+__device__ inline void take_few(const SampleArgs& p, const Row<T>& r, Shared& sh, int64_t row, float u, float t,
+                                int64_t k, float top_p, u64 least) {
+  const int n = r.listed, j = threadIdx.x % kFew, part = threadIdx.x / kFew;
+  const int q = (n + 3) / 4, lo = part * q, hi = min(lo + q, n);
+  Few& few = sh.few;
+  uint32_t key = 0, index = 0;
+  if (j < n) {
+    key = sh.key[j];
+    index = sh.index[j];
+    uint32_t rank = 0, place = 0;
+#pragma unroll 4
+    for (int i = lo; i < hi; ++i) {
+      const uint32_t ki = sh.key[i], ii = sh.index[i];
+      rank += ki > key || (ki == key && ii < index);
+      place += ii < index;
+    }
+    few.rank[part][j] = rank;
+    few.place[part][j] = place;
+  }
+  __syncthreads();
+  if (part == 0 && j < n) {
+    const uint32_t rank = few.rank[0][j] + few.rank[1][j] + few.rank[2][j] + few.rank[3][j];
+    const uint32_t place = few.place[0][j] + few.place[1][j] + few.place[2][j] + few.place[3][j];
+    few.weight[rank] = r.weight(Order<T>::of_key(key));
+    few.rank_at[place] = rank;
+    few.index_at[place] = index;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kWave) return;
+  constexpr int kPer = kFew / kWave;
+  const int first = threadIdx.x * kPer;
+  u64 w[kPer], sum = 0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) sum += w[e] = first + e < n && first + e < k ? few.weight[first + e] : 0;
+  u64 s = upto(sum);
+  const u64 all = last_lane(s), limit = r.few_target ? r.few_target : top_p < 1.f ? cut_of(top_p, all) : ~u64(0);
+  uint32_t mine = 0;  // kept ranks: a run from the first on
+  s -= sum;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    mine += w[e] != 0 && s < limit && w[e] >= least;
+    s += w[e];
+  }
+  const uint32_t kept = uint32_t(__builtin_amdgcn_readlane(int(upto(mine)), 63));
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const uint32_t rank = first + e < n ? few.rank_at[first + e] : kept;
+    sum += w[e] = rank < kept ? few.weight[rank] : 0;
+  }
+  s = upto(sum);
+  const u64 total = last_lane(s), goal = goal_of(u, total);
+  s -= sum;
+  if (s <= goal && goal < s + sum) {
+    int at = -1;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      s += w[e];
+      if (at < 0 && goal < s) at = first + e;
+    }
+    const int i = int(few.index_at[at]);
+    put(p, r, row, t, i, Order<T>::value(r.x[i]), total);
+  }
+}
+
+template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   using O = Order<T>;
   __shared__ Shared sh;
@@ -392,26 +522,27 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   const int lane = threadIdx.x & (kWave - 1);
   Row<T> r;
   r.x = static_cast<const T*>(p.x) + row * p.ld;
-  r.V = p.V;
+  r.V = int(p.V);
   r.shift = p.shift;
   r.listed = -1;
   r.whole = false;
+  r.few_target = 0;
   const float u = p.u[row];
   float t = p.temperature ? p.temperature[row] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
   const float min_p = p.min_p ? p.min_p[row] : p.min_p_all;
   int64_t k = p.top_k ? p.top_k[row] : p.top_k_all;
   bool bad = !(t >= 0.f) || t == INFINITY || top_p != top_p || min_p != min_p || u != u;
+  if (threadIdx.x == 0) sh.n = 0;
+  sh.count[threadIdx.x] = 0;
 
   // The largest value, of this lane's and of all, with the first chunk that holds
   // it; and whether there are more NaN than the places past the row's end.
-  if (threadIdx.x == 0) sh.top = 0, sh.bad = 0;
-  __syncthreads();
   uint32_t mine = 0, nan = 0;
   int mine_at = 0;
   r.template each<3>([&](int c, const Run<T>& v) {
-    const int64_t past = int64_t(c) * kChunk + (lane + 1) * kLane - p.V;
-    nan -= past > 0 ? uint32_t(min(past, int64_t(kLane))) : 0u;
+    const int past = c * kChunk + (lane + 1) * kLane - r.V;
+    nan -= uint32_t(max(0, min(past, kLane)));
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < kLane; ++e) {
@@ -421,15 +552,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     }
     if (m > mine) mine = m, mine_at = c;
   });
-  u64 best = (u64(mine) << 32) | uint32_t(~mine_at);
+  u64 best = nan ? ~u64(0) : (u64(mine) << 32) | uint32_t(~mine_at);
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) best = max(best, u64(__shfl_xor(best, m, kWave)));
-  if (lane == 0) atomicMax(&sh.top, best);
-  if (nan) sh.bad = 1;
+  if (lane == 0) sh.wave_sum[0][threadIdx.x / kWave] = best;
   __syncthreads();
-  const uint32_t top_key = uint32_t(sh.top >> 32);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) best = max(best, sh.wave_sum[0][w]);
+  const uint32_t top_key = uint32_t(best >> 32);
   const float largest = O::of_key(top_key);
-  bad = bad || sh.bad || largest == INFINITY || largest == -INFINITY;
+  bad = bad || best == ~u64(0) || largest == INFINITY || largest == -INFINITY;
   if (bad) {  // the whole workgroup
     if (threadIdx.x == 0) {
       if (p.index_type == MK_S64) static_cast<int64_t*>(p.token)[row] = -1;
@@ -454,34 +586,43 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     r.ties = 1;
     tie_weight = total = u64(1) << p.shift;
     rest = 0;
-    chunk = int(~uint32_t(sh.top));
+    chunk = int(~uint32_t(best));
     ties_before = 0;
   } else {
-    if (k > 0 && k < p.V) {
-      // a lane's maximum is at or above L for at least k lanes: so is the row's
-      // k-th largest value.  L is the lower end of a digit.
-      const int lanes = int(min((p.V + kLane - 1) / kLane, int64_t(kThreads)));  // that hold anything
+    if (k > 0 && k < r.V) {
+      // k lanes have a maximum at most so many steps below the top: so is the
+      // row's k-th largest value.  Each wave finds the step for itself.
+      const int lanes = min((r.V + kLane - 1) / kLane, kThreads);  // that hold anything
       if (k <= lanes / 2) {
-        constexpr int by = O::kShift[0], bits = O::kBits[0];
-        r.template clear<false>(sh, 1 << bits);
-        if (mine) atomicAdd(&sh.count[mine >> by], 1u);
+        if (mine) atomicAdd(&sh.count[min((top_key - mine) >> O::kFine, uint32_t(kThreads - 1))], 1u);
         __syncthreads();
-        r.template place<false>(sh, bits, 0, [&](u64) { return u64(k); });
-        r.whole = r.template make_list<false>(sh, by, uint32_t(sh.found));
+        constexpr int kPer = kThreads / kWave;
+        uint32_t own = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) own += sh.count[kPer * lane + e];
+        uint32_t s = upto(own) - own;
+        uint32_t step = 0;
+        const u64 here = __ballot(s < k && k <= s + own);
+        for (int e = 0; e < kPer; ++e) {
+          if (s + sh.count[kPer * lane + e] >= k) break;
+          s += sh.count[kPer * lane + e];
+          ++step;
+        }
+        step = uint32_t(__builtin_amdgcn_readlane(int(kPer * lane + step), __ffsll(here) - 1));
+        if (step < uint32_t(kThreads - 1)) r.whole = r.make_list(sh, top_key, O::kFine, step);
       }
-      r.template select<false>(sh, [&](u64) { return u64(k); });
+      if (!r.whole || r.listed > kFew) r.template select<false>(sh, [&](u64) { return u64(k); });
     }
-    if (top_p < 1.f)  // of what top-k kept, before min-p
-      r.template select<true>(sh, [&](u64 all) {
-        const double aim = ceil(double(top_p) * double(all));
-        return aim >= 1.0 ? min(u64(aim), all) : u64(1);
-      });
+    const bool few_k = r.whole && r.listed <= kFew && r.cut == 0;  // top-k is still to be taken
+    if (top_p < 1.f && !few_k)  // of what top-k kept, before min-p
+      r.template select<true>(sh, [&](u64 all) { return cut_of(top_p, all); });
+    if (few_k || r.few_target) return take_few(p, r, sh, row, u, t, few_k ? k : int64_t(kFew), top_p, least);
     // weights and ties of each chunk
     tie_weight = r.cut != 0 ? r.weight(O::of_key(r.cut)) : 0;
     if (tie_weight < least) tie_weight = 0;
-    const int chunks = int((p.V + kChunk - 1) / kChunk);
+    const int chunks = (r.V + kChunk - 1) / kChunk;
     r.template clear<true>(sh, chunks);
-    r.template clear<false>(sh, chunks);
+    if (r.cut != 0) r.template clear<false>(sh, chunks);
     if (r.listed >= 0) {
       r.over(sh, [&](int c, uint32_t key) {
         if (key > r.cut) {
@@ -490,6 +631,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
         } else if (key == r.cut) {
           atomicAdd(&sh.count[c], 1u);
         }
+      });
+    } else if (r.cut == 0 && least == 0) {
+      r.template each<1>([&](int c, const Run<T>& v) {
+        u64 own = 0;
+#pragma unroll
+        for (int e = 0; e < kLane; ++e) own += r.raw_weight(r.log2_weight(O::value(v.v[e])));
+        add_all(&sh.mass[c], own - kLane * r.kRaw);
       });
     } else {
       r.template each<1>([&](int c, const Run<T>& v) {
@@ -509,34 +657,34 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     __syncthreads();
     // chunks in order: the ties that each still keeps, then the weights before it
     const int each = (chunks + kThreads - 1) / kThreads, first = int(threadIdx.x) * each;
-    u64 own_ties = 0, all;
-    for (int b = first; b < min(first + each, chunks); ++b) own_ties += sh.count[b];
-    const u64 before_ties = r.cut != 0 ? scan(own_ties, sh, all) : 0;
+    const int last = min(first + each, chunks);
+    u64 before_ties = 0;
+    if (r.cut != 0) {
+      u64 own_ties = 0, all;
+      for (int b = first; b < last; ++b) own_ties += sh.count[b];
+      before_ties = scan(own_ties, sh, 0, all);
+    }
     u64 own = 0, seen = before_ties;
     auto kept = [&](int b) {  // a chunk's weight, `seen` ties before it
-      const u64 left = r.ties > seen ? r.ties - seen : 0;
-      return sh.mass[b] + min(left, u64(sh.count[b])) * tie_weight;
+      if (r.cut == 0) return sh.mass[b];
+      const u64 n = sh.count[b], left = r.ties > seen ? r.ties - seen : 0;
+      seen += n;
+      return sh.mass[b] + min(left, n) * tie_weight;
     };
-    for (int b = first; b < min(first + each, chunks); ++b) {
-      own += kept(b);
-      seen += sh.count[b];
-    }
-    u64 before = scan(own, sh, total);
-    // the first token whose sum exceeds u total: whole numbers exceed its floor
-    const double aim = floor(double(u) * double(total));
-    const u64 goal = aim > 0.0 ? min(u64(min(aim, 0x1p63)), total - 1) : 0;
+    for (int b = first; b < last; ++b) own += kept(b);
+    u64 before = scan(own, sh, 1, total);
+    const u64 goal = goal_of(u, total);
     if (before <= goal && goal < before + own) {
       seen = before_ties;
-      for (int b = first; b < min(first + each, chunks); ++b) {
-        const u64 n = kept(b);
+      for (int b = first; b < last; ++b) {
+        const u64 ties = seen, n = kept(b);
         if (goal < before + n) {
           sh.found = b;
           sh.before = goal - before;
-          sh.ties_before = uint32_t(seen);
+          sh.ties_before = uint32_t(ties);
           break;
         }
         before += n;
-        seen += sh.count[b];
       }
     }
     __syncthreads();
@@ -547,21 +695,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   if (threadIdx.x >= kWave) return;
 
   // within the chunk, one wave
-  const int64_t i0 = int64_t(chunk) * kChunk + lane * kLane;
+  const int i0 = chunk * kChunk + lane * kLane;
   T v[kLane];
   uint32_t equal = 0;
 #pragma unroll
   for (int e = 0; e < kLane; ++e) {
-    v[e] = r.x[min(i0 + e, p.V - 1)];
-    equal += i0 + e < p.V && O::key(v[e]) == r.cut;
+    v[e] = r.x[min(i0 + e, r.V - 1)];
+    equal += i0 + e < r.V && O::key(v[e]) == r.cut;
   }
-  uint32_t tie = equal;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const uint32_t o = uint32_t(__shfl_up(int(tie), d, kWave));
-    if (lane >= d) tie += o;
-  }
-  tie += ties_before - equal;  // ties before this lane's elements
+  uint32_t tie = ties_before + upto(equal) - equal;  // before this lane's elements
   u64 w[kLane], sum = 0;
 #pragma unroll
   for (int e = 0; e < kLane; ++e) {
@@ -569,17 +711,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     w[e] = r.weight(O::value(v[e]));
     w[e] = key > r.cut && w[e] >= least ? w[e] : 0;
     if (key == r.cut) w[e] = u64(tie++) < r.ties ? tie_weight : 0;
-    if (i0 + e >= p.V) w[e] = 0;
+    if (i0 + e >= r.V) w[e] = 0;
     sum += w[e];
   }
-  u64 upto = sum;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const u64 o = shfl_up(upto, d);
-    if (lane >= d) upto += o;
-  }
-  u64 at = upto - sum;
-  if (at <= rest && rest < upto) {
+  const u64 s = upto(sum);
+  u64 at = s - sum;
+  if (at <= rest && rest < s) {
     int e_at = kLane;
     float x_at = 0.f;
 #pragma unroll
@@ -587,10 +724,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
       at += w[e];
       if (e_at == kLane && rest < at) e_at = e, x_at = O::value(v[e]);
     }
-    if (p.index_type == MK_S64) static_cast<int64_t*>(p.token)[row] = i0 + e_at;
-    else static_cast<int32_t*>(p.token)[row] = int32_t(i0 + e_at);
-    if (p.logprob)
-      p.logprob[row] = float((double(x_at) - r.top) / double(t) - log(ldexp(double(total), -p.shift)));
+    put(p, r, row, t, i0 + e_at, x_at, total);
   }
 }
 
