@@ -23,18 +23,26 @@
 //   top-k: the k-th largest of the lanes' own maxima is below the row's k-th
 //   largest value, so what is at or above it holds the first k and is seldom much
 //   more: a second pass puts those tokens into a list in LDS;
-//   top-p alone: a second pass for the weights, a third for the list of the
-//   tokens of the first digit's cut and above;
-//   no cut: a second pass for the weights of each 512 tokens.
-// What remains happens on the list (12288 tokens; rows whose list is longer are
-// read again), then one wave finds the token in its 512.  Bound: one CU's work on
-// a row: barriers and LDS where there is a top-k, else an exponential in 64 bits
-// for each token.  Loops are kept short on purpose: unrolled over a row that
-// stayed in registers they ran slower, waiting for instructions (SLOWER).
+//   top-p alone: a second pass for the weights by 64ths of a power of two, a third
+//   for the list of the tokens from the cut's step up;
+//   min-p alone: a second pass for the list of what is above it;
+//   no limit: a second pass for the weights of each 512 tokens.
+// What remains happens on the list (12288 tokens; where it is longer the row is read
+// again).  A list of at most 256 tokens is ranked by comparing each with each, and
+// one wave does the rest; a longer one is summed by 512 tokens of the row, and one
+// wave finds the token in its 512.
+//
+// Bound: one CU's work on a row.  50257 tokens, one row of bf16 / 256 rows of fp32,
+// us: greedy 7.0 / 12.9 (the first pass: one CU takes in a line every 8 clocks),
+// top-k 50 and top-p 0.9 15 / 24 (two passes and 20 barriers), top-p 0.95 39 / 48 and
+// no limit 20 / 28 (an exponential in 64 bits for each token, 10 us a pass).  Loops are
+// kept short on purpose: with the row in registers and each pass unrolled over it
+// the same steps took 35, 59 and 34 us, waiting for instructions.
 #include "mk_common.h"
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace mk {
 namespace {
@@ -45,9 +53,8 @@ constexpr int kLane = 8;                    // elements a lane takes at once
 constexpr int kChunk = kLane * kWave;       // elements a wave takes at once
 constexpr int kList = 12288;                // tokens of the list
 constexpr int kFew = 256;                   // ... of one that is ranked by comparing each with each
+constexpr int kStep = 512;                  // tokens of a step of list_top that are compared so
 constexpr int64_t kMaxVocab = int64_t(kBins) * kChunk;
-
-constexpr double kLowZ = -16.0;             // log2 of the weights that level 0 of top-p sums without digits
 
 typedef unsigned long long u64;
 
@@ -65,13 +72,14 @@ struct SampleArgs {
 };
 
 // An element type's values as whole numbers that order as they do, -0 as +0.
-// No number and no infinity is 0: that stands for a place past the row's end.
+// No number and no infinity is 0.  Places past the row's end hold -inf, which
+// weighs nothing.
 template <typename T> struct Order;
 template <> struct Order<float> {
   static constexpr int kLevels = 3;
   static constexpr int kShift[3] = {20, 10, 0}, kBits[3] = {12, 10, 10};
   static constexpr int kFine = 17;  // 64 steps from a power of two to the next
-  static __device__ inline float none() { return __builtin_bit_cast(float, 0xffffffffu); }
+  static __device__ inline float none() { return -INFINITY; }
   static __device__ inline float value(float v) { return v; }
   static __device__ inline uint32_t key(float v) {
     uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -91,7 +99,7 @@ __device__ inline uint16_t of_key16(uint32_t k) { return uint16_t(k ^ (k >> 15 ?
 template <> struct Order<uint16_t> {
   static constexpr int kLevels = 2;
   static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4}, kFine = 1;
-  static __device__ inline uint16_t none() { return 0xffffu; }
+  static __device__ inline uint16_t none() { return 0xff80u; }
   static __device__ inline float value(uint16_t v) { return bf16_to_f32(v); }
   static __device__ inline uint32_t key(uint16_t v) { return key16(v); }
   static __device__ inline float of_key(uint32_t k) { return bf16_to_f32(of_key16(k)); }
@@ -99,7 +107,7 @@ template <> struct Order<uint16_t> {
 template <> struct Order<F16> {
   static constexpr int kLevels = 2;
   static constexpr int kShift[2] = {4, 0}, kBits[2] = {12, 4}, kFine = 4;
-  static __device__ inline F16 none() { return F16{0xffffu}; }
+  static __device__ inline F16 none() { return F16{0xfc00u}; }
   static __device__ inline float value(F16 v) { return f16_to_f32(v.bits); }
   static __device__ inline uint32_t key(F16 v) { return key16(v.bits); }
   static __device__ inline float of_key(uint32_t k) { return f16_to_f32(of_key16(k)); }
@@ -124,8 +132,7 @@ struct Shared {
   };
   uint32_t key[kList], index[kList];  // the list
   u64 wave_sum[2][kWaves];
-  u64 top, low;
-  uint32_t bad, n;
+  uint32_t n;
   // what the one thread that found a place leaves for the others
   int found;
   u64 before;
@@ -156,6 +163,16 @@ __device__ inline V upto(V v) {
 __device__ inline u64 last_lane(u64 v) {
   return (u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), 63))) << 32) |
          uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), 63));
+}
+
+__device__ inline uint32_t wave_max(uint32_t v) {
+  v = max(v, dpp<0x111>(v));
+  v = max(v, dpp<0x112>(v));
+  v = max(v, dpp<0x114>(v));
+  v = max(v, dpp<0x118>(v));
+  v = max(v, dpp<0x142, 0xA>(v));
+  v = max(v, dpp<0x143, 0xC>(v));
+  return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
 }
 
 // Sum of v over the threads before this one (and all of them, in total), one
@@ -190,6 +207,19 @@ __device__ inline void add_all(u64* to, u64 v) {
   if (threadIdx.x % 16 == 0 && v) atomicAdd(to, v);
 }
 
+// The first sum that exceeds u times the total exceeds this: whole numbers
+// exceed the product's floor.
+__device__ inline u64 goal_of(float u, u64 total) {
+  const double aim = floor(double(u) * double(total));
+  return aim > 0.0 ? min(u64(min(aim, 0x1p63)), total - 1) : 0;
+}
+// The weight that a cut by top-p reaches: a rank is kept while less than this is
+// before it.
+__device__ inline u64 cut_of(float top_p, u64 all) {
+  const double aim = ceil(double(top_p) * double(all));
+  return aim >= 1.0 ? min(u64(aim), all) : u64(1);
+}
+
 template <typename T>
 struct Row {
   using O = Order<T>;
@@ -201,7 +231,6 @@ struct Row {
   u64 ties;
   int listed;       // tokens in the list, -1: there is none
   bool whole;       // the list holds everything that is kept
-  u64 few_target;   // the weight that a short list is cut at, where it is known
 
   // log2 of a weight, at least -64 (weights below 2^-52 are 0)
   __device__ inline double log2_weight(float v) const { return max((double(v) - top) * per, -64.0); }
@@ -279,72 +308,150 @@ struct Row {
       });
     }
   }
-  // The list of the tokens with first - key (over 2^by) at most `most`; whether
-  // they fit.  sh.n is 0 before it.
-  __device__ inline bool make_list(Shared& sh, uint32_t first, int by, uint32_t most) {
-    each<3>([&](int c, const Run<T>& r) {
-      uint32_t mine = 0;
+  // Puts the elements that the lanes take, a bit each, into the list: one atomic a
+  // wave (one a lane, all on one address, took 7 clocks each; 18 us for the list of
+  // 5000 of 50257 tokens).
+  __device__ inline void append(Shared& sh, int c, const Run<T>& r, uint32_t mine) const {
+    if (!__ballot(mine != 0)) return;
+    const uint32_t n = uint32_t(__popc(mine)), s = upto(n);
+    uint32_t base = 0;
+    if (lane() == kWave - 1) base = atomicAdd(&sh.n, s);
+    uint32_t at = uint32_t(__builtin_amdgcn_readlane(int(base), kWave - 1)) + s - n;
+    if (at > uint32_t(kList - kLane)) return;
+    const uint32_t i = uint32_t(start(c * kChunk + lane() * kLane));
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) {
-        const uint32_t key = O::key(r.v[e]);
-        mine |= uint32_t(key != 0 && ((first - key) >> by) <= most) << e;
+    for (int e = 0; e < kLane; ++e)
+      if (mine >> e & 1) {
+        sh.key[at] = O::key(r.v[e]);
+        sh.index[at] = i + e;
+        ++at;
       }
-      if (mine) {
-        uint32_t at = atomicAdd(&sh.n, uint32_t(__popc(mine)));
-        if (at <= uint32_t(kList - kLane)) {
-          const uint32_t i = uint32_t(start(c * kChunk + lane() * kLane));
-#pragma unroll
-          for (int e = 0; e < kLane; ++e)
-            if (mine >> e & 1) {
-              sh.key[at] = O::key(r.v[e]);
-              sh.index[at] = i + e;
-              ++at;
-            }
-        }
-      }
-    });
+  }
+  // whether what was put into it fits, behind a barrier
+  __device__ inline bool end_list(const Shared& sh) {
     __syncthreads();
     listed = sh.n <= uint32_t(kList - kLane) ? int(sh.n) : -1;
     return listed >= 0;
   }
+  // The list of the tokens from value lo to hi; whether they fit.  sh.n is 0 before it.
+  __device__ inline bool make_list(Shared& sh, float lo, float hi) {
+    each<3>([&](int c, const Run<T>& r) {
+      uint32_t mine = 0;
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) {
+        const float v = O::value(r.v[e]);
+        mine |= uint32_t(v >= lo && v <= hi) << e;
+      }
+      append(sh, c, r, mine);
+    });
+    return end_list(sh);
+  }
 
   // The digit of a level in which the running sum from the largest digit down
   // (`above` before the level) reaches aim(sum of all): left in sh.found, and the
-  // sum above it in sh.before.  No digit where it takes sh.low as well: sh.found -1
-  // as before the call.
+  // sum above it in sh.before.
   template <bool MASS, class Aim>
   __device__ inline void place(Shared& sh, int bits, u64 above, int turn, Aim aim) const {
-    const int bins = 1 << bits, per_thread = bins > kThreads ? bins / kThreads : 1;
+    constexpr int kPer = kBins / kThreads;
+    const int bins = 1 << bits, per_thread = bins > kThreads ? kPer : 1;
     const int first = bins - 1 - int(threadIdx.x) * per_thread;
-    u64 own = 0;
-    for (int k = 0; k < per_thread; ++k)
-      if (first - k >= 0) own += MASS ? sh.mass[first - k] : u64(sh.count[first - k]);
+    u64 n[kPer], own = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const bool in = k < per_thread && first - k >= 0;
+      n[k] = in ? (MASS ? sh.mass[in ? first - k : 0] : u64(sh.count[in ? first - k : 0])) : 0;
+      own += n[k];
+    }
     u64 total;
     u64 before = above + scan(own, sh, turn, total);
-    const u64 target = aim(above + total + (MASS ? sh.low : 0));
+    const u64 target = aim(above + total);
     if (before < target && target <= before + own) {
-      for (int k = 0; k < per_thread; ++k) {
-        const u64 n = MASS ? sh.mass[first - k] : u64(sh.count[first - k]);
-        if (before + n >= target) {
-          sh.found = first - k;
-          sh.before = before;
-          break;
-        }
-        before += n;
-      }
+      int at = 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        if (at == k && before + n[k] < target) before += n[k], ++at;
+      sh.found = first - at;
+      sh.before = before;
     }
     __syncthreads();
   }
-  // an empty level (and list), behind a barrier
+  // an empty level and list, behind a barrier
   template <bool MASS>
   __device__ inline void clear(Shared& sh, int n) const {
     __syncthreads();
-    if (threadIdx.x == 0) sh.low = 0, sh.found = -1;
+    if (threadIdx.x == 0) sh.n = 0;
     for (int b = threadIdx.x; b < n; b += kThreads) {
       if (MASS) sh.mass[b] = 0;
       else sh.count[b] = 0;
     }
     __syncthreads();
+  }
+
+  // which 64th of a power of two below the largest a weight is
+  static __device__ inline int step_of(double z) { return min(int(-64.0 * z), kBins - 1); }
+  // Top-p of a row without a top-k: its weights by their logarithm, in steps of
+  // 1 / 64, say in which step the cut is.  The list of the tokens from that step up
+  // holds all that is kept; few are in the step itself, and are compared with each
+  // other.  Returns the weight that the cut reaches where the cut is still
+  // to be found: on a short list, or where many are in the step or on no list.
+  __device__ inline u64 list_top(Shared& sh, float top_p) {
+    clear<true>(sh, kBins);
+    each<1>([&](int, const Run<T>& r) {
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) {
+        const double z = log2_weight(O::value(r.v[e]));
+        atomicAdd(&sh.mass[kBins - 1 - step_of(z)], weight_of(z));
+      }
+    });
+    __syncthreads();
+    u64 target = 0;
+    place<true>(sh, 12, 0, 0, [&](u64 all) { return target = cut_of(top_p, all); });
+    const int step = kBins - 1 - sh.found;
+    u64 above = sh.before;
+    clear<true>(sh, 0);
+    // a little past the step's ends: what is past them does no harm on the list
+    const float end = float(top - (step + 1) / 64.0 / per), begin = float(top - step / 64.0 / per);
+    const float lo = end - fabsf(end) * 0x1p-22f;
+    whole = make_list(sh, lo, INFINITY);
+    if (whole && listed <= kFew) return target;
+    if (!whole) {  // the step's tokens alone
+      clear<true>(sh, 0);
+      if (!make_list(sh, lo, begin + fabsf(begin) * 0x1p-22f)) return target;
+    }
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    over(sh, [&](int, uint32_t key) {
+      const double z = log2_weight(O::of_key(key));
+      if (step_of(z) != step) return;
+      const uint32_t at = atomicAdd(&sh.n, 1u);
+      if (at >= uint32_t(kStep)) return;
+      sh.count[at] = key;
+      sh.mass[at] = weight_of(z);
+    });
+    __syncthreads();
+    const int n = int(sh.n);
+    if (!whole) listed = -1;
+    if (n > kStep) return target;
+    if (int(threadIdx.x) < n) {
+      const uint32_t key = sh.count[threadIdx.x];
+      const u64 w = sh.mass[threadIdx.x];
+      u64 same = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const uint32_t k = sh.count[i];
+        const u64 v = sh.mass[i];
+        above += k > key ? v : 0;
+        same += k == key ? v : 0;
+      }
+      if (above < target && target <= above + same) {  // the same for all of one key
+        sh.found = int(key);
+        sh.before = (target - above + w - 1) / w;
+      }
+    }
+    __syncthreads();
+    cut = uint32_t(sh.found);
+    ties = sh.before;
+    return 0;
   }
 
   // Moves the cut to where the kept counts (or weights) from the largest value
@@ -358,58 +465,27 @@ struct Row {
     for (int level = 0; level < O::kLevels; ++level) {
       const int by = O::kShift[level], bits = O::kBits[level];
       const uint32_t mask = (1u << bits) - 1;
-      // The weights of the first level: a weight below 2^floor_z is seldom part of a
-      // cut, and goes without its digit into one sum, unless the cut turns out to
-      // need it.
-      const bool all = MASS && level == 0 && listed < 0;
-      double floor_z = all ? kLowZ : -64.0;
-      for (;;) {
-        clear<MASS>(sh, int(mask) + 1);
-        if (all) {
-          u64 low = 0;
-          each<1>([&](int, const Run<T>& r) {
-#pragma unroll
-            for (int e = 0; e < kLane; ++e) {
-              const uint32_t key = O::key(r.v[e]);
-              const double z = log2_weight(O::value(r.v[e]));
-              const u64 w = key > cut ? weight_of(z) : 0;
-              if (z > floor_z) atomicAdd(&sh.mass[(key >> by) & mask], w);
-              else low += w;
-            }
-          });
-          add_all(&sh.low, low);
-        } else {
-          over(sh, [&](int, uint32_t key) {
-            if (key <= (MASS ? cut : 0u) || (level > 0 && (key >> (by + bits)) != prefix)) return;
-            if (MASS) atomicAdd(&sh.mass[(key >> by) & mask], weight(O::of_key(key)));
-            else atomicAdd(&sh.count[(key >> by) & mask], 1u);
-          });
-        }
-        if (MASS && cut != 0 && threadIdx.x == 0 && (level == 0 || (cut >> (by + bits)) == prefix))
-          atomicAdd(&sh.mass[(cut >> by) & mask], ties * tie_weight);
-        __syncthreads();
-        place<MASS>(sh, bits, above, level & 1, [&](u64 total) {
-          if (level == 0) target = aim(total);
-          return target;
-        });
-        if (sh.found >= 0 || floor_z <= -64.0) break;
-        floor_z = -64.0;
-      }
+      clear<MASS>(sh, int(mask) + 1);
+      over(sh, [&](int, uint32_t key) {
+        if (key <= (MASS ? cut : 0u) || (level > 0 && (key >> (by + bits)) != prefix)) return;
+        if (MASS) atomicAdd(&sh.mass[(key >> by) & mask], weight(O::of_key(key)));
+        else atomicAdd(&sh.count[(key >> by) & mask], 1u);
+      });
+      if (MASS && cut != 0 && threadIdx.x == 0 && (level == 0 || (cut >> (by + bits)) == prefix))
+        atomicAdd(&sh.mass[(cut >> by) & mask], ties * tie_weight);
+      __syncthreads();
+      place<MASS>(sh, bits, above, level & 1, [&](u64 total) {
+        if (level == 0) target = aim(total);
+        return target;
+      });
       prefix = (prefix << bits) | uint32_t(sh.found);
       above = sh.before;
       // the other digits on the tokens of this one, with those above where they fit
       if (level == 0 && listed < 0) {
         const uint32_t least = prefix << by, width = (1u << by) - 1;
         for (int only = 0; only < 2 && listed < 0; ++only) {
-          __syncthreads();
-          if (threadIdx.x == 0) sh.n = 0;
-          __syncthreads();
-          const uint32_t first = only ? least + width : 0xffffffffu;
-          whole = make_list(sh, first, 0, first - least) && !only;
-        }
-        if (MASS && whole && listed <= kFew) {
-          few_target = target;
-          return;
+          clear<MASS>(sh, 0);
+          whole = make_list(sh, O::of_key(max(least, O::key(O::none()))), only ? O::of_key(least + width) : INFINITY) && !only;
         }
       }
     }
@@ -432,25 +508,12 @@ __device__ inline void put(const SampleArgs& p, const Row<T>& r, int64_t row, fl
     p.logprob[row] = float((double(x) - r.top) / double(t) - log(ldexp(double(total), -p.shift)));
 }
 
-// The first sum that exceeds u times the total exceeds this: whole numbers
-// exceed the product's floor.
-__device__ inline u64 goal_of(float u, u64 total) {
-  const double aim = floor(double(u) * double(total));
-  return aim > 0.0 ? min(u64(min(aim, 0x1p63)), total - 1) : 0;
-}
-// The weight that a cut by top-p reaches: a rank is kept while less than this is
-// before it.
-__device__ inline u64 cut_of(float top_p, u64 all) {
-  const double aim = ceil(double(top_p) * double(all));
-  return aim >= 1.0 ? min(u64(aim), all) : u64(1);
-}
-
 // The token of a list of at most kFew that holds all that is kept: the first k
-// ranks of it, cut at few_target or by top-p, and by min-p.  Four threads compare a
+// ranks of it, cut at `target` or by top-p, and by min-p.  Four threads compare a
 // token with a quarter of the others each; then one wave sums in both orders.
 template <typename T>
 __device__ inline void take_few(const SampleArgs& p, const Row<T>& r, Shared& sh, int64_t row, float u, float t,
-                                int64_t k, float top_p, u64 least) {
+                                int64_t k, u64 target, float top_p, u64 least) {
   const int n = r.listed, j = threadIdx.x % kFew, part = threadIdx.x / kFew;
   const int q = (n + 3) / 4, lo = part * q, hi = min(lo + q, n);
   Few& few = sh.few;
@@ -484,7 +547,7 @@ __device__ inline void take_few(const SampleArgs& p, const Row<T>& r, Shared& sh
 #pragma unroll
   for (int e = 0; e < kPer; ++e) sum += w[e] = first + e < n && first + e < k ? few.weight[first + e] : 0;
   u64 s = upto(sum);
-  const u64 all = last_lane(s), limit = r.few_target ? r.few_target : top_p < 1.f ? cut_of(top_p, all) : ~u64(0);
+  const u64 all = last_lane(s), limit = target ? target : top_p < 1.f ? cut_of(top_p, all) : ~u64(0);
   uint32_t mine = 0;  // kept ranks: a run from the first on
   s -= sum;
 #pragma unroll
@@ -526,7 +589,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   r.shift = p.shift;
   r.listed = -1;
   r.whole = false;
-  r.few_target = 0;
   const float u = p.u[row];
   float t = p.temperature ? p.temperature[row] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
@@ -537,31 +599,35 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   sh.count[threadIdx.x] = 0;
 
   // The largest value, of this lane's and of all, with the first chunk that holds
-  // it; and whether there are more NaN than the places past the row's end.
-  uint32_t mine = 0, nan = 0;
+  // it; and whether there is a NaN.
+  float lane_top = -INFINITY;
+  bool nan = false;
   int mine_at = 0;
   r.template each<3>([&](int c, const Run<T>& v) {
-    const int past = c * kChunk + (lane + 1) * kLane - r.V;
-    nan -= uint32_t(max(0, min(past, kLane)));
-    uint32_t m = 0;
+    float m = O::value(v.v[0]);
+    nan |= m != m;
 #pragma unroll
-    for (int e = 0; e < kLane; ++e) {
+    for (int e = 1; e < kLane; ++e) {
       const float f = O::value(v.v[e]);
-      nan += f != f;
-      m = max(m, O::key(v.v[e]));
+      nan |= f != f;
+      m = f > m ? f : m;
     }
-    if (m > mine) mine = m, mine_at = c;
+    if (m > lane_top) lane_top = m, mine_at = c;
   });
-  u64 best = nan ? ~u64(0) : (u64(mine) << 32) | uint32_t(~mine_at);
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) best = max(best, u64(__shfl_xor(best, m, kWave)));
-  if (lane == 0) sh.wave_sum[0][threadIdx.x / kWave] = best;
+  uint32_t mine;  // its key
+  if constexpr (sizeof(T) == 4) mine = O::key(lane_top);
+  else if constexpr (std::is_same_v<T, F16>) mine = O::key(F16{f32_to_f16(lane_top)});
+  else mine = O::key(f32_to_bf16(lane_top));
+  const uint32_t wave_top = __ballot(nan) ? 0xffffffffu : wave_max(mine);
+  const uint32_t wave_at = wave_max(mine == wave_top ? uint32_t(~mine_at) : 0u);
+  if (lane == 0) sh.wave_sum[0][threadIdx.x / kWave] = (u64(wave_top) << 32) | wave_at;
   __syncthreads();
+  u64 best = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) best = max(best, sh.wave_sum[0][w]);
   const uint32_t top_key = uint32_t(best >> 32);
   const float largest = O::of_key(top_key);
-  bad = bad || best == ~u64(0) || largest == INFINITY || largest == -INFINITY;
+  bad = bad || top_key == 0xffffffffu || largest == INFINITY || largest == -INFINITY;
   if (bad) {  // the whole workgroup
     if (threadIdx.x == 0) {
       if (p.index_type == MK_S64) static_cast<int64_t*>(p.token)[row] = -1;
@@ -594,29 +660,43 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
       // row's k-th largest value.  Each wave finds the step for itself.
       const int lanes = min((r.V + kLane - 1) / kLane, kThreads);  // that hold anything
       if (k <= lanes / 2) {
-        if (mine) atomicAdd(&sh.count[min((top_key - mine) >> O::kFine, uint32_t(kThreads - 1))], 1u);
-        __syncthreads();
+        // (step b at (b % 16) 64 + b / 16: lane l reads steps 16 l .. side by side)
         constexpr int kPer = kThreads / kWave;
-        uint32_t own = 0;
+        const uint32_t my_step = min((top_key - mine) >> O::kFine, uint32_t(kThreads - 1));
+        if (mine) atomicAdd(&sh.count[my_step % kPer * kWave + my_step / kPer], 1u);
+        __syncthreads();
+        uint32_t n[kPer], own = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) own += sh.count[kPer * lane + e];
+        for (int e = 0; e < kPer; ++e) own += n[e] = sh.count[kWave * e + lane];
         uint32_t s = upto(own) - own;
-        uint32_t step = 0;
         const u64 here = __ballot(s < k && k <= s + own);
-        for (int e = 0; e < kPer; ++e) {
-          if (s + sh.count[kPer * lane + e] >= k) break;
-          s += sh.count[kPer * lane + e];
-          ++step;
+        uint32_t step = uint32_t(kPer * lane);
+#pragma unroll
+        for (int e = 0; e < kPer - 1; ++e)
+          if (step == uint32_t(kPer * lane + e) && s + n[e] < k) s += n[e], ++step;
+        step = uint32_t(__builtin_amdgcn_readlane(int(step), __ffsll(here) - 1));
+        if (step < uint32_t(kThreads - 1)) {
+          const uint32_t below = ((step + 1) << O::kFine) - 1, lowest = O::key(O::none());
+          r.whole = r.make_list(sh, O::of_key(top_key - min(below, top_key - lowest)), INFINITY);
         }
-        step = uint32_t(__builtin_amdgcn_readlane(int(kPer * lane + step), __ffsll(here) - 1));
-        if (step < uint32_t(kThreads - 1)) r.whole = r.make_list(sh, top_key, O::kFine, step);
       }
       if (!r.whole || r.listed > kFew) r.template select<false>(sh, [&](u64) { return u64(k); });
     }
     const bool few_k = r.whole && r.listed <= kFew && r.cut == 0;  // top-k is still to be taken
-    if (top_p < 1.f && !few_k)  // of what top-k kept, before min-p
-      r.template select<true>(sh, [&](u64 all) { return cut_of(top_p, all); });
-    if (few_k || r.few_target) return take_few(p, r, sh, row, u, t, few_k ? k : int64_t(kFew), top_p, least);
+    u64 target = 0;
+    if (top_p < 1.f && !few_k) {  // of what top-k kept, before min-p
+      const bool top_k = r.cut != 0;
+      if (!top_k) target = r.list_top(sh, top_p);
+      if (top_k || (target != 0 && !(r.whole && r.listed <= kFew)))
+        r.template select<true>(sh, [&](u64 all) { return target ? target : cut_of(top_p, all); });
+    }
+    if (r.cut == 0 && r.listed < 0 && least > 0) {  // min-p alone: what may be above it, a little below it
+      r.template clear<true>(sh, 0);
+      const double lo = r.top + double(log2f(fminf(min_p, 1.f))) / r.per;
+      r.whole = r.make_list(sh, float(lo - fabs(lo) * 0x1p-20 - 0x1p-20 / r.per), INFINITY);
+    }
+    if (r.whole && r.listed <= kFew && r.cut == 0)
+      return take_few(p, r, sh, row, u, t, few_k ? k : int64_t(kFew), target, top_p, least);
     // weights and ties of each chunk
     tie_weight = r.cut != 0 ? r.weight(O::of_key(r.cut)) : 0;
     if (tie_weight < least) tie_weight = 0;
@@ -648,7 +728,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
           const uint32_t key = O::key(v.v[e]);
           const u64 w = r.weight(O::value(v.v[e]));
           own += key > r.cut && w >= least ? w : 0;
-          ties += key == r.cut && key != 0;
+          ties += key == r.cut;
         }
         add_all(&sh.mass[c], own);
         if (ties) atomicAdd(&sh.count[c], ties);
@@ -696,22 +776,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
 
   // within the chunk, one wave
   const int i0 = chunk * kChunk + lane * kLane;
-  T v[kLane];
+  const int from = r.start(i0);  // places before i0 hold -inf
+  const Run<T> v = r.load(i0);
   uint32_t equal = 0;
 #pragma unroll
-  for (int e = 0; e < kLane; ++e) {
-    v[e] = r.x[min(i0 + e, r.V - 1)];
-    equal += i0 + e < r.V && O::key(v[e]) == r.cut;
-  }
+  for (int e = 0; e < kLane; ++e) equal += O::key(v.v[e]) == r.cut;
   uint32_t tie = ties_before + upto(equal) - equal;  // before this lane's elements
   u64 w[kLane], sum = 0;
 #pragma unroll
   for (int e = 0; e < kLane; ++e) {
-    const uint32_t key = O::key(v[e]);
-    w[e] = r.weight(O::value(v[e]));
+    const uint32_t key = O::key(v.v[e]);
+    w[e] = r.weight(O::value(v.v[e]));
     w[e] = key > r.cut && w[e] >= least ? w[e] : 0;
     if (key == r.cut) w[e] = u64(tie++) < r.ties ? tie_weight : 0;
-    if (i0 + e >= r.V) w[e] = 0;
     sum += w[e];
   }
   const u64 s = upto(sum);
@@ -722,9 +799,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
 #pragma unroll
     for (int e = 0; e < kLane; ++e) {
       at += w[e];
-      if (e_at == kLane && rest < at) e_at = e, x_at = O::value(v[e]);
+      if (e_at == kLane && rest < at) e_at = e, x_at = O::value(v.v[e]);
     }
-    put(p, r, row, t, i0 + e_at, x_at, total);
+    put(p, r, row, t, from + e_at, x_at, total);
   }
 }
 
