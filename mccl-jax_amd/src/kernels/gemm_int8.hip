@@ -31,14 +31,15 @@ struct Int8Gemm {
   int64_t M, N, K;
   int64_t lda, ldb, ldc;
   int tiles_m, tiles_n;
+  int k_waves;   // few rows: waves of a workgroup that share a column block
   int c_type, epilogue;
   int stream_c;  // C goes past the caches
 };
 
 // one value of C from its sum
 __device__ inline float finish(const Int8Gemm& p, int sum, float sa, int64_t n) {
-  float v = float(sum) * sa * p.b_scale[n];
-  if ((p.epilogue & 3) != 0) v += load_as_f32(p.bias, n, (p.epilogue & 4) ? int(MK_F32) : p.c_type);
+  const float b = (p.epilogue & 3) != 0 ? load_as_f32(p.bias, n, (p.epilogue & 4) ? int(MK_F32) : p.c_type) : 0.f;
+  float v = fmaf(float(sum) * sa, p.b_scale[n], b);
   if ((p.epilogue & 3) == 2) v = v < 0.f ? 0.f : v;  // keeps a NaN
   return v;
 }
@@ -56,10 +57,10 @@ __device__ inline i32x4_t load16_upto(const int8_t* p, int64_t n) {
 }
 
 // ---------------------------------------------------------------- few rows
-// At most 64 rows: reading B (the weights) once is the work.  A workgroup has 16 VN
-// columns and all rows; its NW waves take k in steps of 128 bytes round-robin,
-// kD steps ahead in registers, and their sums meet in LDS (whole numbers: in any
-// order).  Nothing is staged.  A lane (c, g) of v_mfma_i32_16x16x64_i8 loads 32
+// At most 64 rows: reading B (the weights) once is the work.  A wave has 16 VN columns
+// and all rows, and every k_waves-th step of 128 bytes of k, kD steps ahead in
+// registers; the sums of the k_waves waves of a column block meet in LDS (whole
+// numbers: in any order).  Nothing is staged.  A lane (c, g) of v_mfma_i32_16x16x64_i8 loads 32
 // consecutive bytes of row c at k = 32 g, so that 4 lanes take a whole line of a
 // row, and they are the operands of two MFMAs: which k an MFMA's slots mean is
 // free as long as A and B agree.  Rows need no alignment.
@@ -71,7 +72,8 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm 
   __shared__ __attribute__((aligned(16))) int red[NW][16][NT + 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int64_t n0 = int64_t(blockIdx.x) * NT;
+  const int kw = p.k_waves, k_wave = wave % kw, blocks = NW / kw;  // of columns, in this workgroup
+  const int64_t n_first = int64_t(blockIdx.x) * blocks * NT, n0 = n_first + wave / kw * NT;
   // rows past the operands' repeat the last and are not stored
   const int8_t *ap[MT], *bp[VN];
 #pragma unroll
@@ -104,11 +106,11 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm 
   };
   // the loop's loads are unconditional: with a branch around them the compiler
   // waits for every load at the loop's head
-  const int64_t full = p.K / kStep, n = full > wave ? (full - wave + NW - 1) / NW : 0;
+  const int full = int(p.K) / kStep, n = full > k_wave ? (full - k_wave + kw - 1) / kw : 0;
   Step s[kD];
-  auto fetch = [&](int d, int64_t i) __attribute__((always_inline)) { load(s[d], wave + NW * i); };
+  auto fetch = [&](int d, int i) __attribute__((always_inline)) { load(s[d], k_wave + kw * i); };
   if (n >= kD) {
-    int64_t i = 0;
+    int i = 0;
 #pragma unroll
     for (int d = 0; d < kD; ++d) fetch(d, d);
     for (; i + 2 * kD <= n; i += kD) {
@@ -134,8 +136,8 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm 
     for (int d = 0; d < kD - 1; ++d)
       if (d < n) multiply(s[d]);
   }
-  if (p.K % kStep != 0 && full % NW == wave) {  // the last, shorter step: zeros past K
-    const int64_t k = full * kStep, left = p.K - k - 32 * g;
+  if (p.K % kStep != 0 && full % kw == k_wave) {  // the last, shorter step: zeros past K
+    const int64_t k = int64_t(full) * kStep, left = p.K - k - 32 * g;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -152,12 +154,12 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm 
 #pragma unroll
     for (int j = 0; j < VN; ++j) *reinterpret_cast<i32x4_t*>(&red[wave][c][16 * j + 4 * g]) = acc[m][j];
     __syncthreads();
-    for (int e = threadIdx.x; e < 16 * NT; e += 64 * NW) {
-      const int row = e / NT, col = e % NT;
-      int sum = red[0][row][col];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) sum += red[w][row][col];
-      const int64_t mrow = 16 * m + row, nc = n0 + col;
+    const int width = blocks * NT;
+    for (int e = threadIdx.x; e < 16 * width; e += 64 * NW) {
+      const int row = e / width, col = e % width, w0 = col / NT * kw;
+      int sum = red[w0][row][col % NT];
+      for (int w = 1; w < kw; ++w) sum += red[w0 + w][row][col % NT];
+      const int64_t mrow = 16 * m + row, nc = n_first + col;
       if (mrow < p.M && nc < p.N)
         store_from_f32(p.C, mrow * p.ldc + nc, p.c_type, finish(p, sum, p.a_scale[mrow], nc));
     }
@@ -165,39 +167,62 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm 
 }
 
 template <int VN, int MT>
-void launch_rows(hipStream_t s, const Int8Gemm& a) {
-  // sixteen waves where the steps in flight and the sums fit 128 registers, else eight
+void launch_rows(hipStream_t s, Int8Gemm a, int k_waves) {
   constexpr int kWords = 8 * (VN + MT), kSums = 4 * VN * MT;
-  constexpr int NW = 2 * kWords + kSums <= 72 ? 16 : 8;
-  constexpr int kFit = ((NW == 16 ? 72 : 192) - kSums) / kWords, kD = kFit > 4 ? 4 : kFit;
+  // steps in flight within 128 registers (sixteen waves a CU) where two fit, else 256
+  constexpr bool kSlim = 2 * kWords + kSums <= 72;
+  constexpr int kFit = ((kSlim ? 72 : 192) - kSums) / kWords, kD = kFit > 4 ? 4 : kFit;
   static_assert(kD >= 2, "two steps in flight");
-  const int64_t tiles = (a.N + 16 * VN - 1) / (16 * VN);
-  hipLaunchKernelGGL((gemm_int8_rows_kernel<VN, MT, NW, kD>), dim3(unsigned(tiles)), dim3(64 * NW), 0, s, a);
+  constexpr int kMost = kSlim ? 16 : 8;
+  a.k_waves = std::min(k_waves, kMost);
+  const int64_t blocks = (a.N + 16 * VN - 1) / (16 * VN);
+  auto go = [&](auto nw) {
+    constexpr int NW = decltype(nw)::value;
+    const int64_t per = NW / a.k_waves;
+    hipLaunchKernelGGL((gemm_int8_rows_kernel<VN, MT, NW, kD>), dim3(unsigned((blocks + per - 1) / per)), dim3(64 * NW), 0, s, a);
+  };
+  if (a.k_waves == 16) go(Int<kMost>{});
+  else go(Int<8>{});
 }
 
 template <int VN>
-void launch_rows(hipStream_t s, const Int8Gemm& a) {
-  if (a.M <= 16) launch_rows<VN, 1>(s, a);
-  else if (a.M <= 32) launch_rows<VN, 2>(s, a);
-  else launch_rows<VN, 4>(s, a);
+void launch_rows(hipStream_t s, const Int8Gemm& a, int k_waves) {
+  if (a.M <= 16) launch_rows<VN, 1>(s, a, k_waves);
+  else if (a.M <= 32) launch_rows<VN, 2>(s, a, k_waves);
+  else launch_rows<VN, 4>(s, a, k_waves);
+}
+
+// Waves enough to fill the chip, from the columns (64 or 32 a wave where they are
+// many: less of A is read) and then from k.  us, by columns a wave and waves along
+// k: 16 x 4096 x 16384 (M x K x N) 16: 20.6 / 20.9 (2, 4), 32: 17.5 / 18.4 (4, 8),
+// 64: 16.3 (8); 16 x 512 x 16384 16: 4.8 (4), 32: 5.2 (4); 16 x 4096 x 4096 16: 17.1,
+// 10.1, 6.9, 6.9 (2, 4, 8, 16), 32: 8.5 (8); 1 x 768 x 2304 16: 3.1 (8).
+void launch_few_rows(hipStream_t s, const Int8Gemm& a) {
+  const int vn = a.N >= 12288 && a.K >= 2048 ? 4 : a.N >= 8192 ? 2 : 1;
+  const int64_t blocks = (a.N + 16 * vn - 1) / (16 * vn);
+  int kw = 1;
+  while (kw < 16 && kw * blocks < (vn == 1 ? 4096 : 2048) && kw * kStep < a.K) kw *= 2;
+  if (vn == 4) launch_rows<4>(s, a, kw);
+  else if (vn == 2) launch_rows<2>(s, a, kw);
+  else launch_rows<1>(s, a, kw);
 }
 
 // ---------------------------------------------------------------- tiles
 // Rows on the 16-byte grid.  Workgroup tile TM x TN, k in tiles of 128 bytes,
 // WGM x WGN waves of 32 x 32 blocks.  Operand tiles go straight into LDS
-// (buffer_load ... lds, attn_common.h) in two stages: the copies of the next
-// k tile are issued while this one is multiplied, one barrier a tile.  An LDS row is
+// (buffer_load ... lds, attn_common.h) in S stages: the copies of k tile t + S - 1
+// are issued while tile t is multiplied, one barrier a tile.  An LDS row is
 // 128 bytes, its 16-byte chunk c at position c ^ ((row >> 1) & 7), so that the
 // 16 rows a ds_read_b128 takes at one chunk lie on 16 different bank groups.
 // Chunks past M, N or K are loaded from an out-of-range offset, which reads
 // zeros.  Where K is no multiple of 16 the last chunk of a row is loaded whole
-// (16 aligned bytes, so on the row's last page) and, A's bytes past K are
-// cleared as they are read from LDS: what B holds there is multiplied by zero.
+// (16 aligned bytes, so on the row's last page) and A's bytes past K are then
+// cleared in LDS: what B holds there is multiplied by zero.
 //
 // Tile order: workgroups are dealt round-robin to the 8 XCDs, each with its own
 // L2; workgroup i takes tile (i % 8) (tiles / 8) + i / 8 of an order that walks
 // groups of 4 tile rows column by column, so that an XCD's tiles are a compact block.
-constexpr int kBK = 128, kStages = 2;
+constexpr int kBK = 128;
 constexpr int kGroupM = 4;
 constexpr int kInvalid = int(0x80000000u);  // buffer offset past every accepted range
 
@@ -215,6 +240,22 @@ struct Copies {
       off[c] = r0 + row < rows ? uint32_t((r0 + row) * ld + k[c]) : uint32_t(kInvalid);
     }
   }
+  // Clears what this wave copied of the last k tile (at k0, K no multiple of 16) past K.
+  __device__ inline void clear_past(int8_t* tile, int wave, int lane, int k0, int64_t K) const {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int left = int(K) - k0 - k[c];
+      if (left <= 0 || left >= 16) continue;
+      u32x4_t* at = reinterpret_cast<u32x4_t*>(tile + (wave + W * c) * 1024 + 16 * lane);
+      u32x4_t v = *at;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = left - 4 * q;
+        v[q] &= n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+      }
+      *at = v;
+    }
+  }
   // offset for the k tile at k0, or one that reads zeros once the chunk lies past K
   __device__ inline int at(int c, int k0, int64_t K) const {
     return off[c] != uint32_t(kInvalid) && k[c] + k0 < K ? int(off[c] + uint32_t(k0)) : kInvalid;
@@ -227,25 +268,16 @@ __device__ inline i32x4_t read_operand(const int8_t* t, int rb, int ks, int lane
   return *reinterpret_cast<const i32x4_t*>(t + row * kBK + 16 * ch);
 }
 
-// the first n (any whole number) of 16 bytes, zeros for the others
-__device__ inline i32x4_t first_bytes(i32x4_t v, int n) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int b = n - 4 * q;
-    v[q] &= b >= 4 ? -1 : b <= 0 ? 0 : (1 << (8 * b)) - 1;
-  }
-  return v;
-}
-
 template <int N>
 __device__ inline void wait_vm() {
   static_assert(N >= 0 && N < 64, "vmcnt range");
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-template <int TM_, int TN_, int WGM_, int WGN_>
+// workgroup tile, wave grid, LDS stages
+template <int TM_, int TN_, int WGM_, int WGN_, int S_>
 struct Shape {
-  static constexpr int TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_;
+  static constexpr int TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_, S = S_;
 };
 
 typedef uint32_t u32x4_by4_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -253,41 +285,55 @@ typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // C's tile through LDS in passes of as many rows as the operand stages hold:
 // a lane writes 4 consecutive columns at a time, chunk c of staging row r at
-// position c ^ (r & 15) (rows of 8 chunks: c ^ ((r >> 1) & 7)), and the workgroup stores runs of 16 bytes (of whole
+// position c ^ (r & 15) (rows of 8 and 4 chunks: c ^ ((r >> 1) & 7), c ^ ((r >> 2) & 3)), and the workgroup stores runs of 16 bytes (of whole
 // rows; they need no alignment past an element's).
-template <int CT, bool STREAM, int TM, int TN, int kW, int kWM, int kWN, int kI, int kJ>
+template <int CT, bool STREAM, int TM, int TN, int S, int kW, int kWM, int kWN, int kI, int kJ>
 __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm& p, const i32x16_t (&acc)[kI][kJ],
                                                                  int8_t* stage, const float* sa, const float* sb,
                                                                  const float* bias, int64_t m0, int64_t n0, int wm,
                                                                  int wn, int lane) {
   constexpr int kSz = CT == MK_F32 ? 4 : 2, kPer = 16 / kSz, kCpr = TN / kPer, kThreads = 64 * kW;
-  constexpr int kRoom = kStages * kBK * (TM + TN), kFit = kRoom / (TN * kSz) / kWM * kWM;
+  constexpr int kRoom = S * kBK * (TM + TN), kFit = kRoom / (TN * kSz) / kWM * kWM;
   constexpr int kRP = kFit >= TM ? TM : TM % kFit == 0 ? kFit : kWM;  // rows a pass
-  static_assert(kRP > 0 && TM % kRP == 0 && kRP % kWM == 0 && kCpr % 8 == 0, "passes of whole wave rows");
+  static_assert(kRP > 0 && TM % kRP == 0 && kRP % kWM == 0 && kCpr % 4 == 0, "passes of whole wave rows");
   static_assert(kRP * kCpr % kThreads == 0, "chunks split evenly over the threads");
   using out_t = std::conditional_t<CT == MK_F32, u32x4_by4_t, u32x4_by2_t>;
-  auto pos = [](int row, int cn) { return kCpr % 16 == 0 ? cn ^ (row & 15) : cn ^ ((row >> 1) & 7); };
+  auto pos = [](int row, int cn) {
+    return cn ^ (kCpr % 16 == 0 ? row & 15 : kCpr % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3);
+  };
   const int c = lane & 31, g = lane >> 5;
   char* C = static_cast<char*>(p.C);
+  // this lane's scales and biases, ahead of the writes to LDS
+  float s[kI];
+  f32x4 t[kJ][4], u[kJ][4];
+#pragma unroll
+  for (int a = 0; a < kI; ++a) s[a] = sa[wm * kWM + 32 * a + c];
+#pragma unroll
+  for (int b = 0; b < kJ; ++b)
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg) {
+      const int nl = wn * kWN + 32 * b + 8 * rg + 4 * g;
+      t[b][rg] = *reinterpret_cast<const f32x4*>(sb + nl);
+      u[b][rg] = *reinterpret_cast<const f32x4*>(bias + nl);
+    }
 #pragma unroll
   for (int pass = 0; pass < TM / kRP; ++pass) {
     if (pass > 0) lds_barrier();
     if (wm * kWM >= pass * kRP && wm * kWM < (pass + 1) * kRP) {
 #pragma unroll
-      for (int a = 0; a < kI; ++a) {
-        const int ml = wm * kWM + 32 * a + c, row = ml - pass * kRP;
-        const float s = sa[ml];
+      for (int b = 0; b < kJ; ++b)
 #pragma unroll
-        for (int b = 0; b < kJ; ++b)
+        for (int rg = 0; rg < 4; ++rg) {
+          const int nl = wn * kWN + 32 * b + 8 * rg + 4 * g;
 #pragma unroll
-          for (int rg = 0; rg < 4; ++rg) {
-            const int nl = wn * kWN + 32 * b + 8 * rg + 4 * g;
+          for (int a = 0; a < kI; ++a) {
+            const int row = wm * kWM + 32 * a + c - pass * kRP;
             float v[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              v[q] = float(acc[a][b][4 * rg + q]) * s * sb[nl + q];
-              if ((p.epilogue & 3) != 0) v[q] += bias[nl + q];
-              if ((p.epilogue & 3) == 2) v[q] = v[q] < 0.f ? 0.f : v[q];
+            for (int q = 0; q < 4; ++q) v[q] = fmaf(float(acc[a][b][4 * rg + q]) * s[a], t[b][rg].v[q], u[b][rg].v[q]);
+            if ((p.epilogue & 3) == 2) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
             }
             int8_t* to = stage + row * TN * kSz + 16 * pos(row, nl / kPer) + nl % kPer * kSz;
             if constexpr (CT == MK_F32) {
@@ -299,7 +345,7 @@ __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm&
               __builtin_memcpy(to, h, 8);
             }
           }
-      }
+        }
     }
     lds_barrier();
 #pragma unroll 2
@@ -325,17 +371,17 @@ __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm&
   }
 }
 
-template <class Sh, int CT, bool RAGGED>
+template <class Sh, int CT>
 __global__ __launch_bounds__(64 * Sh::WGM * Sh::WGN, 1) void gemm_int8_tiled_kernel(const Int8Gemm p) {
-  constexpr int TM = Sh::TM, TN = Sh::TN, WGN = Sh::WGN, kW = Sh::WGM * WGN;
+  constexpr int TM = Sh::TM, TN = Sh::TN, WGN = Sh::WGN, S = Sh::S, kW = Sh::WGM * WGN;
   constexpr int kWM = TM / Sh::WGM, kWN = TN / WGN, kI = kWM / 32, kJ = kWN / 32;
   constexpr int kCa = TM / 8 / kW, kCb = TN / 8 / kW, kNC = kCa + kCb;
   static_assert(kI * 32 * Sh::WGM == TM && kJ * 32 * WGN == TN, "wave blocks tile the workgroup tile");
   static_assert(kCa * kW * 8 == TM && kCb * kW * 8 == TN, "copies split evenly over the waves");
-  __shared__ __attribute__((aligned(1024))) int8_t lds[kStages * kBK * (TM + TN)];
-  __shared__ float sa[TM], sb[TN], bias[TN];
+  __shared__ __attribute__((aligned(1024))) int8_t lds[S * kBK * (TM + TN)];
+  __shared__ __attribute__((aligned(16))) float sa[TM], sb[TN], bias[TN];
   int8_t (*As)[TM * kBK] = reinterpret_cast<int8_t (*)[TM * kBK]>(lds);
-  int8_t (*Bs)[TN * kBK] = reinterpret_cast<int8_t (*)[TN * kBK]>(lds + kStages * TM * kBK);
+  int8_t (*Bs)[TN * kBK] = reinterpret_cast<int8_t (*)[TN * kBK]>(lds + S * TM * kBK);
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -352,58 +398,91 @@ __global__ __launch_bounds__(64 * Sh::WGM * Sh::WGN, 1) void gemm_int8_tiled_ker
   const Copies<kCa, kW> ca(wave, lane, m0, p.M, p.lda);
   const Copies<kCb, kW> cb(wave, lane, n0, p.N, p.ldb);
   const int K = int(p.K);
-  auto issue = [&](int kt, int stage, int lo, int hi) __attribute__((always_inline)) {
-    const int k0 = kBK * kt;
+  // this wave's copies [lo, hi) of k tile kt (A's, then B's): of a tile wholly below
+  // K, and of the one that crosses it
+  auto issue = [&](int kt, int lo, int hi) __attribute__((always_inline)) {
+    const int st = kt % S;
 #pragma unroll
     for (int c = 0; c < kNC; ++c) {
       if (c < lo || c >= hi) continue;
-      const uint32_t to = c < kCa ? lds_addr(&As[stage][(wave + kW * c) * 1024])
-                                  : lds_addr(&Bs[stage][(wave + kW * (c - kCa)) * 1024]);
-      if (k0 + kBK <= K)
-        copy_to_lds_so(c < kCa ? ra : rb, to, int(c < kCa ? ca.off[c < kCa ? c : 0] : cb.off[c < kCa ? 0 : c - kCa]),
-                       uint32_t(k0));
-      else
-        copy_to_lds(c < kCa ? ra : rb, to, c < kCa ? ca.at(c < kCa ? c : 0, k0, K) : cb.at(c < kCa ? 0 : c - kCa, k0, K));
+      if (c < kCa) copy_to_lds_so(ra, lds_addr(&As[st][(wave + kW * c) * 1024]), int(ca.off[c < kCa ? c : 0]), uint32_t(kBK * kt));
+      else copy_to_lds_so(rb, lds_addr(&Bs[st][(wave + kW * (c - kCa)) * 1024]), int(cb.off[c < kCa ? 0 : c - kCa]), uint32_t(kBK * kt));
     }
   };
+  auto issue_last = [&](int kt) __attribute__((always_inline)) {
+    const int st = kt % S;
+#pragma unroll
+    for (int c = 0; c < kCa; ++c) copy_to_lds(ra, lds_addr(&As[st][(wave + kW * c) * 1024]), ca.at(c, kBK * kt, K));
+#pragma unroll
+    for (int c = 0; c < kCb; ++c) copy_to_lds(rb, lds_addr(&Bs[st][(wave + kW * c) * 1024]), cb.at(c, kBK * kt, K));
+  };
   i32x16_t acc[kI][kJ] = {};
-  const int nk = (K + kBK - 1) / kBK;
-  issue(0, 0, 0, kNC);
+  const int nk = (K + kBK - 1) / kBK, full = K / kBK;
+#pragma unroll
+  for (int kt = 0; kt < S - 1; ++kt) {
+    if (kt < full) issue(kt, 0, kNC);
+    else if (kt < nk) issue_last(kt);
+  }
   // the scales and the bias of the tile, for the end (after the first copies, so
   // that these go first)
   for (int e = threadIdx.x; e < TM; e += 64 * kW) sa[e] = m0 + e < p.M ? p.a_scale[m0 + e] : 0.f;
   for (int e = threadIdx.x; e < TN; e += 64 * kW) {
     sb[e] = n0 + e < p.N ? p.b_scale[n0 + e] : 0.f;
+    bias[e] = 0.f;
     if ((p.epilogue & 3) != 0)
       bias[e] = n0 + e < p.N ? load_as_f32(p.bias, n0 + e, (p.epilogue & 4) ? int(MK_F32) : CT) : 0.f;
   }
-  for (int kt = 0; kt < nk; ++kt) {
-    wait_vm<0>();
-    lds_barrier();
-    const bool more = kt + 1 < nk, last = RAGGED && !more;
-    const int8_t *at = As[kt % 2], *bt = Bs[kt % 2];
+  // Tile kt from stage kt % S, a step's operands read while the step before is
+  // multiplied; MORE: the copies of tile kt + S - 1 in two parts between the first
+  // steps (all at once they fill the memory queue with the MFMAs behind them).
+  auto multiply = [&](int kt, auto more) __attribute__((always_inline)) {
+    const int8_t *at = As[kt % S], *bt = Bs[kt % S];
+    constexpr bool kAhead = kI * kJ == 1;
+    i32x4_t af[2][kI], bf[2][kJ];
+    auto read = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < kI; ++a) {
+        af[ks % 2][a] = read_operand(at, wm * kWM + 32 * a, ks, lane);
+      }
+#pragma unroll
+      for (int b = 0; b < kJ; ++b) bf[ks % 2][b] = read_operand(bt, wn * kWN + 32 * b, ks, lane);
+    };
+    if constexpr (kAhead) read(0);
 #pragma unroll
     for (int ks = 0; ks < kBK / 32; ++ks) {
-      i32x4_t af[kI], bf[kJ];
-#pragma unroll
-      for (int a = 0; a < kI; ++a) af[a] = read_operand(at, wm * kWM + 32 * a, ks, lane);
-#pragma unroll
-      for (int b = 0; b < kJ; ++b) bf[b] = read_operand(bt, wn * kWN + 32 * b, ks, lane);
-      if (more && ks < 2) issue(kt + 1, (kt + 1) % 2, ks * kNC / 2, (ks + 1) * kNC / 2);
-      if (RAGGED && last) {
-#pragma unroll
-        for (int a = 0; a < kI; ++a) af[a] = first_bytes(af[a], K - kBK * kt - 32 * ks - 16 * (lane >> 5));
-      }
+      if constexpr (!kAhead) read(ks);
+      else if (ks + 1 < kBK / 32) read(ks + 1);
+      if constexpr (decltype(more)::value)
+        if (ks < 2) issue(kt + S - 1, ks * kNC / 2, (ks + 1) * kNC / 2);
 #pragma unroll
       for (int a = 0; a < kI; ++a)
 #pragma unroll
         for (int b = 0; b < kJ; ++b)
-          acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[b], af[a], acc[a][b], 0, 0, 0);
+          acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[ks % 2][b], af[ks % 2][a], acc[a][b], 0, 0, 0);
     }
+  };
+  // Each turn waits for this wave's copies of its tile (those of the S - 2 tiles
+  // after it may still be in flight), then for everyone's; the stage of the tile
+  // before is then free for the tile S - 1 further on.
+  int kt = 0;
+  for (; kt + S - 1 < full; ++kt) {
+    wait_vm<(S - 2) * kNC>();
+    lds_barrier();
+    multiply(kt, Flag<true>{});
+  }
+  for (; kt < nk; ++kt) {
+    wait_vm<0>();
+    lds_barrier();
+    if (kt + S - 1 == full && full < nk) issue_last(full);
+    if (kt == nk - 1 && K % 16 != 0) {
+      ca.clear_past(As[kt % S], wave, lane, kBK * kt, K);
+      lds_barrier();
+    }
+    multiply(kt, Flag<false>{});
   }
   lds_barrier();  // every wave is done with the operand stages before they hold C
-  if (p.stream_c) store_tile<CT, true, TM, TN, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
-  else store_tile<CT, false, TM, TN, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
+  if (p.stream_c) store_tile<CT, true, TM, TN, S, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
+  else store_tile<CT, false, TM, TN, S, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
 }
 
 template <class Sh>
@@ -413,12 +492,51 @@ void launch_tiled(hipStream_t s, Int8Gemm a) {
   const dim3 g{unsigned(int64_t(a.tiles_m) * a.tiles_n)}, b{unsigned(64 * Sh::WGM * Sh::WGN)};
   auto go = [&](auto ct) {
     constexpr int CT = decltype(ct)::value;
-    if (a.K % 16 != 0) hipLaunchKernelGGL((gemm_int8_tiled_kernel<Sh, CT, true>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((gemm_int8_tiled_kernel<Sh, CT, false>), g, b, 0, s, a);
+    hipLaunchKernelGGL((gemm_int8_tiled_kernel<Sh, CT>), g, b, 0, s, a);
   };
   if (a.c_type == MK_BF16) go(Int<MK_BF16>{});
   else if (a.c_type == MK_F16) go(Int<MK_F16>{});
   else go(Int<MK_F32>{});
+}
+
+// The tile with the least estimated time: rounds of workgroups of nk + e k tiles,
+// e the first copies and the epilogue; a last round that leaves every workgroup
+// alone on its CU runs each k tile in `alone`.  us, fitted to the shapes' times on
+// 166 products of 17 .. 8192 rows with both C types; the choice costs 1.5% over
+// the fastest on average.  In the order below, us: bf16 C (M x K x N):
+// 8192 x 4096 x 16384 479, 578, 773, 895, 1120; 2048 x 4096 x 4096 54, 44, 58, 67, 83; 512 x
+// 4096 x 4096 41, 23, 18, 18, 24; 64 x 768 x 50257 18, 14, 12.7, 15.5, 17.5; 128 x 768 x 768
+// 12.2, 5.7, 5.1, 4.3, 4.3.
+void launch_best_tile(hipStream_t s, Int8Gemm& a) {
+  struct Option {
+    int tm, tn, per_cu;
+    double each, alone, e16, e32;
+  };
+  static const Option options[] = {{256, 256, 1, 2.08, 1.33, 3.7, 5.6},
+                                   {128, 128, 2, 1.40, 0.70, 2.4, 3.0},
+                                   {64, 128, 2, 0.86, 0.45, 3.1, 3.7},
+                                   {64, 64, 2, 0.50, 0.31, 4.3, 5.1},
+                                   {64, 32, 3, 0.45, 0.27, 4.6, 5.4}};
+  const double nk = double((a.K + kBK - 1) / kBK);
+  int best = 0;
+  double least = 0;
+  for (int o = 0; o < 5; ++o) {
+    const Option& q = options[o];
+    const int64_t tiles = ((a.M + q.tm - 1) / q.tm) * ((a.N + q.tn - 1) / q.tn), slots = 256 * q.per_cu;
+    const double work = nk + (a.c_type == MK_F32 ? q.e32 : q.e16);
+    double t = double(tiles / slots) * work * q.each;
+    if (const int64_t rem = tiles % slots) t += work * (rem <= 256 ? q.alone : q.each);
+    if (o == 0 || t < least) best = o, least = t;
+  }
+  // C past the caches where it is most of the last-level cache and the product is
+  // long (8192 x 4096 x 16384 492 us, 502 with ordinary stores; 8192 x 768 x 50264
+  // 550 and 531)
+  a.stream_c = a.M * a.N * dtype_bytes(a.c_type) >= int64_t(192) << 20 && a.K >= 2048;
+  if (best == 0) launch_tiled<Shape<256, 256, 2, 4, 2>>(s, a);
+  else if (best == 1) launch_tiled<Shape<128, 128, 2, 4, 2>>(s, a);
+  else if (best == 2) launch_tiled<Shape<64, 128, 2, 4, 3>>(s, a);
+  else if (best == 3) launch_tiled<Shape<64, 64, 2, 2, 4>>(s, a);
+  else launch_tiled<Shape<64, 32, 2, 1, 4>>(s, a);
 }
 
 // rows on the 16-byte grid that do not overlap, below the 2^31 bytes of a buffer's offsets
@@ -494,23 +612,12 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
       reinterpret_cast<uintptr_t>(b_scale) % 4 ||
       (epi != 0 && reinterpret_cast<uintptr_t>(bias) % ((epilogue & 4) ? 4 : dtype_bytes(c_type))))
     return fail(MK_ERR_INVALID, at + "an operand is not aligned to its elements");
-  Int8Gemm a{A, B, a_scale, b_scale, C, bias, M, N, K, a_ms, b_ns, c_ms, int((M + 63) / 64), int((N + 63) / 64),
+  Int8Gemm a{A, B, a_scale, b_scale, C, bias, M, N, K, a_ms, b_ns, c_ms, int((M + 63) / 64), int((N + 63) / 64), 1,
              c_type, epilogue, 0};
   hipStream_t s = as_stream(stream);
-  if (M <= 64) {
-    // 64 columns per workgroup where that fills the chip's 256 CUs, else fewer
-    if (N >= 64 * 192) launch_rows<4>(s, a);
-    else if (N >= 32 * 192) launch_rows<2>(s, a);
-    else launch_rows<1>(s, a);
-    return check_launch("mk_gemm_int8");
-  }
-  if (K > 0 && N > 1 && on_grid(A, M, K, a_ms) && on_grid(B, N, K, b_ns)) {
-    a.stream_c = M * N * dtype_bytes(c_type) >= int64_t(192) << 20;
-    if (M >= 256 && N >= 256) launch_tiled<Shape<256, 256, 2, 4>>(s, a);
-    else if (M >= 128 && N >= 128) launch_tiled<Shape<128, 128, 4, 2>>(s, a);
-    else launch_tiled<Shape<64, 64, 2, 2>>(s, a);
-    return check_launch("mk_gemm_int8");
-  }
-  hipLaunchKernelGGL(gemm_int8_any_kernel, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n)), dim3(256), 0, s, a);
+  const bool grid = K > 0 && on_grid(A, M, K, a_ms) && on_grid(B, N, K, b_ns);
+  if (M <= 64 && (!grid || (M <= 16 && N < 32768) || (M <= 32 && N <= 8192))) launch_few_rows(s, a);
+  else if (grid) launch_best_tile(s, a);
+  else hipLaunchKernelGGL(gemm_int8_any_kernel, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n)), dim3(256), 0, s, a);
   return check_launch("mk_gemm_int8");
 }
