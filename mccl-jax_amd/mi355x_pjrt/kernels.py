@@ -707,15 +707,12 @@ def _result(what, name, t, dtype, shape, dev):
         _refuse(what, name, t, (dtype,), shape, dev)
 
 
-def _rows(what, x, name="x"):
-    """(type, shape, row pitch, device) of a 2-D operand that gives a call its shape and type."""
-    dev, t = _here(what, x, name), _ROW_TYPES.get(x.dtype)
+def _refuse_rows(what, name, x):
+    """The ValueError of a 2-D operand that gives a call its shape and type."""
+    dev = _here(what, x, name)
     if x.dim() != 2:
         raise ValueError(f"{what}: {name} must be 2-D")
-    shape, st = x.shape, x.stride()
-    if t is None or (st[1] != 1 and shape[1] > 1):
-        _refuse(what, name, x, _ROW_TYPES, shape, dev)
-    return t, shape, st[0], dev
+    _refuse(what, name, x, _ROW_TYPES, x.shape, dev)
 
 
 def _handle(what, stream, dev):
@@ -727,7 +724,9 @@ def _handle(what, stream, dev):
 
 
 def _new(like, stream, dtype, *shape):
-    """An output on like's device, from the memory of the stream that writes it."""
+    """An output on like's device, from the memory of the stream that writes it
+    (a handle that is no torch stream has no such memory: its caller passes the
+    outputs, or waits before it frees anything)."""
     if stream is None or not isinstance(stream, torch.cuda.Stream):
         return like.new_empty(*shape, dtype=dtype)
     with torch.cuda.stream(stream):
@@ -770,20 +769,24 @@ def add_rmsnorm_int8(x, residual=None, gamma=None, eps=1e-6, sum_out=None, q=Non
     (mk_add_rmsnorm_int8).  Any row pitch; sum_out may be x or residual.
     Outputs that are not given come from the memory of `stream`."""
     what = "add_rmsnorm_int8"
-    t, shape, ld, dev = _rows(what, x)
+    dtype, shape, strides, dev = x.dtype, x.shape, x.stride(), x.get_device()
+    t = _ROW_TYPES.get(dtype)
+    if t is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
+        _refuse_rows(what, "x", x)
+    ld = strides[0]
     total, r_ptr, r_ld, s_ptr, s_ld = x, None, 0, None, 0
     if residual is not None:
-        _operand(what, "residual", residual, x.dtype, shape, dev)
+        _operand(what, "residual", residual, dtype, shape, dev)
         if sum_out is None:
-            total = _new_like(x, stream, x.dtype) if ld == shape[1] else _new(x, stream, x.dtype, *shape)
+            total = _new_like(x, stream, dtype) if ld == shape[1] else _new(x, stream, dtype, *shape)
         else:
             total = sum_out
-            _result(what, "sum_out", total, x.dtype, shape, dev)
+            _result(what, "sum_out", total, dtype, shape, dev)
         r_ptr, r_ld, s_ptr, s_ld = residual.data_ptr(), residual.stride()[0], total.data_ptr(), total.stride()[0]
     elif sum_out is not None:
         raise ValueError(f"{what}: sum_out without a residual")
     if gamma is not None:
-        _operand(what, "gamma", gamma, x.dtype, shape[1:], dev)
+        _operand(what, "gamma", gamma, dtype, shape[1:], dev)
     q, pitch, scale = _int8_outputs(what, x, shape, ld, q, scale, dev, stream)
     rc = lib().mk_add_rmsnorm_int8(_handle(what, stream, dev), t, shape[0], shape[1], x.data_ptr(), ld, r_ptr, r_ld,
                                    None if gamma is None else gamma.data_ptr(), eps, s_ptr, s_ld, q.data_ptr(), pitch,
@@ -798,7 +801,11 @@ def quantize_rows(x, gelu=False, q=None, scale=None, stream=None):
     rows with one fp32 scale each, max |y| / 127 (mk_quantize_rows).  For
     weights x is [out, in] and the product takes q.t()."""
     what = "quantize_rows"
-    t, shape, ld, dev = _rows(what, x)
+    shape, strides, dev = x.shape, x.stride(), x.get_device()
+    t = _ROW_TYPES.get(x.dtype)
+    if t is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
+        _refuse_rows(what, "x", x)
+    ld = strides[0]
     q, pitch, scale = _int8_outputs(what, x, shape, ld, q, scale, dev, stream)
     rc = lib().mk_quantize_rows(_handle(what, stream, dev), t, shape[0], shape[1], x.data_ptr(), ld, 1 if gelu else 0,
                                 q.data_ptr(), pitch, scale.data_ptr())
@@ -882,7 +889,11 @@ def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, 
     tensor of one value a row (top_k int32, the others fp32).  temperature 0 is
     row_argmax.  A row without a valid choice gives token -1 and logprob NaN."""
     what = "sample_rows"
-    mk, shape, ld, dev = _rows(what, logits, "logits")
+    shape, strides, dev = logits.shape, logits.stride(), logits.get_device()
+    mk = _ROW_TYPES.get(logits.dtype)
+    if mk is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
+        _refuse_rows(what, "logits", logits)
+    ld = strides[0]
     per_row = shape[:1]
     _operand(what, "u", u, torch.float32, per_row, dev)
     if index_dtype is not torch.int32 and index_dtype is not torch.int64:

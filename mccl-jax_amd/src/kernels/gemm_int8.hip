@@ -208,8 +208,8 @@ void launch_few_rows(hipStream_t s, const Int8Gemm& a) {
 }
 
 // ---------------------------------------------------------------- tiles
-// Rows on the 16-byte grid.  Workgroup tile TM x TN, k in tiles of 128 bytes,
-// WGM x WGN waves of 32 x 32 blocks.  Operand tiles go straight into LDS
+// Workgroup tile TM x TN, k in tiles of 128 bytes,
+// WGM x WGN waves of 32 x 32 blocks.  Tiles of rows on the 16-byte grid go straight into LDS
 // (buffer_load ... lds, attn_common.h) in S stages: the copies of k tile t + S - 1
 // are issued while tile t is multiplied, one barrier a tile.  An LDS row is
 // 128 bytes, its 16-byte chunk c at position c ^ ((row >> 1) & 7), so that the
@@ -262,6 +262,36 @@ struct Copies {
   }
 };
 
+// The same chunks of rows at any address and pitch, through registers: rows past
+// the operand repeat its last one, k past K is zeros.
+template <int kC, int W>
+struct Loads {
+  const int8_t* at[kC];
+  int32_t k[kC];
+  i32x4_t v[kC];
+  __device__ inline Loads(const int8_t* base, int wave, int lane, int64_t r0, int64_t rows, int64_t ld) {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int row = 8 * (wave + W * c) + lane / 8;
+      k[c] = 16 * ((lane % 8) ^ ((row >> 1) & 7));
+      at[c] = base + std::min<int64_t>(r0 + row, rows - 1) * ld + k[c];
+    }
+  }
+  __device__ inline void load(int k0, int K) {
+    if (k0 + kBK <= K) {
+#pragma unroll
+      for (int c = 0; c < kC; ++c) v[c] = load16(at[c] + k0);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kC; ++c) v[c] = load16_upto(at[c] + k0, K - k0 - k[c]);
+    }
+  }
+  __device__ inline void store(int8_t* tile, int wave, int lane) const {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) *reinterpret_cast<i32x4_t*>(tile + (wave + W * c) * 1024 + 16 * lane) = v[c];
+  }
+};
+
 // MFMA operand for rows rb .. rb + 31 and k 32 ks .. 32 ks + 31 of a tile
 __device__ inline i32x4_t read_operand(const int8_t* t, int rb, int ks, int lane) {
   const int row = rb + (lane & 31), ch = (2 * ks + (lane >> 5)) ^ ((row >> 1) & 7);
@@ -274,10 +304,12 @@ __device__ inline void wait_vm() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-// workgroup tile, wave grid, LDS stages
-template <int TM_, int TN_, int WGM_, int WGN_, int S_>
+// Workgroup tile, wave grid, LDS stages; DIRECT: rows on the 16-byte grid go straight
+// into LDS, any others through registers.
+template <int TM_, int TN_, int WGM_, int WGN_, int S_, bool DIRECT = true>
 struct Shape {
   static constexpr int TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_, S = S_;
+  static constexpr bool kDirect = DIRECT;
 };
 
 typedef uint32_t u32x4_by4_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -418,10 +450,12 @@ __global__ __launch_bounds__(64 * Sh::WGM * Sh::WGN, 1) void gemm_int8_tiled_ker
   };
   i32x16_t acc[kI][kJ] = {};
   const int nk = (K + kBK - 1) / kBK, full = K / kBK;
+  if constexpr (Sh::kDirect) {
 #pragma unroll
-  for (int kt = 0; kt < S - 1; ++kt) {
-    if (kt < full) issue(kt, 0, kNC);
-    else if (kt < nk) issue_last(kt);
+    for (int kt = 0; kt < S - 1; ++kt) {
+      if (kt < full) issue(kt, 0, kNC);
+      else if (kt < nk) issue_last(kt);
+    }
   }
   // the scales and the bias of the tile, for the end (after the first copies, so
   // that these go first)
@@ -461,24 +495,40 @@ __global__ __launch_bounds__(64 * Sh::WGM * Sh::WGN, 1) void gemm_int8_tiled_ker
           acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bf[ks % 2][b], af[ks % 2][a], acc[a][b], 0, 0, 0);
     }
   };
-  // Each turn waits for this wave's copies of its tile (those of the S - 2 tiles
-  // after it may still be in flight), then for everyone's; the stage of the tile
-  // before is then free for the tile S - 1 further on.
-  int kt = 0;
-  for (; kt + S - 1 < full; ++kt) {
-    wait_vm<(S - 2) * kNC>();
-    lds_barrier();
-    multiply(kt, Flag<true>{});
-  }
-  for (; kt < nk; ++kt) {
-    wait_vm<0>();
-    lds_barrier();
-    if (kt + S - 1 == full && full < nk) issue_last(full);
-    if (kt == nk - 1 && K % 16 != 0) {
-      ca.clear_past(As[kt % S], wave, lane, kBK * kt, K);
+  if constexpr (Sh::kDirect) {
+    // Each turn waits for this wave's copies of its tile (those of the S - 2 tiles
+    // after it may still be in flight), then for everyone's; the stage of the tile
+    // before is then free for the tile S - 1 further on.
+    int kt = 0;
+    for (; kt + S - 1 < full; ++kt) {
+      wait_vm<(S - 2) * kNC>();
       lds_barrier();
+      multiply(kt, Flag<true>{});
     }
-    multiply(kt, Flag<false>{});
+    for (; kt < nk; ++kt) {
+      wait_vm<0>();
+      lds_barrier();
+      if (kt + S - 1 == full && full < nk) issue_last(full);
+      if (kt == nk - 1 && K % 16 != 0) {
+        ca.clear_past(As[kt % S], wave, lane, kBK * kt, K);
+        lds_barrier();
+      }
+      multiply(kt, Flag<false>{});
+    }
+  } else {
+    // the next tile's loads are in flight while this one is multiplied; a stage is
+    // written again two barriers after its last reader began
+    static_assert(S == 2 || Sh::kDirect, "two stages");
+    Loads<kCa, kW> la(p.A, wave, lane, m0, p.M, p.lda);
+    Loads<kCb, kW> lb(p.B, wave, lane, n0, p.N, p.ldb);
+    if (nk > 0) la.load(0, K), lb.load(0, K);
+    for (int kt = 0; kt < nk; ++kt) {
+      la.store(As[kt % S], wave, lane);
+      lb.store(Bs[kt % S], wave, lane);
+      __syncthreads();
+      if (kt + 1 < nk) la.load(kBK * (kt + 1), K), lb.load(kBK * (kt + 1), K);
+      multiply(kt, Flag<false>{});
+    }
   }
   lds_barrier();  // every wave is done with the operand stages before they hold C
   if (p.stream_c) store_tile<CT, true, TM, TN, S, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
@@ -507,7 +557,7 @@ void launch_tiled(hipStream_t s, Int8Gemm a) {
 // 8192 x 4096 x 16384 479, 578, 773, 895, 1120; 2048 x 4096 x 4096 54, 44, 58, 67, 83; 512 x
 // 4096 x 4096 41, 23, 18, 18, 24; 64 x 768 x 50257 18, 14, 12.7, 15.5, 17.5; 128 x 768 x 768
 // 12.2, 5.7, 5.1, 4.3, 4.3.
-void launch_best_tile(hipStream_t s, Int8Gemm& a) {
+void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
   struct Option {
     int tm, tn, per_cu;
     double each, alone, e16, e32;
@@ -521,18 +571,21 @@ void launch_best_tile(hipStream_t s, Int8Gemm& a) {
   int best = 0;
   double least = 0;
   for (int o = 0; o < 5; ++o) {
+    if (!grid && o != 1 && o != 3) continue;
     const Option& q = options[o];
     const int64_t tiles = ((a.M + q.tm - 1) / q.tm) * ((a.N + q.tn - 1) / q.tn), slots = 256 * q.per_cu;
     const double work = nk + (a.c_type == MK_F32 ? q.e32 : q.e16);
     double t = double(tiles / slots) * work * q.each;
     if (const int64_t rem = tiles % slots) t += work * (rem <= 256 ? q.alone : q.each);
-    if (o == 0 || t < least) best = o, least = t;
+    if (least == 0 || t < least) best = o, least = t;
   }
   // C past the caches where it is most of the last-level cache and the product is
   // long (8192 x 4096 x 16384 492 us, 502 with ordinary stores; 8192 x 768 x 50264
   // 550 and 531)
   a.stream_c = a.M * a.N * dtype_bytes(a.c_type) >= int64_t(192) << 20 && a.K >= 2048;
-  if (best == 0) launch_tiled<Shape<256, 256, 2, 4, 2>>(s, a);
+  if (!grid && best == 1) launch_tiled<Shape<128, 128, 2, 4, 2, false>>(s, a);
+  else if (!grid) launch_tiled<Shape<64, 64, 2, 2, 2, false>>(s, a);
+  else if (best == 0) launch_tiled<Shape<256, 256, 2, 4, 2>>(s, a);
   else if (best == 1) launch_tiled<Shape<128, 128, 2, 4, 2>>(s, a);
   else if (best == 2) launch_tiled<Shape<64, 128, 2, 4, 3>>(s, a);
   else if (best == 3) launch_tiled<Shape<64, 64, 2, 2, 4>>(s, a);
@@ -545,45 +598,6 @@ bool on_grid(const int8_t* p, int64_t rows, int64_t K, int64_t ld) {
          (rows - 1) * ld + K + 16 < (int64_t(1) << 31);
 }
 
-// ---------------------------------------------------------------- any operands
-// Any shape, pitch and alignment: 64 x 64 tiles, 4 waves of 32 x 32, k 64 deep
-// through registers and LDS.
-__global__ __launch_bounds__(256) void gemm_int8_any_kernel(const Int8Gemm p) {
-  constexpr int T = 64, BK = 64, kPitch = BK + 16;  // rows 80 bytes apart: 16 lanes of a read on different banks
-  __shared__ __attribute__((aligned(16))) int8_t lds[2][T * kPitch];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = lane & 31, g = lane >> 5;
-  const int64_t m0 = int64_t(blockIdx.x / p.tiles_n) * T, n0 = int64_t(blockIdx.x % p.tiles_n) * T;
-  // this thread's chunk of either tile; rows past the operand repeat its last
-  const int row = threadIdx.x / 4, at = 16 * (threadIdx.x % 4);
-  const int8_t* src[2] = {p.A + std::min<int64_t>(m0 + row, p.M - 1) * p.lda + at,
-                          p.B + std::min<int64_t>(n0 + row, p.N - 1) * p.ldb + at};
-  i32x16_t acc = {};
-  for (int64_t k0 = 0; k0 < p.K; k0 += BK) {
-    i32x4_t v[2];
-#pragma unroll
-    for (int o = 0; o < 2; ++o) v[o] = load16_upto(src[o] + k0, p.K - k0 - at);
-    __syncthreads();
-#pragma unroll
-    for (int o = 0; o < 2; ++o) *reinterpret_cast<i32x4_t*>(&lds[o][row * kPitch + at]) = v[o];
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
-      const i32x4_t a = *reinterpret_cast<const i32x4_t*>(&lds[0][(32 * (wave / 2) + c) * kPitch + 32 * ks + 16 * g]);
-      const i32x4_t b = *reinterpret_cast<const i32x4_t*>(&lds[1][(32 * (wave % 2) + c) * kPitch + 32 * ks + 16 * g]);
-      acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(b, a, acc, 0, 0, 0);
-    }
-  }
-  const int64_t m = m0 + 32 * (wave / 2) + c;
-  if (m >= p.M) return;
-  const float sa = p.a_scale[m];
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int64_t n = n0 + 32 * (wave % 2) + 8 * (r / 4) + 4 * g + r % 4;
-    if (n < p.N) store_from_f32(p.C, m * p.ldc + n, p.c_type, finish(p, acc[r], sa, n));
-  }
-}
-
 }  // namespace
 }  // namespace mk
 
@@ -593,31 +607,29 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
                             const float* a_scale, const int8_t* B, int64_t b_ns, const float* b_scale, void* C,
                             int64_t c_ms, const void* bias, int epilogue) {
   clear_error();
-  const std::string at = "mk_gemm_int8: ";
   if (c_type != MK_BF16 && c_type != MK_F16 && c_type != MK_F32)
-    return fail(MK_ERR_UNSUPPORTED, at + "c_type must be bf16/f16/f32");
-  if (M < 0 || N < 0 || K < 0) return fail(MK_ERR_INVALID, at + "negative shape");
-  if (K > kMaxK) return fail(MK_ERR_UNSUPPORTED, at + "K past 131071: the 32-bit sums could overflow");
+    return fail(MK_ERR_UNSUPPORTED, "mk_gemm_int8: c_type must be bf16/f16/f32");
+  if (M < 0 || N < 0 || K < 0) return fail(MK_ERR_INVALID, "mk_gemm_int8: negative shape");
+  if (K > kMaxK) return fail(MK_ERR_UNSUPPORTED, "mk_gemm_int8: K past 131071: the 32-bit sums could overflow");
   // a workgroup of 256 threads per 64 x 64 tile, below HIP's 2^32 threads
   if (M >> 30 || N >> 30 || (M + 63) / 64 * ((N + 63) / 64) >= int64_t(1) << 24)
-    return fail(MK_ERR_UNSUPPORTED, at + "2^24 or more tiles of 64 x 64");
+    return fail(MK_ERR_UNSUPPORTED, "mk_gemm_int8: 2^24 or more tiles of 64 x 64");
   const int epi = epilogue & 3;
   if (epilogue < 0 || epilogue > 6 || epi == 3 || (epilogue == 4))
-    return fail(MK_ERR_INVALID, at + "epilogue must be 0, 1, 2, 5 or 6");
+    return fail(MK_ERR_INVALID, "mk_gemm_int8: epilogue must be 0, 1, 2, 5 or 6");
   if (M == 0 || N == 0) return MK_OK;
   if ((K > 0 && (!A || !B)) || !a_scale || !b_scale || !C || (epi != 0 && !bias))
-    return fail(MK_ERR_INVALID, at + "null pointer");
-  if ((M > 1 && (a_ms < 0 || c_ms < N)) || (N > 1 && b_ns < 0)) return fail(MK_ERR_INVALID, at + "bad stride");
+    return fail(MK_ERR_INVALID, "mk_gemm_int8: null pointer");
+  if ((M > 1 && (a_ms < 0 || c_ms < N)) || (N > 1 && b_ns < 0)) return fail(MK_ERR_INVALID, "mk_gemm_int8: bad stride");
   if (reinterpret_cast<uintptr_t>(C) % dtype_bytes(c_type) || reinterpret_cast<uintptr_t>(a_scale) % 4 ||
       reinterpret_cast<uintptr_t>(b_scale) % 4 ||
       (epi != 0 && reinterpret_cast<uintptr_t>(bias) % ((epilogue & 4) ? 4 : dtype_bytes(c_type))))
-    return fail(MK_ERR_INVALID, at + "an operand is not aligned to its elements");
-  Int8Gemm a{A, B, a_scale, b_scale, C, bias, M, N, K, a_ms, b_ns, c_ms, int((M + 63) / 64), int((N + 63) / 64), 1,
+    return fail(MK_ERR_INVALID, "mk_gemm_int8: an operand is not aligned to its elements");
+  Int8Gemm a{A, B, a_scale, b_scale, C, bias, M, N, K, a_ms, b_ns, c_ms, 0, 0, 1,
              c_type, epilogue, 0};
   hipStream_t s = as_stream(stream);
   const bool grid = K > 0 && on_grid(A, M, K, a_ms) && on_grid(B, N, K, b_ns);
   if (M <= 64 && (!grid || (M <= 16 && N < 32768) || (M <= 32 && N <= 8192))) launch_few_rows(s, a);
-  else if (grid) launch_best_tile(s, a);
-  else hipLaunchKernelGGL(gemm_int8_any_kernel, dim3(unsigned(int64_t(a.tiles_m) * a.tiles_n)), dim3(256), 0, s, a);
+  else launch_best_tile(s, a, grid);
   return check_launch("mk_gemm_int8");
 }

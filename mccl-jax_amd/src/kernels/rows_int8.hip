@@ -308,19 +308,25 @@ int launch_dequantize(hipStream_t s, int64_t rows, int64_t cols, const int8_t* q
   return check_launch("mk_dequantize_rows");
 }
 
-// what every entry point of this file asks of its shape and of one operand of
-// it; "" when it holds
-std::string bad_shape(int type, int64_t rows, int64_t cols) {
+// What every entry point of this file asks of its shape, and of one operand of
+// it; null when it holds.
+const char* bad_shape(int type, int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 1) return "need rows >= 0 and cols >= 1";
   if (type != MK_BF16 && type != MK_F16 && type != MK_F32) return "type must be bf16/f16/f32";
-  if (rows < 0 || rows > kMaxRows || cols < 1) return "need 0 <= rows <= 2^36 and cols >= 1";
-  return "";
+  if (rows > kMaxRows) return "more than 2^36 rows";
+  return nullptr;
 }
-std::string bad_operand(const char* name, const void* p, int bytes, int64_t rows, int64_t cols, int64_t ld,
-                        bool written) {
-  if (!p) return std::string("null ") + name;
-  if (reinterpret_cast<uintptr_t>(p) % bytes) return std::string(name) + " is not aligned to its elements";
-  if (ld < 0 || (written && rows > 1 && ld < cols)) return std::string(name) + ": row pitch below its columns";
-  return "";
+const char* bad_operand(const void* p, int bytes, int64_t rows, int64_t cols, int64_t ld, bool written) {
+  if (!p) return "null ";
+  if (reinterpret_cast<uintptr_t>(p) % bytes) return "not aligned to its elements: ";
+  if (ld < 0 || (written && rows > 1 && ld < cols)) return "row pitch below the columns: ";
+  return nullptr;
+}
+int refuse(const char* entry, const char* why, const char* operand = "") {
+  return fail(MK_ERR_INVALID, std::string(entry) + ": " + why + operand);
+}
+int refuse_shape(const char* entry, const char* why, int64_t rows, int64_t cols) {
+  return fail(rows < 0 || cols < 1 ? MK_ERR_INVALID : MK_ERR_UNSUPPORTED, std::string(entry) + ": " + why);
 }
 
 }  // namespace
@@ -332,51 +338,48 @@ extern "C" int mk_add_rmsnorm_int8(void* stream, int io_type, int64_t rows, int6
                                    const void* residual, int64_t ld_residual, const void* gamma, float eps, void* sum,
                                    int64_t ld_sum, int8_t* q, int64_t ld_q, float* scale) {
   clear_error();
-  const std::string at = "mk_add_rmsnorm_int8: ";
-  std::string bad = bad_shape(io_type, rows, cols);
-  if (!bad.empty()) return fail(rows >= 0 && cols >= 1 ? MK_ERR_UNSUPPORTED : MK_ERR_INVALID, at + bad);
-  if (!(eps >= 0.f)) return fail(MK_ERR_INVALID, at + "eps must be a number >= 0");
+  const char* at = "mk_add_rmsnorm_int8";
+  if (const char* w = bad_shape(io_type, rows, cols)) return refuse_shape(at, w, rows, cols);
+  if (!(eps >= 0.f)) return refuse(at, "eps must be a number >= 0");
   if (rows == 0) return MK_OK;
   const int bytes = dtype_bytes(io_type);
-  bad = bad_operand("x", x, bytes, rows, cols, ld_x, false);
-  if (bad.empty() && residual) bad = bad_operand("residual", residual, bytes, rows, cols, ld_residual, false);
-  if (bad.empty() && residual) bad = bad_operand("sum", sum, bytes, rows, cols, ld_sum, true);
-  if (bad.empty() && gamma) bad = bad_operand("gamma", gamma, bytes, 1, cols, cols, false);
-  if (bad.empty()) bad = bad_operand("q", q, 1, rows, cols, ld_q, true);
-  if (bad.empty()) bad = bad_operand("scale", scale, 4, 1, 1, 1, true);
-  if (!bad.empty()) return fail(MK_ERR_INVALID, at + bad);
+  if (const char* w = bad_operand(x, bytes, rows, cols, ld_x, false)) return refuse(at, w, "x");
+  if (residual) {
+    if (const char* w = bad_operand(residual, bytes, rows, cols, ld_residual, false)) return refuse(at, w, "residual");
+    if (const char* w = bad_operand(sum, bytes, rows, cols, ld_sum, true)) return refuse(at, w, "sum");
+  }
+  if (gamma)
+    if (const char* w = bad_operand(gamma, bytes, 1, cols, cols, false)) return refuse(at, w, "gamma");
+  if (const char* w = bad_operand(q, 1, rows, cols, ld_q, true)) return refuse(at, w, "q");
+  if (const char* w = bad_operand(scale, 4, 1, 1, 1, true)) return refuse(at, w, "scale");
   const RowsArgs a{x, residual, gamma, sum, q, scale, rows, cols, ld_x, ld_residual, ld_sum, ld_q, eps};
-  return residual ? launch_typed<kAddNorm>(as_stream(stream), io_type, a, "mk_add_rmsnorm_int8")
-                  : launch_typed<kNorm>(as_stream(stream), io_type, a, "mk_add_rmsnorm_int8");
+  return residual ? launch_typed<kAddNorm>(as_stream(stream), io_type, a, at)
+                  : launch_typed<kNorm>(as_stream(stream), io_type, a, at);
 }
 
 extern "C" int mk_quantize_rows(void* stream, int io_type, int64_t rows, int64_t cols, const void* x, int64_t ld_x,
                                 int gelu, int8_t* q, int64_t ld_q, float* scale) {
   clear_error();
-  const std::string at = "mk_quantize_rows: ";
-  std::string bad = bad_shape(io_type, rows, cols);
-  if (!bad.empty()) return fail(rows >= 0 && cols >= 1 ? MK_ERR_UNSUPPORTED : MK_ERR_INVALID, at + bad);
+  const char* at = "mk_quantize_rows";
+  if (const char* w = bad_shape(io_type, rows, cols)) return refuse_shape(at, w, rows, cols);
   if (rows == 0) return MK_OK;
-  bad = bad_operand("x", x, dtype_bytes(io_type), rows, cols, ld_x, false);
-  if (bad.empty()) bad = bad_operand("q", q, 1, rows, cols, ld_q, true);
-  if (bad.empty()) bad = bad_operand("scale", scale, 4, 1, 1, 1, true);
-  if (!bad.empty()) return fail(MK_ERR_INVALID, at + bad);
+  if (const char* w = bad_operand(x, dtype_bytes(io_type), rows, cols, ld_x, false)) return refuse(at, w, "x");
+  if (const char* w = bad_operand(q, 1, rows, cols, ld_q, true)) return refuse(at, w, "q");
+  if (const char* w = bad_operand(scale, 4, 1, 1, 1, true)) return refuse(at, w, "scale");
   const RowsArgs a{x, nullptr, nullptr, nullptr, q, scale, rows, cols, ld_x, 0, 0, ld_q, 0.f};
-  return gelu ? launch_typed<kGelu>(as_stream(stream), io_type, a, "mk_quantize_rows")
-              : launch_typed<kPlain>(as_stream(stream), io_type, a, "mk_quantize_rows");
+  return gelu ? launch_typed<kGelu>(as_stream(stream), io_type, a, at)
+              : launch_typed<kPlain>(as_stream(stream), io_type, a, at);
 }
 
 extern "C" int mk_dequantize_rows(void* stream, int out_type, int64_t rows, int64_t cols, const int8_t* q,
                                   int64_t ld_q, const float* scale, void* y, int64_t ld_y) {
   clear_error();
-  const std::string at = "mk_dequantize_rows: ";
-  std::string bad = bad_shape(out_type, rows, cols);
-  if (!bad.empty()) return fail(rows >= 0 && cols >= 1 ? MK_ERR_UNSUPPORTED : MK_ERR_INVALID, at + bad);
+  const char* at = "mk_dequantize_rows";
+  if (const char* w = bad_shape(out_type, rows, cols)) return refuse_shape(at, w, rows, cols);
   if (rows == 0) return MK_OK;
-  bad = bad_operand("q", q, 1, rows, cols, ld_q, false);
-  if (bad.empty()) bad = bad_operand("scale", scale, 4, 1, 1, 1, false);
-  if (bad.empty()) bad = bad_operand("y", y, dtype_bytes(out_type), rows, cols, ld_y, true);
-  if (!bad.empty()) return fail(MK_ERR_INVALID, at + bad);
+  if (const char* w = bad_operand(q, 1, rows, cols, ld_q, false)) return refuse(at, w, "q");
+  if (const char* w = bad_operand(scale, 4, 1, 1, 1, false)) return refuse(at, w, "scale");
+  if (const char* w = bad_operand(y, dtype_bytes(out_type), rows, cols, ld_y, true)) return refuse(at, w, "y");
   hipStream_t s = as_stream(stream);
   if (out_type == MK_BF16) return launch_dequantize<uint16_t>(s, rows, cols, q, ld_q, scale, y, ld_y);
   if (out_type == MK_F16) return launch_dequantize<F16>(s, rows, cols, q, ld_q, scale, y, ld_y);

@@ -815,27 +815,26 @@ extern "C" int mk_sample_rows(void* stream, int io_type, int64_t rows, int64_t v
                               const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
                               const float* min_p, float min_p_all, int index_type, void* tokens, float* logprobs) {
   clear_error();
-  const std::string at = "mk_sample_rows: ";
   if (io_type != MK_BF16 && io_type != MK_F16 && io_type != MK_F32)
-    return fail(MK_ERR_UNSUPPORTED, at + "io_type must be bf16/f16/f32");
+    return fail(MK_ERR_UNSUPPORTED, "mk_sample_rows: io_type must be bf16/f16/f32");
   if (index_type != MK_S32 && index_type != MK_S64)
-    return fail(MK_ERR_UNSUPPORTED, at + "index_type must be s32/s64");
-  if (rows < 0 || vocab < 1) return fail(MK_ERR_INVALID, at + "need rows >= 0 and vocab >= 1");
-  if (vocab > kMaxVocab) return fail(MK_ERR_UNSUPPORTED, at + "more than 2097152 tokens");
-  if (rows >= int64_t(1) << 22) return fail(MK_ERR_UNSUPPORTED, at + "2^22 rows or more");
+    return fail(MK_ERR_UNSUPPORTED, "mk_sample_rows: index_type must be s32/s64");
+  if (rows < 0 || vocab < 1) return fail(MK_ERR_INVALID, "mk_sample_rows: need rows >= 0 and vocab >= 1");
+  if (vocab > kMaxVocab) return fail(MK_ERR_UNSUPPORTED, "mk_sample_rows: more than 2097152 tokens");
+  if (rows >= int64_t(1) << 22) return fail(MK_ERR_UNSUPPORTED, "mk_sample_rows: 2^22 rows or more");
   if (!temperature && !(temperature_all >= 0.f && temperature_all < INFINITY))
-    return fail(MK_ERR_INVALID, at + "temperature must be a number >= 0");
+    return fail(MK_ERR_INVALID, "mk_sample_rows: temperature must be a number >= 0");
   if ((!top_p && top_p_all != top_p_all) || (!min_p && min_p_all != min_p_all))
-    return fail(MK_ERR_INVALID, at + "top_p and min_p must be numbers");
+    return fail(MK_ERR_INVALID, "mk_sample_rows: top_p and min_p must be numbers");
   if (rows == 0) return MK_OK;
-  if (!logits || !u || !tokens) return fail(MK_ERR_INVALID, at + "null pointer");
-  if (ld_logits < 0) return fail(MK_ERR_INVALID, at + "negative row pitch");
+  if (!logits || !u || !tokens) return fail(MK_ERR_INVALID, "mk_sample_rows: null pointer");
+  if (ld_logits < 0) return fail(MK_ERR_INVALID, "mk_sample_rows: negative row pitch");
   if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(io_type) ||
       reinterpret_cast<uintptr_t>(tokens) % dtype_bytes(index_type) || reinterpret_cast<uintptr_t>(u) % 4 ||
       reinterpret_cast<uintptr_t>(temperature) % 4 || reinterpret_cast<uintptr_t>(top_k) % 4 ||
       reinterpret_cast<uintptr_t>(top_p) % 4 || reinterpret_cast<uintptr_t>(min_p) % 4 ||
       reinterpret_cast<uintptr_t>(logprobs) % 4)
-    return fail(MK_ERR_INVALID, at + "an operand is not aligned to its elements");
+    return fail(MK_ERR_INVALID, "mk_sample_rows: an operand is not aligned to its elements");
   int bits = 0;
   while ((int64_t(1) << bits) < vocab) ++bits;
   const SampleArgs a{logits, rows, vocab, ld_logits, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all,
