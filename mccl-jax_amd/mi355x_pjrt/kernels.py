@@ -664,9 +664,11 @@ def sdpa_bwd(q, k, v, o, dout, lse, scale, causal=True, dq=None, dk=None, dv=Non
 
 
 # ------------------------------------------------------------------ eight-bit serving
-# The smallest of these calls are this layer's time too: operands are looked at
-# once by _fits, and what is wrong with one is worked out only for the error
-# (a norm of 1 x 768 with its residual: HOST_BEFORE -> HOST_AFTER us a call).
+# The smallest of these calls are this layer's time: of 7 us for a product of 1 x 768 x
+# 768, 3.4 are the launch, 1 its result's memory and 0.7 ctypes.  So each wrapper
+# looks at its operands in one expression, the usual call's outputs are made where
+# they are needed, and what is wrong with an operand is worked out only for the
+# error (with a helper called for each operand: norm of 1 x 768 10.0 us, now NORM_US).
 _ROW_TYPES = {torch.bfloat16: MK["BF16"], torch.float16: MK["F16"], torch.float32: MK["F32"]}
 
 
@@ -707,12 +709,12 @@ def _result(what, name, t, dtype, shape, dev):
         _refuse(what, name, t, (dtype,), shape, dev)
 
 
-def _refuse_rows(what, name, x):
+def _refuse_rows(what, name, x, dtypes=_ROW_TYPES):
     """The ValueError of a 2-D operand that gives a call its shape and type."""
     dev = _here(what, x, name)
     if x.dim() != 2:
         raise ValueError(f"{what}: {name} must be 2-D")
-    _refuse(what, name, x, _ROW_TYPES, x.shape, dev)
+    _refuse(what, name, x, dtypes, x.shape, dev)
 
 
 def _handle(what, stream, dev):
@@ -733,25 +735,14 @@ def _new(like, stream, dtype, *shape):
         return like.new_empty(*shape, dtype=dtype)
 
 
-def _new_like(x, stream, dtype):
-    """An output of the shape of rows x, which is dense."""
-    if stream is None or not isinstance(stream, torch.cuda.Stream):
-        return torch.empty_like(x, dtype=dtype)
-    with torch.cuda.stream(stream):
-        return torch.empty_like(x, dtype=dtype)
-
-
-def _int8_outputs(what, x, shape, ld, q, scale, dev, stream):
+def _int8_outputs(what, x, shape, q, scale, dev, stream):
     """q, its row pitch and scale: a new q has its rows on 16-byte boundaries, which gemm_int8 multiplies fastest."""
     rows, cols = shape
     if q is None:
         pitch = (cols + 15) // 16 * 16
-        if pitch == cols == ld:
-            q = _new_like(x, stream, torch.int8)
-        else:
-            q = _new(x, stream, torch.int8, rows, pitch)
-            if pitch != cols:
-                q = q[:, :cols]
+        q = _new(x, stream, torch.int8, rows, pitch)
+        if pitch != cols:
+            q = q[:, :cols]
     else:
         _result(what, "q", q, torch.int8, shape, dev)
         pitch = q.stride()[0]
@@ -773,24 +764,38 @@ def add_rmsnorm_int8(x, residual=None, gamma=None, eps=1e-6, sum_out=None, q=Non
     t = _ROW_TYPES.get(dtype)
     if t is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
         _refuse_rows(what, "x", x)
+    rows, cols = shape
     ld = strides[0]
     total, r_ptr, r_ld, s_ptr, s_ld = x, None, 0, None, 0
     if residual is not None:
-        _operand(what, "residual", residual, dtype, shape, dev)
+        r_strides = residual.stride()
+        if residual.dtype is not dtype or residual.shape != shape or residual.get_device() != dev or \
+                (r_strides[1] != 1 and cols > 1):
+            _refuse(what, "residual", residual, (dtype,), shape, dev)
         if sum_out is None:
-            total = _new_like(x, stream, dtype) if ld == shape[1] else _new(x, stream, dtype, *shape)
+            if stream is None and ld == cols:
+                total = torch.empty_like(x)
+            else:
+                total = _new(x, stream, dtype, rows, cols)
         else:
             total = sum_out
             _result(what, "sum_out", total, dtype, shape, dev)
-        r_ptr, r_ld, s_ptr, s_ld = residual.data_ptr(), residual.stride()[0], total.data_ptr(), total.stride()[0]
+        r_ptr, r_ld, s_ptr, s_ld = residual.data_ptr(), r_strides[0], total.data_ptr(), total.stride()[0]
     elif sum_out is not None:
         raise ValueError(f"{what}: sum_out without a residual")
+    g_ptr = None
     if gamma is not None:
-        _operand(what, "gamma", gamma, dtype, shape[1:], dev)
-    q, pitch, scale = _int8_outputs(what, x, shape, ld, q, scale, dev, stream)
-    rc = lib().mk_add_rmsnorm_int8(_handle(what, stream, dev), t, shape[0], shape[1], x.data_ptr(), ld, r_ptr, r_ld,
-                                   None if gamma is None else gamma.data_ptr(), eps, s_ptr, s_ld, q.data_ptr(), pitch,
-                                   scale.data_ptr())
+        if gamma.dtype is not dtype or gamma.shape != (cols,) or gamma.get_device() != dev or \
+                (cols > 1 and gamma.stride()[0] != 1):
+            _refuse(what, "gamma", gamma, (dtype,), (cols,), dev)
+        g_ptr = gamma.data_ptr()
+    if q is None and scale is None and stream is None and ld == cols and cols % 16 == 0:
+        q, pitch, scale = torch.empty_like(x, dtype=torch.int8), cols, x.new_empty(rows, dtype=torch.float32)
+    else:
+        q, pitch, scale = _int8_outputs(what, x, shape, q, scale, dev, stream)
+    handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
+    rc = (_lib._kernels or lib()).mk_add_rmsnorm_int8(handle, t, rows, cols, x.data_ptr(), ld, r_ptr, r_ld, g_ptr, eps,
+                                                      s_ptr, s_ld, q.data_ptr(), pitch, scale.data_ptr())
     if rc:
         _check(rc, "mk_add_rmsnorm_int8")
     return q, scale, total
@@ -805,10 +810,15 @@ def quantize_rows(x, gelu=False, q=None, scale=None, stream=None):
     t = _ROW_TYPES.get(x.dtype)
     if t is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
         _refuse_rows(what, "x", x)
+    rows, cols = shape
     ld = strides[0]
-    q, pitch, scale = _int8_outputs(what, x, shape, ld, q, scale, dev, stream)
-    rc = lib().mk_quantize_rows(_handle(what, stream, dev), t, shape[0], shape[1], x.data_ptr(), ld, 1 if gelu else 0,
-                                q.data_ptr(), pitch, scale.data_ptr())
+    if q is None and scale is None and stream is None and ld == cols and cols % 16 == 0:
+        q, pitch, scale = torch.empty_like(x, dtype=torch.int8), cols, x.new_empty(rows, dtype=torch.float32)
+    else:
+        q, pitch, scale = _int8_outputs(what, x, shape, q, scale, dev, stream)
+    handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
+    rc = (_lib._kernels or lib()).mk_quantize_rows(handle, t, rows, cols, x.data_ptr(), ld, 1 if gelu else 0,
+                                                   q.data_ptr(), pitch, scale.data_ptr())
     if rc:
         _check(rc, "mk_quantize_rows")
     return q, scale
@@ -816,21 +826,26 @@ def quantize_rows(x, gelu=False, q=None, scale=None, stream=None):
 
 def dequantize_rows(q, scale, dtype=torch.bfloat16, out=None, stream=None):
     """The values q * scale that 8-bit rows stand for, in `dtype`."""
-    what, t = "dequantize_rows", _ROW_TYPES.get(dtype)
-    dev = _here(what, q, "q")
+    what = "dequantize_rows"
+    shape, strides, dev, t = q.shape, q.stride(), q.get_device(), _ROW_TYPES.get(dtype)
     if t is None:
         raise ValueError(f"{what}: no rows of {dtype}")
-    if q.dim() != 2:
-        raise ValueError(f"{what}: q must be 2-D")
-    shape = q.shape
-    _operand(what, "q", q, torch.int8, shape, dev)
-    _operand(what, "scale", scale, torch.float32, shape[:1], dev)
+    if q.dtype is not torch.int8 or len(shape) != 2 or dev < 0 or dev != _device() or \
+            (strides[1] != 1 and shape[1] > 1):
+        _refuse_rows(what, "q", q, (torch.int8,))
+    rows, cols = shape
+    if scale.dtype is not torch.float32 or scale.shape != (rows,) or scale.get_device() != dev or \
+            (rows > 1 and scale.stride()[0] != 1):
+        _refuse(what, "scale", scale, (torch.float32,), (rows,), dev)
     if out is None:
-        out = _new_like(q, stream, dtype) if q.stride()[0] == shape[1] else _new(q, stream, dtype, *shape)
+        out = q.new_empty(rows, cols, dtype=dtype) if stream is None else _new(q, stream, dtype, rows, cols)
+        ld = cols
     else:
         _result(what, "out", out, dtype, shape, dev)
-    rc = lib().mk_dequantize_rows(_handle(what, stream, dev), t, shape[0], shape[1], q.data_ptr(), q.stride()[0],
-                                  scale.data_ptr(), out.data_ptr(), out.stride()[0])
+        ld = out.stride()[0]
+    handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
+    rc = (_lib._kernels or lib()).mk_dequantize_rows(handle, t, rows, cols, q.data_ptr(), strides[0], scale.data_ptr(),
+                                                     out.data_ptr(), ld)
     if rc:
         _check(rc, "mk_dequantize_rows")
     return out
@@ -842,22 +857,26 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16, bias=None, relu=
     add_rmsnorm_int8 give it, b the transposed view of weights stored by output
     channel (quantize_rows(w)[0].t()).  a_scale [M], b_scale [N] fp32; the sum
     over k is exact (mk_gemm_int8)."""
-    what, t = "gemm_int8", _ROW_TYPES.get(out_dtype)
-    dev = _here(what, a, "a")
+    what = "gemm_int8"
+    shape_a, shape_b, sa, sb, dev = a.shape, b.shape, a.stride(), b.stride(), a.get_device()
+    t = _ROW_TYPES.get(out_dtype)
     if t is None:
         raise ValueError(f"{what}: no results in {out_dtype}")
-    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[0]:
-        raise ValueError(f"{what}: a [M, K] and b [K, N] expected, got {tuple(a.shape)} and {tuple(b.shape)}")
-    shape_a, sb = a.shape, b.stride()
-    M, Kd = shape_a
-    N = b.shape[1]
-    _operand(what, "a", a, torch.int8, shape_a, dev)
-    if b.dtype is not torch.int8 or b.get_device() != dev or (sb[0] != 1 and Kd > 1):
-        _refuse(what, "b, transposed,", b.t(), (torch.int8,), (N, Kd), dev)
-    _operand(what, "a_scale", a_scale, torch.float32, (M,), dev)
-    _operand(what, "b_scale", b_scale, torch.float32, (N,), dev)
+    if len(shape_a) != 2 or len(shape_b) != 2 or shape_a[1] != shape_b[0]:
+        raise ValueError(f"{what}: a [M, K] and b [K, N] expected, got {tuple(shape_a)} and {tuple(shape_b)}")
+    (M, Kd), N = shape_a, shape_b[1]
+    if a.dtype is not torch.int8 or b.dtype is not torch.int8 or a_scale.dtype is not torch.float32 or \
+            b_scale.dtype is not torch.float32 or dev < 0 or dev != _device() or b.get_device() != dev or \
+            a_scale.get_device() != dev or b_scale.get_device() != dev or a_scale.shape != (M,) or \
+            b_scale.shape != (N,) or (Kd > 1 and (sa[1] != 1 or sb[0] != 1)) or \
+            (M > 1 and a_scale.stride()[0] != 1) or (N > 1 and b_scale.stride()[0] != 1):
+        _here(what, a, "a")
+        _operand(what, "a", a, torch.int8, shape_a, dev)
+        _operand(what, "b, transposed,", b.t(), torch.int8, (N, Kd), dev)
+        _operand(what, "a_scale", a_scale, torch.float32, (M,), dev)
+        _operand(what, "b_scale", b_scale, torch.float32, (N,), dev)
     if out is None:
-        out = _new(a, stream, out_dtype, M, N)
+        out = a.new_empty(M, N, dtype=out_dtype) if stream is None else _new(a, stream, out_dtype, M, N)
         ld = N
     else:
         _result(what, "out", out, out_dtype, (M, N), dev)
@@ -872,8 +891,10 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16, bias=None, relu=
         bias_ptr = bias.data_ptr()
     elif relu:
         raise ValueError(f"{what}: relu goes with a bias")
-    rc = lib().mk_gemm_int8(_handle(what, stream, dev), t, M, N, Kd, a.data_ptr(), a.stride()[0], a_scale.data_ptr(),
-                            b.data_ptr(), sb[1], b_scale.data_ptr(), out.data_ptr(), ld, bias_ptr, epi)
+    handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
+    rc = (_lib._kernels or lib()).mk_gemm_int8(handle, t, M, N, Kd, a.data_ptr(), sa[0], a_scale.data_ptr(),
+                                               b.data_ptr(), sb[1], b_scale.data_ptr(), out.data_ptr(), ld, bias_ptr,
+                                               epi)
     if rc:
         _check(rc, "mk_gemm_int8")
     return out
@@ -923,9 +944,10 @@ def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, 
         m_all = min_p
     token = _new(logits, stream, index_dtype, shape[0])
     logprob = _new(logits, stream, torch.float32, shape[0]) if with_logprob else None
-    rc = lib().mk_sample_rows(_handle(what, stream, dev), mk, shape[0], shape[1], logits.data_ptr(), ld, u.data_ptr(), t,
-                              t_all, k, k_all, p, p_all, m, m_all, _TORCH_TO_MK[index_dtype], token.data_ptr(),
-                              _ptr(logprob))
+    handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
+    rc = (_lib._kernels or lib()).mk_sample_rows(handle, mk, shape[0], shape[1], logits.data_ptr(), ld, u.data_ptr(), t,
+                                                 t_all, k, k_all, p, p_all, m, m_all, _TORCH_TO_MK[index_dtype],
+                                                 token.data_ptr(), _ptr(logprob))
     if rc:
         _check(rc, "mk_sample_rows")
     return token, logprob
