@@ -668,7 +668,7 @@ def sdpa_bwd(q, k, v, o, dout, lse, scale, causal=True, dq=None, dk=None, dv=Non
 # 768, 3.4 are the launch, 1 its result's memory and 0.7 ctypes.  So each wrapper
 # looks at its operands in one expression, the usual call's outputs are made where
 # they are needed, and what is wrong with an operand is worked out only for the
-# error (with a helper called for each operand: norm of 1 x 768 10.0 us, now NORM_US).
+# error (with a helper called for each operand: norm of 1 x 768 10.0 us, now 8.0).
 _ROW_TYPES = {torch.bfloat16: MK["BF16"], torch.float16: MK["F16"], torch.float32: MK["F32"]}
 
 

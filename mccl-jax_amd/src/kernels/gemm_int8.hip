@@ -74,10 +74,11 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm 
   const int c = lane & 15, g = lane >> 4;
   const int kw = p.k_waves, k_wave = wave % kw, blocks = NW / kw;  // of columns, in this workgroup
   const int64_t n_first = int64_t(blockIdx.x) * blocks * NT, n0 = n_first + wave / kw * NT;
+  const int64_t m_first = int64_t(blockIdx.y) * 16 * MT;
   // rows past the operands' repeat the last and are not stored
   const int8_t *ap[MT], *bp[VN];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) ap[m] = p.A + std::min<int64_t>(16 * m + c, p.M - 1) * p.lda + 32 * g;
+  for (int m = 0; m < MT; ++m) ap[m] = p.A + std::min<int64_t>(m_first + 16 * m + c, p.M - 1) * p.lda + 32 * g;
 #pragma unroll
   for (int j = 0; j < VN; ++j) bp[j] = p.B + std::min<int64_t>(n0 + 16 * j + c, p.N - 1) * p.ldb + 32 * g;
   struct Step {
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(const Int8Gemm 
       const int row = e / width, col = e % width, w0 = col / NT * kw;
       int sum = red[w0][row][col % NT];
       for (int w = 1; w < kw; ++w) sum += red[w0 + w][row][col % NT];
-      const int64_t mrow = 16 * m + row, nc = n_first + col;
+      const int64_t mrow = m_first + 16 * m + row, nc = n_first + col;
       if (mrow < p.M && nc < p.N)
         store_from_f32(p.C, mrow * p.ldc + nc, p.c_type, finish(p, sum, p.a_scale[mrow], nc));
     }
@@ -179,17 +180,10 @@ void launch_rows(hipStream_t s, Int8Gemm a, int k_waves) {
   auto go = [&](auto nw) {
     constexpr int NW = decltype(nw)::value;
     const int64_t per = NW / a.k_waves;
-    hipLaunchKernelGGL((gemm_int8_rows_kernel<VN, MT, NW, kD>), dim3(unsigned((blocks + per - 1) / per)), dim3(64 * NW), 0, s, a);
+    hipLaunchKernelGGL((gemm_int8_rows_kernel<VN, MT, NW, kD>), dim3(unsigned((blocks + per - 1) / per), unsigned((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * NW), 0, s, a);
   };
   if (a.k_waves == 16) go(Int<kMost>{});
   else go(Int<8>{});
-}
-
-template <int VN>
-void launch_rows(hipStream_t s, const Int8Gemm& a, int k_waves) {
-  if (a.M <= 16) launch_rows<VN, 1>(s, a, k_waves);
-  else if (a.M <= 32) launch_rows<VN, 2>(s, a, k_waves);
-  else launch_rows<VN, 4>(s, a, k_waves);
 }
 
 // Waves enough to fill the chip, from the columns (64 or 32 a wave where they are
@@ -197,14 +191,33 @@ void launch_rows(hipStream_t s, const Int8Gemm& a, int k_waves) {
 // k: 16 x 4096 x 16384 (M x K x N) 16: 20.6 / 20.9 (2, 4), 32: 17.5 / 18.4 (4, 8),
 // 64: 16.3 (8); 16 x 512 x 16384 16: 4.8 (4), 32: 5.2 (4); 16 x 4096 x 4096 16: 17.1,
 // 10.1, 6.9, 6.9 (2, 4, 8, 16), 32: 8.5 (8); 1 x 768 x 2304 16: 3.1 (8).
+template <int VN>
 void launch_few_rows(hipStream_t s, const Int8Gemm& a) {
-  const int vn = a.N >= 12288 && a.K >= 2048 ? 4 : a.N >= 8192 ? 2 : 1;
-  const int64_t blocks = (a.N + 16 * vn - 1) / (16 * vn);
+  const int64_t blocks = (a.N + 16 * VN - 1) / (16 * VN);
   int kw = 1;
-  while (kw < 16 && kw * blocks < (vn == 1 ? 4096 : 2048) && kw * kStep < a.K) kw *= 2;
-  if (vn == 4) launch_rows<4>(s, a, kw);
-  else if (vn == 2) launch_rows<2>(s, a, kw);
-  else launch_rows<1>(s, a, kw);
+  while (kw < 16 && kw * blocks < (VN == 1 ? 4096 : 2048) && kw * kStep < a.K) kw *= 2;
+  if (a.M <= 16) launch_rows<VN, 1>(s, a, kw);
+  else if (a.M <= 32) launch_rows<VN, 2>(s, a, kw);
+  else launch_rows<VN, 4>(s, a, kw);
+}
+void launch_few_rows(hipStream_t s, const Int8Gemm& a) {
+  if (a.N >= 12288 && a.K >= 2048) launch_few_rows<4>(s, a);
+  else if (a.N >= 8192) launch_few_rows<2>(s, a);
+  else launch_few_rows<1>(s, a);
+}
+
+// A small C: 16 x 16 blocks, k over the waves of a workgroup each.  Where those find
+// a CU each they are ahead of the tiles, whose few workgroups have all of k in
+// series; off the 16-byte grid for longer.  us, so / else: 64 x 16384 x 256 16.8 / 27.6;
+// 256 x 4096 x 256 6.7 / 9.6; 128 x 2048 x 512 (256 blocks) 4.8 / 6.5; 106 x 4720 x 857
+// (378) 10.3 / 11.0; 128 x 4096 x 1024 (512) 11.2 / 9.7; 42 x 6055 x 208 18 / 37.
+bool small_c(const Int8Gemm& a, bool grid) {
+  return (a.M + 15) / 16 * ((a.N + 15) / 16) <= (grid ? 256 : 512);
+}
+void launch_small(hipStream_t s, const Int8Gemm& a) {
+  int kw = 1;
+  while (kw < 16 && kw * kStep < a.K) kw *= 2;
+  launch_rows<1, 1>(s, a, kw);
 }
 
 // ---------------------------------------------------------------- tiles
@@ -629,7 +642,11 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
              c_type, epilogue, 0};
   hipStream_t s = as_stream(stream);
   const bool grid = K > 0 && on_grid(A, M, K, a_ms) && on_grid(B, N, K, b_ns);
-  if (M <= 64 && (!grid || (M <= 16 && N < 32768) || (M <= 32 && N <= 8192))) launch_few_rows(s, a);
+  // few rows off the grid, or where the weights alone are the work; from 17 rows or
+  // 32768 columns on the tiles share A's reads (32 x 4096 x 16384 19.1 us, 22 so; 16 x
+  // 768 x 50257 11.4, 14.1; 32 x 4096 x 4096 9.7, 9.2)
+  if (small_c(a, grid)) launch_small(s, a);
+  else if (M <= 64 && (!grid || (M <= 16 && N < 32768) || (M <= 32 && N <= 8192))) launch_few_rows(s, a);
   else launch_best_tile(s, a, grid);
   return check_launch("mk_gemm_int8");
 }
