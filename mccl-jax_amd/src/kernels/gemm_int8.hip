@@ -624,9 +624,9 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
     return fail(MK_ERR_UNSUPPORTED, "mk_gemm_int8: c_type must be bf16/f16/f32");
   if (M < 0 || N < 0 || K < 0) return fail(MK_ERR_INVALID, "mk_gemm_int8: negative shape");
   if (K > kMaxK) return fail(MK_ERR_UNSUPPORTED, "mk_gemm_int8: K past 131071: the 32-bit sums could overflow");
-  // a workgroup of 256 threads per 64 x 64 tile, below HIP's 2^32 threads
-  if (M >> 30 || N >> 30 || (M + 63) / 64 * ((N + 63) / 64) >= int64_t(1) << 24)
-    return fail(MK_ERR_UNSUPPORTED, "mk_gemm_int8: 2^24 or more tiles of 64 x 64");
+  // a workgroup of 256 threads per 64 x 64 tile, or of 512 per two, below HIP's 2^32 threads
+  if (M >> 30 || N >> 30 || (M + 63) / 64 * ((N + 63) / 64) >= (int64_t(1) << 24) - 1)
+    return fail(MK_ERR_UNSUPPORTED, "mk_gemm_int8: 2^24 - 1 or more tiles of 64 x 64");
   const int epi = epilogue & 3;
   if (epilogue < 0 || epilogue > 6 || epi == 3 || (epilogue == 4))
     return fail(MK_ERR_INVALID, "mk_gemm_int8: epilogue must be 0, 1, 2, 5 or 6");

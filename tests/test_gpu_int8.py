@@ -196,7 +196,8 @@ SHAPES = [
     (17, 128, 1000), (33, 640, 96), (48, 48, 48), (64, 2048, 257), (65, 2048, 256), (100, 130, 515), (127, 64, 128),
     (128, 128, 128), (129, 192, 130), (200, 1024, 4100), (255, 272, 384), (256, 256, 256), (257, 1040, 640),
     (300, 31, 300), (333, 768, 1003), (512, 2064, 512), (1000, 100, 1000), (1024, 1008, 2048), (2048, 4096, 768),
-    (1, 16, 70001), (3, 131071, 5), (70, 131071, 70), (2500, 16, 64),
+    (1, 16, 70001), (3, 131071, 5), (70, 131071, 70), (2500, 16, 64), (128, 512, 4096), (2048, 768, 2304),
+    (40, 768, 20011), (64, 272, 9000), (300, 1001, 2000), (130, 4097, 3001),
 ]
 
 
@@ -477,6 +478,90 @@ def test_the_operators_together(K, rows, d, ff, vocab):
             eager = block(*fresh[i])
             for n in eager:
                 assert torch.equal(outs[i][n], eager[n]), (step, i, n)
+
+
+def test_sample_rows_where_a_step_ends_at_zero(K):
+    """The largest value a whole number of 64ths of a power of two above the others, which lie at and around 0: the
+    step they are in ends there to within roundings.  On the list (5000 tokens), past it (20000), one step's 400."""
+    tiny = torch.tensor([0.0, 1e-30, -1e-30, 1e-45, -1e-45, -0.0])
+    for vocab in (400, 5000, 20000):
+        g = torch.Generator().manual_seed(vocab)
+        x = tiny[torch.randint(0, 6, (24, vocab), generator=g)]
+        t = torch.tensor([1.0, 0.7, 3.0, 1e-3])[torch.arange(24) % 4]
+        steps = torch.tensor([1, 2, 64, 65, 100, 128])[torch.arange(24) // 4]
+        x[torch.arange(24), torch.randint(0, vocab, (24,), generator=g)] = (steps / 64 * math.log(2.0) * t.double()).float()
+        print(f"case: sample_rows, steps ending at 0, {vocab}", flush=True)
+        for p in (0.31, 0.9):
+            _check_sample(K, x.cuda(), _u(vocab, 24), t.cuda(), 0, p)
+            _check_sample(K, x.cuda(), _u(vocab, 24), t.cuda(), 0, p, 0.2)
+
+
+def test_sample_rows_flat_rows(K):
+    """All tokens alike, more than a list holds; far from 0; at the largest temperatures, masked with -inf or the lowest value."""
+    x = torch.full((6, 160001), 3.0, dtype=torch.bfloat16, device="cuda")
+    for k, p, m in ((50001, 1.0, 0.0), (0, 0.31, 0.0), (50001, 0.31, 0.5), (0, 1.0, 1.0), (0, 1.0, 1e-30), (3, 1.0, 0.0)):
+        print(f"case: sample_rows, flat, {k} {p} {m}", flush=True)
+        _check_sample(K, x, _u(k, 6), 1.0, k, p, m)
+    x = _normal(31, (16, 9001)) + 1e6
+    for p, m in ((0.9, 0.0), (1.0, 1e-30), (1.0, 0.37), (0.5, 0.2)):
+        _check_sample(K, x, _u(32, 16), 0.8, 0, p, m)
+    low = torch.finfo(torch.float32).min
+    x = torch.tensor([0.0, low, -math.inf, -low])[torch.randint(0, 4, (16, 3001), generator=torch.Generator().manual_seed(5))]
+    for k, p, m in ((0, 0.97, 0.0), (0, 1.0, 1e-45), (2900, 0.97, 1e-45), (0, 0.1, 0.3)):
+        _check_sample(K, x.cuda(), _u(33, 16), -low, k, p, m)
+
+
+def test_rows_far_apart(K):
+    """Rows whose offsets pass 2^31 bytes and 2^31 elements, of every operand."""
+    def far(t, pitch):
+        v = torch.empty((t.shape[0] - 1) * pitch + t.shape[1] + 64, dtype=t.dtype, device="cuda")
+        v = v.as_strided(t.shape, (pitch, 1))
+        return v.copy_(t)
+
+    for Kd, off in ((256, 0), (250, 1)):
+        for M, N in ((20, 70), (70, 200)):
+            a, w, sa, sb = _int8(1, (M, Kd)), _int8(2, (N, Kd)), _scales(1, M), _scales(2, N)
+            want = K.gemm_int8(a, sa, w.t(), sb)
+            print(f"case: gemm_int8 far apart {M} x {Kd} x {N}", flush=True)
+            assert torch.equal(K.gemm_int8(far(a, (1 << 27) + off), sa, w.t(), sb), want)
+            assert torch.equal(K.gemm_int8(a, sa, far(w, (1 << 25) + off).t(), sb), want)
+            out = far(want, (1 << 26) + off)
+            K.gemm_int8(a, sa, w.t(), sb, out=out.zero_())
+            assert torch.equal(out, want)
+    x, u = _normal(3, (5, 1001), torch.bfloat16), _u(4, 5)
+    v = far(x, (1 << 29) + 1)
+    assert all(torch.equal(i, j) for i, j in zip(K.sample_rows(v, u, 0.8, 50, 0.9), K.sample_rows(x, u, 0.8, 50, 0.9)))
+    q, scale, total = K.add_rmsnorm_int8(x, x)
+    s = far(x, (1 << 29) + 1)
+    got = K.add_rmsnorm_int8(v, v, q=far(q, (1 << 30) + 1), sum_out=s)
+    assert got[2] is s and all(torch.equal(i, j) for i, j in zip(got, (q, scale, total)))
+    assert torch.equal(K.dequantize_rows(got[0], scale), K.dequantize_rows(q, scale))
+
+
+def test_one_row_of_weights_for_every_column(K):
+    a, w, sa, sb = _int8(1, (100, 768)), _int8(2, (1, 768)), _scales(1, 100), _scales(2, 600)
+    want = K.gemm_int8(a, sa, w.expand(600, 768).contiguous().t(), sb)
+    assert torch.equal(K.gemm_int8(a, sa, w.expand(600, 768).t(), sb), want)
+    want = K.gemm_int8(a[:1].expand(100, 768).contiguous(), sa, w.expand(600, 768).contiguous().t(), sb)
+    assert torch.equal(K.gemm_int8(a[:1].expand(100, 768), sa, w.expand(600, 768).t(), sb), want)
+
+
+def test_two_streams_at_once(K):
+    """Nothing is shared between calls: the same results with every call in flight on two streams."""
+    blocks = [_Block(K, rows, 512, 1024, 5003) for rows in (40, 300)]
+    ins = [(_normal(i, (b.rows, 512), torch.bfloat16), _normal(i + 9, (b.rows, 512), torch.bfloat16), _u(i, b.rows))
+           for i, b in enumerate(blocks)]
+    want = [b(*v) for b, v in zip(blocks, ins)]
+    streams = [torch.cuda.Stream() for _ in blocks]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        got.append([b(*v, stream=s) for b, v, s in zip(blocks, ins, streams)])
+    torch.cuda.synchronize()
+    for both in got:
+        for o, w in zip(both, want):
+            for n in w:
+                assert torch.equal(o[n], w[n]), n
 
 
 def test_refusals(K):
