@@ -8,9 +8,9 @@
 //
 // What is kept is one cut (key, ties): the tokens whose x is above a value, and
 // the first `ties` of those equal to it, in the order of the vocabulary.  So no
-// row is sorted: the cut's value is found digit by digit from a histogram of
-// counts (top-k) or of weights (top-p) over x's bits, taken as a whole number
-// that orders as x does.
+// row is sorted: in general the cut's value is found digit by digit from a histogram
+// of counts (top-k) or of weights (top-p) over x's bits, taken as a whole number that
+// orders as x does.
 //
 // Weights are whole numbers: w 2^s, with 2^z to 2^-33 of itself in 64 bits, s
 // such that a row's sum stays below 2^63 (46 bits for 50257 tokens).  Their sums
@@ -411,13 +411,14 @@ struct Row {
     clear<true>(sh, 0);
     // a little past the step's ends: what is past them does no harm on the list
     const float end = float(top - (step + 1) / 64.0 / per), begin = float(top - step / 64.0 / per);
-    const float lo = end - fabsf(end) * 0x1p-22f;
+    const float slack = float(fabs(top)) * 0x1p-40f, lo = end - fabsf(end) * 0x1p-22f - slack;
     whole = make_list(sh, lo, INFINITY);
     if (whole && listed <= kFew) return target;
     if (!whole) {  // the step's tokens alone
       clear<true>(sh, 0);
-      if (!make_list(sh, lo, begin + fabsf(begin) * 0x1p-22f)) return target;
+      if (!make_list(sh, lo, begin + fabsf(begin) * 0x1p-22f + slack)) return target;
     }
+    __syncthreads();  // everyone has read the list's length
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     over(sh, [&](int, uint32_t key) {
@@ -485,7 +486,8 @@ struct Row {
         const uint32_t least = prefix << by, width = (1u << by) - 1;
         for (int only = 0; only < 2 && listed < 0; ++only) {
           clear<MASS>(sh, 0);
-          whole = make_list(sh, O::of_key(max(least, O::key(O::none()))), only ? O::of_key(least + width) : INFINITY) && !only;
+          const float from = O::of_key(max(least, O::key(O::none()))), to = only ? O::of_key(least + width) : INFINITY;
+          whole = make_list(sh, from, to) && !only;
         }
       }
     }
@@ -693,7 +695,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     if (r.cut == 0 && r.listed < 0 && least > 0) {  // min-p alone: what may be above it, a little below it
       r.template clear<true>(sh, 0);
       const double lo = r.top + double(log2f(fminf(min_p, 1.f))) / r.per;
-      r.whole = r.make_list(sh, float(lo - fabs(lo) * 0x1p-20 - 0x1p-20 / r.per), INFINITY);
+      r.whole = r.make_list(sh, float(lo - (fabs(lo) + fabs(r.top)) * 0x1p-20 - 0x1p-10 / r.per), INFINITY);
     }
     if (r.whole && r.listed <= kFew && r.cut == 0)
       return take_few(p, r, sh, row, u, t, few_k ? k : int64_t(kFew), target, top_p, least);
