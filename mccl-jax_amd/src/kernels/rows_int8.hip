@@ -13,11 +13,13 @@
 // square in 32.  The maximum is taken over the bits of |t| as whole numbers,
 // where NaN is above infinity is above every number, so neither is lost.
 //
-// Bound: HBM, each operand once.  A team of W waves has a row; its lanes hold
-// up to NV chunks of 16 bytes each.  The last chunk of a row that is no whole
-// number of chunks is the row's last 16 bytes: what it shares with the chunk
-// before it is left out of the sum and written twice with the same values
-// (after every load of the row, so that outputs may be inputs).
+// Bound: HBM, each operand once: the norm of 8192 x 4096 in bf16 (235 MB) takes 38 us,
+// rounding 50257 x 768 of fp32 (193 MB) 34 us, the way back 36 us, where a copy of
+// 200 MiB moves 5.4 MB a us.  One row is a launch and two round trips to memory: 768 in
+// 2.7 us.  A team of W waves has a row; its lanes hold up to NV chunks of 16 bytes each.
+// The last chunk of a row that is no whole number of chunks is the row's last 16 bytes:
+// what it shares with the chunk before it is left out of the sum and written twice
+// with the same values (after every load of the row, so that outputs may be inputs).
 #include "mk_common.h"
 
 #include <algorithm>
@@ -227,29 +229,35 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rows_int8_any_kernel(co
   if (t == 0) p.scale[row] = step.y;
 }
 
-// y = q scale: 8 elements a lane and step, the row's last ones one by one
+// y = q scale: a lane writes 16 bytes of four places of the row in a step, all four
+// loaded first; the elements behind the last whole chunk one by one
 template <typename T, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void dequantize_kernel(int64_t rows, int64_t cols, const int8_t* q,
                                                                            int64_t ld_q, const float* scale, T* y,
                                                                            int64_t ld_y) {
-  constexpr int S = 64 * W, kRows = W == 1 ? 4 : 1;
-  struct __attribute__((packed, aligned(1))) In { int8_t v[8]; };
-  struct __attribute__((packed, aligned(sizeof(T)))) Out { T v[8]; };
+  constexpr int E = kE<T>, S = 64 * W, kRows = W == 1 ? 4 : 1, kSteps = 4;
+  struct __attribute__((packed, aligned(1))) In { int8_t v[E]; };
   const int t = int(threadIdx.x) % S;
   const int64_t row = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * kRows + int(threadIdx.x) / S;
   if (row >= rows) return;
   const float f = scale[row];
   q += row * ld_q;
   y += row * ld_y;
-  const int64_t whole = cols / 8;
-  for (int64_t i = t; i < whole; i += S) {
-    const In in = *reinterpret_cast<const In*>(q + 8 * i);
-    Out out;
+  const int64_t whole = cols / E;
+  for (int64_t i = t; i < whole; i += S * kSteps) {
+    In in[kSteps];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out.v[e] = narrow<T>(float(in.v[e]) * f);
-    *reinterpret_cast<Out*>(y + 8 * i) = out;
+    for (int v = 0; v < kSteps; ++v) in[v] = *reinterpret_cast<const In*>(q + E * std::min(i + S * v, whole - 1));
+#pragma unroll
+    for (int v = 0; v < kSteps; ++v) {
+      if (i + S * v >= whole) continue;
+      Chunk<T> out;
+#pragma unroll
+      for (int e = 0; e < E; ++e) out.v[e] = narrow<T>(float(in[v].v[e]) * f);
+      *reinterpret_cast<Chunk<T>*>(y + E * (i + S * v)) = out;
+    }
   }
-  if (const int64_t c = 8 * whole + t; c < cols) y[c] = narrow<T>(float(q[c]) * f);
+  if (const int64_t c = E * whole + t; c < cols) y[c] = narrow<T>(float(q[c]) * f);
 }
 
 // teams of W waves over `rows` rows: below HIP's 2^32 threads an axis
@@ -265,6 +273,13 @@ void launch_held(hipStream_t s, const RowsArgs& a) {
   hipLaunchKernelGGL((rows_int8_kernel<T, M, W, NV>), row_grid<W>(a.rows), dim3(W == 1 ? 256 : 64 * W), 0, s, a);
 }
 
+// Teams by the row's chunks: as few waves as hold the row in 2 to 4 chunks a lane, more
+// where they would leave CUs idle.  us, for W x NV, bf16: norm of 8192 x 768 1 x 2: 11.2,
+// 2 x 1: 12.7, 4 x 1: 18.6; of 8192 x 2048 2 x 2: 21.2, 1 x 4: 22.2, 4 x 1: 22.2; of 256 x
+// 2048 2 x 2: 3.8, 4 x 1: 3.6; of 8192 x 4096 4 x 2: 38.1, 1 x 8: 42.9, 8 x 1: 43.8, 16 x 1:
+// 72; of 1 x 8192 4 x 4: 3.6, 8 x 2: 3.6, 16 x 1: 4.0; of 4096 x 16384 8 x 4: 91, 4 x 8: 88,
+// 16 x 2: 99; of 64 x 16384 5.5, 6.0, 6.0.  50257 x 768 of fp32 to 8 bits 2 x 2: 34, 4 x 1: 46.
+// Longer rows than 16 x 4 holds are read twice: 1024 x 16384 of fp32 47 us held, 69 so.
 template <typename T, Mode M>
 int launch_rows(hipStream_t s, const RowsArgs& a, const char* what) {
   const int64_t chunks = (a.cols + kE<T> - 1) / kE<T>;
@@ -273,15 +288,12 @@ int launch_rows(hipStream_t s, const RowsArgs& a, const char* what) {
   else if (chunks > 4096)
     hipLaunchKernelGGL((rows_int8_any_kernel<T, M, 16>), row_grid<16>(a.rows), dim3(1024), 0, s, a);
   else if (chunks <= 64) launch_held<T, M, 1, 1>(s, a);
-  else if (chunks <= 128 && a.rows >= 512) launch_held<T, M, 1, 2>(s, a);
-  else if (chunks <= 256 && a.rows >= 1024) launch_held<T, M, 1, 4>(s, a);
-  else if (chunks <= 512 && a.rows >= 2048) launch_held<T, M, 1, 8>(s, a);
+  else if (chunks <= 128) launch_held<T, M, 1, 2>(s, a);
+  else if (chunks <= 256 && a.rows >= 1024) launch_held<T, M, 2, 2>(s, a);
   else if (chunks <= 256) launch_held<T, M, 4, 1>(s, a);
   else if (chunks <= 512) launch_held<T, M, 4, 2>(s, a);
-  else if (chunks <= 1024 && a.rows >= 512) launch_held<T, M, 4, 4>(s, a);
-  else if (chunks <= 2048 && a.rows >= 512) launch_held<T, M, 4, 8>(s, a);
-  else if (chunks <= 1024) launch_held<T, M, 16, 1>(s, a);
-  else if (chunks <= 2048) launch_held<T, M, 16, 2>(s, a);
+  else if (chunks <= 1024) launch_held<T, M, 4, 4>(s, a);
+  else if (chunks <= 2048) launch_held<T, M, 8, 4>(s, a);
   else launch_held<T, M, 16, 4>(s, a);
   return check_launch(what);
 }
@@ -296,10 +308,13 @@ int launch_typed(hipStream_t s, int io_type, const RowsArgs& a, const char* what
 template <typename T>
 int launch_dequantize(hipStream_t s, int64_t rows, int64_t cols, const int8_t* q, int64_t ld_q, const float* scale,
                       void* y, int64_t ld_y) {
-  if (cols <= 512 || (cols <= 4096 && rows >= 1024))
+  // us, 1, 4 and 16 waves a row: 8192 x 2048 of bf16 11.3, 14.8, 17.5; 8192 x 4096 21.6,
+  // 20.0, 27.5; 1 x 8192 3.1, 2.1, 2.2; 64 x 40000 16.1, 5.8, 4.6; 50257 x 768 of fp32 36, 43, 80
+  const int64_t chunks = cols / kE<T>;
+  if (chunks <= 256)
     hipLaunchKernelGGL((dequantize_kernel<T, 1>), row_grid<1>(rows), dim3(256), 0, s, rows, cols, q, ld_q, scale,
                        static_cast<T*>(y), ld_y);
-  else if (cols <= 2048 || rows >= 512)
+  else if (chunks <= 2048)
     hipLaunchKernelGGL((dequantize_kernel<T, 4>), row_grid<4>(rows), dim3(256), 0, s, rows, cols, q, ld_q, scale,
                        static_cast<T*>(y), ld_y);
   else

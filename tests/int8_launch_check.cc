@@ -69,7 +69,10 @@ int main() {
       for (int t : {MK_BF16, MK_F16, MK_F32}) {
         const std::string at = " of " + std::to_string(rows) + " x " + std::to_string(cols);
         launched("norm" + at, mk_add_rmsnorm_int8(nullptr, t, rows, cols, X, cols, X, cols, X, 1e-6f, Y, cols, i8(Y), cols, f32(Y)));
-        const uint64_t teams = g_x * g_y * (g_block_size == 256 && g_kernel.find("Li1E") != std::string::npos ? 4 : 1);
+// waves a row: the number after the mode, ...ModeE0ELi<W>E
+        const int waves = std::atoi(g_kernel.c_str() + g_kernel.find("ModeE") + 9);
+        const uint64_t teams = g_x * g_y * (waves == 1 ? 4 : 1);
+        expect(g_block_size == (waves == 1 ? 256 : 64 * waves), "norm" + at + ": threads of " + g_kernel);
         expect(teams >= uint64_t(rows), "norm" + at + ": rows left out");
         launched("rows" + at, mk_quantize_rows(nullptr, t, rows, cols, X, cols, 1, i8(Y), cols, f32(Y)));
         launched("values" + at, mk_dequantize_rows(nullptr, t, rows, cols, i8(X), cols, f32(X), Y, cols));
