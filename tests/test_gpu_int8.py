@@ -511,6 +511,16 @@ def test_sample_rows_flat_rows(K):
         _check_sample(K, x.cuda(), _u(33, 16), -low, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_rows_where_the_list_overflows(K, dtype):
+    """More kept than a list holds: the cut's step alone on it, of few tokens (spread), of many (16-bit values, narrow) and past it too."""
+    for vocab, std in ((130001, 3.0), (130001, 1.0), (40000, 0.05), (150000, 0.003)):
+        print(f"case: sample_rows, long lists, {vocab} {std} {dtype}", flush=True)
+        x = _normal(vocab, (6, vocab), dtype, std)
+        for p, m in ((0.95, 0.0), (0.5, 0.0), (0.9, 0.3)):
+            _check_sample(K, x, _u(41, 6), torch.tensor([1.0, 1.0, 0.8, 1.3, 1.0, 2.0], device="cuda"), 0, p, m)
+
+
 def test_rows_far_apart(K):
     """Rows whose offsets pass 2^31 bytes and 2^31 elements, of every operand."""
     def far(t, pitch):
