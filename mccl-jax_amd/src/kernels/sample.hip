@@ -23,8 +23,9 @@
 //   top-k: the k-th largest of the lanes' own maxima is below the row's k-th
 //   largest value, so what is at or above it holds the first k and is seldom much
 //   more: a second pass puts those tokens into a list in LDS;
-//   top-p alone: a second pass for the weights by 64ths of a power of two, a third
-//   for the list of the tokens from the cut's step up;
+//   top-p alone: a second pass for the weights by 64ths of a power of two, a third for
+//   the list of the tokens from the cut's step up or, where they are many, for their
+//   weights by 512 tokens;
 //   min-p alone: a second pass for the list of what is above it;
 //   no limit: a second pass for the weights of each 512 tokens.
 // What remains happens on the list (12288 tokens; where it is longer the row is read
@@ -34,7 +35,7 @@
 //
 // Bound: one CU's work on a row.  50257 tokens, one row of bf16 / 256 rows of fp32,
 // us: greedy 7.0 / 12.9 (the first pass: one CU takes in a line every 8 clocks),
-// top-k 50 and top-p 0.9 15 / 24 (two passes and 20 barriers), top-p 0.95 39 / 48 and
+// top-k 50 and top-p 0.9 15 / 24 (two passes and 20 barriers), top-p 0.95 39 / 49 and
 // no limit 20 / 28 (an exponential in 64 bits for each token, 10 us a pass).  Loops are
 // kept short on purpose: with the row in registers and each pass unrolled over it
 // the same steps took 35, 59 and 34 us, waiting for instructions.
@@ -53,7 +54,7 @@ constexpr int kLane = 8;                    // elements a lane takes at once
 constexpr int kChunk = kLane * kWave;       // elements a wave takes at once
 constexpr int kList = 12288;                // tokens of the list
 constexpr int kFew = 256;                   // ... of one that is ranked by comparing each with each
-constexpr int kStep = 512;                  // tokens of a step of list_top that are compared so
+constexpr int kStep = 512;                  // tokens of a step of find_top that are compared so
 constexpr int64_t kMaxVocab = int64_t(kBins) * kChunk;
 
 typedef unsigned long long u64;
@@ -131,12 +132,14 @@ struct Shared {
     Few few;
   };
   uint32_t key[kList], index[kList];  // the list
+  u64 step_weight[kStep];            // of a step's tokens
+  uint32_t step_key[kStep], step_chunk[kStep];
   u64 wave_sum[2][kWaves];
   uint32_t n;
   // what the one thread that found a place leaves for the others
   int found;
   u64 before;
-  uint32_t ties_before;
+  uint32_t ties_before, kept, in_step;
 };
 
 // v of the lane that a DPP control word names, 0 where there is none
@@ -231,6 +234,7 @@ struct Row {
   u64 ties;
   int listed;       // tokens in the list, -1: there is none
   bool whole;       // the list holds everything that is kept
+  bool summed;      // sh.mass and sh.count hold what is kept of each chunk
 
   // log2 of a weight, at least -64 (weights below 2^-52 are 0)
   __device__ inline double log2_weight(float v) const { return max((double(v) - top) * per, -64.0); }
@@ -390,11 +394,15 @@ struct Row {
   // which 64th of a power of two below the largest a weight is
   static __device__ inline int step_of(double z) { return min(int(-64.0 * z), kBins - 1); }
   // Top-p of a row without a top-k: its weights by their logarithm, in steps of
-  // 1 / 64, say in which step the cut is.  The list of the tokens from that step up
-  // holds all that is kept; few are in the step itself, and are compared with each
-  // other.  Returns the weight that the cut reaches where the cut is still
-  // to be found: on a short list, or where many are in the step or on no list.
-  __device__ inline u64 list_top(Shared& sh, float top_p) {
+  // 1 / 64, say in which step the cut is, and about how many tokens are above it.  Few
+  // are in the step itself, and are compared with each other.  Where little is kept, a
+  // list of the tokens from that step up holds all of it; else another pass sums the
+  // weights above the step by chunk and puts the step's own tokens aside.  Returns the
+  // weight that the cut reaches where the cut is still to be found: on a short list, or
+  // where many are in the step.  us, list / pass by tokens kept: 5000 of 50257 39.1 /
+  // 40.3, 13000 57.7 (more than the list holds) / 42; 2000 of 32000 64.5 / 64.8, 7000
+  // 78 / 68; 8000 of 128000 77 / 89.
+  __device__ inline u64 find_top(Shared& sh, float top_p, u64 least) {
     clear<true>(sh, kBins);
     each<1>([&](int, const Run<T>& r) {
 #pragma unroll
@@ -404,43 +412,83 @@ struct Row {
       }
     });
     __syncthreads();
-    u64 target = 0;
-    place<true>(sh, 12, 0, 0, [&](u64 all) { return target = cut_of(top_p, all); });
-    const int step = kBins - 1 - sh.found;
-    u64 above = sh.before;
-    clear<true>(sh, 0);
-    // a little past the step's ends: what is past them does no harm on the list
-    const float end = float(top - (step + 1) / 64.0 / per), begin = float(top - step / 64.0 / per);
-    const float slack = float(fabs(top)) * 0x1p-40f, lo = end - fabsf(end) * 0x1p-22f - slack;
-    whole = make_list(sh, lo, INFINITY);
-    if (whole && listed <= kFew) return target;
-    if (!whole) {  // the step's tokens alone
-      clear<true>(sh, 0);
-      if (!make_list(sh, lo, begin + fabsf(begin) * 0x1p-22f + slack)) return target;
+    // each thread's steps from the largest weight down: their weights, and how many
+    // tokens that is (the weight over one of the step's)
+    constexpr int kPer = kBins / kThreads;
+    u64 mass[kPer], own = 0, all;
+    uint32_t tokens[kPer], some = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int j = int(threadIdx.x) * kPer + k;
+      own += mass[k] = sh.mass[kBins - 1 - j];
+      some += tokens[k] = uint32_t(float(mass[k]) * exp2f(float(j) / 64.f - float(shift)) + 0.5f);
     }
-    __syncthreads();  // everyone has read the list's length
-    if (threadIdx.x == 0) sh.n = 0;
+    some = upto(some) - some;
+    if (lane() == kWave - 1) sh.wave_sum[1][wave()] = some + tokens[0] + tokens[1] + tokens[2] + tokens[3];
+    u64 above = scan(own, sh, 0, all);
+    const u64 target = cut_of(top_p, all);
+    if (above < target && target <= above + own) {
+      for (int w = 0; w < int(threadIdx.x) / kWave; ++w) some += uint32_t(sh.wave_sum[1][w]);
+      int at = 0;
+      uint32_t in_step = 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        if (at == k) some += tokens[k], in_step = tokens[k];
+        if (at == k && above + mass[k] < target) above += mass[k], ++at;
+      }
+      sh.found = int(threadIdx.x) * kPer + at;
+      sh.before = above;
+      sh.kept = some;
+      sh.in_step = in_step;
+    }
     __syncthreads();
-    over(sh, [&](int, uint32_t key) {
-      const double z = log2_weight(O::of_key(key));
-      if (step_of(z) != step) return;
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at >= uint32_t(kStep)) return;
-      sh.count[at] = key;
-      sh.mass[at] = weight_of(z);
-    });
+    const int step = sh.found;
+    const uint32_t kept = sh.kept;
+    const bool many = sh.in_step > uint32_t(kStep);  // at least as many are in the step
+    above = sh.before;
+    clear<true>(sh, (V + kChunk - 1) / kChunk);
+    clear<false>(sh, (V + kChunk - 1) / kChunk);
+    if (kept <= uint32_t(min(V / 8, kList - kList / 32))) {
+      // a little past the step's end: what is past it does no harm on the list
+      const float end = float(top - (step + 1) / 64.0 / per);
+      whole = make_list(sh, end - fabsf(end) * 0x1p-22f - float(fabs(top)) * 0x1p-40f, INFINITY);
+      if (whole && listed <= kFew) return target;
+      if (!whole || many) return target;
+      __syncthreads();  // everyone has read the list's length
+      if (threadIdx.x == 0) sh.n = 0;
+      __syncthreads();
+      over(sh, [&](int c, uint32_t key) {
+        const double z = log2_weight(O::of_key(key));
+        if (step_of(z) == step) put_aside(sh, c, key, weight_of(z));
+      });
+    } else {
+      if (many) return target;
+      const double from = -(step + 1) / 64.0, to = -step / 64.0;  // z in (from, to]
+      const u64 low = kRaw + least;
+      each<1>([&](int c, const Run<T>& r) {
+        u64 own = 0;
+#pragma unroll
+        for (int e = 0; e < kLane; ++e) {
+          const float v = O::value(r.v[e]);
+          const double z = log2_weight(v);
+          const u64 w = raw_weight(z);
+          own += z > to && w >= low ? w : kRaw;
+          if (z > from && z <= to) put_aside(sh, c, O::key(r.v[e]), w - kRaw);
+        }
+        add_all(&sh.mass[c], own - kLane * kRaw);
+      });
+    }
     __syncthreads();
     const int n = int(sh.n);
-    if (!whole) listed = -1;
     if (n > kStep) return target;
     if (int(threadIdx.x) < n) {
-      const uint32_t key = sh.count[threadIdx.x];
-      const u64 w = sh.mass[threadIdx.x];
+      const uint32_t key = sh.step_key[threadIdx.x];
+      const u64 w = sh.step_weight[threadIdx.x];
       u64 same = 0;
 #pragma unroll 4
       for (int i = 0; i < n; ++i) {
-        const uint32_t k = sh.count[i];
-        const u64 v = sh.mass[i];
+        const uint32_t k = sh.step_key[i];
+        const u64 v = sh.step_weight[i];
         above += k > key ? v : 0;
         same += k == key ? v : 0;
       }
@@ -452,7 +500,22 @@ struct Row {
     __syncthreads();
     cut = uint32_t(sh.found);
     ties = sh.before;
+    summed = !whole;
+    if (summed && int(threadIdx.x) < n) {
+      const uint32_t key = sh.step_key[threadIdx.x], c = sh.step_chunk[threadIdx.x];
+      const u64 w = sh.step_weight[threadIdx.x];
+      if (key > cut && w >= least) atomicAdd(&sh.mass[c], w);
+      if (key == cut) atomicAdd(&sh.count[c], 1u);
+    }
     return 0;
+  }
+  // one of the step's tokens
+  __device__ inline void put_aside(Shared& sh, int c, uint32_t key, u64 w) const {
+    const uint32_t at = atomicAdd(&sh.n, 1u);
+    if (at >= uint32_t(kStep)) return;
+    sh.step_key[at] = key;
+    sh.step_chunk[at] = uint32_t(c);
+    sh.step_weight[at] = w;
   }
 
   // Moves the cut to where the kept counts (or weights) from the largest value
@@ -590,7 +653,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
   r.V = int(p.V);
   r.shift = p.shift;
   r.listed = -1;
-  r.whole = false;
+  r.whole = r.summed = false;
   const float u = p.u[row];
   float t = p.temperature ? p.temperature[row] : p.temperature_all;
   const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
@@ -688,7 +751,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     u64 target = 0;
     if (top_p < 1.f && !few_k) {  // of what top-k kept, before min-p
       const bool top_k = r.cut != 0;
-      if (!top_k) target = r.list_top(sh, top_p);
+      if (!top_k) target = r.find_top(sh, top_p, least);
       if (top_k || (target != 0 && !(r.whole && r.listed <= kFew)))
         r.template select<true>(sh, [&](u64 all) { return target ? target : cut_of(top_p, all); });
     }
@@ -703,9 +766,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     tie_weight = r.cut != 0 ? r.weight(O::of_key(r.cut)) : 0;
     if (tie_weight < least) tie_weight = 0;
     const int chunks = (r.V + kChunk - 1) / kChunk;
-    r.template clear<true>(sh, chunks);
-    if (r.cut != 0) r.template clear<false>(sh, chunks);
-    if (r.listed >= 0) {
+    if (!r.summed) {
+      r.template clear<true>(sh, chunks);
+      if (r.cut != 0) r.template clear<false>(sh, chunks);
+    }
+    if (r.summed) {
+      // by find_top
+    } else if (r.listed >= 0) {
       r.over(sh, [&](int c, uint32_t key) {
         if (key > r.cut) {
           const u64 w = r.weight(O::of_key(key));
