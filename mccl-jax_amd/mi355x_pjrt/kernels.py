@@ -794,7 +794,7 @@ def add_rmsnorm_int8(x, residual=None, gamma=None, eps=1e-6, sum_out=None, q=Non
     else:
         q, pitch, scale = _int8_outputs(what, x, shape, q, scale, dev, stream)
     handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
-    rc = (_lib._kernels or lib()).mk_add_rmsnorm_int8(handle, t, rows, cols, x.data_ptr(), ld, r_ptr, r_ld, g_ptr, eps,
+    rc = (_lib._kernels or lib()).mk_add_rmsnorm_int8(handle, t, rows, cols, x.data_ptr(), ld, r_ptr, r_ld, g_ptr, float(eps),
                                                       s_ptr, s_ld, q.data_ptr(), pitch, scale.data_ptr())
     if rc:
         _check(rc, "mk_add_rmsnorm_int8")
@@ -926,7 +926,7 @@ def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, 
         _operand(what, "temperature", temperature, torch.float32, per_row, dev)
         t = temperature.data_ptr()
     elif temperature is not None:
-        t_all = temperature
+        t_all = float(temperature)
     if isinstance(top_k, torch.Tensor):
         _operand(what, "top_k", top_k, torch.int32, per_row, dev)
         k = top_k.data_ptr()
@@ -936,12 +936,12 @@ def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, 
         _operand(what, "top_p", top_p, torch.float32, per_row, dev)
         p = top_p.data_ptr()
     elif top_p is not None:
-        p_all = top_p
+        p_all = float(top_p)
     if isinstance(min_p, torch.Tensor):
         _operand(what, "min_p", min_p, torch.float32, per_row, dev)
         m = min_p.data_ptr()
     elif min_p is not None:
-        m_all = min_p
+        m_all = float(min_p)
     token = _new(logits, stream, index_dtype, shape[0])
     logprob = _new(logits, stream, torch.float32, shape[0]) if with_logprob else None
     handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)

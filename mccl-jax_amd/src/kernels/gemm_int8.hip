@@ -8,6 +8,11 @@
 // operand row c and 16 consecutive k of group g.  They are issued with B's rows
 // first, so that a lane's accumulator holds 4 consecutive columns of one row of
 // C (lane (c, g), reg r of the 32 x 32 form: row c, column 8 (r / 4) + 4 g + r % 4).
+//
+// Bound: the matrix cores at the power limit for many rows (8192 x 4096 x 16384, M x K x N,
+// 479 us, 2296 TOP/s; 8192 cubed 454 us, 389 us on zeros), HBM for few, where the weights
+// are the traffic (16 x 4096 x 16384 13.7 us, 67 MB), launches and latency for one (1 x
+// 768 x 2304 3.9 us).
 #include "attn_common.h"
 
 #include <algorithm>
@@ -60,10 +65,10 @@ __device__ inline i32x4_t load16_upto(const int8_t* p, int64_t n) {
 // At most 64 rows: reading B (the weights) once is the work.  A wave has 16 VN columns
 // and all rows, and every k_waves-th step of 128 bytes of k, kD steps ahead in
 // registers; the sums of the k_waves waves of a column block meet in LDS (whole
-// numbers: in any order).  Nothing is staged.  A lane (c, g) of v_mfma_i32_16x16x64_i8 loads 32
-// consecutive bytes of row c at k = 32 g, so that 4 lanes take a whole line of a
-// row, and they are the operands of two MFMAs: which k an MFMA's slots mean is
-// free as long as A and B agree.  Rows need no alignment.
+// numbers: in any order).  Nothing is staged.  A lane (c, g) of v_mfma_i32_16x16x64_i8
+// loads 32 consecutive bytes of row c at k = 32 g, so that 4 lanes take a whole line of
+// a row, and they are the operands of two MFMAs: which k an MFMA's slots mean is free
+// as long as A and B agree.  Rows need no alignment.
 constexpr int kStep = 128;
 
 template <int VN, int MT, int NW, int kD>
@@ -221,10 +226,10 @@ void launch_small(hipStream_t s, const Int8Gemm& a) {
 }
 
 // ---------------------------------------------------------------- tiles
-// Workgroup tile TM x TN, k in tiles of 128 bytes,
-// WGM x WGN waves of 32 x 32 blocks.  Tiles of rows on the 16-byte grid go straight into LDS
-// (buffer_load ... lds, attn_common.h) in S stages: the copies of k tile t + S - 1
-// are issued while tile t is multiplied, one barrier a tile.  An LDS row is
+// Workgroup tile TM x TN, k in tiles of 128 bytes, WGM x WGN waves of 32 x 32 blocks.
+// Tiles of rows on the 16-byte grid go straight into LDS (buffer_load ... lds,
+// attn_common.h) in S stages: the copies of k tile t + S - 1 are issued while tile t is
+// multiplied, one barrier a tile.  An LDS row is
 // 128 bytes, its 16-byte chunk c at position c ^ ((row >> 1) & 7), so that the
 // 16 rows a ds_read_b128 takes at one chunk lie on 16 different bank groups.
 // Chunks past M, N or K are loaded from an out-of-range offset, which reads
@@ -329,9 +334,10 @@ typedef uint32_t u32x4_by4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // C's tile through LDS in passes of as many rows as the operand stages hold:
-// a lane writes 4 consecutive columns at a time, chunk c of staging row r at
-// position c ^ (r & 15) (rows of 8 and 4 chunks: c ^ ((r >> 1) & 7), c ^ ((r >> 2) & 3)), and the workgroup stores runs of 16 bytes (of whole
-// rows; they need no alignment past an element's).
+// a lane writes 4 consecutive columns at a time, chunk c of staging row r at position
+// c ^ (r & 15) (rows of 8 and 4 chunks: c ^ ((r >> 1) & 7), c ^ ((r >> 2) & 3)), and the
+// workgroup stores runs of 16 bytes (of whole rows; they need no alignment past an
+// element's).
 template <int CT, bool STREAM, int TM, int TN, int S, int kW, int kWM, int kWN, int kI, int kJ>
 __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm& p, const i32x16_t (&acc)[kI][kJ],
                                                                  int8_t* stage, const float* sa, const float* sb,
@@ -607,7 +613,7 @@ void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
 
 // rows on the 16-byte grid that do not overlap, below the 2^31 bytes of a buffer's offsets
 bool on_grid(const int8_t* p, int64_t rows, int64_t K, int64_t ld) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld >= K &&
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld >= K && ld < (int64_t(1) << 31) &&
          (rows - 1) * ld + K + 16 < (int64_t(1) << 31);
 }
 
@@ -638,6 +644,9 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
       reinterpret_cast<uintptr_t>(b_scale) % 4 ||
       (epi != 0 && reinterpret_cast<uintptr_t>(bias) % ((epilogue & 4) ? 4 : dtype_bytes(c_type))))
     return fail(MK_ERR_INVALID, "mk_gemm_int8: an operand is not aligned to its elements");
+  // one row's pitch says nothing
+  if (M == 1) a_ms = (K + 15) & ~int64_t(15);
+  if (N == 1) b_ns = (K + 15) & ~int64_t(15);
   Int8Gemm a{A, B, a_scale, b_scale, C, bias, M, N, K, a_ms, b_ns, c_ms, 0, 0, 1,
              c_type, epilogue, 0};
   hipStream_t s = as_stream(stream);

@@ -390,6 +390,8 @@ def test_sample_rows_views_and_agreement(K):
     assert torch.equal(K.sample_rows(x, u, 0.0)[0], K.row_argmax(x)[0])
     assert torch.equal(K.sample_rows(x, u, top_k=1)[0], K.row_argmax(x)[0])
     assert K.sample_rows(x, u, with_logprob=False)[1] is None
+    got = K.sample_rows(x, u, np.float32(0.8), np.int64(50), np.float64(0.9), np.float32(0.01))
+    assert torch.equal(got[0], want[0])
     assert K.sample_rows(x[:0], u[:0])[0].shape == (0,)
 
 
@@ -554,6 +556,14 @@ def test_one_row_of_weights_for_every_column(K):
     assert torch.equal(K.gemm_int8(a, sa, w.expand(600, 768).t(), sb), want)
     want = K.gemm_int8(a[:1].expand(100, 768).contiguous(), sa, w.expand(600, 768).contiguous().t(), sb)
     assert torch.equal(K.gemm_int8(a[:1].expand(100, 768), sa, w.expand(600, 768).t(), sb), want)
+    # a single row, whose pitch says nothing
+    for Kd in (768, 750):
+        v = _int8(3, (600, Kd))
+        row = a[:1, :Kd].contiguous()
+        want = K.gemm_int8(row, sa[:1], v.t(), sb)
+        assert torch.equal(K.gemm_int8(row.as_strided((1, Kd), (1, 1)), sa[:1], v.t(), sb), want)
+        want = K.gemm_int8(v, sb, row.t(), sa[:1])
+        assert torch.equal(K.gemm_int8(v, sb, row.as_strided((1, Kd), (1, 1)).t(), sa[:1]), want)
 
 
 def test_two_streams_at_once(K):
