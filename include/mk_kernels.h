@@ -620,7 +620,7 @@ int mk_dequantize_rows(void* stream, int out_type, int64_t rows, int64_t cols, c
  * fp32, a_scale first, and rounded once to c_type in {MK_F32, MK_BF16, MK_F16}.
  * a_scale [M] and b_scale [N] are fp32.  epilogue and bias as mk_gemm's (0 none,
  * 1 + bias, 2 + bias then max(., 0), 5 / 6 as 1 / 2 with an fp32 bias).  K = 0 is a
- * sum of 0. */
+ * sum of 0.  M and N in 64s, times each other, stay below 2^24 - 1. */
 int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int64_t K, const int8_t* A, int64_t a_ms,
                  const float* a_scale, const int8_t* B, int64_t b_ns, const float* b_scale, void* C, int64_t c_ms,
                  const void* bias, int epilogue);
@@ -638,8 +638,8 @@ int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int64_t K, cons
  *            more than u times all kept weights
  *   logprob = log(w_token / sum of kept weights), fp32 (logprobs may be NULL)
  * temperature 0 takes the largest logit, the lowest index among equals, whatever
- * the other limits say.  Sums are exact sums of weights rounded to whole multiples
- * of 2^-s, s >= 41 (46 for 50257 tokens).  temperature, top_k, top_p and min_p: a
+ * the other limits say.  A weight is within 2^-33 of itself and a whole multiple of
+ * 2^-s, s >= 41 (46 for 50257 tokens); sums of weights are exact.  temperature, top_k, top_p and min_p: a
  * device array of one value a row, or NULL and the value `*_all` for every row.
  * -inf logits are never drawn.  A row that holds a NaN or +inf, or nothing above
  * -inf, and a row whose u, temperature, top_p or min_p is NaN or whose temperature
