@@ -10,7 +10,7 @@
 // C (lane (c, g), reg r of the 32 x 32 form: row c, column 8 (r / 4) + 4 g + r % 4).
 //
 // Bound: the matrix cores at the power limit for many rows (8192 x 4096 x 16384, M x K x N,
-// 479 us, 2296 TOP/s; 8192 cubed 454 us, 389 us on zeros), HBM for few, where the weights
+// 467 us, 2355 TOP/s; 8192 cubed 443 us), HBM for few, where the weights
 // are the traffic (16 x 4096 x 16384 13.7 us, 67 MB), launches and latency for one (1 x
 // 768 x 2304 3.9 us).
 #include "attn_common.h"
@@ -333,28 +333,26 @@ struct Shape {
 typedef uint32_t u32x4_by4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
 
-// C's tile through LDS in passes of as many rows as the operand stages hold:
-// a lane writes 4 consecutive columns at a time, chunk c of staging row r at position
-// c ^ (r & 15) (rows of 8 and 4 chunks: c ^ ((r >> 1) & 7), c ^ ((r >> 2) & 3)), and the
-// workgroup stores runs of 16 bytes (of whole rows; they need no alignment past an
-// element's).
-template <int CT, bool STREAM, int TM, int TN, int S, int kW, int kWM, int kWN, int kI, int kJ>
+// C's tile through LDS, each wave for itself and without barriers: 32 rows of its
+// columns at a time, in its part of the operand stages (8192 x 768 x 50304 in bf16 466
+// us, 495 with the workgroup storing whole rows of the tile between barriers).  A lane writes 4 consecutive
+// columns, chunk c of staging row r at position c ^ (r & 15) (rows of 8 and 4 chunks:
+// c ^ ((r >> 1) & 7), c ^ ((r >> 2) & 3)), and the wave stores runs of 16 bytes (of whole
+// rows; they need no alignment past an element's).
+template <int CT, bool STREAM, int kWM, int kWN, int kI, int kJ>
 __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm& p, const i32x16_t (&acc)[kI][kJ],
                                                                  int8_t* stage, const float* sa, const float* sb,
                                                                  const float* bias, int64_t m0, int64_t n0, int wm,
                                                                  int wn, int lane) {
-  constexpr int kSz = CT == MK_F32 ? 4 : 2, kPer = 16 / kSz, kCpr = TN / kPer, kThreads = 64 * kW;
-  constexpr int kRoom = S * kBK * (TM + TN), kFit = kRoom / (TN * kSz) / kWM * kWM;
-  constexpr int kRP = kFit >= TM ? TM : TM % kFit == 0 ? kFit : kWM;  // rows a pass
-  static_assert(kRP > 0 && TM % kRP == 0 && kRP % kWM == 0 && kCpr % 4 == 0, "passes of whole wave rows");
-  static_assert(kRP * kCpr % kThreads == 0, "chunks split evenly over the threads");
+  constexpr int kSz = CT == MK_F32 ? 4 : 2, kPer = 16 / kSz, kCpr = kWN / kPer;
+  static_assert(kCpr % 4 == 0 && 32 * kCpr % 64 == 0, "whole chunks, evenly over the lanes");
   using out_t = std::conditional_t<CT == MK_F32, u32x4_by4_t, u32x4_by2_t>;
   auto pos = [](int row, int cn) {
     return cn ^ (kCpr % 16 == 0 ? row & 15 : kCpr % 8 == 0 ? (row >> 1) & 7 : (row >> 2) & 3);
   };
   const int c = lane & 31, g = lane >> 5;
   char* C = static_cast<char*>(p.C);
-  // this lane's scales and biases, ahead of the writes to LDS
+  // this lane's scales and biases
   float s[kI];
   f32x4 t[kJ][4], u[kJ][4];
 #pragma unroll
@@ -368,43 +366,36 @@ __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm&
       u[b][rg] = *reinterpret_cast<const f32x4*>(bias + nl);
     }
 #pragma unroll
-  for (int pass = 0; pass < TM / kRP; ++pass) {
-    if (pass > 0) lds_barrier();
-    if (wm * kWM >= pass * kRP && wm * kWM < (pass + 1) * kRP) {
+  for (int a = 0; a < kI; ++a) {
 #pragma unroll
-      for (int b = 0; b < kJ; ++b)
+    for (int b = 0; b < kJ; ++b)
 #pragma unroll
-        for (int rg = 0; rg < 4; ++rg) {
-          const int nl = wn * kWN + 32 * b + 8 * rg + 4 * g;
+      for (int rg = 0; rg < 4; ++rg) {
+        const int nl = 32 * b + 8 * rg + 4 * g;
+        float v[4];
 #pragma unroll
-          for (int a = 0; a < kI; ++a) {
-            const int row = wm * kWM + 32 * a + c - pass * kRP;
-            float v[4];
+        for (int q = 0; q < 4; ++q) v[q] = fmaf(float(acc[a][b][4 * rg + q]) * s[a], t[b][rg].v[q], u[b][rg].v[q]);
+        if ((p.epilogue & 3) == 2) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = fmaf(float(acc[a][b][4 * rg + q]) * s[a], t[b][rg].v[q], u[b][rg].v[q]);
-            if ((p.epilogue & 3) == 2) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
-            }
-            int8_t* to = stage + row * TN * kSz + 16 * pos(row, nl / kPer) + nl % kPer * kSz;
-            if constexpr (CT == MK_F32) {
-              *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
-            } else {
-              uint16_t h[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) h[q] = CT == MK_BF16 ? f32_to_bf16(v[q]) : f32_to_f16(v[q]);
-              __builtin_memcpy(to, h, 8);
-            }
-          }
+          for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
         }
-    }
-    lds_barrier();
-#pragma unroll 2
-    for (int it = 0; it < kRP * kCpr / kThreads; ++it) {
-      const int e = it * kThreads + int(threadIdx.x);
+        int8_t* to = stage + c * kWN * kSz + 16 * pos(c, nl / kPer) + nl % kPer * kSz;
+        if constexpr (CT == MK_F32) {
+          *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
+        } else {
+          uint16_t h[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) h[q] = CT == MK_BF16 ? f32_to_bf16(v[q]) : f32_to_f16(v[q]);
+          __builtin_memcpy(to, h, 8);
+        }
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int it = 0; it < 32 * kCpr / 64; ++it) {
+      const int e = it * 64 + lane;
       const int row = e / kCpr, cn = e % kCpr;
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + row * TN * kSz + 16 * pos(row, cn));
-      const int64_t m = m0 + pass * kRP + row, n = n0 + cn * kPer;
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + row * kWN * kSz + 16 * pos(row, cn));
+      const int64_t m = m0 + wm * kWM + 32 * a + row, n = n0 + wn * kWN + cn * kPer;
       if (m >= p.M || n >= p.N) continue;
       char* to = C + kSz * (m * p.ldc + n);
       if (n + kPer <= p.N) {
@@ -419,6 +410,7 @@ __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm&
           }
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -550,8 +542,11 @@ __global__ __launch_bounds__(64 * Sh::WGM * Sh::WGN, 1) void gemm_int8_tiled_ker
     }
   }
   lds_barrier();  // every wave is done with the operand stages before they hold C
-  if (p.stream_c) store_tile<CT, true, TM, TN, S, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
-  else store_tile<CT, false, TM, TN, S, kW, kWM, kWN>(p, acc, lds, sa, sb, bias, m0, n0, wm, wn, lane);
+  constexpr int kStage = 32 * kWN * (CT == MK_F32 ? 4 : 2);  // bytes a wave
+  static_assert(kStage * kW <= S * kBK * (TM + TN), "room for C");
+  int8_t* stage = lds + wave * kStage;
+  if (p.stream_c) store_tile<CT, true, kWM, kWN>(p, acc, stage, sa, sb, bias, m0, n0, wm, wn, lane);
+  else store_tile<CT, false, kWM, kWN>(p, acc, stage, sa, sb, bias, m0, n0, wm, wn, lane);
 }
 
 template <class Sh>
@@ -568,12 +563,13 @@ void launch_tiled(hipStream_t s, Int8Gemm a) {
   else go(Int<MK_F32>{});
 }
 
-// The tile with the least estimated time: rounds of workgroups of nk + e k tiles,
-// e the first copies and the epilogue; a last round that leaves every workgroup
-// alone on its CU runs each k tile in `alone`.  us, fitted to the shapes' times on
-// 166 products of 17 .. 8192 rows with both C types; the choice costs 1.5% over
-// the fastest on average.  In the order below, us: bf16 C (M x K x N):
-// 8192 x 4096 x 16384 479, 578, 773, 895, 1120; 2048 x 4096 x 4096 54, 44, 58, 67, 83; 512 x
+// The tile with the least estimated time: rounds of workgroups of nk + e k tiles, e the
+// first copies and the epilogue; a last round that leaves every workgroup alone on its
+// CU runs each k tile in `alone`, and 256 x 256 tiles, one on a CU, in a time that
+// grows with their number (the power limit).  us, fitted to the shapes' times on 166
+// products of 17 .. 8192 rows with both C types; the choice costs 1.0% over the fastest
+// on average (1.6% without that last term).  In the order below, us: bf16 C (M x K x N):
+// 8192 x 4096 x 16384 467, 578, 773, 895, 1120; 2048 x 4096 x 4096 54, 43, 58, 67, 83; 512 x
 // 4096 x 4096 41, 23, 18, 18, 24; 64 x 768 x 50257 18, 14, 12.7, 15.5, 17.5; 128 x 768 x 768
 // 12.2, 5.7, 5.1, 4.3, 4.3.
 void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
@@ -581,8 +577,8 @@ void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
     int tm, tn, per_cu;
     double each, alone, e16, e32;
   };
-  static const Option options[] = {{256, 256, 1, 2.08, 1.33, 3.7, 5.6},
-                                   {128, 128, 2, 1.40, 0.70, 2.4, 3.0},
+  static const Option options[] = {{256, 256, 1, 2.04, 1.21, 3.2, 5.1},
+                                   {128, 128, 2, 1.40, 0.70, 2.3, 3.0},
                                    {64, 128, 2, 0.86, 0.45, 3.1, 3.7},
                                    {64, 64, 2, 0.50, 0.31, 4.3, 5.1},
                                    {64, 32, 3, 0.45, 0.27, 4.6, 5.4}};
@@ -595,13 +591,17 @@ void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
     const int64_t tiles = ((a.M + q.tm - 1) / q.tm) * ((a.N + q.tn - 1) / q.tn), slots = 256 * q.per_cu;
     const double work = nk + (a.c_type == MK_F32 ? q.e32 : q.e16);
     double t = double(tiles / slots) * work * q.each;
-    if (const int64_t rem = tiles % slots) t += work * (rem <= 256 ? q.alone : q.each);
+    const int64_t rem = tiles % slots;
+    if (q.per_cu == 1) t += rem ? work * (q.alone + (q.each - q.alone) * double(rem) / 256) : 0;
+    else if (rem) t += work * (rem <= 256 ? q.alone : q.each);
     if (least == 0 || t < least) best = o, least = t;
   }
-  // C past the caches where it is most of the last-level cache and the product is
-  // long (8192 x 4096 x 16384 492 us, 502 with ordinary stores; 8192 x 768 x 50264
-  // 550 and 531)
-  a.stream_c = a.M * a.N * dtype_bytes(a.c_type) >= int64_t(192) << 20 && a.K >= 2048;
+  // C past the caches where it is most of the last-level cache and its rows lie on the
+  // 128-byte lines; us, so / with ordinary stores: bf16 8192 x 768 x 50304 430 / 454,
+  // 8192 x 4096 x 16384 475 / 478, fp32 8192 x 768 x 50304 566 / 578, 8192 x 2048 x 16384
+  // 333 / 326; off the lines, bf16 8192 x 768 x 50264 584 / 495, fp32 x 50257 818 / 663
+  const int64_t pitch = a.ldc * dtype_bytes(a.c_type);
+  a.stream_c = a.M * pitch >= int64_t(192) << 20 && pitch % 128 == 0 && reinterpret_cast<uintptr_t>(a.C) % 128 == 0;
   if (!grid && best == 1) launch_tiled<Shape<128, 128, 2, 4, 2, false>>(s, a);
   else if (!grid) launch_tiled<Shape<64, 64, 2, 2, 2, false>>(s, a);
   else if (best == 0) launch_tiled<Shape<256, 256, 2, 4, 2>>(s, a);
