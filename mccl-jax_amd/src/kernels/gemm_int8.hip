@@ -10,7 +10,7 @@
 // C (lane (c, g), reg r of the 32 x 32 form: row c, column 8 (r / 4) + 4 g + r % 4).
 //
 // Bound: the matrix cores at the power limit for many rows (8192 x 4096 x 16384, M x K x N,
-// 467 us, 2355 TOP/s; 8192 cubed 443 us), HBM for few, where the weights
+// 466 us, 2360 TOP/s; 8192 cubed 443 us), HBM for few, where the weights
 // are the traffic (16 x 4096 x 16384 13.7 us, 67 MB), launches and latency for one (1 x
 // 768 x 2304 3.9 us).
 #include "attn_common.h"
