@@ -794,8 +794,8 @@ def add_rmsnorm_int8(x, residual=None, gamma=None, eps=1e-6, sum_out=None, q=Non
     else:
         q, pitch, scale = _int8_outputs(what, x, shape, q, scale, dev, stream)
     handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
-    rc = (_lib._kernels or lib()).mk_add_rmsnorm_int8(handle, t, rows, cols, x.data_ptr(), ld, r_ptr, r_ld, g_ptr, float(eps),
-                                                      s_ptr, s_ld, q.data_ptr(), pitch, scale.data_ptr())
+    rc = (_lib._kernels or lib()).mk_add_rmsnorm_int8(handle, t, rows, cols, x.data_ptr(), ld, r_ptr, r_ld, g_ptr,
+                                                      float(eps), s_ptr, s_ld, q.data_ptr(), pitch, scale.data_ptr())
     if rc:
         _check(rc, "mk_add_rmsnorm_int8")
     return q, scale, total

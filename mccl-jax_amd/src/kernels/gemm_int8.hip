@@ -185,7 +185,8 @@ void launch_rows(hipStream_t s, Int8Gemm a, int k_waves) {
   auto go = [&](auto nw) {
     constexpr int NW = decltype(nw)::value;
     const int64_t per = NW / a.k_waves;
-    hipLaunchKernelGGL((gemm_int8_rows_kernel<VN, MT, NW, kD>), dim3(unsigned((blocks + per - 1) / per), unsigned((a.M + 16 * MT - 1) / (16 * MT))), dim3(64 * NW), 0, s, a);
+    const dim3 g{unsigned((blocks + per - 1) / per), unsigned((a.M + 16 * MT - 1) / (16 * MT))};
+    hipLaunchKernelGGL((gemm_int8_rows_kernel<VN, MT, NW, kD>), g, dim3(64 * NW), 0, s, a);
   };
   if (a.k_waves == 16) go(Int<kMost>{});
   else go(Int<8>{});
@@ -448,8 +449,9 @@ __global__ __launch_bounds__(64 * Sh::WGM * Sh::WGN, 1) void gemm_int8_tiled_ker
 #pragma unroll
     for (int c = 0; c < kNC; ++c) {
       if (c < lo || c >= hi) continue;
-      if (c < kCa) copy_to_lds_so(ra, lds_addr(&As[st][(wave + kW * c) * 1024]), int(ca.off[c < kCa ? c : 0]), uint32_t(kBK * kt));
-      else copy_to_lds_so(rb, lds_addr(&Bs[st][(wave + kW * (c - kCa)) * 1024]), int(cb.off[c < kCa ? 0 : c - kCa]), uint32_t(kBK * kt));
+      const uint32_t at = uint32_t(kBK * kt);
+      if (c < kCa) copy_to_lds_so(ra, lds_addr(&As[st][(wave + kW * c) * 1024]), int(ca.off[c < kCa ? c : 0]), at);
+      else copy_to_lds_so(rb, lds_addr(&Bs[st][(wave + kW * (c - kCa)) * 1024]), int(cb.off[c < kCa ? 0 : c - kCa]), at);
     }
   };
   auto issue_last = [&](int kt) __attribute__((always_inline)) {

@@ -72,7 +72,8 @@ __device__ inline Stats join(Stats a, Stats b) { return {a.squares + b.squares, 
 
 __device__ inline Stats wave_join(Stats s) {
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) s = join(s, {__shfl_xor(s.squares, m, kWave), uint32_t(__shfl_xor(int(s.top), m, kWave))});
+  for (int m = 32; m >= 1; m >>= 1)
+    s = join(s, {__shfl_xor(s.squares, m, kWave), uint32_t(__shfl_xor(int(s.top), m, kWave))});
   return s;
 }
 

@@ -523,6 +523,19 @@ def test_sample_rows_where_the_list_overflows(K, dtype):
             _check_sample(K, x, _u(41, 6), torch.tensor([1.0, 1.0, 0.8, 1.3, 1.0, 2.0], device="cuda"), 0, p, m)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_rows_of_mostly_masked_tokens(K, dtype):
+    """Fewer tokens left than top_k, more, and more than a list holds; masked with -inf, the lowest value, 60 below."""
+    for vocab, left in ((50257, 1), (50257, 10), (50257, 400), (50257, 20000), (3000, 7), (9, 3)):
+        print(f"case: sample_rows, {left} of {vocab} left, {dtype}", flush=True)
+        x = _normal(left, (6, vocab), dtype, 2.0)
+        at = torch.rand((6, vocab), generator=torch.Generator().manual_seed(left)).argsort(dim=1) >= left
+        for mask in (-math.inf, torch.finfo(dtype).min, -60.0):
+            y = x.masked_fill(at.cuda(), mask)
+            for k, p, m in ((50, 1.0, 0.0), (50, 0.9, 0.0), (1000, 0.9, 0.0), (30000, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.1)):
+                _check_sample(K, y, _u(51, 6), 0.7, k, p, m)
+
+
 def test_rows_far_apart(K):
     """Rows whose offsets pass 2^31 bytes and 2^31 elements, of every operand."""
     def far(t, pitch):
