@@ -591,7 +591,8 @@ int mk_sdpa_bwd(void* stream, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int6
 /* Residual add, RMS norm and rounding to 8 bits in one pass over rows of `cols`:
  *   s = x + residual        (fp32 add, one RNE rounding to io_type, stored to sum)
  *   y = s / sqrt(mean(s^2) + eps) * gamma
- *   scale = max |y| / 127,  q = y / scale rounded to the nearest whole number
+ *   scale = max |y| / 127,  q = y / scale rounded to the nearest whole number, halves
+ *           to the even one (of s gamma 127 / max |s gamma|, rounded to fp32 before)
  * io_type in {MK_BF16, MK_F16, MK_F32} for x, residual, gamma and sum.  residual
  * NULL: s = x and sum is not written (sum may be x or residual, at its pitch);
  * gamma NULL: 1.  The mean is summed in 64 bits.  A row with max |s gamma| below
@@ -604,7 +605,7 @@ int mk_add_rmsnorm_int8(void* stream, int io_type, int64_t rows, int64_t cols, c
 /* Rows to 8 bits: scale = max |y| / 127, q = y / scale rounded, with y = x or
  * (gelu != 0) gelu_tanh(x) in fp32: an attention output, an MLP's hidden rows, or
  * weights with a scale for each output channel.  Zeros, NaN and infinities as
- * above (for y). */
+ * above (for y), halves too, but a GELU's, which go either way. */
 int mk_quantize_rows(void* stream, int io_type, int64_t rows, int64_t cols, const void* x, int64_t ld_x, int gelu,
                      int8_t* q, int64_t ld_q, float* scale);
 
