@@ -179,7 +179,7 @@ void launch_rows(hipStream_t s, Int8Gemm a, int k_waves) {
   constexpr bool kSlim = 2 * kWords + kSums <= 72;
   constexpr int kFit = ((kSlim ? 72 : 192) - kSums) / kWords, kD = kFit > 4 ? 4 : kFit;
   static_assert(kD >= 2, "two steps in flight");
-  constexpr int kMost = kSlim ? 16 : 8;
+  constexpr int kMost = kSlim && VN == 1 ? 16 : 8;  // (32 columns a wave and more are never cut further)
   a.k_waves = std::min(k_waves, kMost);
   const int64_t blocks = (a.N + 16 * VN - 1) / (16 * VN);
   auto go = [&](auto nw) {
