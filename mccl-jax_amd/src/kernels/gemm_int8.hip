@@ -603,7 +603,8 @@ void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
   // 8192 x 4096 x 16384 475 / 478, fp32 8192 x 768 x 50304 566 / 578, 8192 x 2048 x 16384
   // 333 / 326; off the lines, bf16 8192 x 768 x 50264 584 / 495, fp32 x 50257 818 / 663
   const int64_t pitch = a.ldc * dtype_bytes(a.c_type);
-  a.stream_c = a.M * pitch >= int64_t(192) << 20 && pitch % 128 == 0 && reinterpret_cast<uintptr_t>(a.C) % 128 == 0;
+  a.stream_c = a.M * a.N * dtype_bytes(a.c_type) >= int64_t(192) << 20 && pitch % 128 == 0 &&
+               reinterpret_cast<uintptr_t>(a.C) % 128 == 0;
   if (!grid && best == 1) launch_tiled<Shape<128, 128, 2, 4, 2, false>>(s, a);
   else if (!grid) launch_tiled<Shape<64, 64, 2, 2, 2, false>>(s, a);
   else if (best == 0) launch_tiled<Shape<256, 256, 2, 4, 2>>(s, a);
@@ -649,6 +650,7 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
   // one row's pitch says nothing
   if (M == 1) a_ms = (K + 15) & ~int64_t(15);
   if (N == 1) b_ns = (K + 15) & ~int64_t(15);
+  if (M == 1) c_ms = N;
   Int8Gemm a{A, B, a_scale, b_scale, C, bias, M, N, K, a_ms, b_ns, c_ms, 0, 0, 1,
              c_type, epilogue, 0};
   hipStream_t s = as_stream(stream);

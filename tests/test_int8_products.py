@@ -69,3 +69,14 @@ def test_each_product_runs_on_its_kernel_and_each_kernel_has_one(routes):
     for p, g, w in zip(asked, got, want):
         assert g == w, p
     assert {g.split(">")[0] for g in got} == {c.split(">")[0] for c in compiled}
+
+
+def test_what_goes_past_the_caches(routes):
+    """C of 192 MiB and more with whole rows on the 128-byte lines; not a few columns of a wide buffer."""
+    mib = 1 << 20
+    got, _ = routes([(BF16, 8192, 4096, 16384, 4096, 4096, 16384), (BF16, 8192, 4096, 16384, 4096, 4096, 16385),
+                     (BF16, 8192, 4096, 64, 4096, 4096, 16384), (F32, 65536, 256, 512, 256, 256, 65536),
+                     (F32, 65536, 256, 768, 256, 256, 65536), (BF16, 6144, 512, 16384, 512, 512, 16384),
+                     (BF16, 6143, 512, 16384, 512, 512, 32768)])
+    assert 6144 * 16384 * 2 == 192 * mib and 65536 * 768 * 4 == 192 * mib
+    assert [g.split("> ")[1] for g in got] == ["streamed", "cached", "cached", "cached", "streamed", "streamed", "cached"]
