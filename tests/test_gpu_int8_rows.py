@@ -8,6 +8,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_int8 import _check_rows, _f64, _normal
+
 pytestmark = pytest.mark.gpu
 
 HALF_TYPES = [torch.bfloat16, torch.float16]
@@ -81,3 +83,42 @@ def test_halves_go_to_the_even_number(K, dtype, cols):
     # at the type's largest and least normal exponents
     for f in (2.0 ** 14, 2.0 ** -5) if dtype == torch.float16 else (2.0 ** 126, 2.0 ** -117):
         assert torch.equal(K.quantize_rows(x * f)[0].cpu(), q)
+
+
+@pytest.mark.parametrize("cols", [5, 768, 4104, 33000])
+@pytest.mark.parametrize("dtype", HALF_TYPES + [torch.float32])
+def test_zeros_nan_infinities_and_the_ends_of_the_range(K, dtype, cols):
+    """Of every type, plain, normed and through GELU, whose value at -inf is NaN (-inf times 0) and at the
+    lowest number -0."""
+    info = torch.finfo(dtype)
+    x = _normal(1, (11, cols), dtype)
+    x[0] = 0
+    x[1, cols // 2] = math.nan
+    x[2, cols - 1] = math.inf
+    x[3, 0] = -math.inf
+    x[4] = info.max
+    x[5] = info.smallest_normal * info.eps  # the least number there is
+    x[6] = -0.0
+    x[7] = info.min
+    x[8, 0] = info.max  # the others are a fraction of a step
+    for mode in ("plain", "norm", "gelu"):
+        print(f"case: {mode}, special values, {cols} {dtype}", flush=True)
+        q, scale = K.add_rmsnorm_int8(x, eps=1e-6)[:2] if mode == "norm" else K.quantize_rows(x, gelu=mode == "gelu")
+        zeros = {0, 6} | ({7} if mode == "gelu" else set()) | (set() if dtype == torch.float16 else {5})
+        for r in zeros:
+            assert float(scale[r]) == 0 and not bool(q[r].any()), r
+        for r in (1, 2, 3):
+            assert math.isnan(float(scale[r])) and not bool(q[r].any()), r
+            assert bool(torch.isnan(K.dequantize_rows(q, scale, dtype)[r]).all())
+        keep = [r for r in range(11) if r not in zeros | {1, 2, 3}]
+        v = _f64(x)[keep]
+        if mode == "norm":
+            v = v / torch.sqrt((v * v).mean(dim=1, keepdim=True) + np.float64(np.float32(1e-6)))
+        elif mode == "gelu":
+            v = v / (1 + torch.exp(-2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))
+        # GELU: half a step of the exponent's rounding at each of 3, the exponential, the
+        # reciprocal and the product, of the row's largest value (a positive one)
+        _check_rows(q[keep], scale[keep], v, 16 * 2.0 ** -24 if mode == "gelu" else 2.0 ** -24)
+        for r in (4, 5):
+            assert r in zeros or bool((q[r] == 127).all())
+        assert mode == "gelu" or bool((q[7] == -127).all())
