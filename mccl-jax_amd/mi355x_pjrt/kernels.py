@@ -901,14 +901,16 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16, bias=None, relu=
 
 
 def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, index_dtype=torch.int32,
-                with_logprob=True, stream=None):
+                with_logprob=True, stream=None, token=None, logprob=None):
     """(token, logprob) of each row of [rows, vocab] logits, drawn with the
     random numbers u [rows] (fp32, in [0, 1)): softmax(logits / temperature)
     limited to the top_k largest, then to the fewest of those that hold top_p of
     their weight, then to those with at least min_p of the largest one's
     (mk_sample_rows has the exact terms).  Each limit is a number, None, or a
     tensor of one value a row (top_k int32, the others fp32).  temperature 0 is
-    row_argmax.  A row without a valid choice gives token -1 and logprob NaN."""
+    row_argmax.  A row without a valid choice gives token -1 and logprob NaN.
+    A given token [rows] (int32 or int64, whatever index_dtype says) and logprob
+    [rows] (fp32) are written in place of new ones."""
     what = "sample_rows"
     shape, strides, dev = logits.shape, logits.stride(), logits.get_device()
     mk = _ROW_TYPES.get(logits.dtype)
@@ -942,8 +944,17 @@ def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, 
         m = min_p.data_ptr()
     elif min_p is not None:
         m_all = float(min_p)
-    token = _new(logits, stream, index_dtype, shape[0])
-    logprob = _new(logits, stream, torch.float32, shape[0]) if with_logprob else None
+    if token is None:
+        token = _new(logits, stream, index_dtype, shape[0])
+    else:
+        index_dtype = token.dtype if token.dtype is torch.int64 else torch.int32
+        _operand(what, "token", token, index_dtype, per_row, dev)
+    if logprob is not None:
+        if not with_logprob:
+            raise ValueError(f"{what}: a logprob to write, and with_logprob false")
+        _operand(what, "logprob", logprob, torch.float32, per_row, dev)
+    elif with_logprob:
+        logprob = _new(logits, stream, torch.float32, shape[0])
     handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
     rc = (_lib._kernels or lib()).mk_sample_rows(handle, mk, shape[0], shape[1], logits.data_ptr(), ld, u.data_ptr(), t,
                                                  t_all, k, k_all, p, p_all, m, m_all, _TORCH_TO_MK[index_dtype],
