@@ -10,9 +10,9 @@
 // C (lane (c, g), reg r of the 32 x 32 form: row c, column 8 (r / 4) + 4 g + r % 4).
 //
 // Bound: the matrix cores at the power limit for many rows (8192 x 4096 x 16384, M x K x N,
-// 466 us, 2360 TOP/s; 8192 cubed 443 us), HBM for few, where the weights
-// are the traffic (16 x 4096 x 16384 13.7 us, 67 MB), launches and latency for one (1 x
-// 768 x 2304 3.9 us).
+// 466 to 505 us by the card, 2180 to 2360 TOP/s), HBM for few, where the weights
+// are the traffic (16 x 4096 x 16384 13.9 us, 67 MB), launches and latency for one (1 x
+// 768 x 2304 3.2 to 3.8 us).
 #include "attn_common.h"
 
 #include <algorithm>
@@ -194,9 +194,9 @@ void launch_rows(hipStream_t s, Int8Gemm a, int k_waves) {
 
 // Waves enough to fill the chip, from the columns (64 or 32 a wave where they are
 // many: less of A is read) and then from k.  us, by columns a wave and waves along
-// k: 16 x 4096 x 16384 (M x K x N) 16: 20.6 / 20.9 (2, 4), 32: 17.5 / 18.4 (4, 8),
-// 64: 16.3 (8); 16 x 512 x 16384 16: 4.8 (4), 32: 5.2 (4); 16 x 4096 x 4096 16: 17.1,
-// 10.1, 6.9, 6.9 (2, 4, 8, 16), 32: 8.5 (8); 1 x 768 x 2304 16: 3.1 (8).
+// k: 16 x 4096 x 16384 (M x K x N) 16: 17.5 / 17.6 (2, 4), 32: 15.1 / 15.8 (4, 8),
+// 64: 14.0 (8); 16 x 512 x 16384 16: 4.6 (4), 32: 4.6 (4); 16 x 4096 x 4096 16: 17.4,
+// 10.3, 7.2, 7.2 (2, 4, 8, 16), 32: 8.7 (8); 1 x 768 x 2304 16: 3.2 (8).
 template <int VN>
 void launch_few_rows(hipStream_t s, const Int8Gemm& a) {
   const int64_t blocks = (a.N + 16 * VN - 1) / (16 * VN);
@@ -335,11 +335,11 @@ typedef uint32_t u32x4_by4_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // C's tile through LDS, each wave for itself and without barriers: 32 rows of its
-// columns at a time, in its part of the operand stages (8192 x 768 x 50304 in bf16 466
-// us, 495 with the workgroup storing whole rows of the tile between barriers).  A lane writes 4 consecutive
-// columns, chunk c of staging row r at position c ^ (r & 15) (rows of 8 and 4 chunks:
-// c ^ ((r >> 1) & 7), c ^ ((r >> 2) & 3)), and the wave stores runs of 16 bytes (of whole
-// rows; they need no alignment past an element's).
+// columns at a time, in its part of the operand stages (8192 x 768 x 50304 in bf16, with
+// ordinary stores: 6% less than with the workgroup storing whole rows of the tile between
+// barriers).  A lane writes 4 consecutive columns, chunk c of staging row r at position
+// c ^ (r & 15) (rows of 8 and 4 chunks: c ^ ((r >> 1) & 7), c ^ ((r >> 2) & 3)), and the
+// wave stores runs of 16 bytes (of whole rows; they need no alignment past an element's).
 template <int CT, bool STREAM, int kWM, int kWN, int kI, int kJ>
 __device__ __attribute__((always_inline)) inline void store_tile(const Int8Gemm& p, const i32x16_t (&acc)[kI][kJ],
                                                                  int8_t* stage, const float* sa, const float* sb,
@@ -599,9 +599,10 @@ void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
     if (least == 0 || t < least) best = o, least = t;
   }
   // C past the caches where it is most of the last-level cache and its rows lie on the
-  // 128-byte lines; us, so / with ordinary stores: bf16 8192 x 768 x 50304 430 / 454,
-  // 8192 x 4096 x 16384 475 / 478, fp32 8192 x 768 x 50304 566 / 578, 8192 x 2048 x 16384
-  // 333 / 326; off the lines, bf16 8192 x 768 x 50264 584 / 495, fp32 x 50257 818 / 663
+  // 128-byte lines; us, so / with ordinary stores: bf16 8192 x 768 x 50304 394 / 473,
+  // 8192 x 4096 x 16384 475 / 490, fp32 8192 x 768 x 50304 482 / 590, 8192 x 2048 x 16384
+  // 291 / 326.  Off the lines not every C gains: fp32 8192 x 768 x 50257 680 / 672, x 50260
+  // 632 / 655, bf16 x 50264 402 / 494; all of those take ordinary stores
   const int64_t pitch = a.ldc * dtype_bytes(a.c_type);
   a.stream_c = a.M * a.N * dtype_bytes(a.c_type) >= int64_t(192) << 20 && pitch % 128 == 0 &&
                reinterpret_cast<uintptr_t>(a.C) % 128 == 0;
@@ -615,6 +616,8 @@ void launch_best_tile(hipStream_t s, Int8Gemm& a, bool grid) {
 }
 
 // rows on the 16-byte grid that do not overlap, below the 2^31 bytes of a buffer's offsets
+// (an operand of more is loaded through registers: 131056 x 16384 x 4096 7.0 ms, 131088
+// rows 10.9)
 bool on_grid(const int8_t* p, int64_t rows, int64_t K, int64_t ld) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 16 == 0 && ld >= K && ld < (int64_t(1) << 31) &&
          (rows - 1) * ld + K + 16 < (int64_t(1) << 31);
@@ -655,9 +658,11 @@ extern "C" int mk_gemm_int8(void* stream, int c_type, int64_t M, int64_t N, int6
              c_type, epilogue, 0};
   hipStream_t s = as_stream(stream);
   const bool grid = K > 0 && on_grid(A, M, K, a_ms) && on_grid(B, N, K, b_ns);
-  // few rows off the grid, or where the weights alone are the work; from 17 rows or
-  // 32768 columns on the tiles share A's reads (32 x 4096 x 16384 19.1 us, 22 so; 16 x
-  // 768 x 50257 11.4, 14.1; 32 x 4096 x 4096 9.7, 9.2)
+  // few rows off the grid, or up to where the tiles are ahead (from 17 rows on they share
+  // A's reads; for wide weights they are from one row on).  us, rows kernel / tiles:
+  // 32 x 4096 x 16384 16.9 / 13.4; 32 x 4096 x 4096 9.5 / 10.0; 32 x 4096 x 8192 11.7 / 10.3;
+  // fp32 C 1 x 768 x 50257 10.5 / 9.1, 16 rows 13.0 / 9.6; 1 x 4096 x 128256 118 / 108, 16 rows
+  // 126 / 113; bf16 C 1 x 4096 x 32768 30 / 33
   if (small_c(a, grid)) launch_small(s, a);
   else if (M <= 64 && (!grid || (M <= 16 && N < 32768) || (M <= 32 && N <= 8192))) launch_few_rows(s, a);
   else launch_best_tile(s, a, grid);

@@ -13,13 +13,14 @@
 // square in 32.  The maximum is taken over the bits of |t| as whole numbers,
 // where NaN is above infinity is above every number, so neither is lost.
 //
-// Bound: HBM, each operand once: the norm of 8192 x 4096 in bf16 (235 MB) takes 38 us,
-// rounding 50257 x 768 of fp32 (193 MB) 34 us, the way back 36 us, where a copy of
-// 200 MiB moves 5.4 MB a us.  One row is a launch and two round trips to memory: 768 in
-// 2.7 us.  A team of W waves has a row; its lanes hold up to NV chunks of 16 bytes each.
+// Bound: HBM, each operand once, at the 5.4 MB a us of a 200 MiB copy: the norm of 8192 x
+// 4096 in bf16 (235 MB) takes 43 us, rounding 50257 x 768 of fp32 (193 MB) 34 us, the way
+// back 36 us (operands of three calls in turn; of one call, part of them stays in the
+// last-level cache: 37, 28, 29 us).  One row is a launch and two round trips to memory: 768 in
+// 2.8 us.  A team of W waves has a row; its lanes hold up to NV chunks of 16 bytes each.
 // The last chunk of a row that is no whole number of chunks is the row's last 16 bytes:
 // what it shares with the chunk before it is left out of the sum and written twice
-// with the same values (after every load of the row, so that outputs may be inputs).
+// with the same values (after every load of the row, so that the sum may be x or r).
 #include "mk_common.h"
 
 #include <algorithm>
@@ -289,11 +290,12 @@ void launch_held(hipStream_t s, const RowsArgs& a) {
 }
 
 // Teams by the row's chunks: as few waves as hold the row in 2 to 4 chunks a lane, more
-// where they would leave CUs idle.  us, for W x NV, bf16: norm of 8192 x 768 1 x 2: 11.2,
-// 2 x 1: 12.7, 4 x 1: 18.6; of 8192 x 2048 2 x 2: 21.2, 1 x 4: 22.2, 4 x 1: 22.2; of 256 x
-// 2048 2 x 2: 3.8, 4 x 1: 3.6; of 8192 x 4096 4 x 2: 38.1, 1 x 8: 42.9, 8 x 1: 43.8, 16 x 1:
-// 72; of 1 x 8192 4 x 4: 3.6, 8 x 2: 3.6, 16 x 1: 4.0; of 4096 x 16384 8 x 4: 91, 4 x 8: 88,
-// 16 x 2: 99; of 64 x 16384 5.5, 6.0, 6.0.  50257 x 768 of fp32 to 8 bits 2 x 2: 34, 4 x 1: 46.
+// where they would leave CUs idle.  us, for W x NV, bf16 (every sum to the same memory,
+// which stays in the last-level cache): norm of 8192 x 768 1 x 2: 11.2, 2 x 1: 12.7, 4 x 1:
+// 18.6; of 8192 x 2048 2 x 2: 21.2, 1 x 4: 22.2, 4 x 1: 22.2; of 256 x 2048 2 x 2: 3.8, 4 x 1:
+// 3.6; of 8192 x 4096 4 x 2: 38.1, 1 x 8: 42.9, 8 x 1: 43.8, 16 x 1: 72; of 1 x 8192 4 x 4:
+// 3.6, 8 x 2: 3.6, 16 x 1: 4.0; of 4096 x 16384 8 x 4: 91, 4 x 8: 88, 16 x 2: 99; of 64 x 16384
+// 5.5, 6.0, 6.0.  50257 x 768 of fp32 to 8 bits 2 x 2: 34, 4 x 1: 46.
 // Longer rows than 16 x 4 holds are read twice: 1024 x 16384 of fp32 47 us held, 69 so.
 template <typename T, Mode M>
 int launch_rows(hipStream_t s, const RowsArgs& a, const char* what) {
