@@ -578,6 +578,78 @@ int mk_sdpa_bwd(void* stream, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int6
                 float scale, int causal, void* workspace);
 
 /* ========================================================================
+ * What a training step needs beside the above and the reference has no
+ * counterpart of: the loss over a large vocabulary without the logits in
+ * memory, and dropout without its mask in memory.  Rows are `ld_*` elements
+ * apart (inputs: any pitch >= 0, outputs: at least their columns), their
+ * elements contiguous; pointers need the alignment of their elements.
+ * io_type in {MK_BF16, MK_F16, MK_F32}.
+ * ====================================================================== */
+
+/* Softmax cross entropy of the logits x wᵀ, x [rows, width] and w [vocab, width]
+ * (mk_gemm and mk_softmax_xent in one, the logits never stored):
+ *   s[n][v] = sum_d x[n][d] w[v][d]          (fp32 accumulation)
+ *   lse[n] = log sum_v exp(s[n][v]);  loss_rows[n] = lse[n] - s[n][labels[n]]
+ * Labels are MK_S32 or MK_S64.  A label outside [0, vocab) has no target term
+ * (loss_rows[n] = lse[n], as in mk_softmax_xent); with has_ignore, rows whose
+ * label is ignore_index have loss 0.  lse is each row's, ignored or not.
+ * loss_rows and lse are fp32 [rows], either may be NULL.  The vocabulary is
+ * gone through in tiles, of which the workspace holds each row's maximum and
+ * sum.  Operands off the 16-byte boundaries (base, pitch or width) are copied
+ * to them first, w piece by piece; the size of the workspace counts that, so
+ * the pointers and pitches given to it are those of the call. */
+size_t mk_linear_xent_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
+                                      int64_t ld_x, const void* w, int64_t ld_w);
+int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x, int64_t ld_x,
+                   const void* w, int64_t ld_w, int label_type, const void* labels, int has_ignore,
+                   int64_t ignore_index, float* loss_rows, float* lse, void* workspace);
+
+/* Its gradient, from lse of the forward pass:
+ *   g[n][v] = (exp(s[n][v] - lse[n]) - [v == labels[n]]) * row_grad[n] * grad_scale
+ *   dx[n][d] = sum_v g[n][v] w[v][d],  dw[v][d] = sum_n g[n][v] x[n][d]
+ * row_grad (fp32 [rows]) may be NULL (1).  grad_scale = 1 / rows gives the
+ * gradient of the mean loss.  With has_ignore, rows whose label is
+ * ignore_index have a gradient of 0 and add nothing to dw, whatever their x
+ * holds.  g is formed in pieces of the vocabulary and rounded to io_type (before
+ * grad_scale; for MK_F16 scaled by powers of two out of the subnormals), the
+ * operand of the products with w and x; their sums are fp32, in a fixed order:
+ * the same inputs give the same bits.  dx is of io_type, dw of dw_type (io_type
+ * or MK_F32); either may be NULL, then only the other is computed.  dx may not
+ * overlap x, nor dw w.  Workspace as above. */
+size_t mk_linear_xent_bwd_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
+                                          int64_t ld_x, const void* w, int64_t ld_w, int has_ignore);
+int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_t rows, int64_t width, int64_t vocab,
+                       const void* x, int64_t ld_x, const void* w, int64_t ld_w, int label_type, const void* labels,
+                       int has_ignore, int64_t ignore_index, const float* lse, const float* row_grad,
+                       float grad_scale, void* dx, int64_t ld_dx, void* dw, int64_t ld_dw, void* workspace);
+
+/* Dropout of a branch and its way into the residual stream, in one pass:
+ *   out[r][c] = residual[r][c] + keep(r, c) * (x[r][c] + bias[c]) * 65536 / (65536 - T)
+ * with T = p * 65536 rounded to a whole number (halves to even), so that p is a
+ * multiple of 2^-16 and the scale undoes exactly what is dropped.  keep(r, c) is
+ * 1 where f >= T, f the 16-bit field c % 8 (low half of word 0 first) of the four
+ * 32-bit words that Philox-4x32 of 10 rounds (Salmon, Moraes, Dror, Shaw, SC
+ * 2011) gives for the key (seed mod 2^32, seed / 2^32) and the counter (c / 8, r,
+ * o mod 2^32, o / 2^32), o = offset + *step (step: one 64-bit number on the
+ * device, which a captured launch reads anew on every replay; NULL: 0).  A call
+ * with the same seed, o and p drops the same elements, whatever their type,
+ * pitch and device.  A dropped element is the residual itself (0 without one),
+ * whatever x holds.  fp32 math, one rounding.  bias and residual may be NULL;
+ * out may be x or residual, at its pitch.  p in [0, 1]; rows below 2^32, cols up to 2^31. */
+int mk_dropout_add(void* stream, int io_type, int64_t rows, int64_t cols, const void* x, int64_t ld_x,
+                   const void* bias, const void* residual, int64_t ld_residual, double p, uint64_t seed,
+                   uint64_t offset, const uint64_t* step, void* out, int64_t ld_out);
+
+/* Its gradient: dx[r][c] = keep(r, c) * dy[r][c] * 65536 / (65536 - T), the
+ * branch's, and dx_colsum[c] = sum_r dx[r][c] before its rounding, the bias's
+ * (fp32, in a fixed order; may be NULL, then no workspace is needed).  The
+ * residual's is dy.  dx may be dy, at its pitch. */
+size_t mk_dropout_add_bwd_workspace_bytes(int64_t rows, int64_t cols);
+int mk_dropout_add_bwd(void* stream, int io_type, int64_t rows, int64_t cols, const void* dy, int64_t ld_dy, double p,
+                       uint64_t seed, uint64_t offset, const uint64_t* step, void* dx, int64_t ld_dx,
+                       float* dx_colsum, void* workspace);
+
+/* ========================================================================
  * Eight-bit serving.  No counterpart in the reference: products whose operands
  * are rows of whole numbers of 8 bits with an fp32 scale each (half the bytes of
  * bf16 and twice its matrix rate), what makes such rows, and the choice of

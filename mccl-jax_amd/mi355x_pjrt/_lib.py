@@ -100,6 +100,16 @@ SIGNATURES = {
     "mk_sdpa_bwd": (_I, [_P, _I64, _I64, _I64, _I64, _I64]
                     + [_P, _I64, _I64, _I64] * 5 + [_P]
                     + [_P, _I64, _I64, _I64] * 3 + [_F, _I, _P]),
+    "mk_linear_xent_workspace_bytes": (ctypes.c_size_t, [_I, _I64, _I64, _I64, _P, _I64, _P, _I64]),
+    "mk_linear_xent": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I64, _I, _P, _I, _I64, _P, _P, _P]),
+    "mk_linear_xent_bwd_workspace_bytes": (ctypes.c_size_t, [_I, _I64, _I64, _I64, _P, _I64, _P, _I64, _I]),
+    "mk_linear_xent_bwd": (_I, [_P, _I, _I, _I64, _I64, _I64, _P, _I64, _P, _I64, _I, _P, _I, _I64, _P, _P, _F, _P,
+                                _I64, _P, _I64, _P]),
+    "mk_dropout_add": (_I, [_P, _I, _I64, _I64, _P, _I64, _P, _P, _I64, ctypes.c_double, ctypes.c_uint64,
+                            ctypes.c_uint64, _P, _P, _I64]),
+    "mk_dropout_add_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "mk_dropout_add_bwd": (_I, [_P, _I, _I64, _I64, _P, _I64, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _P,
+                                _P, _I64, _P, _P]),
     "mk_add_rmsnorm_int8": (_I, [_P, _I, _I64, _I64, _P, _I64, _P, _I64, _P, _F, _P, _I64, _P, _I64, _P]),
     "mk_quantize_rows": (_I, [_P, _I, _I64, _I64, _P, _I64, _I, _P, _I64, _P]),
     "mk_dequantize_rows": (_I, [_P, _I, _I64, _I64, _P, _I64, _P, _P, _I64]),

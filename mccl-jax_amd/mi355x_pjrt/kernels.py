@@ -962,3 +962,192 @@ def sample_rows(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, 
     if rc:
         _check(rc, "mk_sample_rows")
     return token, logprob
+
+
+# ------------------------------------------------------------------ loss without logits, dropout without a mask
+def _labels(what, labels, rows, dev):
+    if labels.dtype is not torch.int32 and labels.dtype is not torch.int64:
+        raise ValueError(f"{what}: labels must be int32 or int64")
+    if labels.numel() != rows or not labels.is_contiguous():
+        raise ValueError(f"{what}: labels must be one contiguous number a row")
+    if labels.get_device() != dev:
+        raise ValueError(f"{what}: labels is not on the current device")
+    return _TORCH_TO_MK[labels.dtype]
+
+
+def _xent_operands(what, x, w):
+    """(type, rows, width, vocab, device) of x [rows, width] and w [vocab, width]."""
+    dev = x.get_device()
+    t = _ROW_TYPES.get(x.dtype)
+    shape, strides = x.shape, x.stride()
+    if t is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
+        _refuse_rows(what, "x", x)
+    if w.dim() != 2 or w.shape[1] != shape[1]:
+        raise ValueError(f"{what}: x [rows, width] and w [vocab, width] expected, got {tuple(shape)} and {tuple(w.shape)}")
+    _operand(what, "w", w, x.dtype, w.shape, dev)
+    return t, shape[0], shape[1], w.shape[0], dev
+
+
+def _bytes(what, like, nbytes, workspace, stream, dev):
+    if workspace is None:
+        return _new(like, stream, torch.uint8, max(int(nbytes), 1))
+    if workspace.get_device() != dev or not workspace.is_contiguous() or workspace.data_ptr() % 16 or \
+            workspace.numel() * workspace.element_size() < nbytes:
+        raise ValueError(f"{what}: workspace must be {int(nbytes)} contiguous bytes or more on the current device, "
+                         "on a 16-byte boundary")
+    return workspace
+
+
+def linear_xent(x, w, labels, ignore_index=None, loss_rows=None, lse=None, workspace=None, stream=None):
+    """(loss_rows, lse): softmax cross entropy of the logits x @ w.t() and their
+    log-sum-exp, fp32 [rows] each, for x [rows, width] and w [vocab, width]; the
+    logits are not stored (mk_linear_xent).  Rows with label ignore_index have
+    loss 0; another label outside the vocabulary has no target term, as in
+    softmax_xent.  Outputs and a workspace that are not given come from the
+    memory of `stream`."""
+    what = "linear_xent"
+    t, rows, width, vocab, dev = _xent_operands(what, x, w)
+    label_type = _labels(what, labels, rows, dev)
+    if loss_rows is None:
+        loss_rows = _new(x, stream, torch.float32, rows)
+    else:
+        _operand(what, "loss_rows", loss_rows, torch.float32, (rows,), dev)
+    if lse is None:
+        lse = _new(x, stream, torch.float32, rows)
+    else:
+        _operand(what, "lse", lse, torch.float32, (rows,), dev)
+    L = _lib._kernels or lib()
+    at = (x.data_ptr(), x.stride()[0], w.data_ptr(), w.stride()[0])
+    ws = _bytes(what, x, L.mk_linear_xent_workspace_bytes(t, rows, width, vocab, *at), workspace, stream, dev)
+    rc = L.mk_linear_xent(_handle(what, stream, dev), t, rows, width, vocab, *at, label_type, labels.data_ptr(),
+                          ignore_index is not None, ignore_index or 0, loss_rows.data_ptr(), lse.data_ptr(),
+                          ws.data_ptr())
+    if rc:
+        _check(rc, "mk_linear_xent")
+    return loss_rows, lse
+
+
+def linear_xent_bwd(x, w, labels, lse, grad_scale=1.0, row_grad=None, ignore_index=None, dx=None, dw=None,
+                    dw_dtype=None, want_dx=True, want_dw=True, workspace=None, stream=None):
+    """(dx, dw) of sum_n row_grad[n] * grad_scale * loss_rows[n], with lse of
+    linear_xent (mk_linear_xent_bwd); grad_scale 1 / rows is the mean loss's.
+    row_grad: fp32 [rows] or None (1).  Rows with label ignore_index get a dx of 0
+    and add nothing to dw, whatever their x holds.  dw is of w's type, or fp32
+    (dw_dtype, or a given dw's); want_dx and want_dw leave one out (None)."""
+    what = "linear_xent_bwd"
+    t, rows, width, vocab, dev = _xent_operands(what, x, w)
+    label_type = _labels(what, labels, rows, dev)
+    _operand(what, "lse", lse, torch.float32, (rows,), dev)
+    if row_grad is not None:
+        _operand(what, "row_grad", row_grad, torch.float32, (rows,), dev)
+    if not want_dx:
+        dx = None
+    elif dx is None:
+        dx = _new(x, stream, x.dtype, rows, width)
+    else:
+        _result(what, "dx", dx, x.dtype, (rows, width), dev)
+    if not want_dw:
+        dw = None
+    else:
+        dw_dtype = dw_dtype or (w.dtype if dw is None else dw.dtype)
+        if dw_dtype is not w.dtype and dw_dtype is not torch.float32:
+            raise ValueError(f"{what}: dw must be of w's type or fp32")
+        if dw is None:
+            dw = _new(x, stream, dw_dtype, vocab, width)
+        else:
+            _result(what, "dw", dw, dw_dtype, (vocab, width), dev)
+    L = _lib._kernels or lib()
+    at = (x.data_ptr(), x.stride()[0], w.data_ptr(), w.stride()[0])
+    ws = _bytes(what, x, L.mk_linear_xent_bwd_workspace_bytes(t, rows, width, vocab, *at,
+                                                                       ignore_index is not None),
+                         workspace, stream, dev)
+    rc = L.mk_linear_xent_bwd(_handle(what, stream, dev), t, t if dw is None else _TORCH_TO_MK[dw.dtype], rows, width,
+                              vocab, *at, label_type, labels.data_ptr(), ignore_index is not None, ignore_index or 0,
+                              lse.data_ptr(), _ptr(row_grad), float(grad_scale), _ptr(dx),
+                              0 if dx is None else dx.stride()[0], _ptr(dw), 0 if dw is None else dw.stride()[0],
+                              ws.data_ptr())
+    if rc:
+        _check(rc, "mk_linear_xent_bwd")
+    return dx, dw
+
+
+def _draw(what, seed, offset, step, dev):
+    """seed, offset and the address of step as the C-ABI takes them."""
+    if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
+        raise ValueError(f"{what}: seed and offset are whole numbers of 64 bits")
+    if step is None:
+        return None
+    if step.dtype is not torch.int64 or step.numel() != 1 or step.get_device() != dev:
+        raise ValueError(f"{what}: step must be one int64 on the current device")
+    return step.data_ptr()
+
+
+def dropout_add(x, p, seed, offset=0, step=None, bias=None, residual=None, out=None, stream=None):
+    """residual + dropout(x + bias) for 2-D x (mk_dropout_add; bias [cols] and
+    residual are optional).  Elements are dropped by the counter-based generator's
+    numbers for (seed, offset + step, row, column): the same call drops the same
+    ones, and dropout_add_bwd with the same numbers knows which.  step: one int64
+    on the device, for a captured step that draws anew on every replay.  out may
+    be x or residual."""
+    what = "dropout_add"
+    dtype, shape, strides, dev = x.dtype, x.shape, x.stride(), x.get_device()
+    t = _ROW_TYPES.get(dtype)
+    if t is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
+        _refuse_rows(what, "x", x)
+    rows, cols = shape
+    r_ptr, r_ld, b_ptr = None, 0, None
+    if residual is not None:
+        _operand(what, "residual", residual, dtype, shape, dev)
+        r_ptr, r_ld = residual.data_ptr(), residual.stride()[0]
+    if bias is not None:
+        _operand(what, "bias", bias, dtype, (cols,), dev)
+        b_ptr = bias.data_ptr()
+    if out is None:
+        out = x.new_empty(shape) if stream is None else _new(x, stream, dtype, rows, cols)
+        ld = cols
+    else:
+        _result(what, "out", out, dtype, shape, dev)
+        ld = out.stride()[0]
+    s_ptr = _draw(what, seed, offset, step, dev)
+    handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
+    rc = (_lib._kernels or lib()).mk_dropout_add(handle, t, rows, cols, x.data_ptr(), strides[0], b_ptr, r_ptr, r_ld, p,
+                                                 seed, offset, s_ptr, out.data_ptr(), ld)
+    if rc:
+        _check(rc, "mk_dropout_add")
+    return out
+
+
+def dropout_add_bwd(dy, p, seed, offset=0, step=None, want_colsum=False, dx=None, colsum=None, workspace=None,
+                    stream=None):
+    """(dx, colsum) of dropout_add with the same p, seed, offset and step: dx of
+    its branch, and (want_colsum, or a colsum [cols] fp32 to write) the column
+    sums of dx before rounding, the bias's gradient; else None
+    (mk_dropout_add_bwd).  The residual's gradient is dy itself; dx may be dy."""
+    what = "dropout_add_bwd"
+    dtype, shape, strides, dev = dy.dtype, dy.shape, dy.stride(), dy.get_device()
+    t = _ROW_TYPES.get(dtype)
+    if t is None or len(shape) != 2 or dev < 0 or dev != _device() or (strides[1] != 1 and shape[1] > 1):
+        _refuse_rows(what, "dy", dy)
+    rows, cols = shape
+    if dx is None:
+        dx = dy.new_empty(shape) if stream is None else _new(dy, stream, dtype, rows, cols)
+        ld = cols
+    else:
+        _result(what, "dx", dx, dtype, shape, dev)
+        ld = dx.stride()[0]
+    L = _lib._kernels or lib()
+    c_ptr = w_ptr = None
+    if colsum is not None:
+        _operand(what, "colsum", colsum, torch.float32, (cols,), dev)
+    elif want_colsum:
+        colsum = _new(dy, stream, torch.float32, cols)
+    if colsum is not None:
+        workspace = _bytes(what, dy, L.mk_dropout_add_bwd_workspace_bytes(rows, cols), workspace, stream, dev)
+        c_ptr, w_ptr = colsum.data_ptr(), workspace.data_ptr()
+    s_ptr = _draw(what, seed, offset, step, dev)
+    handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
+    rc = L.mk_dropout_add_bwd(handle, t, rows, cols, dy.data_ptr(), strides[0], p, seed, offset, s_ptr, dx.data_ptr(), ld,
+                              c_ptr, w_ptr)
+    if rc:
+        _check(rc, "mk_dropout_add_bwd")
+    return dx, colsum

@@ -1,0 +1,921 @@
+// Softmax cross entropy over a large vocabulary from the hidden rows and the
+// embedding (mk_linear_xent), and its gradient (mk_linear_xent_bwd), without
+// the logits in memory.
+//
+//   s[n][v] = x[n] . w[v];  lse[n] = log sum_v exp s[n][v];  loss[n] = lse[n] - s[n][label]
+//   g[n][v] = (exp(s[n][v] - lse[n]) - [v == label]) row_grad[n] grad_scale
+//   dx = g w,  dw = gᵀ x
+//
+// Forward: one product, tile by tile; a tile ends with each of its rows' maximum
+// and sum of exponentials (8 bytes a row for TN logits), and a second launch joins
+// a row's tiles.  Backward, piece by piece of the vocabulary: the same product
+// again, ending with g in the operands' type (a matrix product reads it next;
+// its rounding is as small as that of the gradients themselves, and it is formed
+// from fp32 logits), then dx and dw of the piece in one launch.
+// The products are tiles as in gemm_tiled.hip (copies HBM -> LDS, two stages, k
+// tiles of 128 bytes a row); fp32 operands take the same bytes and the fp32 MFMA.
+// Operand bases move along k in 64 bits, so no operand's size is limited by a
+// buffer's 32-bit offsets.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <string>
+
+#include "gemm_tile.h"
+
+namespace mk {
+namespace {
+
+using namespace attn;
+
+constexpr int kGroupM = 4;                  // tile rows per group of the tile order
+constexpr int kInvalid = int(0x80000000u);  // buffer offset past the range of every copy
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kThreads = 256;               // of the kernels without products
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// Element types: bytes, elements of a 16-byte chunk, and the MFMA step of one
+// chunk an operand: 16 k of 16 bits, or 8 k of 32 bits in four instructions of 2
+// (lane half g has k 4 g .. 4 g + 3 of them, in both operands).
+struct Bf16 {
+  static constexpr int esz = 2, mk = MK_BF16;
+  static __device__ inline f32x16_t mma(const u32x4_t& b, const u32x4_t& a, const f32x16_t& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(b), as_bf16x8(a), c, 0, 0, 0);
+  }
+};
+struct F16 {
+  static constexpr int esz = 2, mk = MK_F16;
+  static __device__ inline f32x16_t mma(const u32x4_t& b, const u32x4_t& a, const f32x16_t& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, b), __builtin_bit_cast(f16x8_t, a), c, 0,
+                                                  0, 0);
+  }
+};
+struct F32 {
+  static constexpr int esz = 4, mk = MK_F32;
+  static __device__ inline f32x16_t mma(const u32x4_t& b, const u32x4_t& a, f32x16_t c) {
+    const f32x4_t bf = __builtin_bit_cast(f32x4_t, b), af = __builtin_bit_cast(f32x4_t, a);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(bf[e], af[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// BK: 16-bit elements of a k tile (128 bytes a row whatever the type)
+using Big = Shape<256, 256, 2, 4, 64, 2>;
+using Mid = Shape<128, 128, 4, 2, 64, 2>;
+
+template <class Sh>
+struct Geo {
+  static constexpr int W = Sh::WGM * Sh::WGN, threads = 64 * W;
+  static constexpr int WM = Sh::TM / Sh::WGM, WN = Sh::TN / Sh::WGN;  // wave block
+  static constexpr int I = WM / 32, J = WN / 32;                      // MFMA blocks of it
+  static constexpr int lds_bytes = Sh::S * 128 * (Sh::TM + Sh::TN);
+  static_assert(Sh::TM * Sh::TN * 2 <= lds_bytes, "a 16-bit tile is staged where the operands were");
+  static_assert(Sh::S == 2 && Sh::BK == 64, "the k loop below");
+};
+template <class Sh>
+using Acc = f32x16_t[Geo<Sh>::I][Geo<Sh>::J];
+
+// ---------------------------------------------------------------- operand copies
+// The 1 KB copies one wave makes of one operand's k tile (gemm_tiled.hip's
+// Copies): their byte offsets from the tile's base, and the first k each reads.
+// `base` is the tile's first row (KC) or column (!KC) at its first k; rows: those
+// of the tile inside the operand.
+template <class T, bool KC, int R, int W>
+struct Operand {
+  static constexpr int kE = 16 / T::esz, kDeep = 128 / T::esz, kC = R / (8 * W);
+  static constexpr int kCpr = KC ? 8 : R / kE;  // chunks of an LDS row
+  static_assert(kC * 8 * W == R, "copies split evenly over the waves");
+  const char* base;
+  int64_t step;  // bytes from a k tile to the next
+  uint32_t off[kC];
+  int32_t k[kC];
+  __device__ inline Operand(int wave, int lane, const char* base, int64_t rows, int64_t ld)
+      : base(base), step(KC ? 128 : kDeep * ld * T::esz) {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const int u = 64 * (wave + W * c) + lane, r = u / kCpr;
+      int row;
+      if constexpr (KC) {
+        row = r;
+        k[c] = kE * ((u % kCpr) ^ kc_swizzle<64>(row));
+        off[c] = uint32_t(row * ld * T::esz + k[c] * T::esz);
+      } else {
+        row = kE * ((u % kCpr) ^ (T::esz == 2 ? nc_swizzle<R>(r) : 0));
+        k[c] = r;
+        off[c] = uint32_t(r * ld * T::esz + row * T::esz);
+      }
+      if (row >= rows) off[c] = uint32_t(kInvalid), k[c] = 0x7fffffff - kDeep;
+    }
+  }
+  // copies [lo, hi) of k tile kt, of which the operand has K - kDeep kt k
+  __device__ inline void issue(int kt, int64_t K, char* tile, int wave, int lo, int hi) const {
+    const i32x4_t r = tile_desc(base + kt * step, uint32_t(kInvalid));
+    const int64_t left = K - int64_t(kDeep) * kt;
+    if (left >= kDeep) {
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        if (c >= lo && c < hi) copy_to_lds_so(r, lds_addr(tile + 1024 * (wave + W * c)), int(off[c]), 0);
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+      if (c >= lo && c < hi)
+        copy_to_lds(r, lds_addr(tile + 1024 * (wave + W * c)), k[c] < left ? int(off[c]) : kInvalid);
+  }
+};
+
+template <class T, bool KC, int R>
+__device__ inline u32x4_t read_chunk(const char* t, int rb, int ks, int lane) {
+  if constexpr (KC || T::esz == 2) {  // a k-contiguous row is 8 chunks of 16 bytes in either width
+    return read_operand16<KC, R, 64>(reinterpret_cast<const uint16_t*>(t), rb, ks, lane);
+  } else {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(t) + (8 * ks + 4 * (lane >> 5)) * R + rb + (lane & 31);
+    return u32x4_t{p[0], p[R], p[2 * R], p[3 * R]};
+  }
+}
+
+// acc += A B of one workgroup tile over K: the k loop of gemm_tiled.hip.  A wave
+// waits for its own copies of tile kt, the barrier publishes all and frees the
+// other stage, whose copies are issued beside the first k-steps' MFMAs.  Ends with
+// a barrier: the operands' LDS is free.
+template <class T, class Sh, bool AKC, bool BKC>
+__device__ __attribute__((always_inline)) inline void product(const char* A, int64_t lda, int64_t a_rows,
+                                                              const char* B, int64_t ldb, int64_t b_rows, int64_t K,
+                                                              char* lds, int wave, int lane, Acc<Sh>& acc) {
+  using G = Geo<Sh>;
+  const int wm = wave / Sh::WGN, wn = wave % Sh::WGN;
+  const Operand<T, AKC, Sh::TM, G::W> oa(wave, lane, A, a_rows, lda);
+  const Operand<T, BKC, Sh::TN, G::W> ob(wave, lane, B, b_rows, ldb);
+  constexpr int kCa = Sh::TM / (8 * G::W), kCb = Sh::TN / (8 * G::W), kA = Sh::TM * 128, kStage = 128 * (Sh::TM + Sh::TN);
+  constexpr int kDeep = 128 / T::esz;
+  const int nk = int((K + kDeep - 1) / kDeep);
+  if (nk > 0) {
+    oa.issue(0, K, lds, wave, 0, kCa);
+    ob.issue(0, K, lds + kA, wave, 0, kCb);
+  }
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_vm<0>();
+    lds_barrier();
+    const char* at = lds + (kt & 1) * kStage;
+    char* next = lds + ((kt + 1) & 1) * kStage;
+    const bool more = kt + 1 < nk;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      u32x4_t af[G::I], bf[G::J];
+#pragma unroll
+      for (int a = 0; a < G::I; ++a) af[a] = read_chunk<T, AKC, Sh::TM>(at, wm * G::WM + 32 * a, ks, lane);
+#pragma unroll
+      for (int b = 0; b < G::J; ++b) bf[b] = read_chunk<T, BKC, Sh::TN>(at + kA, wn * G::WN + 32 * b, ks, lane);
+      if (more && ks < 2) {
+        if (ks == 0) oa.issue(kt + 1, K, next, wave, 0, kCa);
+        else ob.issue(kt + 1, K, next + kA, wave, 0, kCb);
+      }
+#pragma unroll
+      for (int a = 0; a < G::I; ++a)
+#pragma unroll
+        for (int b = 0; b < G::J; ++b) acc[a][b] = T::mma(bf[b], af[a], acc[a][b]);
+    }
+  }
+  lds_barrier();
+}
+
+template <class Sh>
+__device__ inline void zero(Acc<Sh>& acc) {
+#pragma unroll
+  for (int a = 0; a < Geo<Sh>::I; ++a)
+#pragma unroll
+    for (int b = 0; b < Geo<Sh>::J; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+}
+
+// Tile t of a tiles_m x tiles_n grid, for workgroup i of nt: an XCD (i % 8) has a
+// run of tiles, which walk groups of 4 tile rows column by column.
+__device__ inline void tile_of(uint32_t i, uint32_t nt, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+  const uint32_t per = nt / 8, t = i < 8 * per ? (i % 8) * per + i / 8 : i;
+  const uint32_t first = t / (kGroupM * tiles_n) * kGroupM, gm = min(uint32_t(kGroupM), tiles_m - first);
+  const uint32_t in = t - first * tiles_n;
+  tm = first + in % gm;
+  tn = in / gm;
+}
+
+// ---------------------------------------------------------------- labels
+struct Labels {
+  const void* p;
+  int wide;  // int64
+  int has_ignore;
+  int64_t ignore;
+  __device__ inline int64_t at(int64_t n) const {
+    return wide ? static_cast<const int64_t*>(p)[n] : int64_t(static_cast<const int32_t*>(p)[n]);
+  }
+  __device__ inline bool ignored(int64_t label) const { return has_ignore && label == ignore; }
+};
+
+// ---------------------------------------------------------------- forward
+struct LossArgs {
+  const char *x, *w;       // w: of this piece
+  int64_t rows, width, vocab;  // vocab: of this piece
+  int64_t ld_x, ld_w;
+  int64_t v0;              // the piece's first class
+  int tiles_m, tiles_n;
+  Labels labels;
+  float2* part;            // [tiles_n][rows]: maximum and sum of exponentials
+  float* target;           // [rows]: the label's logit
+};
+
+template <class T, class Sh>
+__global__ __launch_bounds__(Geo<Sh>::threads, 1) void loss_kernel(const LossArgs p) {
+  using G = Geo<Sh>;
+  __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, gridDim.x, uint32_t(p.tiles_m), uint32_t(p.tiles_n), tm, tn);
+  const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
+  Acc<Sh> acc;
+  zero<Sh>(acc);
+  product<T, Sh, true, true>(p.x + m0 * p.ld_x * T::esz, p.ld_x, p.rows - m0, p.w + n0 * p.ld_w * T::esz, p.ld_w,
+                             p.vocab - n0, p.width, lds, wave, lane, acc);
+  // a lane has, of row 32 a + c, the columns 32 b + 8 (r / 4) + 4 g + r % 4
+  const int nl = wn * G::WN + 4 * g;
+  if (n0 + Sh::TN > p.vocab) {
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (n0 + nl + 32 * b + 8 * (r / 4) + r % 4 >= p.vocab)
+#pragma unroll
+          for (int a = 0; a < G::I; ++a) acc[a][b][r] = -INFINITY;
+  }
+  float2* red = reinterpret_cast<float2*>(lds);  // [WGN][TM]
+#pragma unroll
+  for (int a = 0; a < G::I; ++a) {
+    const int ml = wm * G::WM + 32 * a + c;
+    const int64_t m = m0 + ml;
+    if (m < p.rows) {
+      const int64_t rel = p.labels.at(m) - p.v0 - n0 - wn * G::WN;  // the label's column of this wave's
+      if (rel >= 0 && rel < G::WN) {
+#pragma unroll
+        for (int b = 0; b < G::J; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (rel == 32 * b + 8 * (r / 4) + 4 * g + r % 4) p.target[m] = acc[a][b][r];
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[a][b][r]);
+    float lo, hi;
+    lane_halves_sched(top, lo, hi);
+    top = fmaxf(lo, hi);
+    const float from = top == -INFINITY ? 0.f : top;  // nothing but -inf: a sum of 0
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[a][b][r] - from) * kLog2e);
+    lane_halves_sched(sum, lo, hi);
+    if (g == 0) red[wn * Sh::TM + ml] = float2{top, lo + hi};
+  }
+  lds_barrier();
+  for (int i = int(threadIdx.x); i < Sh::TM; i += G::threads) {
+    if (m0 + i >= p.rows) break;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < Sh::WGN; ++q) top = fmaxf(top, red[q * Sh::TM + i].x);
+    const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int q = 0; q < Sh::WGN; ++q) {
+      const float2 v = red[q * Sh::TM + i];
+      sum += v.y * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
+    }
+    p.part[int64_t(tn) * p.rows + m0 + i] = float2{top, sum};
+  }
+}
+
+// A row's tiles joined: 16 rows a block, 16 threads a row over the tiles.
+__global__ __launch_bounds__(kThreads) void loss_final_kernel(const float2* part, const float* target, int64_t rows,
+                                                              int64_t vocab, int64_t tiles, Labels labels, float* loss,
+                                                              float* lse) {
+  __shared__ float2 red[16][16];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int64_t n = int64_t(blockIdx.x) * 16 + tx;
+  float top = -INFINITY, sum = 0.f;
+  if (n < rows) {
+    for (int64_t t = ty; t < tiles; t += 16) {
+      const float2 v = part[t * rows + n];
+      const float to = fmaxf(top, v.x), from = to == -INFINITY ? 0.f : to;
+      sum = sum * __builtin_amdgcn_exp2f((top - from) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
+      top = to;
+    }
+  }
+  red[ty][tx] = float2{top, sum};
+  __syncthreads();
+  if (ty != 0 || n >= rows) return;
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, red[i][tx].x);
+  const float from = top == -INFINITY ? 0.f : top;
+  sum = 0.f;
+  for (int i = 0; i < 16; ++i) sum += red[i][tx].y * __builtin_amdgcn_exp2f((red[i][tx].x - from) * kLog2e);
+  const float z = top + logf(sum);
+  if (lse) lse[n] = z;
+  if (!loss) return;
+  const int64_t label = labels.at(n);
+  loss[n] = labels.ignored(label) ? 0.f : (label >= 0 && label < vocab ? z - target[n] : z);
+}
+
+// ---------------------------------------------------------------- backward: g
+struct GradArgs {
+  const char *x, *w;
+  int64_t rows, width, vocab;  // vocab: of this piece
+  int64_t ld_x, ld_w, v0;
+  int tiles_m, tiles_n;
+  Labels labels;
+  const float *lse, *row_grad;
+  const float* dyn;  // {factor of g, factor of the products} on the device, or null: `unit`
+  float unit;        // factor of g
+  char* g;           // [rows][ld_g], columns past vocab up to a whole chunk are zeros
+  int64_t ld_g;
+};
+
+__device__ inline uint32_t pack2(Bf16, float a, float b) {
+  return uint32_t(f32_to_bf16(a)) | (uint32_t(f32_to_bf16(b)) << 16);
+}
+__device__ inline uint32_t pack2(F16, float a, float b) { return uint32_t(f32_to_f16(a)) | (uint32_t(f32_to_f16(b)) << 16); }
+
+// A tile of 16-bit results through LDS (gemm_tiled.hip's store_staged): value
+// v(a, b, rg, acc) of the 4 columns 32 b + 8 rg + 4 g .. + 3 of a lane's row 32 a +
+// c, then whole 16-byte chunks of rows, or (vec false) element by element.
+// rows, cols: what of the tile is stored.
+template <class T, class Sh, class V>
+__device__ __attribute__((always_inline)) inline void store16(Acc<Sh>& acc, char* lds, int wave, int lane, char* out,
+                                                              int64_t ld, int64_t rows, int64_t cols, bool vec,
+                                                              V&& value) {
+  using G = Geo<Sh>;
+  constexpr int kCpr = Sh::TN / 8;
+  static_assert(kCpr % 16 == 0, "staging rows of whole 16-chunk groups");
+  const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
+  uint16_t* st = reinterpret_cast<uint16_t*>(lds);
+#pragma unroll
+  for (int a = 0; a < G::I; ++a) {
+    const int ml = wm * G::WM + 32 * a + c;
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint2 w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v[4];
+          value(a, b, 2 * h + e, v);
+          w[e] = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
+        }
+        // lanes l and l + 32 trade halves, so that each has 8 consecutive columns
+        const auto s0 = __builtin_amdgcn_permlane32_swap(w[0].x, w[1].x, false, false);
+        const auto s1 = __builtin_amdgcn_permlane32_swap(w[0].y, w[1].y, false, false);
+        const u32x4_t chunk = {static_cast<uint32_t>(s0[0]), static_cast<uint32_t>(s1[0]),
+                               static_cast<uint32_t>(s0[1]), static_cast<uint32_t>(s1[1])};
+        const int cn = (wn * G::WN + 32 * b + 16 * h + 8 * g) >> 3;
+        *reinterpret_cast<u32x4_t*>(st + ml * Sh::TN + 8 * (cn ^ (ml & 15))) = chunk;
+      }
+  }
+  lds_barrier();
+  if (vec) {
+#pragma unroll 2
+    for (int it = 0; it < Sh::TM * kCpr / G::threads; ++it) {
+      const int e = it * G::threads + int(threadIdx.x), row = e / kCpr, cn = e % kCpr;
+      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(st + row * Sh::TN + 8 * (cn ^ (row & 15)));
+      if (row < rows && 8 * cn < cols) *reinterpret_cast<u32x4_t*>(out + (row * ld + 8 * cn) * 2) = v;
+    }
+  } else {
+    for (int it = 0; it < Sh::TM * Sh::TN / G::threads; ++it) {
+      const int e = it * G::threads + int(threadIdx.x), row = e / Sh::TN, col = e % Sh::TN;
+      const uint16_t v = st[row * Sh::TN + 8 * ((col >> 3) ^ (row & 15)) + (col & 7)];
+      if (row < rows && col < cols) reinterpret_cast<uint16_t*>(out)[row * ld + col] = v;
+    }
+  }
+}
+
+// A tile of fp32 results straight from the accumulators: 16 bytes a lane (two
+// lanes' are neighbours), or (vec false) element by element.
+template <class Sh, class V>
+__device__ __attribute__((always_inline)) inline void store32(Acc<Sh>& acc, int wave, int lane, float* out, int64_t ld,
+                                                              int64_t rows, int64_t cols, bool vec, V&& value) {
+  using G = Geo<Sh>;
+  const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
+#pragma unroll
+  for (int a = 0; a < G::I; ++a) {
+    const int ml = wm * G::WM + 32 * a + c;
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {
+        const int nl = wn * G::WN + 32 * b + 8 * rg + 4 * g;
+        float v[4];
+        value(a, b, rg, v);
+        float* to = out + ml * ld + nl;
+        if (ml >= rows) continue;
+        if (vec && nl + 4 <= cols) {
+          *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (nl + q < cols) to[q] = v[q];
+        }
+      }
+  }
+}
+
+template <class T, class Sh>
+__global__ __launch_bounds__(Geo<Sh>::threads, 1) void grad_kernel(const GradArgs p) {
+  using G = Geo<Sh>;
+  __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, gridDim.x, uint32_t(p.tiles_m), uint32_t(p.tiles_n), tm, tn);
+  const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
+  Acc<Sh> acc;
+  zero<Sh>(acc);
+  product<T, Sh, true, true>(p.x + m0 * p.ld_x * T::esz, p.ld_x, p.rows - m0, p.w + n0 * p.ld_w * T::esz, p.ld_w,
+                             p.vocab - n0, p.width, lds, wave, lane, acc);
+  const float unit = p.dyn ? p.dyn[0] : p.unit;
+  float lse[G::I], factor[G::I];
+  int target[G::I];  // the label's column of this lane's, -1: none
+  bool counts[G::I];
+#pragma unroll
+  for (int a = 0; a < G::I; ++a) {
+    const int64_t m = m0 + wm * G::WM + 32 * a + c;
+    counts[a] = false, target[a] = -1, lse[a] = 0.f, factor[a] = 0.f;
+    if (m < p.rows) {
+      const int64_t label = p.labels.at(m), rel = label - p.v0 - n0 - wn * G::WN - 4 * g;
+      target[a] = rel >= 0 && rel < G::WN ? int(rel) : -1;
+      counts[a] = !p.labels.ignored(label);
+      lse[a] = p.lse[m];
+      factor[a] = unit * (p.row_grad ? p.row_grad[m] : 1.f);
+    }
+  }
+  const int left = int(min(int64_t(Sh::TN), p.vocab - n0)) - wn * G::WN - 4 * g;  // columns below it exist
+  auto value = [&](int a, int b, int rg, float (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int col = 32 * b + 8 * rg + q;
+      const float e = __builtin_amdgcn_exp2f((acc[a][b][4 * rg + q] - lse[a]) * kLog2e);
+      const float d = (e - (col == target[a] ? 1.f : 0.f)) * factor[a];
+      v[q] = counts[a] && col < left ? d : 0.f;  // selected: an ignored row's x may hold anything
+    }
+  };
+  constexpr int kE = 16 / T::esz;
+  const int64_t rows = p.rows - m0, cols = (p.vocab + kE - 1) / kE * kE - n0;
+  char* out = p.g + (m0 * p.ld_g + n0) * T::esz;
+  if constexpr (T::esz == 2) store16<T, Sh>(acc, lds, wave, lane, out, p.ld_g, rows, cols, true, value);
+  else store32<Sh>(acc, wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, true, value);
+}
+
+// ---------------------------------------------------------------- backward: dx and dw of a piece
+struct ProductsArgs {
+  const char *g, *x, *w;
+  int64_t rows, width, vocab;  // vocab: of this piece
+  int64_t ld_g, ld_x, ld_w;
+  // dx: tiles of rows x width, the piece's classes cut into `slices` runs of `run`
+  int dx_m, dx_n, slices;
+  int64_t run;
+  int first;       // the first piece: sums start from zero
+  float* sums;     // [slices][dx tile][accumulators]
+  // dw: tiles of classes x width
+  int dw_m, dw_n;
+  char* dw;        // the piece's rows
+  int64_t ld_dw;
+  int dw_f32, dw_vec;
+  const float* dyn;
+  float unit;      // factor of dw
+};
+
+template <class T, class Sh>
+__global__ __launch_bounds__(Geo<Sh>::threads, 1) void products_kernel(const ProductsArgs p) {
+  using G = Geo<Sh>;
+  __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t n_dx = uint32_t(p.dx_m) * p.dx_n * p.slices;
+  Acc<Sh> acc;
+  uint32_t tm, tn;
+  if (blockIdx.x < n_dx) {
+    const uint32_t slice = blockIdx.x % p.slices, tile = blockIdx.x / p.slices;
+    tm = tile / p.dx_n, tn = tile % p.dx_n;
+    const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN, k0 = slice * p.run;
+    f32x4* sums = reinterpret_cast<f32x4*>(p.sums) + (int64_t(slice) * p.dx_m * p.dx_n + tile) * (Sh::TM * Sh::TN / 4);
+    zero<Sh>(acc);
+    if (!p.first) {
+#pragma unroll
+      for (int a = 0; a < G::I; ++a)
+#pragma unroll
+        for (int b = 0; b < G::J; ++b)
+#pragma unroll
+          for (int rg = 0; rg < 4; ++rg) {
+            const f32x4 v = sums[((a * G::J + b) * 4 + rg) * G::threads + threadIdx.x];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[a][b][4 * rg + q] = v.v[q];
+          }
+    }
+    product<T, Sh, true, false>(p.g + (m0 * p.ld_g + k0) * T::esz, p.ld_g, p.rows - m0,
+                                p.w + (k0 * p.ld_w + n0) * T::esz, p.ld_w, p.width - n0,
+                                min(p.run, p.vocab - k0), lds, wave, lane, acc);
+#pragma unroll
+    for (int a = 0; a < G::I; ++a)
+#pragma unroll
+      for (int b = 0; b < G::J; ++b)
+#pragma unroll
+        for (int rg = 0; rg < 4; ++rg)
+          sums[((a * G::J + b) * 4 + rg) * G::threads + threadIdx.x] =
+              f32x4{{acc[a][b][4 * rg], acc[a][b][4 * rg + 1], acc[a][b][4 * rg + 2], acc[a][b][4 * rg + 3]}};
+    return;
+  }
+  tile_of(blockIdx.x - n_dx, gridDim.x - n_dx, uint32_t(p.dw_m), uint32_t(p.dw_n), tm, tn);
+  const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
+  zero<Sh>(acc);
+  product<T, Sh, false, false>(p.g + m0 * T::esz, p.ld_g, p.vocab - m0, p.x + n0 * T::esz, p.ld_x, p.width - n0, p.rows,
+                               lds, wave, lane, acc);
+  const float unit = p.dyn ? p.dyn[1] : p.unit;
+  auto value = [&](int a, int b, int rg, float (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = acc[a][b][4 * rg + q] * unit;
+  };
+  const int64_t rows = p.vocab - m0, cols = p.width - n0;
+  if constexpr (T::esz == 2) {
+    if (!p.dw_f32) {
+      store16<T, Sh>(acc, lds, wave, lane, p.dw + (m0 * p.ld_dw + n0) * 2, p.ld_dw, rows, cols, p.dw_vec, value);
+      return;
+    }
+  }
+  store32<Sh>(acc, wave, lane, reinterpret_cast<float*>(p.dw) + m0 * p.ld_dw + n0, p.ld_dw, rows, cols, p.dw_vec, value);
+}
+
+// dx = the slices' sums, in order, times the factor.  A thread has one group of 4
+// columns of a tile, as the products' accumulators lay.
+template <class T, class Sh>
+__global__ __launch_bounds__(kThreads) void dx_kernel(const float* sums, int64_t rows, int64_t width, int dx_m, int dx_n,
+                                                      int slices, const float* dyn, float unit, char* dx, int64_t ld) {
+  using G = Geo<Sh>;
+  constexpr int kGroups = Sh::TM * Sh::TN / 4;
+  const int64_t tiles = int64_t(dx_m) * dx_n, i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t tile = i / kGroups;
+  const int at = int(i % kGroups), tid = at % G::threads, reg = at / G::threads;
+  const int lane = tid & 63, wave = tid >> 6, rg = reg & 3, b = reg / 4 % G::J, a = reg / 4 / G::J;
+  const int64_t m = tile / dx_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a + (lane & 31);
+  const int64_t n = tile % dx_n * Sh::TN + wave % Sh::WGN * G::WN + 32 * b + 8 * rg + 4 * (lane >> 5);
+  if (m >= rows || n >= width) return;
+  const f32x4* p = reinterpret_cast<const f32x4*>(sums) + i;
+  f32x4 s = p[0];
+  for (int q = 1; q < slices; ++q) {
+    const f32x4 v = p[q * tiles * kGroups];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
+  }
+  const float f = dyn ? dyn[1] : unit;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < width) store_from_f32(dx, m * ld + n + e, T::mk, s.v[e] * f);
+}
+
+// ---------------------------------------------------------------- operands off the 16-byte boundaries
+// Rows copied to a pitch of whole 16-byte chunks with zeros past their end, and
+// (has_ignore) zeros for ignored rows, which g's zeros would not keep out of dw
+// if they held infinities.
+template <typename U>
+__global__ __launch_bounds__(kThreads) void pack_kernel(const U* src, int64_t ld, int64_t rows, int64_t cols, U* dst,
+                                                        int64_t ld_dst, Labels labels) {
+  constexpr int kE = 16 / int(sizeof(U));
+  const int64_t chunks = ld_dst / kE, i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t row = i / chunks, col = i % chunks * kE;
+  if (row >= rows) return;
+  const bool zero = labels.has_ignore && labels.ignored(labels.at(row));
+  struct alignas(16) Chunk { U v[kE]; } c;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) c.v[e] = !zero && col + e < cols ? src[row * ld + col + e] : U(0);
+  *reinterpret_cast<Chunk*>(dst + row * ld_dst + col) = c;
+}
+
+// rows x cols of zeros (words of U): the gradient of no rows
+template <typename U>
+__global__ __launch_bounds__(kThreads) void zero_kernel(U* p, int64_t ld, int64_t rows, int64_t cols) {
+  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  if (i < rows * cols) p[i / cols * ld + i % cols] = U(0);
+}
+
+// dyn = {factor of g, factor of the products} for fp16: |g| <= max |row_grad|, and
+// 2^15 times that over its power of two is below fp16's largest value, while the
+// smallest normal value is 2^-29 of it.
+__global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad, int64_t rows, float scale, float* dyn) {
+  __shared__ float red[kThreads / kWave];
+  float top = 0.f;
+  for (int64_t n = threadIdx.x; n < rows; n += kThreads) {
+    const float v = fabsf(row_grad[n]);
+    if (v < INFINITY) top = fmaxf(top, v);
+  }
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int i = 1; i < kThreads / kWave; ++i) top = fmaxf(top, red[i]);
+  int e = 0;
+  if (top > 0.f) (void)frexpf(top, &e);  // top <= 2^e
+  e = max(-100, min(100, e));
+  dyn[0] = ldexpf(1.f, 15 - e);
+  dyn[1] = ldexpf(scale, e - 15);
+}
+
+// ---------------------------------------------------------------- host
+constexpr int64_t kGBytes = int64_t(512) << 20;     // of g a piece
+constexpr int64_t kPackBytes = int64_t(256) << 20;  // of w copied a piece
+
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+bool on_grid(const void* p, int64_t ld, int64_t width, int esz) {
+  // 256 rows of a tile lie within a buffer's 32-bit offsets
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld * esz % 16 == 0 && width * esz % 16 == 0 && ld >= width &&
+         ld * esz < (int64_t(1) << 23);
+}
+
+// One call's sizes and its workspace, from the shapes and the operands' alignment alone.
+struct Plan {
+  int esz;
+  int64_t rows, width, vocab;
+  bool big;                       // tiles of 256 x 256, else 128 x 128
+  int64_t tm, tn;
+  bool pack_x, pack_w;
+  int64_t pitch;                  // of packed rows, elements
+  int64_t piece, pieces;          // classes of a piece
+  int64_t ld_g;
+  int64_t slices;
+  int64_t x_at, w_at, part_at, target_at, g_at, sums_at, dyn_at, bytes;
+};
+
+Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x, int64_t ld_x, const void* w,
+          int64_t ld_w, bool has_ignore) {
+  Plan q{};
+  q.esz = dtype_bytes(io_type);
+  q.rows = rows, q.width = width, q.vocab = vocab;
+  q.big = rows > 128;
+  q.tm = q.tn = q.big ? 256 : 128;
+  q.pack_x = !on_grid(x, ld_x, width, q.esz) || (bwd && has_ignore);
+  q.pack_w = !on_grid(w, ld_w, width, q.esz);
+  q.pitch = up(width, 16 / q.esz);
+  int64_t most = vocab;
+  if (q.pack_w) most = std::min(most, std::max<int64_t>(q.tn, kPackBytes / (q.pitch * q.esz)));
+  if (bwd) most = std::min(most, std::max<int64_t>(q.tn, std::min<int64_t>(kGBytes / (rows * q.esz), int64_t(1) << 20)));
+  q.pieces = (vocab + most - 1) / most;
+  q.piece = up((vocab + q.pieces - 1) / q.pieces, 256);
+  q.pieces = (vocab + q.piece - 1) / q.piece;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t here = at; at += align256(bytes); return here; };
+  if (q.pack_x) q.x_at = take(rows * q.pitch * q.esz);
+  if (q.pack_w) q.w_at = take(std::min(vocab, q.piece) * q.pitch * q.esz);
+  if (!bwd) {
+    q.part_at = take(((vocab + q.tn - 1) / q.tn + q.pieces) * rows * 8);
+    q.target_at = take(rows * 4);
+  } else {
+    const int64_t classes = std::min(vocab, q.piece);
+    q.ld_g = up(classes, 64);
+    q.g_at = take(rows * q.ld_g * q.esz);
+    // dx's slices: three rounds of the 256 CUs
+    const int64_t tiles = (rows + q.tm - 1) / q.tm * ((width + q.tn - 1) / q.tn), deep = 128 / q.esz;
+    q.slices = std::max<int64_t>(1, std::min<int64_t>({768 / tiles, 64, (classes + 4 * deep - 1) / (4 * deep)}));
+    q.sums_at = take(q.slices * tiles * q.tm * q.tn * 4);
+    q.dyn_at = take(8);
+  }
+  q.bytes = at;
+  return q;
+}
+
+int check_shapes(const std::string& what, int io_type, int64_t rows, int64_t width, int64_t vocab, int64_t ld_x,
+                 int64_t ld_w, int label_type) {
+  if (io_type != MK_BF16 && io_type != MK_F16 && io_type != MK_F32)
+    return fail(MK_ERR_UNSUPPORTED, what + ": io_type must be bf16, f16 or f32");
+  if (label_type != MK_S32 && label_type != MK_S64) return fail(MK_ERR_UNSUPPORTED, what + ": label_type must be s32 or s64");
+  if (rows < 0 || width <= 0 || vocab <= 0) return fail(MK_ERR_INVALID, what + ": bad shape");
+  if (ld_x < 0 || ld_w < 0) return fail(MK_ERR_INVALID, what + ": negative pitch");
+  if (rows >= int64_t(1) << 31 || vocab >= int64_t(1) << 31 || width > int64_t(1) << 20)
+    return fail(MK_ERR_UNSUPPORTED, what + ": rows and vocab must be below 2^31, width at most 2^20");
+  return MK_OK;
+}
+
+int check_pointer(const std::string& what, const char* name, const void* p, int bytes, bool needed) {
+  if (!p) return needed ? fail(MK_ERR_INVALID, what + ": null " + name) : MK_OK;
+  if (reinterpret_cast<uintptr_t>(p) % bytes) return fail(MK_ERR_INVALID, what + ": not aligned: " + name);
+  return MK_OK;
+}
+
+int check_tiles(const std::string& what, int64_t tiles, int threads) {
+  if (tiles * threads >= int64_t(1) << 32) return fail(MK_ERR_UNSUPPORTED, what + ": too many tiles");
+  return MK_OK;
+}
+
+int pack(const char* what, hipStream_t s, const Plan& q, const void* src, int64_t ld, int64_t rows, char* dst,
+         const Labels& labels) {
+  const int64_t blocks = (rows * (q.pitch * q.esz / 16) + kThreads - 1) / kThreads;
+  if (int rc = check_tiles(what, blocks, kThreads)) return rc;
+  const dim3 g{unsigned(blocks)}, b{kThreads};
+  if (q.esz == 2)
+    hipLaunchKernelGGL(pack_kernel<uint16_t>, g, b, 0, s, static_cast<const uint16_t*>(src), ld, rows, q.width,
+                       reinterpret_cast<uint16_t*>(dst), q.pitch, labels);
+  else
+    hipLaunchKernelGGL(pack_kernel<uint32_t>, g, b, 0, s, static_cast<const uint32_t*>(src), ld, rows, q.width,
+                       reinterpret_cast<uint32_t*>(dst), q.pitch, labels);
+  return check_launch(what);
+}
+
+// f(type, shape) of the call's
+template <class F>
+int with_kernels(int io_type, bool big, F&& f) {
+  if (io_type == MK_BF16) return big ? f(Bf16{}, Big{}) : f(Bf16{}, Mid{});
+  if (io_type == MK_F16) return big ? f(F16{}, Big{}) : f(F16{}, Mid{});
+  return big ? f(F32{}, Big{}) : f(F32{}, Mid{});
+}
+
+}  // namespace
+}  // namespace mk
+
+using namespace mk;
+
+extern "C" size_t mk_linear_xent_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
+                                                 int64_t ld_x, const void* w, int64_t ld_w) {
+  if (check_shapes("", io_type, rows, width, vocab, ld_x, ld_w, MK_S32) || rows == 0) return 0;
+  return size_t(plan(false, io_type, rows, width, vocab, x, ld_x, w, ld_w, false).bytes);
+}
+
+extern "C" int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
+                              int64_t ld_x, const void* w, int64_t ld_w, int label_type, const void* labels,
+                              int has_ignore, int64_t ignore_index, float* loss_rows, float* lse, void* workspace) {
+  clear_error();
+  const char* what = "mk_linear_xent";
+  if (int rc = check_shapes(what, io_type, rows, width, vocab, ld_x, ld_w, label_type)) return rc;
+  if (rows == 0) return MK_OK;
+  const int esz = dtype_bytes(io_type);
+  const struct { const char* name; const void* p; int bytes; bool needed; } ptrs[] = {
+      {"x", x, esz, true}, {"w", w, esz, true}, {"labels", labels, dtype_bytes(label_type), true},
+      {"loss_rows", loss_rows, 4, false}, {"lse", lse, 4, false}, {"workspace", workspace, 16, true}};
+  for (const auto& e : ptrs)
+    if (int rc = check_pointer(what, e.name, e.p, e.bytes, e.needed)) return rc;
+  const Plan q = plan(false, io_type, rows, width, vocab, x, ld_x, w, ld_w, false);
+  hipStream_t s = as_stream(stream);
+  char* ws = static_cast<char*>(workspace);
+  LossArgs a{};
+  a.labels = {labels, label_type == MK_S64, has_ignore != 0, ignore_index};
+  a.x = static_cast<const char*>(x), a.ld_x = ld_x;
+  a.rows = rows, a.width = width;
+  a.part = reinterpret_cast<float2*>(ws + q.part_at);
+  a.target = reinterpret_cast<float*>(ws + q.target_at);
+  a.tiles_m = int((rows + q.tm - 1) / q.tm);
+  if (int rc = check_tiles(what, a.tiles_m * ((q.piece + q.tn - 1) / q.tn), 512)) return rc;
+  if (q.pack_x) {
+    if (int rc = pack(what, s, q, x, ld_x, rows, ws + q.x_at, Labels{})) return rc;
+    a.x = ws + q.x_at, a.ld_x = q.pitch;
+  }
+  const float2* part = a.part;
+  int64_t tiles = 0;
+  for (int64_t v0 = 0; v0 < vocab; v0 += q.piece) {
+    a.v0 = v0;
+    a.vocab = std::min(q.piece, vocab - v0);
+    a.w = static_cast<const char*>(w) + v0 * ld_w * esz, a.ld_w = ld_w;
+    if (q.pack_w) {
+      if (int rc = pack(what, s, q, a.w, ld_w, a.vocab, ws + q.w_at, Labels{})) return rc;
+      a.w = ws + q.w_at, a.ld_w = q.pitch;
+    }
+    a.tiles_n = int((a.vocab + q.tn - 1) / q.tn);
+    const int rc = with_kernels(io_type, q.big, [&](auto t, auto sh) {
+      using T = decltype(t);
+      using Sh = decltype(sh);
+      hipLaunchKernelGGL((loss_kernel<T, Sh>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)), dim3(Geo<Sh>::threads), 0,
+                         s, a);
+      return check_launch(what);
+    });
+    if (rc) return rc;
+    a.part += a.tiles_n * rows;
+    tiles += a.tiles_n;
+  }
+  hipLaunchKernelGGL(loss_final_kernel, dim3(unsigned((rows + 15) / 16)), dim3(kThreads), 0, s, part, a.target, rows, vocab,
+                     tiles, a.labels, loss_rows, lse);
+  return check_launch(what);
+}
+
+extern "C" size_t mk_linear_xent_bwd_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab,
+                                                     const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                                     int has_ignore) {
+  if (check_shapes("", io_type, rows, width, vocab, ld_x, ld_w, MK_S32) || rows == 0) return 0;
+  return size_t(plan(true, io_type, rows, width, vocab, x, ld_x, w, ld_w, has_ignore != 0).bytes);
+}
+
+extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_t rows, int64_t width, int64_t vocab,
+                                  const void* x, int64_t ld_x, const void* w, int64_t ld_w, int label_type,
+                                  const void* labels, int has_ignore, int64_t ignore_index, const float* lse,
+                                  const float* row_grad, float grad_scale, void* dx, int64_t ld_dx, void* dw,
+                                  int64_t ld_dw, void* workspace) {
+  clear_error();
+  const char* what = "mk_linear_xent_bwd";
+  if (int rc = check_shapes(what, io_type, rows, width, vocab, ld_x, ld_w, label_type)) return rc;
+  if (dw && dw_type != io_type && dw_type != MK_F32)
+    return fail(MK_ERR_UNSUPPORTED, std::string(what) + ": dw_type must be io_type or f32");
+  const int esz = dtype_bytes(io_type), dwsz = dw ? dtype_bytes(dw_type) : 1;
+  if ((dx && rows > 1 && ld_dx < width) || (dw && vocab > 1 && ld_dw < width))
+    return fail(MK_ERR_INVALID, std::string(what) + ": rows of dx or dw overlap");
+  if (int rc = check_pointer(what, "dw", dw, dwsz, false)) return rc;
+  hipStream_t s = as_stream(stream);
+  if (!dx && !dw) return MK_OK;
+  const struct { const char* name; const void* p; int bytes; bool needed; } ptrs[] = {
+      {"x", x, esz, true}, {"w", w, esz, true}, {"labels", labels, dtype_bytes(label_type), true}, {"lse", lse, 4, true},
+      {"row_grad", row_grad, 4, false}, {"dx", dx, esz, false}, {"workspace", workspace, 16, true}};
+  if (rows == 0) {
+    if (!dw) return MK_OK;
+    const int64_t blocks = (vocab * width + kThreads - 1) / kThreads;
+    if (int rc = check_tiles(what, blocks, kThreads)) return rc;
+    if (dwsz == 2)
+      hipLaunchKernelGGL(zero_kernel<uint16_t>, dim3(unsigned(blocks)), dim3(kThreads), 0, s, static_cast<uint16_t*>(dw),
+                         ld_dw, vocab, width);
+    else
+      hipLaunchKernelGGL(zero_kernel<uint32_t>, dim3(unsigned(blocks)), dim3(kThreads), 0, s, static_cast<uint32_t*>(dw),
+                         ld_dw, vocab, width);
+    return check_launch(what);
+  }
+  for (const auto& e : ptrs)
+    if (int rc = check_pointer(what, e.name, e.p, e.bytes, e.needed)) return rc;
+  if (dx == x || (dw && dw == w)) return fail(MK_ERR_INVALID, std::string(what) + ": dx over x, or dw over w");
+  const Plan q = plan(true, io_type, rows, width, vocab, x, ld_x, w, ld_w, has_ignore != 0);
+  char* ws = static_cast<char*>(workspace);
+  const Labels lab = {labels, label_type == MK_S64, has_ignore != 0, ignore_index};
+  GradArgs a{};
+  ProductsArgs b{};
+  a.rows = b.rows = rows, a.width = b.width = width;
+  a.labels = lab;
+  a.lse = lse, a.row_grad = row_grad;
+  a.x = static_cast<const char*>(x), a.ld_x = ld_x;
+  a.g = ws + q.g_at, a.ld_g = q.ld_g;
+  a.tiles_m = int((rows + q.tm - 1) / q.tm);
+  b.dx_m = dx ? a.tiles_m : 0;
+  b.dx_n = b.dw_n = int((width + q.tn - 1) / q.tn);
+  b.slices = int(q.slices);
+  const int64_t most = a.tiles_m * ((q.piece + q.tn - 1) / q.tn),
+                most2 = int64_t(a.tiles_m) * b.dx_n * q.slices + (q.piece + q.tm - 1) / q.tm * b.dw_n;
+  if (int rc = check_tiles(what, std::max(most, most2), 512)) return rc;
+  // fp16: g out of the subnormals, by a power of two of the largest row_grad
+  a.unit = io_type == MK_F16 ? 32768.f : 1.f;
+  b.unit = io_type == MK_F16 ? grad_scale / 32768.f : grad_scale;
+  if (io_type == MK_F16 && row_grad) {
+    float* dyn = reinterpret_cast<float*>(ws + q.dyn_at);
+    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(kThreads), 0, s, row_grad, rows, grad_scale, dyn);
+    if (int rc = check_launch(what)) return rc;
+    a.dyn = b.dyn = dyn;
+  }
+  if (q.pack_x) {
+    if (int rc = pack(what, s, q, x, ld_x, rows, ws + q.x_at, lab)) return rc;
+    a.x = ws + q.x_at, a.ld_x = q.pitch;
+  }
+  b.g = a.g, b.ld_g = a.ld_g;
+  b.x = a.x, b.ld_x = a.ld_x;
+  b.sums = reinterpret_cast<float*>(ws + q.sums_at);
+  b.dw_f32 = dw_type == MK_F32;
+  b.ld_dw = ld_dw;
+  b.dw_vec = (reinterpret_cast<uintptr_t>(dw) & 15u) == 0 && ld_dw * dwsz % 16 == 0 && width * esz % 16 == 0;
+  for (int64_t v0 = 0; v0 < vocab; v0 += q.piece) {
+    a.v0 = v0;
+    a.vocab = b.vocab = std::min(q.piece, vocab - v0);
+    a.w = static_cast<const char*>(w) + v0 * ld_w * esz, a.ld_w = ld_w;
+    if (q.pack_w) {
+      if (int rc = pack(what, s, q, a.w, ld_w, a.vocab, ws + q.w_at, Labels{})) return rc;
+      a.w = ws + q.w_at, a.ld_w = q.pitch;
+    }
+    b.w = a.w, b.ld_w = a.ld_w;
+    b.first = v0 == 0;
+    const int64_t deep = 128 / esz;
+    b.run = up((a.vocab + q.slices - 1) / q.slices, deep);
+    b.dw = static_cast<char*>(dw) + v0 * ld_dw * dwsz;
+    a.tiles_n = int((a.vocab + q.tn - 1) / q.tn);
+    b.dw_m = dw ? int((a.vocab + q.tm - 1) / q.tm) : 0;
+    const int rc = with_kernels(io_type, q.big, [&](auto t, auto sh) {
+      using T = decltype(t);
+      using Sh = decltype(sh);
+      hipLaunchKernelGGL((grad_kernel<T, Sh>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)), dim3(Geo<Sh>::threads), 0,
+                         s, a);
+      if (int r = check_launch(what)) return r;
+      const unsigned tiles = unsigned(b.dx_m) * b.dx_n * b.slices + unsigned(b.dw_m) * b.dw_n;
+      hipLaunchKernelGGL((products_kernel<T, Sh>), dim3(tiles), dim3(Geo<Sh>::threads), 0, s, b);
+      return check_launch(what);
+    });
+    if (rc) return rc;
+  }
+  if (!dx) return MK_OK;
+  return with_kernels(io_type, q.big, [&](auto t, auto sh) {
+    using T = decltype(t);
+    using Sh = decltype(sh);
+    const int64_t blocks = int64_t(b.dx_m) * b.dx_n * Sh::TM * Sh::TN / 4 / kThreads;
+    if (int r = check_tiles(what, blocks, kThreads)) return r;
+    hipLaunchKernelGGL((dx_kernel<T, Sh>), dim3(unsigned(blocks)), dim3(kThreads), 0, s, b.sums, rows, width, b.dx_m, b.dx_n,
+                       b.slices, b.dyn, b.unit, static_cast<char*>(dx), ld_dx);
+    return check_launch(what);
+  });
+}
