@@ -62,7 +62,7 @@ struct F32 {
   }
 };
 
-// BK: 16-bit elements of a k tile (128 bytes a row whatever the type)
+// BK: 16-bit elements of a k tile (2 BK bytes a row whatever the type)
 using Big = Shape<256, 256, 2, 4, 64, 2>;
 using Mid = Shape<128, 128, 4, 2, 64, 2>;
 
@@ -71,9 +71,9 @@ struct Geo {
   static constexpr int W = Sh::WGM * Sh::WGN, threads = 64 * W;
   static constexpr int WM = Sh::TM / Sh::WGM, WN = Sh::TN / Sh::WGN;  // wave block
   static constexpr int I = WM / 32, J = WN / 32;                      // MFMA blocks of it
-  static constexpr int lds_bytes = Sh::S * 128 * (Sh::TM + Sh::TN);
+  static constexpr int row_bytes = 2 * Sh::BK, steps = row_bytes / 32;  // of a k tile; its MFMA steps
+  static constexpr int stage = row_bytes * (Sh::TM + Sh::TN), lds_bytes = Sh::S * stage;
   static_assert(Sh::TM * Sh::TN * 2 <= lds_bytes, "a 16-bit tile is staged where the operands were");
-  static_assert(Sh::S == 2 && Sh::BK == 64, "the k loop below");
 };
 template <class Sh>
 using Acc = f32x16_t[Geo<Sh>::I][Geo<Sh>::J];
@@ -83,24 +83,25 @@ using Acc = f32x16_t[Geo<Sh>::I][Geo<Sh>::J];
 // Copies): their byte offsets from the tile's base, and the first k each reads.
 // `base` is the tile's first row (KC) or column (!KC) at its first k; rows: those
 // of the tile inside the operand.
-template <class T, bool KC, int R, int W>
+template <class T, bool KC, int R, int W, int BK>
 struct Operand {
-  static constexpr int kE = 16 / T::esz, kDeep = 128 / T::esz, kC = R / (8 * W);
-  static constexpr int kCpr = KC ? 8 : R / kE;  // chunks of an LDS row
-  static_assert(kC * 8 * W == R, "copies split evenly over the waves");
+  static constexpr int kRow = 2 * BK;  // bytes of k a tile row has
+  static constexpr int kE = 16 / T::esz, kDeep = kRow / T::esz, kC = R * kRow / (1024 * W);
+  static constexpr int kCpr = KC ? kRow / 16 : R / kE;  // chunks of an LDS row
+  static_assert(kC * 1024 * W == R * kRow, "copies split evenly over the waves");
   const char* base;
   int64_t step;  // bytes from a k tile to the next
   uint32_t off[kC];
   int32_t k[kC];
   __device__ inline Operand(int wave, int lane, const char* base, int64_t rows, int64_t ld)
-      : base(base), step(KC ? 128 : kDeep * ld * T::esz) {
+      : base(base), step(KC ? kRow : kDeep * ld * T::esz) {
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
       const int u = 64 * (wave + W * c) + lane, r = u / kCpr;
       int row;
       if constexpr (KC) {
         row = r;
-        k[c] = kE * ((u % kCpr) ^ kc_swizzle<64>(row));
+        k[c] = kE * ((u % kCpr) ^ kc_swizzle<BK>(row));
         off[c] = uint32_t(row * ld * T::esz + k[c] * T::esz);
       } else {
         row = kE * ((u % kCpr) ^ (T::esz == 2 ? nc_swizzle<R>(r) : 0));
@@ -110,27 +111,25 @@ struct Operand {
       if (row >= rows) off[c] = uint32_t(kInvalid), k[c] = 0x7fffffff - kDeep;
     }
   }
-  // copies [lo, hi) of k tile kt, of which the operand has K - kDeep kt k
-  __device__ inline void issue(int kt, int64_t K, char* tile, int wave, int lo, int hi) const {
+  // the copies of k tile kt, of which the operand has K - kDeep kt k
+  __device__ inline void issue(int kt, int64_t K, char* tile, int wave) const {
     const i32x4_t r = tile_desc(base + kt * step, uint32_t(kInvalid));
     const int64_t left = K - int64_t(kDeep) * kt;
     if (left >= kDeep) {
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
-        if (c >= lo && c < hi) copy_to_lds_so(r, lds_addr(tile + 1024 * (wave + W * c)), int(off[c]), 0);
+      for (int c = 0; c < kC; ++c) copy_to_lds_so(r, lds_addr(tile + 1024 * (wave + W * c)), int(off[c]), 0);
       return;
     }
 #pragma unroll
     for (int c = 0; c < kC; ++c)
-      if (c >= lo && c < hi)
-        copy_to_lds(r, lds_addr(tile + 1024 * (wave + W * c)), k[c] < left ? int(off[c]) : kInvalid);
+      copy_to_lds(r, lds_addr(tile + 1024 * (wave + W * c)), k[c] < left ? int(off[c]) : kInvalid);
   }
 };
 
-template <class T, bool KC, int R>
+template <class T, bool KC, int R, int BK>
 __device__ inline u32x4_t read_chunk(const char* t, int rb, int ks, int lane) {
-  if constexpr (KC || T::esz == 2) {  // a k-contiguous row is 8 chunks of 16 bytes in either width
-    return read_operand16<KC, R, 64>(reinterpret_cast<const uint16_t*>(t), rb, ks, lane);
+  if constexpr (KC || T::esz == 2) {  // a k-contiguous row is chunks of 16 bytes in either width
+    return read_operand16<KC, R, BK>(reinterpret_cast<const uint16_t*>(t), rb, ks, lane);
   } else {
     const uint32_t* p = reinterpret_cast<const uint32_t*>(t) + (8 * ks + 4 * (lane >> 5)) * R + rb + (lane & 31);
     return u32x4_t{p[0], p[R], p[2 * R], p[3 * R]};
@@ -138,46 +137,53 @@ __device__ inline u32x4_t read_chunk(const char* t, int rb, int ks, int lane) {
 }
 
 // acc += A B of one workgroup tile over K: the k loop of gemm_tiled.hip.  A wave
-// waits for its own copies of tile kt, the barrier publishes all and frees the
-// other stage, whose copies are issued beside the first k-steps' MFMAs.  Ends with
-// a barrier: the operands' LDS is free.
+// waits for its own copies of tile kt (those of the S - 2 tiles after it may be in
+// flight), the barrier publishes all and frees the stage of tile kt - 1, whose
+// next copies are issued beside the first k-steps' MFMAs.  Ends with a barrier:
+// the operands' LDS is free.
 template <class T, class Sh, bool AKC, bool BKC>
 __device__ __attribute__((always_inline)) inline void product(const char* A, int64_t lda, int64_t a_rows,
                                                               const char* B, int64_t ldb, int64_t b_rows, int64_t K,
                                                               char* lds, int wave, int lane, Acc<Sh>& acc) {
   using G = Geo<Sh>;
+  constexpr int S = Sh::S, BK = Sh::BK;
   const int wm = wave / Sh::WGN, wn = wave % Sh::WGN;
-  const Operand<T, AKC, Sh::TM, G::W> oa(wave, lane, A, a_rows, lda);
-  const Operand<T, BKC, Sh::TN, G::W> ob(wave, lane, B, b_rows, ldb);
-  constexpr int kCa = Sh::TM / (8 * G::W), kCb = Sh::TN / (8 * G::W), kA = Sh::TM * 128, kStage = 128 * (Sh::TM + Sh::TN);
-  constexpr int kDeep = 128 / T::esz;
-  const int nk = int((K + kDeep - 1) / kDeep);
-  if (nk > 0) {
-    oa.issue(0, K, lds, wave, 0, kCa);
-    ob.issue(0, K, lds + kA, wave, 0, kCb);
-  }
-  for (int kt = 0; kt < nk; ++kt) {
-    wait_vm<0>();
-    lds_barrier();
-    const char* at = lds + (kt & 1) * kStage;
-    char* next = lds + ((kt + 1) & 1) * kStage;
-    const bool more = kt + 1 < nk;
+  using OA = Operand<T, AKC, Sh::TM, G::W, BK>;
+  using OB = Operand<T, BKC, Sh::TN, G::W, BK>;
+  const OA oa(wave, lane, A, a_rows, lda);
+  const OB ob(wave, lane, B, b_rows, ldb);
+  constexpr int kA = Sh::TM * G::row_bytes;
+  const int nk = int((K + OA::kDeep - 1) / OA::kDeep);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+  for (int st = 0; st < S - 1; ++st)
+    if (st < nk) {
+      oa.issue(st, K, lds + st * G::stage, wave);
+      ob.issue(st, K, lds + st * G::stage + kA, wave);
+    }
+  int stage = 0, fill = S - 1;
+  for (int kt = 0; kt < nk; ++kt) {
+    if (kt + S - 2 < nk) wait_vm<(S - 2) * (OA::kC + OB::kC)>();
+    else wait_vm<0>();
+    lds_barrier();
+    const char* at = lds + stage * G::stage;
+    char* next = lds + fill * G::stage;
+    const bool more = kt + S - 1 < nk;
+#pragma unroll
+    for (int ks = 0; ks < G::steps; ++ks) {
       u32x4_t af[G::I], bf[G::J];
 #pragma unroll
-      for (int a = 0; a < G::I; ++a) af[a] = read_chunk<T, AKC, Sh::TM>(at, wm * G::WM + 32 * a, ks, lane);
+      for (int a = 0; a < G::I; ++a) af[a] = read_chunk<T, AKC, Sh::TM, BK>(at, wm * G::WM + 32 * a, ks, lane);
 #pragma unroll
-      for (int b = 0; b < G::J; ++b) bf[b] = read_chunk<T, BKC, Sh::TN>(at + kA, wn * G::WN + 32 * b, ks, lane);
-      if (more && ks < 2) {
-        if (ks == 0) oa.issue(kt + 1, K, next, wave, 0, kCa);
-        else ob.issue(kt + 1, K, next + kA, wave, 0, kCb);
-      }
+      for (int b = 0; b < G::J; ++b) bf[b] = read_chunk<T, BKC, Sh::TN, BK>(at + kA, wn * G::WN + 32 * b, ks, lane);
+      if (more && ks == 0) oa.issue(kt + S - 1, K, next, wave);
+      if (more && ks == 1) ob.issue(kt + S - 1, K, next + kA, wave);
 #pragma unroll
       for (int a = 0; a < G::I; ++a)
 #pragma unroll
         for (int b = 0; b < G::J; ++b) acc[a][b] = T::mma(bf[b], af[a], acc[a][b]);
     }
+    stage = stage + 1 == S ? 0 : stage + 1;
+    fill = fill + 1 == S ? 0 : fill + 1;
   }
   lds_barrier();
 }
@@ -192,14 +198,18 @@ __device__ inline void zero(Acc<Sh>& acc) {
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
 }
 
-// Tile t of a tiles_m x tiles_n grid, for workgroup i of nt: an XCD (i % 8) has a
-// run of tiles, which walk groups of 4 tile rows column by column.
-__device__ inline void tile_of(uint32_t i, uint32_t nt, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+// The tile of a tiles_m x tiles_n grid that workgroup i of nt has: an XCD (i % 8)
+// has a run of tiles, which walk groups of 4 tile rows column by column.  False:
+// there are fewer than nt.
+__device__ inline bool tile_of(uint32_t i, uint32_t nt, uint32_t tiles_m, uint32_t tiles_n, uint32_t& tm, uint32_t& tn) {
+  if (nt == 0) return false;
   const uint32_t per = nt / 8, t = i < 8 * per ? (i % 8) * per + i / 8 : i;
+  if (t >= tiles_m * tiles_n) return false;
   const uint32_t first = t / (kGroupM * tiles_n) * kGroupM, gm = min(uint32_t(kGroupM), tiles_m - first);
   const uint32_t in = t - first * tiles_n;
   tm = first + in % gm;
   tn = in / gm;
+  return t < tiles_m * tiles_n;
 }
 
 // ---------------------------------------------------------------- labels
@@ -227,7 +237,7 @@ struct LossArgs {
 };
 
 template <class T, class Sh>
-__global__ __launch_bounds__(Geo<Sh>::threads, 1) void loss_kernel(const LossArgs p) {
+__global__ __launch_bounds__(Geo<Sh>::threads, 2) void loss_kernel(const LossArgs p) {
   using G = Geo<Sh>;
   __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -298,28 +308,39 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 1) void loss_kernel(const LossArg
   }
 }
 
-// A row's tiles joined: 16 rows a block, 16 threads a row over the tiles.
+// A row's tiles joined: 16 rows a block, 16 threads a row over the tiles, 8 of
+// them loaded at a time (one after the other a row's 393 tiles took 9 us).
 __global__ __launch_bounds__(kThreads) void loss_final_kernel(const float2* part, const float* target, int64_t rows,
                                                               int64_t vocab, int64_t tiles, Labels labels, float* loss,
                                                               float* lse) {
+  constexpr int kAt = 8;
   __shared__ float2 red[16][16];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int64_t n = int64_t(blockIdx.x) * 16 + tx;
   float top = -INFINITY, sum = 0.f;
   if (n < rows) {
-    for (int64_t t = ty; t < tiles; t += 16) {
-      const float2 v = part[t * rows + n];
-      const float to = fmaxf(top, v.x), from = to == -INFINITY ? 0.f : to;
-      sum = sum * __builtin_amdgcn_exp2f((top - from) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
+    for (int64_t t = ty; t < tiles; t += 16 * kAt) {
+      float2 v[kAt];
+#pragma unroll
+      for (int i = 0; i < kAt; ++i) v[i] = t + 16 * i < tiles ? part[(t + 16 * i) * rows + n] : float2{-INFINITY, 0.f};
+      float to = top;
+#pragma unroll
+      for (int i = 0; i < kAt; ++i) to = fmaxf(to, v[i].x);
+      const float from = to == -INFINITY ? 0.f : to;  // nothing but -inf: a sum of 0
+      sum *= __builtin_amdgcn_exp2f((top - from) * kLog2e);
+#pragma unroll
+      for (int i = 0; i < kAt; ++i) sum += v[i].y * __builtin_amdgcn_exp2f((v[i].x - from) * kLog2e);
       top = to;
     }
   }
   red[ty][tx] = float2{top, sum};
   __syncthreads();
   if (ty != 0 || n >= rows) return;
+#pragma unroll
   for (int i = 1; i < 16; ++i) top = fmaxf(top, red[i][tx].x);
   const float from = top == -INFINITY ? 0.f : top;
   sum = 0.f;
+#pragma unroll
   for (int i = 0; i < 16; ++i) sum += red[i][tx].y * __builtin_amdgcn_exp2f((red[i][tx].x - from) * kLog2e);
   const float z = top + logf(sum);
   if (lse) lse[n] = z;
@@ -340,6 +361,7 @@ struct GradArgs {
   float unit;        // factor of g
   char* g;           // [rows][ld_g], columns past vocab up to a whole chunk are zeros
   int64_t ld_g;
+  int stream;        // g goes past the caches
 };
 
 __device__ inline uint32_t pack2(Bf16, float a, float b) {
@@ -352,9 +374,9 @@ __device__ inline uint32_t pack2(F16, float a, float b) { return uint32_t(f32_to
 // c, then whole 16-byte chunks of rows, or (vec false) element by element.
 // rows, cols: what of the tile is stored.
 template <class T, class Sh, class V>
-__device__ __attribute__((always_inline)) inline void store16(Acc<Sh>& acc, char* lds, int wave, int lane, char* out,
+__device__ __attribute__((always_inline)) inline void store16(char* lds, int wave, int lane, char* out,
                                                               int64_t ld, int64_t rows, int64_t cols, bool vec,
-                                                              V&& value) {
+                                                              bool stream, V&& value) {
   using G = Geo<Sh>;
   constexpr int kCpr = Sh::TN / 8;
   static_assert(kCpr % 16 == 0, "staging rows of whole 16-chunk groups");
@@ -384,13 +406,23 @@ __device__ __attribute__((always_inline)) inline void store16(Acc<Sh>& acc, char
       }
   }
   lds_barrier();
-  if (vec) {
-#pragma unroll 2
+  auto chunks = [&](auto past) __attribute__((always_inline)) {
+#pragma unroll 4
     for (int it = 0; it < Sh::TM * kCpr / G::threads; ++it) {
       const int e = it * G::threads + int(threadIdx.x), row = e / kCpr, cn = e % kCpr;
       const u32x4_t v = *reinterpret_cast<const u32x4_t*>(st + row * Sh::TN + 8 * (cn ^ (row & 15)));
-      if (row < rows && 8 * cn < cols) *reinterpret_cast<u32x4_t*>(out + (row * ld + 8 * cn) * 2) = v;
+      u32x4_t* const to = reinterpret_cast<u32x4_t*>(out + (row * ld + 8 * cn) * 2);
+      if (row < rows && 8 * cn < cols) {
+        if constexpr (decltype(past)::value) __builtin_nontemporal_store(v, to);
+        else *to = v;
+      }
     }
+  };
+  if (vec && stream) {
+    chunks(std::true_type{});
+    asm volatile("");  // keeps the two loops' stores apart
+  } else if (vec) {
+    chunks(std::false_type{});
   } else {
     for (int it = 0; it < Sh::TM * Sh::TN / G::threads; ++it) {
       const int e = it * G::threads + int(threadIdx.x), row = e / Sh::TN, col = e % Sh::TN;
@@ -403,7 +435,7 @@ __device__ __attribute__((always_inline)) inline void store16(Acc<Sh>& acc, char
 // A tile of fp32 results straight from the accumulators: 16 bytes a lane (two
 // lanes' are neighbours), or (vec false) element by element.
 template <class Sh, class V>
-__device__ __attribute__((always_inline)) inline void store32(Acc<Sh>& acc, int wave, int lane, float* out, int64_t ld,
+__device__ __attribute__((always_inline)) inline void store32(int wave, int lane, float* out, int64_t ld,
                                                               int64_t rows, int64_t cols, bool vec, V&& value) {
   using G = Geo<Sh>;
   const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
@@ -431,7 +463,7 @@ __device__ __attribute__((always_inline)) inline void store32(Acc<Sh>& acc, int 
 }
 
 template <class T, class Sh>
-__global__ __launch_bounds__(Geo<Sh>::threads, 1) void grad_kernel(const GradArgs p) {
+__global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArgs p) {
   using G = Geo<Sh>;
   __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -443,37 +475,61 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 1) void grad_kernel(const GradArg
   zero<Sh>(acc);
   product<T, Sh, true, true>(p.x + m0 * p.ld_x * T::esz, p.ld_x, p.rows - m0, p.w + n0 * p.ld_w * T::esz, p.ld_w,
                              p.vocab - n0, p.width, lds, wave, lane, acc);
+  // Most tiles have every class, and waves no ignored row: an exponential, its
+  // exponent and a factor for each element.  The label's -1 is put in afterwards
+  // by the few lanes that have one.
   const float unit = p.dyn ? p.dyn[0] : p.unit;
-  float lse[G::I], factor[G::I];
-  int target[G::I];  // the label's column of this lane's, -1: none
-  bool counts[G::I];
+  float factor[G::I];
+  bool counts = true;
 #pragma unroll
   for (int a = 0; a < G::I; ++a) {
     const int64_t m = m0 + wm * G::WM + 32 * a + c;
-    counts[a] = false, target[a] = -1, lse[a] = 0.f, factor[a] = 0.f;
+    int64_t rel = -1;  // the label's column of this lane's
+    float lse = 0.f;
+    factor[a] = 0.f;
     if (m < p.rows) {
-      const int64_t label = p.labels.at(m), rel = label - p.v0 - n0 - wn * G::WN - 4 * g;
-      target[a] = rel >= 0 && rel < G::WN ? int(rel) : -1;
-      counts[a] = !p.labels.ignored(label);
-      lse[a] = p.lse[m];
+      const int64_t label = p.labels.at(m);
+      rel = label - p.v0 - n0 - wn * G::WN - 4 * g;
+      lse = p.lse[m];
       factor[a] = unit * (p.row_grad ? p.row_grad[m] : 1.f);
+      if (p.labels.ignored(label)) factor[a] = 0.f, rel = -1, counts = false;
+    }
+    const float from = -lse * kLog2e;
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        // 32-bit results: the difference first, which is exact where it is small
+        acc[a][b][r] = __builtin_amdgcn_exp2f(T::esz == 4 ? (acc[a][b][r] - lse) * kLog2e
+                                                          : fmaf(acc[a][b][r], kLog2e, from));
+    if (rel >= 0 && rel < G::WN) {
+#pragma unroll
+      for (int b = 0; b < G::J; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (rel == 32 * b + 8 * (r / 4) + r % 4) acc[a][b][r] -= 1.f;
     }
   }
-  const int left = int(min(int64_t(Sh::TN), p.vocab - n0)) - wn * G::WN - 4 * g;  // columns below it exist
+  if (!__all(counts) || n0 + Sh::TN > p.vocab) {
+    const int64_t left = p.vocab - n0 - wn * G::WN - 4 * g;  // columns below it exist
+#pragma unroll
+    for (int a = 0; a < G::I; ++a)
+#pragma unroll
+      for (int b = 0; b < G::J; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          // selected: an ignored row's logits may be anything
+          if (factor[a] == 0.f || 32 * b + 8 * (r / 4) + r % 4 >= left) acc[a][b][r] = 0.f;
+  }
   auto value = [&](int a, int b, int rg, float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int col = 32 * b + 8 * rg + q;
-      const float e = __builtin_amdgcn_exp2f((acc[a][b][4 * rg + q] - lse[a]) * kLog2e);
-      const float d = (e - (col == target[a] ? 1.f : 0.f)) * factor[a];
-      v[q] = counts[a] && col < left ? d : 0.f;  // selected: an ignored row's x may hold anything
-    }
+    for (int q = 0; q < 4; ++q) v[q] = acc[a][b][4 * rg + q] * factor[a];
   };
   constexpr int kE = 16 / T::esz;
   const int64_t rows = p.rows - m0, cols = (p.vocab + kE - 1) / kE * kE - n0;
   char* out = p.g + (m0 * p.ld_g + n0) * T::esz;
-  if constexpr (T::esz == 2) store16<T, Sh>(acc, lds, wave, lane, out, p.ld_g, rows, cols, true, value);
-  else store32<Sh>(acc, wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, true, value);
+  if constexpr (T::esz == 2) store16<T, Sh>(lds, wave, lane, out, p.ld_g, rows, cols, true, p.stream, value);
+  else store32<Sh>(wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, true, value);
 }
 
 // ---------------------------------------------------------------- backward: dx and dw of a piece
@@ -496,15 +552,19 @@ struct ProductsArgs {
 };
 
 template <class T, class Sh>
-__global__ __launch_bounds__(Geo<Sh>::threads, 1) void products_kernel(const ProductsArgs p) {
+__global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const ProductsArgs p) {
   using G = Geo<Sh>;
   __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t n_dx = uint32_t(p.dx_m) * p.dx_n * p.slices;
+  // dw's tiles first: they are the long ones where there are many rows, and dx's
+  // runs fill the last round (8192 x 768 x 25088: 404 k steps a CU the other way
+  // round, 320 so).  Both start at a multiple of 8, an XCD each.
+  const uint32_t dw_tiles = uint32_t(p.dw_m) * p.dw_n, n_dw = (dw_tiles + 7) / 8 * 8;
   Acc<Sh> acc;
   uint32_t tm, tn;
-  if (blockIdx.x < n_dx) {
-    const uint32_t slice = blockIdx.x % p.slices, tile = blockIdx.x / p.slices;
+  if (blockIdx.x >= n_dw) {
+    // a slice of the classes is one XCD's (of 8 slices), with all of dx's tiles
+    const uint32_t j = blockIdx.x - n_dw, slice = j % p.slices, tile = j / p.slices;
     tm = tile / p.dx_n, tn = tile % p.dx_n;
     const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN, k0 = slice * p.run;
     f32x4* sums = reinterpret_cast<f32x4*>(p.sums) + (int64_t(slice) * p.dx_m * p.dx_n + tile) * (Sh::TM * Sh::TN / 4);
@@ -534,7 +594,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 1) void products_kernel(const Pro
               f32x4{{acc[a][b][4 * rg], acc[a][b][4 * rg + 1], acc[a][b][4 * rg + 2], acc[a][b][4 * rg + 3]}};
     return;
   }
-  tile_of(blockIdx.x - n_dx, gridDim.x - n_dx, uint32_t(p.dw_m), uint32_t(p.dw_n), tm, tn);
+  if (!tile_of(blockIdx.x, n_dw, uint32_t(p.dw_m), uint32_t(p.dw_n), tm, tn)) return;
   const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
   zero<Sh>(acc);
   product<T, Sh, false, false>(p.g + m0 * T::esz, p.ld_g, p.vocab - m0, p.x + n0 * T::esz, p.ld_x, p.width - n0, p.rows,
@@ -547,38 +607,61 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 1) void products_kernel(const Pro
   const int64_t rows = p.vocab - m0, cols = p.width - n0;
   if constexpr (T::esz == 2) {
     if (!p.dw_f32) {
-      store16<T, Sh>(acc, lds, wave, lane, p.dw + (m0 * p.ld_dw + n0) * 2, p.ld_dw, rows, cols, p.dw_vec, value);
+      store16<T, Sh>(lds, wave, lane, p.dw + (m0 * p.ld_dw + n0) * 2, p.ld_dw, rows, cols, p.dw_vec, false, value);
       return;
     }
   }
-  store32<Sh>(acc, wave, lane, reinterpret_cast<float*>(p.dw) + m0 * p.ld_dw + n0, p.ld_dw, rows, cols, p.dw_vec, value);
+  store32<Sh>(wave, lane, reinterpret_cast<float*>(p.dw) + m0 * p.ld_dw + n0, p.ld_dw, rows, cols, p.dw_vec, value);
 }
 
-// dx = the slices' sums, in order, times the factor.  A thread has one group of 4
-// columns of a tile, as the products' accumulators lay.
+// dx = the slices' sums, in order, times the factor.  A block has the 32 rows x WN
+// columns of one of a wave's accumulator rows, as they lay, and stores them in
+// rows through LDS.
 template <class T, class Sh>
 __global__ __launch_bounds__(kThreads) void dx_kernel(const float* sums, int64_t rows, int64_t width, int dx_m, int dx_n,
-                                                      int slices, const float* dyn, float unit, char* dx, int64_t ld) {
+                                                      int slices, const float* dyn, float unit, char* dx, int64_t ld,
+                                                      int vec) {
   using G = Geo<Sh>;
-  constexpr int kGroups = Sh::TM * Sh::TN / 4;
-  const int64_t tiles = int64_t(dx_m) * dx_n, i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t tile = i / kGroups;
-  const int at = int(i % kGroups), tid = at % G::threads, reg = at / G::threads;
-  const int lane = tid & 63, wave = tid >> 6, rg = reg & 3, b = reg / 4 % G::J, a = reg / 4 / G::J;
-  const int64_t m = tile / dx_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a + (lane & 31);
-  const int64_t n = tile % dx_n * Sh::TN + wave % Sh::WGN * G::WN + 32 * b + 8 * rg + 4 * (lane >> 5);
-  if (m >= rows || n >= width) return;
-  const f32x4* p = reinterpret_cast<const f32x4*>(sums) + i;
-  f32x4 s = p[0];
-  for (int q = 1; q < slices; ++q) {
-    const f32x4 v = p[q * tiles * kGroups];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
-  }
+  constexpr int kPitch = G::WN + 4;
+  __shared__ float lds[32 * kPitch];
+  const int64_t tiles = int64_t(dx_m) * dx_n, tile = blockIdx.x / (G::W * G::I);
+  const int part = int(blockIdx.x % (G::W * G::I)), wave = part / G::I, a = part % G::I;
+  const f32x4* from = reinterpret_cast<const f32x4*>(sums) + tile * (Sh::TM * Sh::TN / 4);
   const float f = dyn ? dyn[1] : unit;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (n + e < width) store_from_f32(dx, m * ld + n + e, T::mk, s.v[e] * f);
+  for (int i = int(threadIdx.x); i < G::J * 4 * 64; i += kThreads) {
+    const int lane = i & 63, br = i >> 6;  // accumulator group: b, rg
+    const f32x4* p = from + (a * G::J * 4 + br) * G::threads + wave * 64 + lane;
+    f32x4 s = p[0];
+#pragma unroll 8
+    for (int q = 1; q < slices; ++q) {
+      const f32x4 v = p[q * tiles * (Sh::TM * Sh::TN / 4)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      lds[(lane & 31) * kPitch + 32 * (br >> 2) + 8 * (br & 3) + 4 * (lane >> 5) + e] = s.v[e] * f;
+  }
+  __syncthreads();
+  const int64_t m0 = tile / dx_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a;
+  const int64_t n0 = tile % dx_n * Sh::TN + wave % Sh::WGN * G::WN;
+#pragma unroll
+  for (int i = int(threadIdx.x); i < 32 * G::WN / 4; i += kThreads) {
+    const int row = i / (G::WN / 4), col = i % (G::WN / 4) * 4;
+    const int64_t m = m0 + row, n = n0 + col;
+    if (m >= rows || n >= width) continue;
+    const float* v = lds + row * kPitch + col;
+    char* to = dx + (m * ld + n) * T::esz;
+    if (vec && n + 4 <= width) {
+      if constexpr (T::esz == 2) *reinterpret_cast<uint2*>(to) = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
+      else *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < width) store_from_f32(to, e, T::mk, v[e]);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- operands off the 16-byte boundaries
@@ -589,13 +672,24 @@ template <typename U>
 __global__ __launch_bounds__(kThreads) void pack_kernel(const U* src, int64_t ld, int64_t rows, int64_t cols, U* dst,
                                                         int64_t ld_dst, Labels labels) {
   constexpr int kE = 16 / int(sizeof(U));
-  const int64_t chunks = ld_dst / kE, i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t row = i / chunks, col = i % chunks * kE;
+  struct __attribute__((packed, aligned(sizeof(U)))) Loose { U v[kE]; };  // 16 bytes at any element
+  struct alignas(16) Chunk { U v[kE]; };
+  const int64_t chunks = ld_dst / kE, first = int64_t(blockIdx.x) * kThreads;
+  const uint32_t in = uint32_t(first % chunks) + threadIdx.x;
+  const int64_t row = first / chunks + in / uint32_t(chunks), col = int64_t(in % uint32_t(chunks)) * kE;
   if (row >= rows) return;
-  const bool zero = labels.has_ignore && labels.ignored(labels.at(row));
-  struct alignas(16) Chunk { U v[kE]; } c;
+  Chunk c;
+  if (labels.has_ignore && labels.ignored(labels.at(row))) {
 #pragma unroll
-  for (int e = 0; e < kE; ++e) c.v[e] = !zero && col + e < cols ? src[row * ld + col + e] : U(0);
+    for (int e = 0; e < kE; ++e) c.v[e] = U(0);
+  } else if (col + kE <= cols) {
+    const Loose l = *reinterpret_cast<const Loose*>(src + row * ld + col);
+#pragma unroll
+    for (int e = 0; e < kE; ++e) c.v[e] = l.v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) c.v[e] = col + e < cols ? src[row * ld + col + e] : U(0);
+  }
   *reinterpret_cast<Chunk*>(dst + row * ld_dst + col) = c;
 }
 
@@ -631,6 +725,7 @@ __global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad,
 
 // ---------------------------------------------------------------- host
 constexpr int64_t kGBytes = int64_t(512) << 20;     // of g a piece
+constexpr int64_t kStreamBytes = int64_t(192) << 20;
 constexpr int64_t kPackBytes = int64_t(256) << 20;  // of w copied a piece
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -643,11 +738,12 @@ bool on_grid(const void* p, int64_t ld, int64_t width, int esz) {
 }
 
 // One call's sizes and its workspace, from the shapes and the operands' alignment alone.
+enum { kBig, kMid };
 struct Plan {
   int esz;
   int64_t rows, width, vocab;
-  bool big;                       // tiles of 256 x 256, else 128 x 128
-  int64_t tm, tn;
+  int logits, products;           // shapes of the kernels that form the logits, and of dx's and dw's
+  int64_t tm, tn, pm, pn;         // their tiles
   bool pack_x, pack_w;
   int64_t pitch;                  // of packed rows, elements
   int64_t piece, pieces;          // classes of a piece
@@ -661,8 +757,10 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   Plan q{};
   q.esz = dtype_bytes(io_type);
   q.rows = rows, q.width = width, q.vocab = vocab;
-  q.big = rows > 128;
-  q.tm = q.tn = q.big ? 256 : 128;
+  q.logits = q.products = rows > 128 ? kBig : kMid;
+  const int64_t sizes[][2] = {{256, 256}, {128, 128}};
+  q.tm = sizes[q.logits][0], q.tn = sizes[q.logits][1];
+  q.pm = sizes[q.products][0], q.pn = sizes[q.products][1];
   q.pack_x = !on_grid(x, ld_x, width, q.esz) || (bwd && has_ignore);
   q.pack_w = !on_grid(w, ld_w, width, q.esz);
   q.pitch = up(width, 16 / q.esz);
@@ -684,9 +782,9 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
     q.ld_g = up(classes, 64);
     q.g_at = take(rows * q.ld_g * q.esz);
     // dx's slices: three rounds of the 256 CUs
-    const int64_t tiles = (rows + q.tm - 1) / q.tm * ((width + q.tn - 1) / q.tn), deep = 128 / q.esz;
+    const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn), deep = 128 / q.esz;
     q.slices = std::max<int64_t>(1, std::min<int64_t>({768 / tiles, 64, (classes + 4 * deep - 1) / (4 * deep)}));
-    q.sums_at = take(q.slices * tiles * q.tm * q.tn * 4);
+    q.sums_at = take(q.slices * tiles * q.pm * q.pn * 4);
     q.dyn_at = take(8);
   }
   q.bytes = at;
@@ -730,12 +828,16 @@ int pack(const char* what, hipStream_t s, const Plan& q, const void* src, int64_
   return check_launch(what);
 }
 
-// f(type, shape) of the call's
+// f(type, shape) of a kernel
+template <class T, class F>
+int with_shape(T t, int shape, F&& f) {
+  return shape == kBig ? f(t, Big{}) : f(t, Mid{});
+}
 template <class F>
-int with_kernels(int io_type, bool big, F&& f) {
-  if (io_type == MK_BF16) return big ? f(Bf16{}, Big{}) : f(Bf16{}, Mid{});
-  if (io_type == MK_F16) return big ? f(F16{}, Big{}) : f(F16{}, Mid{});
-  return big ? f(F32{}, Big{}) : f(F32{}, Mid{});
+int with_kernels(int io_type, int shape, F&& f) {
+  if (io_type == MK_BF16) return with_shape(Bf16{}, shape, f);
+  if (io_type == MK_F16) return with_shape(F16{}, shape, f);
+  return with_shape(F32{}, shape, f);
 }
 
 }  // namespace
@@ -788,7 +890,7 @@ extern "C" int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t w
       a.w = ws + q.w_at, a.ld_w = q.pitch;
     }
     a.tiles_n = int((a.vocab + q.tn - 1) / q.tn);
-    const int rc = with_kernels(io_type, q.big, [&](auto t, auto sh) {
+    const int rc = with_kernels(io_type, q.logits, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
       hipLaunchKernelGGL((loss_kernel<T, Sh>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)), dim3(Geo<Sh>::threads), 0,
@@ -855,12 +957,13 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   a.lse = lse, a.row_grad = row_grad;
   a.x = static_cast<const char*>(x), a.ld_x = ld_x;
   a.g = ws + q.g_at, a.ld_g = q.ld_g;
+  a.stream = rows * q.ld_g * esz >= kStreamBytes;
   a.tiles_m = int((rows + q.tm - 1) / q.tm);
-  b.dx_m = dx ? a.tiles_m : 0;
-  b.dx_n = b.dw_n = int((width + q.tn - 1) / q.tn);
+  b.dx_m = dx ? int((rows + q.pm - 1) / q.pm) : 0;
+  b.dx_n = b.dw_n = int((width + q.pn - 1) / q.pn);
   b.slices = int(q.slices);
   const int64_t most = a.tiles_m * ((q.piece + q.tn - 1) / q.tn),
-                most2 = int64_t(a.tiles_m) * b.dx_n * q.slices + (q.piece + q.tm - 1) / q.tm * b.dw_n;
+                most2 = int64_t(b.dx_m) * b.dx_n * q.slices + (q.piece + q.pm - 1) / q.pm * b.dw_n + 8;
   if (int rc = check_tiles(what, std::max(most, most2), 512)) return rc;
   // fp16: g out of the subnormals, by a power of two of the largest row_grad
   a.unit = io_type == MK_F16 ? 32768.f : 1.f;
@@ -895,27 +998,33 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     b.run = up((a.vocab + q.slices - 1) / q.slices, deep);
     b.dw = static_cast<char*>(dw) + v0 * ld_dw * dwsz;
     a.tiles_n = int((a.vocab + q.tn - 1) / q.tn);
-    b.dw_m = dw ? int((a.vocab + q.tm - 1) / q.tm) : 0;
-    const int rc = with_kernels(io_type, q.big, [&](auto t, auto sh) {
+    b.dw_m = dw ? int((a.vocab + q.pm - 1) / q.pm) : 0;
+    int rc = with_kernels(io_type, q.logits, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
       hipLaunchKernelGGL((grad_kernel<T, Sh>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)), dim3(Geo<Sh>::threads), 0,
                          s, a);
-      if (int r = check_launch(what)) return r;
-      const unsigned tiles = unsigned(b.dx_m) * b.dx_n * b.slices + unsigned(b.dw_m) * b.dw_n;
+      return check_launch(what);
+    });
+    if (rc) return rc;
+    rc = with_kernels(io_type, q.products, [&](auto t, auto sh) {
+      using T = decltype(t);
+      using Sh = decltype(sh);
+      const unsigned tiles = unsigned(b.dx_m) * b.dx_n * b.slices + (unsigned(b.dw_m) * b.dw_n + 7) / 8 * 8;
       hipLaunchKernelGGL((products_kernel<T, Sh>), dim3(tiles), dim3(Geo<Sh>::threads), 0, s, b);
       return check_launch(what);
     });
     if (rc) return rc;
   }
   if (!dx) return MK_OK;
-  return with_kernels(io_type, q.big, [&](auto t, auto sh) {
+  const int dx_vec = reinterpret_cast<uintptr_t>(dx) % (4 * esz) == 0 && ld_dx % 4 == 0;
+  return with_kernels(io_type, q.products, [&](auto t, auto sh) {
     using T = decltype(t);
     using Sh = decltype(sh);
-    const int64_t blocks = int64_t(b.dx_m) * b.dx_n * Sh::TM * Sh::TN / 4 / kThreads;
+    const int64_t blocks = int64_t(b.dx_m) * b.dx_n * Geo<Sh>::W * Geo<Sh>::I;
     if (int r = check_tiles(what, blocks, kThreads)) return r;
     hipLaunchKernelGGL((dx_kernel<T, Sh>), dim3(unsigned(blocks)), dim3(kThreads), 0, s, b.sums, rows, width, b.dx_m, b.dx_n,
-                       b.slices, b.dyn, b.unit, static_cast<char*>(dx), ld_dx);
+                       b.slices, b.dyn, b.unit, static_cast<char*>(dx), ld_dx, dx_vec);
     return check_launch(what);
   });
 }
