@@ -13,11 +13,12 @@
 // p is then a multiple of 2^-16, and the scale is that of the rounded p.
 // The rows start at field 0, so the mask does not depend on their pitch.
 //
-// A thread has a group of 8 columns and walks down the rows, with the bias of its
-// columns (forward) or their sums (backward) in registers; a block is CT groups
-// wide (a power of two that wastes little of the last tile) and 256 / CT rows
-// high.  Sums of columns go through LDS, then as one partial row a block to the
-// workspace, and a second launch adds the partial rows in order.
+// A thread has 16 bytes of a row (8 columns of 16 bits, or half a draw's 4 of 32:
+// lanes that are neighbours read neighbouring bytes) and walks down the rows, with
+// the bias of its columns (forward) or their sums (backward) in registers; a block
+// is CT chunks wide (a power of two that wastes little of the last tile) and 256 /
+// CT rows high.  Sums of columns go through LDS, then as one partial row a block to
+// the workspace, and a second launch adds the partial rows in order.
 #include "mk_common.h"
 
 #include <algorithm>
@@ -28,8 +29,8 @@ namespace mk {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroup = 8;         // columns a thread has: one draw of the generator
-constexpr int64_t kMaxParts = 256;  // partial rows of the column sums
+constexpr int kGroup = 8;  // columns of one draw of the generator
+constexpr int64_t kEach = 4;
 
 struct DropArgs {
   const void *x, *bias, *residual;
@@ -60,38 +61,6 @@ template <> __device__ inline F16 narrow<F16>(float v) { return F16{f32_to_f16(v
 template <typename T> constexpr int kE = 16 / int(sizeof(T));
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Chunk { T v[kE<T>]; };
 
-// the group's n columns at p (n < 8: the row's last)
-template <typename T>
-__device__ inline void load8(const T* p, int n, float (&v)[kGroup]) {
-  if (n == kGroup) {
-#pragma unroll
-    for (int h = 0; h < kGroup / kE<T>; ++h) {
-      const Chunk<T> c = *reinterpret_cast<const Chunk<T>*>(p + kE<T> * h);
-#pragma unroll
-      for (int e = 0; e < kE<T>; ++e) v[kE<T> * h + e] = widen(c.v[e]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kGroup; ++e) v[e] = e < n ? widen(p[e]) : 0.f;
-  }
-}
-template <typename T>
-__device__ inline void store8(T* p, int n, const float (&v)[kGroup]) {
-  if (n == kGroup) {
-#pragma unroll
-    for (int h = 0; h < kGroup / kE<T>; ++h) {
-      Chunk<T> c;
-#pragma unroll
-      for (int e = 0; e < kE<T>; ++e) c.v[e] = narrow<T>(v[kE<T> * h + e]);
-      *reinterpret_cast<Chunk<T>*>(p + kE<T> * h) = c;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kGroup; ++e)
-      if (e < n) p[e] = narrow<T>(v[e]);
-  }
-}
-
 // The 8 fields of group g of row r: Philox-4x32, 10 rounds.
 struct Fields { uint32_t w[4]; };
 __device__ inline Fields philox(uint32_t g, uint32_t r, uint32_t o0, uint32_t o1, uint32_t k0, uint32_t k1) {
@@ -99,9 +68,9 @@ __device__ inline Fields philox(uint32_t g, uint32_t r, uint32_t o0, uint32_t o1
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t p0 = uint64_t(c0) * 0xD2511F53u, p1 = uint64_t(c2) * 0xCD9E8D57u;
-    c0 = uint32_t(p1 >> 32) ^ c1 ^ k0;
+    c0 = __builtin_amdgcn_bitop3_b32(uint32_t(p1 >> 32), c1, k0, 0x96);  // three-way exclusive or
     c1 = uint32_t(p1);
-    c2 = uint32_t(p0 >> 32) ^ c3 ^ k1;
+    c2 = __builtin_amdgcn_bitop3_b32(uint32_t(p0 >> 32), c3, k1, 0x96);
     c3 = uint32_t(p0);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -109,100 +78,152 @@ __device__ inline Fields philox(uint32_t g, uint32_t r, uint32_t o0, uint32_t o1
   return {{c0, c1, c2, c3}};
 }
 
-template <typename T, bool BWD>
+// One element from x (or dy), its bias and residual.
+template <bool BWD>
+__device__ inline float drop(bool keep, float x, float bias, float residual, float scale) {
+  // selected, not multiplied: a dropped infinity or NaN is dropped
+  return BWD ? (keep ? x : 0.f) : (keep ? fmaf(x + bias, scale, residual) : residual);
+}
+__device__ inline uint32_t field(const Fields& f, int e) {
+  return e & 1 ? f.w[e / 2] >> 16 : f.w[e / 2] & 0xFFFFu;
+}
+
+// NR: rows a thread has in flight.  Their loads come first: a row after the other
+// would wait for memory each time, since a store may be what the next load reads
+// as far as the compiler knows.
+template <typename T, bool BWD, int NR>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(const DropArgs a) {
+  constexpr int E = kE<T>;
   const int ct = 1 << a.ct_log2;
   const int tx = int(threadIdx.x) & (ct - 1), ty = int(threadIdx.x) >> a.ct_log2, high = kThreads >> a.ct_log2;
-  const uint32_t tile = blockIdx.x % a.col_tiles;
-  const int64_t block_row = blockIdx.x / a.col_tiles;
-  const int64_t g = int64_t(tile) * ct + tx;
-  const int64_t col = g * kGroup;
-  const int n = int(std::min<int64_t>(a.cols - col, kGroup));  // below 1: no columns here
+  // a run of rows is one XCD's (workgroups are dealt to the 8 of them in turn): rows
+  // off the 128-byte lines have lines that two tiles write
+  const uint32_t turn = blockIdx.x / 8, tile = turn % a.col_tiles;
+  const int64_t block_row = int64_t(turn / a.col_tiles) * 8 + blockIdx.x % 8;
+  const int64_t chunk = int64_t(tile) * ct + tx, col = chunk * E, chunks = a.cols / E;  // whole ones
+  const bool upper = E < kGroup && (chunk & 1);  // of the group's fields
   const uint64_t o = a.offset + (a.step ? *a.step : 0);
   const uint32_t o0 = uint32_t(o), o1 = uint32_t(o >> 32);
-  const T* x = static_cast<const T*>(a.x) + col;
-  const T* res = static_cast<const T*>(a.residual) + col;
-  T* out = static_cast<T*>(a.out) + col;
-  float bias[kGroup], sum[kGroup];
-#pragma unroll
-  for (int e = 0; e < kGroup; ++e) bias[e] = sum[e] = 0.f;
-  if (!BWD && a.bias && n > 0) load8(static_cast<const T*>(a.bias) + col, n, bias);
+  const T* x = static_cast<const T*>(a.x);
+  const T* res = static_cast<const T*>(a.residual);
+  const T* bias_p = static_cast<const T*>(a.bias);
+  T* out = static_cast<T*>(a.out);
   const int64_t r0 = block_row * a.rows_per_block, r1 = std::min(a.rows, r0 + a.rows_per_block);
-  if (n > 0) {
-#pragma unroll 2
-    for (int64_t r = r0 + ty; r < r1; r += high) {
-      float v[kGroup], rv[kGroup];
-      load8(x + r * a.ld_x, n, v);
-      if (!BWD && a.residual) {
-        load8(res + r * a.ld_r, n, rv);
-      } else {
+  if (r0 >= a.rows) return;
+  float bias[E], sum[E];
 #pragma unroll
-        for (int e = 0; e < kGroup; ++e) rv[e] = 0.f;
+  for (int e = 0; e < E; ++e) bias[e] = sum[e] = 0.f;
+  if (chunk < chunks) {
+    if (!BWD && a.bias) {
+      const Chunk<T> b = *reinterpret_cast<const Chunk<T>*>(bias_p + col);
+#pragma unroll
+      for (int e = 0; e < E; ++e) bias[e] = widen(b.v[e]);
+    }
+    for (int64_t r = r0 + ty; r < r1; r += int64_t(high) * NR) {
+      Chunk<T> xv[NR], rv[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int64_t row = r + int64_t(high) * i;
+        if (i > 0 && row >= r1) break;
+        xv[i] = *reinterpret_cast<const Chunk<T>*>(x + row * a.ld_x + col);
+        if (!BWD && a.residual) rv[i] = *reinterpret_cast<const Chunk<T>*>(res + row * a.ld_r + col);
       }
-      const Fields f = philox(uint32_t(g), uint32_t(r), o0, o1, a.k0, a.k1);
 #pragma unroll
-      for (int e = 0; e < kGroup; ++e) {
-        const uint32_t field = e & 1 ? f.w[e / 2] >> 16 : f.w[e / 2] & 0xFFFFu;
-        // selected, not multiplied: a dropped infinity or NaN is dropped
-        const bool keep = field >= a.cut;
-        if (BWD) {
-          v[e] = keep ? v[e] : 0.f;
-          sum[e] += v[e];
-          v[e] *= a.scale;
-        } else {
-          v[e] = keep ? fmaf(v[e] + bias[e], a.scale, rv[e]) : rv[e];
+      for (int i = 0; i < NR; ++i) {
+        const int64_t row = r + int64_t(high) * i;
+        if (i > 0 && row >= r1) break;
+        const Fields f = philox(uint32_t(col / kGroup), uint32_t(row), o0, o1, a.k0, a.k1);
+        Chunk<T> c;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t at = E < kGroup && upper ? field(f, e + E) : field(f, e);
+          float v = drop<BWD>(at >= a.cut, widen(xv[i].v[e]), bias[e], !BWD && a.residual ? widen(rv[i].v[e]) : 0.f, a.scale);
+          if (BWD) sum[e] += v, v *= a.scale;
+          c.v[e] = narrow<T>(v);
         }
+        *reinterpret_cast<Chunk<T>*>(out + row * a.ld_out + col) = c;
       }
-      store8(out + r * a.ld_out, n, v);
+    }
+  }
+  // what is left of the rows past their whole chunks: a thread a row (beside the
+  // chunks, their element loads would be another path through every wave that ends a row)
+  const int left = int(a.cols - chunks * E);
+  const bool has_left = left > 0 && tile + 1 == a.col_tiles;
+  float last[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) last[e] = 0.f;
+  if (has_left) {
+    const int64_t c0 = chunks * E;
+    for (int64_t row = r0 + threadIdx.x; row < r1; row += kThreads) {
+      const Fields f = philox(uint32_t(c0 / kGroup), uint32_t(row), o0, o1, a.k0, a.k1);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (e >= left) break;
+        const uint32_t at = E < kGroup && (chunks & 1) ? field(f, e + E) : field(f, e);
+        float v = drop<BWD>(at >= a.cut, widen(x[row * a.ld_x + c0 + e]), !BWD && a.bias ? widen(bias_p[c0 + e]) : 0.f,
+                            !BWD && a.residual ? widen(res[row * a.ld_r + c0 + e]) : 0.f, a.scale);
+        if (BWD) last[e] += v, v *= a.scale;
+        out[row * a.ld_out + c0 + e] = narrow<T>(v);
+      }
     }
   }
   if (!BWD || !a.part) return;
-  // column sums: the block's rows in order of ty
-  __shared__ float lds[kThreads * kGroup];
+  // column sums: the block's rows in order of ty, the last columns' in the order of the waves
+  __shared__ float lds[kThreads * E];
+  __shared__ float ends[kThreads / kWave][E];
 #pragma unroll
-  for (int e = 0; e < kGroup; ++e) lds[e * kThreads + threadIdx.x] = sum[e];
+  for (int e = 0; e < E; ++e) {
+    lds[threadIdx.x * E + e] = sum[e];
+    last[e] = wave_sum_dpp(last[e]);
+    if ((threadIdx.x & 63) == 0) ends[threadIdx.x >> 6][e] = last[e];
+  }
   __syncthreads();
   float* part = a.part + block_row * a.cols;
-  for (int i = int(threadIdx.x); i < ct * kGroup; i += kThreads) {
-    const int e = i & (kGroup - 1), t = i / kGroup;
+  for (int i = int(threadIdx.x); i < ct * E; i += kThreads) {
     float s = 0.f;
-    for (int y = 0; y < high; ++y) s += lds[e * kThreads + (y << a.ct_log2) + t];
-    const int64_t c = (int64_t(tile) * ct + t) * kGroup + e;
-    if (c < a.cols) part[c] = s;
+    for (int y = 0; y < high; ++y) s += lds[y * ct * E + i];
+    const int64_t c = int64_t(tile) * ct * E + i;
+    if (c < chunks * E) part[c] = s;
+  }
+  if (has_left && int(threadIdx.x) < left) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) s += ends[w][threadIdx.x];
+    part[chunks * E + threadIdx.x] = s;
   }
 }
 
-// y[c] = scale * (the partial rows' sum, 8 runs of them in order)
-__global__ __launch_bounds__(kThreads) void colsum_final_kernel(const float* part, int64_t parts, int64_t cols, float scale,
-                                                                float* y) {
-  __shared__ float lds[8][32];
+// y[c] = scale * (the partial rows' sum, 32 runs of them in order)
+__global__ __launch_bounds__(1024) void colsum_final_kernel(const float* part, int64_t parts, int64_t cols, float scale,
+                                                            float* y) {
+  __shared__ float lds[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = int64_t(blockIdx.x) * 32 + tx;
-  const int64_t run = (parts + 7) / 8, p0 = ty * run, p1 = std::min(parts, p0 + run);
+  const int64_t run = (parts + 31) / 32, p0 = ty * run, p1 = std::min(parts, p0 + run);
   float s = 0.f;
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 8
     for (int64_t p = p0; p < p1; ++p) s += part[p * cols + c];
+  }
   lds[ty][tx] = s;
   __syncthreads();
   if (ty != 0 || c >= cols) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += lds[i][tx];
+  for (int i = 1; i < 32; ++i) s += lds[i][tx];
   y[c] = s * scale;
 }
 
-// Groups a block is wide: the widest power of two that pads the row least.
-int ct_log2(int64_t groups) {
+// Chunks a block is wide: the widest power of two that pads the row least.
+int ct_log2(int64_t chunks) {
   int best = 0;
   int64_t best_pad = -1;
-  for (int l = 8; l >= 3 || (int64_t(1) << l) >= groups; --l) {
-    const int64_t ct = int64_t(1) << l, pad = (groups + ct - 1) / ct * ct;
+  for (int l = 8; l >= 3 || (int64_t(1) << l) >= chunks; --l) {
+    const int64_t ct = int64_t(1) << l, pad = (chunks + ct - 1) / ct * ct;
     if (best_pad < 0 || pad * 16 < best_pad * 15) best = l, best_pad = pad;
     if (l == 0) break;
   }
   return best;
 }
-
-int64_t row_parts(int64_t rows, int high) { return std::min(kMaxParts, (rows + high - 1) / high); }
 
 const char* bad_pointer(const void* p, int bytes, bool needed) {
   if (!p) return needed ? "null " : nullptr;
@@ -220,27 +241,46 @@ int check(const char* what, int io_type, int64_t rows, int64_t cols, double p) {
   return MK_OK;
 }
 
-void draw_args(DropArgs& a, int64_t rows, int64_t cols, double p, uint64_t seed, uint64_t offset, const uint64_t* step) {
+void draw_args(DropArgs& a, int io_type, int64_t rows, int64_t cols, double p, uint64_t seed, uint64_t offset, const uint64_t* step) {
   a.rows = rows, a.cols = cols;
   a.k0 = uint32_t(seed), a.k1 = uint32_t(seed >> 32);
   a.offset = offset, a.step = step;
   a.cut = uint32_t(std::nearbyint(p * 65536.0));
   a.scale = a.cut < 65536u ? float(65536.0 / (65536.0 - a.cut)) : 0.f;
-  const int64_t groups = (cols + kGroup - 1) / kGroup;
-  a.ct_log2 = ct_log2(groups);
-  a.col_tiles = uint32_t((groups + (int64_t(1) << a.ct_log2) - 1) >> a.ct_log2);
+  const int64_t each = io_type == MK_F32 ? 4 : 8, chunks = std::max<int64_t>(1, cols / each);
+  a.ct_log2 = ct_log2(chunks);
+  a.col_tiles = uint32_t((chunks + (int64_t(1) << a.ct_log2) - 1) >> a.ct_log2);
 }
 
+// Rows a thread walks down.  One until the chip is full, then up to 4, which are in
+// flight together; more only with sums of columns, for fewer partial rows.
+int64_t rows_each(const DropArgs& a, bool sums) {
+  const int64_t high = kThreads >> a.ct_log2, deep = (a.rows + high - 1) / high;  // rows of a column of threads
+  auto cut = [&](int64_t blocks) { return (deep + std::max<int64_t>(1, blocks / a.col_tiles) - 1) / std::max<int64_t>(1, blocks / a.col_tiles); };
+  if (!sums) return std::min<int64_t>(kEach, cut(2048));
+  const int64_t each = cut(1024);
+  return each < 8 ? each : cut(512);
+}
+
+template <typename T, bool BWD>
+void launch_rows(hipStream_t s, const DropArgs& a, dim3 g, int64_t each) {
+  const dim3 b{kThreads};
+  if (each >= 4) hipLaunchKernelGGL((dropout_kernel<T, BWD, 4>), g, b, 0, s, a);
+  else if (each >= 2) hipLaunchKernelGGL((dropout_kernel<T, BWD, 2>), g, b, 0, s, a);
+  else hipLaunchKernelGGL((dropout_kernel<T, BWD, 1>), g, b, 0, s, a);
+}
+
+int64_t row_parts(const DropArgs& a) { return (a.rows + a.rows_per_block - 1) / a.rows_per_block; }
+
 template <bool BWD>
-int launch(const char* what, hipStream_t s, int io_type, DropArgs& a, int64_t parts) {
-  a.rows_per_block = (a.rows + parts - 1) / parts;
-  parts = (a.rows + a.rows_per_block - 1) / a.rows_per_block;
-  const uint64_t blocks = uint64_t(parts) * a.col_tiles;
+int launch(const char* what, hipStream_t s, int io_type, DropArgs& a) {
+  const int64_t each = rows_each(a, a.part != nullptr), parts = (a.rows_per_block = each * (kThreads >> a.ct_log2), row_parts(a));
+  const uint64_t blocks = uint64_t((parts + 7) / 8 * 8) * a.col_tiles;
   if (blocks >= uint64_t(1) << 24) return fail(MK_ERR_UNSUPPORTED, std::string(what) + ": too many elements");
-  const dim3 g{unsigned(blocks)}, b{kThreads};
-  if (io_type == MK_BF16) hipLaunchKernelGGL((dropout_kernel<uint16_t, BWD>), g, b, 0, s, a);
-  else if (io_type == MK_F16) hipLaunchKernelGGL((dropout_kernel<F16, BWD>), g, b, 0, s, a);
-  else hipLaunchKernelGGL((dropout_kernel<float, BWD>), g, b, 0, s, a);
+  const dim3 g{unsigned(blocks)};
+  if (io_type == MK_BF16) launch_rows<uint16_t, BWD>(s, a, g, each);
+  else if (io_type == MK_F16) launch_rows<F16, BWD>(s, a, g, each);
+  else launch_rows<float, BWD>(s, a, g, each);
   return check_launch(what);
 }
 
@@ -266,18 +306,22 @@ extern "C" int mk_dropout_add(void* stream, int io_type, int64_t rows, int64_t c
   if (ld_x < 0 || ld_residual < 0 || (rows > 1 && ld_out < cols))
     return fail(MK_ERR_INVALID, std::string(what) + ": a pitch below 0, or rows of out that overlap");
   DropArgs a{};
-  draw_args(a, rows, cols, p, seed, offset, step);
+  draw_args(a, io_type, rows, cols, p, seed, offset, step);
   a.x = x, a.bias = bias, a.residual = residual, a.out = out;
   a.ld_x = ld_x, a.ld_r = ld_residual, a.ld_out = ld_out;
-  // a row a thread until 16 blocks a CU are there, then longer walks
-  const int high = kThreads >> a.ct_log2;
-  const int64_t most = (rows + high - 1) / high, want = std::max<int64_t>(1, 8192 / a.col_tiles);
-  return launch<false>(what, as_stream(stream), io_type, a, std::min(most, want));
+  return launch<false>(what, as_stream(stream), io_type, a);
 }
 
 extern "C" size_t mk_dropout_add_bwd_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return size_t(std::min(kMaxParts, rows) * cols * 4);
+  DropArgs a{};
+  int64_t parts = 0;
+  for (int t : {MK_BF16, MK_F32}) {  // 8 or 4 columns a thread
+    draw_args(a, t, rows, cols, 0.0, 0, 0, nullptr);
+    a.rows_per_block = rows_each(a, true) * (kThreads >> a.ct_log2);
+    parts = std::max(parts, row_parts(a));
+  }
+  return size_t(parts * cols * 4);
 }
 
 extern "C" int mk_dropout_add_bwd(void* stream, int io_type, int64_t rows, int64_t cols, const void* dy, int64_t ld_dy,
@@ -300,15 +344,14 @@ extern "C" int mk_dropout_add_bwd(void* stream, int io_type, int64_t rows, int64
   if (ld_dy < 0 || (rows > 1 && ld_dx < cols))
     return fail(MK_ERR_INVALID, std::string(what) + ": a pitch below 0, or rows of dx that overlap");
   DropArgs a{};
-  draw_args(a, rows, cols, p, seed, offset, step);
+  draw_args(a, io_type, rows, cols, p, seed, offset, step);
   a.x = dy, a.out = dx;
   a.ld_x = ld_dy, a.ld_out = ld_dx;
   a.part = dx_colsum ? static_cast<float*>(workspace) : nullptr;
   hipStream_t s = as_stream(stream);
-  if (int rc = launch<true>(what, s, io_type, a, row_parts(rows, kThreads >> a.ct_log2))) return rc;
+  if (int rc = launch<true>(what, s, io_type, a)) return rc;
   if (!dx_colsum) return MK_OK;
-  const int64_t parts = (rows + a.rows_per_block - 1) / a.rows_per_block;
-  hipLaunchKernelGGL(colsum_final_kernel, dim3(unsigned((cols + 31) / 32)), dim3(kThreads), 0, s, a.part, parts, cols,
+  hipLaunchKernelGGL(colsum_final_kernel, dim3(unsigned((cols + 31) / 32)), dim3(1024), 0, s, a.part, row_parts(a), cols,
                      a.scale, dx_colsum);
   return check_launch(what);
 }

@@ -91,8 +91,12 @@ def test_workspaces(lib):
     assert grad(65536, 131072) < 65536 * 131072 * 2 // 10
     assert grad(1000, 5000, 1) == grad(1000, 5000) + 1000 * 768 * 2
     assert lib.mk_dropout_add_bwd_workspace_bytes(0, 768) == 0
-    assert lib.mk_dropout_add_bwd_workspace_bytes(3, 768) == 3 * 768 * 4
-    assert lib.mk_dropout_add_bwd_workspace_bytes(1 << 20, 768) <= 1 << 20
+    # a partial row for each run of rows, never more than there are rows; and at most 1024 blocks
+    # of 256 threads write them, 8 columns a thread, so no more than 1024 * 2048 numbers
+    for rows in (1, 3, 1000, 1 << 20):
+        for cols in (1, 100, 768, 1001, 16384):
+            size = lib.mk_dropout_add_bwd_workspace_bytes(rows, cols)
+            assert cols * 4 <= size <= min(rows * cols, 1024 * 2048) * 4
 
 
 def test_dropout(lib):
