@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <numeric>
 #include <string>
 
 #include "gemm_tile.h"
@@ -30,7 +31,7 @@ using namespace attn;
 
 constexpr int kGroupM = 4;                  // tile rows per group of the tile order
 constexpr int kInvalid = int(0x80000000u);  // buffer offset past the range of every copy
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 256;               // of the kernels without products
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -92,27 +93,23 @@ struct Operand {
   const char* base;
   int64_t step;  // bytes from a k tile to the next
   uint32_t off[kC];
-  int32_t k[kC];
+  // the tile row and the k of this lane's chunk of copy c
+  static __device__ inline void chunk(int c, int wave, int lane, int& row, int& k) {
+    const int u = 64 * (wave + W * c) + lane, r = u / kCpr;
+    row = KC ? r : kE * ((u % kCpr) ^ (T::esz == 2 ? nc_swizzle<R>(r) : 0));
+    k = KC ? kE * ((u % kCpr) ^ kc_swizzle<BK>(r)) : r;
+  }
   __device__ inline Operand(int wave, int lane, const char* base, int64_t rows, int64_t ld)
       : base(base), step(KC ? kRow : kDeep * ld * T::esz) {
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      const int u = 64 * (wave + W * c) + lane, r = u / kCpr;
-      int row;
-      if constexpr (KC) {
-        row = r;
-        k[c] = kE * ((u % kCpr) ^ kc_swizzle<BK>(row));
-        off[c] = uint32_t(row * ld * T::esz + k[c] * T::esz);
-      } else {
-        row = kE * ((u % kCpr) ^ (T::esz == 2 ? nc_swizzle<R>(r) : 0));
-        k[c] = r;
-        off[c] = uint32_t(r * ld * T::esz + row * T::esz);
-      }
-      if (row >= rows) off[c] = uint32_t(kInvalid), k[c] = 0x7fffffff - kDeep;
+      int row, k;
+      chunk(c, wave, lane, row, k);
+      off[c] = row < rows ? uint32_t((KC ? row * ld + k : k * ld + row) * T::esz) : uint32_t(kInvalid);
     }
   }
   // the copies of k tile kt, of which the operand has K - kDeep kt k
-  __device__ inline void issue(int kt, int64_t K, char* tile, int wave) const {
+  __device__ inline void issue(int kt, int64_t K, char* tile, int wave, int lane) const {
     const i32x4_t r = tile_desc(base + kt * step, uint32_t(kInvalid));
     const int64_t left = K - int64_t(kDeep) * kt;
     if (left >= kDeep) {
@@ -120,9 +117,13 @@ struct Operand {
       for (int c = 0; c < kC; ++c) copy_to_lds_so(r, lds_addr(tile + 1024 * (wave + W * c)), int(off[c]), 0);
       return;
     }
+    asm volatile("" : "+v"(lane));  // nothing of the last tile's is held through the loop
 #pragma unroll
-    for (int c = 0; c < kC; ++c)
-      copy_to_lds(r, lds_addr(tile + 1024 * (wave + W * c)), k[c] < left ? int(off[c]) : kInvalid);
+    for (int c = 0; c < kC; ++c) {
+      int row, k;
+      chunk(c, wave, lane, row, k);
+      copy_to_lds(r, lds_addr(tile + 1024 * (wave + W * c)), k < left ? int(off[c]) : kInvalid);
+    }
   }
 };
 
@@ -137,56 +138,55 @@ __device__ inline u32x4_t read_chunk(const char* t, int rb, int ks, int lane) {
 }
 
 // acc += A B of one workgroup tile over K: the k loop of gemm_tiled.hip.  A wave
-// waits for its own copies of tile kt (those of the S - 2 tiles after it may be in
-// flight), the barrier publishes all and frees the stage of tile kt - 1, whose
-// next copies are issued beside the first k-steps' MFMAs.  Ends with a barrier:
-// the operands' LDS is free.
+// waits for its own copies of tile kt, the barrier publishes all and frees the
+// other stage, whose next copies are issued beside the first k-steps' MFMAs.
+// start() issues the first k tile's copies, into the first stage; run() ends with a
+// barrier: the operands' LDS is free, and start() of the next product may follow.
 template <class T, class Sh, bool AKC, bool BKC>
-__device__ __attribute__((always_inline)) inline void product(const char* A, int64_t lda, int64_t a_rows,
-                                                              const char* B, int64_t ldb, int64_t b_rows, int64_t K,
-                                                              char* lds, int wave, int lane, Acc<Sh>& acc) {
+struct Product {
   using G = Geo<Sh>;
-  constexpr int S = Sh::S, BK = Sh::BK;
-  const int wm = wave / Sh::WGN, wn = wave % Sh::WGN;
-  using OA = Operand<T, AKC, Sh::TM, G::W, BK>;
-  using OB = Operand<T, BKC, Sh::TN, G::W, BK>;
-  const OA oa(wave, lane, A, a_rows, lda);
-  const OB ob(wave, lane, B, b_rows, ldb);
-  constexpr int kA = Sh::TM * G::row_bytes;
-  const int nk = int((K + OA::kDeep - 1) / OA::kDeep);
-#pragma unroll
-  for (int st = 0; st < S - 1; ++st)
-    if (st < nk) {
-      oa.issue(st, K, lds + st * G::stage, wave);
-      ob.issue(st, K, lds + st * G::stage + kA, wave);
-    }
-  int stage = 0, fill = S - 1;
-  for (int kt = 0; kt < nk; ++kt) {
-    if (kt + S - 2 < nk) wait_vm<(S - 2) * (OA::kC + OB::kC)>();
-    else wait_vm<0>();
-    lds_barrier();
-    const char* at = lds + stage * G::stage;
-    char* next = lds + fill * G::stage;
-    const bool more = kt + S - 1 < nk;
-#pragma unroll
-    for (int ks = 0; ks < G::steps; ++ks) {
-      u32x4_t af[G::I], bf[G::J];
-#pragma unroll
-      for (int a = 0; a < G::I; ++a) af[a] = read_chunk<T, AKC, Sh::TM, BK>(at, wm * G::WM + 32 * a, ks, lane);
-#pragma unroll
-      for (int b = 0; b < G::J; ++b) bf[b] = read_chunk<T, BKC, Sh::TN, BK>(at + kA, wn * G::WN + 32 * b, ks, lane);
-      if (more && ks == 0) oa.issue(kt + S - 1, K, next, wave);
-      if (more && ks == 1) ob.issue(kt + S - 1, K, next + kA, wave);
-#pragma unroll
-      for (int a = 0; a < G::I; ++a)
-#pragma unroll
-        for (int b = 0; b < G::J; ++b) acc[a][b] = T::mma(bf[b], af[a], acc[a][b]);
-    }
-    stage = stage + 1 == S ? 0 : stage + 1;
-    fill = fill + 1 == S ? 0 : fill + 1;
+  using OA = Operand<T, AKC, Sh::TM, G::W, Sh::BK>;
+  using OB = Operand<T, BKC, Sh::TN, G::W, Sh::BK>;
+  static constexpr int kA = Sh::TM * G::row_bytes;
+  static_assert(Sh::S == 2, "two stages");
+  OA oa;
+  OB ob;
+  int64_t K;
+  __device__ inline Product(const char* A, int64_t lda, int64_t a_rows, const char* B, int64_t ldb, int64_t b_rows,
+                            int64_t K, int wave, int lane)
+      : oa(wave, lane, A, a_rows, lda), ob(wave, lane, B, b_rows, ldb), K(K) {}
+  __device__ inline void start(char* lds, int wave, int lane) const {
+    if (K <= 0) return;
+    oa.issue(0, K, lds, wave, lane);
+    ob.issue(0, K, lds + kA, wave, lane);
   }
-  lds_barrier();
-}
+  __device__ __attribute__((always_inline)) inline void run(char* lds, int wave, int lane, Acc<Sh>& acc) const {
+    const int wm = wave / Sh::WGN, wn = wave % Sh::WGN;
+    const int nk = int((K + OA::kDeep - 1) / OA::kDeep);
+    for (int kt = 0; kt < nk; ++kt) {
+      wait_vm<0>();
+      lds_barrier();
+      const char* at = lds + (kt & 1) * G::stage;
+      char* next = lds + ((kt + 1) & 1) * G::stage;
+      const bool more = kt + 1 < nk;
+#pragma unroll
+      for (int ks = 0; ks < G::steps; ++ks) {
+        u32x4_t af[G::I], bf[G::J];
+#pragma unroll
+        for (int a = 0; a < G::I; ++a) af[a] = read_chunk<T, AKC, Sh::TM, Sh::BK>(at, wm * G::WM + 32 * a, ks, lane);
+#pragma unroll
+        for (int b = 0; b < G::J; ++b) bf[b] = read_chunk<T, BKC, Sh::TN, Sh::BK>(at + kA, wn * G::WN + 32 * b, ks, lane);
+        if (more && ks == 0) oa.issue(kt + 1, K, next, wave, lane);
+        if (more && ks == 1) ob.issue(kt + 1, K, next + kA, wave, lane);
+#pragma unroll
+        for (int a = 0; a < G::I; ++a)
+#pragma unroll
+          for (int b = 0; b < G::J; ++b) acc[a][b] = T::mma(bf[b], af[a], acc[a][b]);
+      }
+    }
+    lds_barrier();
+  }
+};
 
 template <class Sh>
 __device__ inline void zero(Acc<Sh>& acc) {
@@ -232,79 +232,100 @@ struct LossArgs {
   int64_t v0;              // the piece's first class
   int tiles_m, tiles_n;
   Labels labels;
-  float2* part;            // [tiles_n][rows]: maximum and sum of exponentials
+  float2* part;            // [tiles_n][rows]: t and the sum of 2^(s log2(e) - t)
   float* target;           // [rows]: the label's logit
 };
 
+// Exponentials are of base 2, of s log2(e) - t with t the rounded product of the
+// row's maximum and log2(e): t is what the tile's sum is relative to, exactly.
+// A workgroup has every gridDim-th tile, and the next one's first copies in flight
+// while it ends a tile.
 template <class T, class Sh>
 __global__ __launch_bounds__(Geo<Sh>::threads, 2) void loss_kernel(const LossArgs p) {
   using G = Geo<Sh>;
+  using P = Product<T, Sh, true, true>;
   __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
+  __shared__ float2 red[Sh::WGN * Sh::TM];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
-  uint32_t tm, tn;
-  tile_of(blockIdx.x, gridDim.x, uint32_t(p.tiles_m), uint32_t(p.tiles_n), tm, tn);
-  const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
-  Acc<Sh> acc;
-  zero<Sh>(acc);
-  product<T, Sh, true, true>(p.x + m0 * p.ld_x * T::esz, p.ld_x, p.rows - m0, p.w + n0 * p.ld_w * T::esz, p.ld_w,
-                             p.vocab - n0, p.width, lds, wave, lane, acc);
-  // a lane has, of row 32 a + c, the columns 32 b + 8 (r / 4) + 4 g + r % 4
-  const int nl = wn * G::WN + 4 * g;
-  if (n0 + Sh::TN > p.vocab) {
+  const uint32_t nt = uint32_t(p.tiles_m) * uint32_t(p.tiles_n);
+  auto tile = [&](uint32_t i, int64_t& m0, int64_t& n0) __attribute__((always_inline)) {
+    uint32_t tm, tn;
+    tile_of(i, nt, uint32_t(p.tiles_m), uint32_t(p.tiles_n), tm, tn);
+    m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
+    return P(p.x + m0 * p.ld_x * T::esz, p.ld_x, p.rows - m0, p.w + n0 * p.ld_w * T::esz, p.ld_w, p.vocab - n0, p.width,
+             wave, lane);
+  };
+  int64_t m0, n0;
+  P now = tile(blockIdx.x, m0, n0);
+  now.start(lds, wave, lane);
+  for (uint32_t i = blockIdx.x;;) {
+    int rel[G::I];  // the label's column of this wave's, -1: none
 #pragma unroll
-    for (int b = 0; b < G::J; ++b)
+    for (int a = 0; a < G::I; ++a) {
+      const int64_t m = m0 + wm * G::WM + 32 * a + c;
+      const int64_t at = m < p.rows ? p.labels.at(m) - p.v0 - n0 - wn * G::WN : -1;
+      rel[a] = at >= 0 && at < G::WN ? int(at) : -1;
+    }
+    Acc<Sh> acc;
+    zero<Sh>(acc);
+    now.run(lds, wave, lane, acc);
+    const int64_t m_now = m0, n_now = n0;
+    i += gridDim.x;
+    if (i < nt) {
+      now = tile(i, m0, n0);
+      now.start(lds, wave, lane);
+    }
+    // a lane has, of row 32 a + c, the columns 32 b + 8 (r / 4) + 4 g + r % 4
+    if (n_now + Sh::TN > p.vocab) {
+      const int64_t left = p.vocab - n_now - wn * G::WN - 4 * g;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (n0 + nl + 32 * b + 8 * (r / 4) + r % 4 >= p.vocab)
+      for (int b = 0; b < G::J; ++b)
 #pragma unroll
-          for (int a = 0; a < G::I; ++a) acc[a][b][r] = -INFINITY;
-  }
-  float2* red = reinterpret_cast<float2*>(lds);  // [WGN][TM]
+        for (int r = 0; r < 16; ++r)
+          if (32 * b + 8 * (r / 4) + r % 4 >= left)
 #pragma unroll
-  for (int a = 0; a < G::I; ++a) {
-    const int ml = wm * G::WM + 32 * a + c;
-    const int64_t m = m0 + ml;
-    if (m < p.rows) {
-      const int64_t rel = p.labels.at(m) - p.v0 - n0 - wn * G::WN;  // the label's column of this wave's
-      if (rel >= 0 && rel < G::WN) {
+            for (int a = 0; a < G::I; ++a) acc[a][b][r] = -INFINITY;
+    }
+#pragma unroll
+    for (int a = 0; a < G::I; ++a) {
+      const int ml = wm * G::WM + 32 * a + c;
+      if (rel[a] >= 0) {
 #pragma unroll
         for (int b = 0; b < G::J; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (rel == 32 * b + 8 * (r / 4) + 4 * g + r % 4) p.target[m] = acc[a][b][r];
+            if (rel[a] == 32 * b + 8 * (r / 4) + 4 * g + r % 4) p.target[m_now + ml] = acc[a][b][r];
       }
+      float top = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < G::J; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[a][b][r]);
+      float lo, hi;
+      lane_halves_sched(top, lo, hi);
+      top = fmaxf(lo, hi);
+      const float t = top * kLog2e, from = t == -INFINITY ? 0.f : t;  // nothing but -inf: a sum of 0
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < G::J; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[a][b][r], kLog2e, -from));
+      lane_halves_sched(sum, lo, hi);
+      if (g == 0) red[wn * Sh::TM + ml] = float2{t, lo + hi};
     }
-    float top = -INFINITY;
+    lds_barrier();
+    for (int e = int(threadIdx.x); e < Sh::TM; e += G::threads) {
+      if (m_now + e >= p.rows) break;
+      float t = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int b = 0; b < G::J; ++b)
+      for (int q = 0; q < Sh::WGN; ++q) t = fmaxf(t, red[q * Sh::TM + e].x);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[a][b][r]);
-    float lo, hi;
-    lane_halves_sched(top, lo, hi);
-    top = fmaxf(lo, hi);
-    const float from = top == -INFINITY ? 0.f : top;  // nothing but -inf: a sum of 0
-    float sum = 0.f;
-#pragma unroll
-    for (int b = 0; b < G::J; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[a][b][r] - from) * kLog2e);
-    lane_halves_sched(sum, lo, hi);
-    if (g == 0) red[wn * Sh::TM + ml] = float2{top, lo + hi};
-  }
-  lds_barrier();
-  for (int i = int(threadIdx.x); i < Sh::TM; i += G::threads) {
-    if (m0 + i >= p.rows) break;
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int q = 0; q < Sh::WGN; ++q) top = fmaxf(top, red[q * Sh::TM + i].x);
-    const float from = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int q = 0; q < Sh::WGN; ++q) {
-      const float2 v = red[q * Sh::TM + i];
-      sum += v.y * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
+      for (int q = 0; q < Sh::WGN; ++q)
+        sum += red[q * Sh::TM + e].y * __builtin_amdgcn_exp2f(red[q * Sh::TM + e].x - (t == -INFINITY ? 0.f : t));
+      p.part[n_now / Sh::TN * p.rows + m_now + e] = float2{t, sum};
     }
-    p.part[int64_t(tn) * p.rows + m0 + i] = float2{top, sum};
+    if (i >= nt) return;
   }
 }
 
@@ -326,10 +347,10 @@ __global__ __launch_bounds__(kThreads) void loss_final_kernel(const float2* part
       float to = top;
 #pragma unroll
       for (int i = 0; i < kAt; ++i) to = fmaxf(to, v[i].x);
-      const float from = to == -INFINITY ? 0.f : to;  // nothing but -inf: a sum of 0
-      sum *= __builtin_amdgcn_exp2f((top - from) * kLog2e);
+      const float from = to == -INFINITY ? 0.f : to;
+      sum *= __builtin_amdgcn_exp2f(top - from);
 #pragma unroll
-      for (int i = 0; i < kAt; ++i) sum += v[i].y * __builtin_amdgcn_exp2f((v[i].x - from) * kLog2e);
+      for (int i = 0; i < kAt; ++i) sum += v[i].y * __builtin_amdgcn_exp2f(v[i].x - from);
       top = to;
     }
   }
@@ -341,8 +362,8 @@ __global__ __launch_bounds__(kThreads) void loss_final_kernel(const float2* part
   const float from = top == -INFINITY ? 0.f : top;
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum += red[i][tx].y * __builtin_amdgcn_exp2f((red[i][tx].x - from) * kLog2e);
-  const float z = top + logf(sum);
+  for (int i = 0; i < 16; ++i) sum += red[i][tx].y * __builtin_amdgcn_exp2f(red[i][tx].x - from);
+  const float z = (top + log2f(sum)) * kLn2;
   if (lse) lse[n] = z;
   if (!loss) return;
   const int64_t label = labels.at(n);
@@ -361,7 +382,6 @@ struct GradArgs {
   float unit;        // factor of g
   char* g;           // [rows][ld_g], columns past vocab up to a whole chunk are zeros
   int64_t ld_g;
-  int stream;        // g goes past the caches
 };
 
 __device__ inline uint32_t pack2(Bf16, float a, float b) {
@@ -369,14 +389,50 @@ __device__ inline uint32_t pack2(Bf16, float a, float b) {
 }
 __device__ inline uint32_t pack2(F16, float a, float b) { return uint32_t(f32_to_f16(a)) | (uint32_t(f32_to_f16(b)) << 16); }
 
-// A tile of 16-bit results through LDS (gemm_tiled.hip's store_staged): value
-// v(a, b, rg, acc) of the 4 columns 32 b + 8 rg + 4 g .. + 3 of a lane's row 32 a +
-// c, then whole 16-byte chunks of rows, or (vec false) element by element.
-// rows, cols: what of the tile is stored.
+// 16 bits: the 8 columns 32 b + 16 h + 8 g .. + 7 of a lane's row 32 a + c as one
+// chunk.  value(a, b, rg, v) gives the 4 columns 32 b + 8 rg + 4 g .. + 3; lanes l
+// and l + 32 trade halves of them.
+template <class T, class V>
+__device__ __attribute__((always_inline)) inline u32x4_t chunk16(int a, int b, int h, V&& value) {
+  uint2 w[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float v[4];
+    value(a, b, 2 * h + e, v);
+    w[e] = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
+  }
+  const auto s0 = __builtin_amdgcn_permlane32_swap(w[0].x, w[1].x, false, false);
+  const auto s1 = __builtin_amdgcn_permlane32_swap(w[0].y, w[1].y, false, false);
+  return u32x4_t{static_cast<uint32_t>(s0[0]), static_cast<uint32_t>(s1[0]), static_cast<uint32_t>(s0[1]),
+                 static_cast<uint32_t>(s1[1])};
+}
+
+// A tile of 16-bit results straight from the accumulators, whole chunks of rows (cols
+// a multiple of 8).  rows, cols: what of the tile is stored.
 template <class T, class Sh, class V>
-__device__ __attribute__((always_inline)) inline void store16(char* lds, int wave, int lane, char* out,
-                                                              int64_t ld, int64_t rows, int64_t cols, bool vec,
-                                                              bool stream, V&& value) {
+__device__ __attribute__((always_inline)) inline void store16_direct(int wave, int lane, char* out, int64_t ld,
+                                                                     int64_t rows, int64_t cols, V&& value) {
+  using G = Geo<Sh>;
+  const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
+#pragma unroll
+  for (int a = 0; a < G::I; ++a) {
+    const int ml = wm * G::WM + 32 * a + c;
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4_t chunk = chunk16<T>(a, b, h, value);
+        const int nl = wn * G::WN + 32 * b + 16 * h + 8 * g;
+        if (ml < rows && nl < cols) *reinterpret_cast<u32x4_t*>(out + (ml * ld + nl) * 2) = chunk;
+      }
+  }
+}
+
+// The same through LDS (gemm_tiled.hip's store_staged): rows go out in runs, as whole
+// chunks or (vec false) element by element.
+template <class T, class Sh, class V>
+__device__ __attribute__((always_inline)) inline void store16(char* lds, int wave, int lane, char* out, int64_t ld,
+                                                              int64_t rows, int64_t cols, bool vec, V&& value) {
   using G = Geo<Sh>;
   constexpr int kCpr = Sh::TN / 8;
   static_assert(kCpr % 16 == 0, "staging rows of whole 16-chunk groups");
@@ -389,40 +445,18 @@ __device__ __attribute__((always_inline)) inline void store16(char* lds, int wav
     for (int b = 0; b < G::J; ++b)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint2 w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v[4];
-          value(a, b, 2 * h + e, v);
-          w[e] = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
-        }
-        // lanes l and l + 32 trade halves, so that each has 8 consecutive columns
-        const auto s0 = __builtin_amdgcn_permlane32_swap(w[0].x, w[1].x, false, false);
-        const auto s1 = __builtin_amdgcn_permlane32_swap(w[0].y, w[1].y, false, false);
-        const u32x4_t chunk = {static_cast<uint32_t>(s0[0]), static_cast<uint32_t>(s1[0]),
-                               static_cast<uint32_t>(s0[1]), static_cast<uint32_t>(s1[1])};
         const int cn = (wn * G::WN + 32 * b + 16 * h + 8 * g) >> 3;
-        *reinterpret_cast<u32x4_t*>(st + ml * Sh::TN + 8 * (cn ^ (ml & 15))) = chunk;
+        *reinterpret_cast<u32x4_t*>(st + ml * Sh::TN + 8 * (cn ^ (ml & 15))) = chunk16<T>(a, b, h, value);
       }
   }
   lds_barrier();
-  auto chunks = [&](auto past) __attribute__((always_inline)) {
+  if (vec) {
 #pragma unroll 4
     for (int it = 0; it < Sh::TM * kCpr / G::threads; ++it) {
       const int e = it * G::threads + int(threadIdx.x), row = e / kCpr, cn = e % kCpr;
       const u32x4_t v = *reinterpret_cast<const u32x4_t*>(st + row * Sh::TN + 8 * (cn ^ (row & 15)));
-      u32x4_t* const to = reinterpret_cast<u32x4_t*>(out + (row * ld + 8 * cn) * 2);
-      if (row < rows && 8 * cn < cols) {
-        if constexpr (decltype(past)::value) __builtin_nontemporal_store(v, to);
-        else *to = v;
-      }
+      if (row < rows && 8 * cn < cols) *reinterpret_cast<u32x4_t*>(out + (row * ld + 8 * cn) * 2) = v;
     }
-  };
-  if (vec && stream) {
-    chunks(std::true_type{});
-    asm volatile("");  // keeps the two loops' stores apart
-  } else if (vec) {
-    chunks(std::false_type{});
   } else {
     for (int it = 0; it < Sh::TM * Sh::TN / G::threads; ++it) {
       const int e = it * G::threads + int(threadIdx.x), row = e / Sh::TN, col = e % Sh::TN;
@@ -462,6 +496,10 @@ __device__ __attribute__((always_inline)) inline void store32(int wave, int lane
   }
 }
 
+// One tile a workgroup: its 128 KB of stores leave while the next workgroup begins
+// (a workgroup that goes on from tile to tile as loss_kernel's, with the next
+// tile's copies and rows ahead of the stores, took the same time, 1975 us for the
+// gradient of 8192 x 768 x 50257, and held registers the compiler had to spill).
 template <class T, class Sh>
 __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArgs p) {
   using G = Geo<Sh>;
@@ -471,43 +509,47 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
   uint32_t tm, tn;
   tile_of(blockIdx.x, gridDim.x, uint32_t(p.tiles_m), uint32_t(p.tiles_n), tm, tn);
   const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
-  Acc<Sh> acc;
-  zero<Sh>(acc);
-  product<T, Sh, true, true>(p.x + m0 * p.ld_x * T::esz, p.ld_x, p.rows - m0, p.w + n0 * p.ld_w * T::esz, p.ld_w,
-                             p.vocab - n0, p.width, lds, wave, lane, acc);
-  // Most tiles have every class, and waves no ignored row: an exponential, its
-  // exponent and a factor for each element.  The label's -1 is put in afterwards
-  // by the few lanes that have one.
+  const Product<T, Sh, true, true> logits(p.x + m0 * p.ld_x * T::esz, p.ld_x, p.rows - m0, p.w + n0 * p.ld_w * T::esz,
+                                          p.ld_w, p.vocab - n0, p.width, wave, lane);
+  logits.start(lds, wave, lane);
   const float unit = p.dyn ? p.dyn[0] : p.unit;
-  float factor[G::I];
+  float lse[G::I], factor[G::I];
+  int rel[G::I];  // the label's column of this lane's, -1: none
   bool counts = true;
 #pragma unroll
   for (int a = 0; a < G::I; ++a) {
     const int64_t m = m0 + wm * G::WM + 32 * a + c;
-    int64_t rel = -1;  // the label's column of this lane's
-    float lse = 0.f;
-    factor[a] = 0.f;
+    lse[a] = factor[a] = 0.f, rel[a] = -1;
     if (m < p.rows) {
-      const int64_t label = p.labels.at(m);
-      rel = label - p.v0 - n0 - wn * G::WN - 4 * g;
-      lse = p.lse[m];
+      const int64_t label = p.labels.at(m), at = label - p.v0 - n0 - wn * G::WN - 4 * g;
+      lse[a] = p.lse[m];
       factor[a] = unit * (p.row_grad ? p.row_grad[m] : 1.f);
-      if (p.labels.ignored(label)) factor[a] = 0.f, rel = -1, counts = false;
+      if (p.labels.ignored(label)) factor[a] = 0.f, counts = false;
+      else if (at >= 0 && at < G::WN) rel[a] = int(at);
     }
-    const float from = -lse * kLog2e;
+  }
+  Acc<Sh> acc;
+  zero<Sh>(acc);
+  logits.run(lds, wave, lane, acc);
+  // Most tiles have every class, and waves no ignored row: an exponential, its
+  // exponent and a factor for each element.  The label's -1 is put in afterwards
+  // by the few lanes that have one.
+#pragma unroll
+  for (int a = 0; a < G::I; ++a) {
+    const float from = -lse[a] * kLog2e;
 #pragma unroll
     for (int b = 0; b < G::J; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         // 32-bit results: the difference first, which is exact where it is small
-        acc[a][b][r] = __builtin_amdgcn_exp2f(T::esz == 4 ? (acc[a][b][r] - lse) * kLog2e
+        acc[a][b][r] = __builtin_amdgcn_exp2f(T::esz == 4 ? (acc[a][b][r] - lse[a]) * kLog2e
                                                           : fmaf(acc[a][b][r], kLog2e, from));
-    if (rel >= 0 && rel < G::WN) {
+    if (rel[a] >= 0) {
 #pragma unroll
       for (int b = 0; b < G::J; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (rel == 32 * b + 8 * (r / 4) + r % 4) acc[a][b][r] -= 1.f;
+          if (rel[a] == 32 * b + 8 * (r / 4) + r % 4) acc[a][b][r] -= 1.f;
     }
   }
   if (!__all(counts) || n0 + Sh::TN > p.vocab) {
@@ -528,7 +570,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
   constexpr int kE = 16 / T::esz;
   const int64_t rows = p.rows - m0, cols = (p.vocab + kE - 1) / kE * kE - n0;
   char* out = p.g + (m0 * p.ld_g + n0) * T::esz;
-  if constexpr (T::esz == 2) store16<T, Sh>(lds, wave, lane, out, p.ld_g, rows, cols, true, p.stream, value);
+  if constexpr (T::esz == 2) store16_direct<T, Sh>(wave, lane, out, p.ld_g, rows, cols, value);
   else store32<Sh>(wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, true, value);
 }
 
@@ -581,9 +623,11 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
             for (int q = 0; q < 4; ++q) acc[a][b][4 * rg + q] = v.v[q];
           }
     }
-    product<T, Sh, true, false>(p.g + (m0 * p.ld_g + k0) * T::esz, p.ld_g, p.rows - m0,
-                                p.w + (k0 * p.ld_w + n0) * T::esz, p.ld_w, p.width - n0,
-                                min(p.run, p.vocab - k0), lds, wave, lane, acc);
+    const Product<T, Sh, true, false> dx(p.g + (m0 * p.ld_g + k0) * T::esz, p.ld_g, p.rows - m0,
+                                         p.w + (k0 * p.ld_w + n0) * T::esz, p.ld_w, p.width - n0,
+                                         min(p.run, p.vocab - k0), wave, lane);
+    dx.start(lds, wave, lane);
+    dx.run(lds, wave, lane, acc);
 #pragma unroll
     for (int a = 0; a < G::I; ++a)
 #pragma unroll
@@ -597,8 +641,10 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   if (!tile_of(blockIdx.x, n_dw, uint32_t(p.dw_m), uint32_t(p.dw_n), tm, tn)) return;
   const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
   zero<Sh>(acc);
-  product<T, Sh, false, false>(p.g + m0 * T::esz, p.ld_g, p.vocab - m0, p.x + n0 * T::esz, p.ld_x, p.width - n0, p.rows,
-                               lds, wave, lane, acc);
+  const Product<T, Sh, false, false> dw(p.g + m0 * T::esz, p.ld_g, p.vocab - m0, p.x + n0 * T::esz, p.ld_x, p.width - n0,
+                                        p.rows, wave, lane);
+  dw.start(lds, wave, lane);
+  dw.run(lds, wave, lane, acc);
   const float unit = p.dyn ? p.dyn[1] : p.unit;
   auto value = [&](int a, int b, int rg, float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
@@ -607,7 +653,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   const int64_t rows = p.vocab - m0, cols = p.width - n0;
   if constexpr (T::esz == 2) {
     if (!p.dw_f32) {
-      store16<T, Sh>(lds, wave, lane, p.dw + (m0 * p.ld_dw + n0) * 2, p.ld_dw, rows, cols, p.dw_vec, false, value);
+      store16<T, Sh>(lds, wave, lane, p.dw + (m0 * p.ld_dw + n0) * 2, p.ld_dw, rows, cols, p.dw_vec, value);
       return;
     }
   }
@@ -725,8 +771,20 @@ __global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad,
 
 // ---------------------------------------------------------------- host
 constexpr int64_t kGBytes = int64_t(512) << 20;     // of g a piece
-constexpr int64_t kStreamBytes = int64_t(192) << 20;
 constexpr int64_t kPackBytes = int64_t(256) << 20;  // of w copied a piece
+
+// compute units of the current device (cached per device)
+int64_t cu_count() {
+  static std::atomic<int> cache[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = cache[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cache[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
@@ -752,6 +810,41 @@ struct Plan {
   int64_t x_at, w_at, part_at, target_at, g_at, sums_at, dyn_at, bytes;
 };
 
+// k tiles that the last of the chip's workgroups ends with, of dw's `dw` tiles of kw
+// k tiles and then dx's `dx` runs of kx, an XCD's share on its `slots` workgroups:
+// each takes the next one when it is free.
+int64_t ends(int64_t dw, int64_t kw, int64_t dx, int64_t kx, int64_t slots) {
+  const int64_t rounds = dw / slots, more = dw % slots, most = (dx + slots - 1) / slots;
+  int64_t lo = (rounds + (more > 0)) * kw, hi = lo + most * kx;
+  auto fits = [&](int64_t t) {
+    const int64_t late = std::max<int64_t>(0, t - (rounds + 1) * kw) / kx, early = std::max<int64_t>(0, t - rounds * kw) / kx;
+    return more * late + (slots - more) * early >= dx;
+  };
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (fits(mid)) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// Runs that dx's sums over a piece's classes are cut into: the fewest k tiles in a
+// row, against what a run costs, its tile of sums written and read again in each
+// piece and by the last launch (256 x 256: 256 KB at about 4.5 TB/s, where a k tile
+// takes 1.75 us).
+int64_t dx_slices(int64_t dx_tiles, int64_t kx, int64_t dw_tiles, int64_t kw, int64_t tile_bytes, bool big) {
+  const int64_t slots = std::max<int64_t>(1, cu_count() / 8 * (big ? 1 : 2));
+  const double step = big ? 1.75 : 1.2;
+  int64_t best = 1;
+  double best_t = 0;
+  for (int64_t n = 1; n <= 64 && n <= kx; n *= 2) {
+    const double t = double(ends((dw_tiles + 7) / 8, kw, (dx_tiles * n + 7) / 8, (kx + n - 1) / n, slots)) * step +
+                     double(dx_tiles * n * tile_bytes) * 2 / 4.5e6;
+    if (n == 1 || t < best_t) best = n, best_t = t;
+  }
+  return best;
+}
+
 Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x, int64_t ld_x, const void* w,
           int64_t ld_w, bool has_ignore) {
   Plan q{};
@@ -769,6 +862,10 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   if (bwd) most = std::min(most, std::max<int64_t>(q.tn, std::min<int64_t>(kGBytes / (rows * q.esz), int64_t(1) << 20)));
   q.pieces = (vocab + most - 1) / most;
   q.piece = up((vocab + q.pieces - 1) / q.pieces, 256);
+  if (q.pieces > 1) {  // whole rounds of tiles in all but the last piece, where they fit
+    const int64_t tiles_m = (rows + q.tm - 1) / q.tm, round = cu_count() / std::gcd(tiles_m, cu_count()) * q.tn;
+    if (up(q.piece, round) <= most) q.piece = up(q.piece, round);
+  }
   q.pieces = (vocab + q.piece - 1) / q.piece;
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t here = at; at += align256(bytes); return here; };
@@ -781,9 +878,9 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
     const int64_t classes = std::min(vocab, q.piece);
     q.ld_g = up(classes, 64);
     q.g_at = take(rows * q.ld_g * q.esz);
-    // dx's slices: three rounds of the 256 CUs
     const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn), deep = 128 / q.esz;
-    q.slices = std::max<int64_t>(1, std::min<int64_t>({768 / tiles, 64, (classes + 4 * deep - 1) / (4 * deep)}));
+    q.slices = dx_slices(tiles, (classes + deep - 1) / deep, (classes + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn),
+                         (rows + deep - 1) / deep, q.pm * q.pn * 4, q.products == kBig);
     q.sums_at = take(q.slices * tiles * q.pm * q.pn * 4);
     q.dyn_at = take(8);
   }
@@ -826,6 +923,14 @@ int pack(const char* what, hipStream_t s, const Plan& q, const void* src, int64_
     hipLaunchKernelGGL(pack_kernel<uint32_t>, g, b, 0, s, static_cast<const uint32_t*>(src), ld, rows, q.width,
                        reinterpret_cast<uint32_t*>(dst), q.pitch, labels);
   return check_launch(what);
+}
+
+// Workgroups of a kernel whose workgroups go on from tile to tile: those that the
+// chip holds at once (multiples of 8, so that a workgroup's tiles are one XCD's).
+template <class Sh>
+unsigned resident(int64_t tiles) {
+  const int64_t most = cu_count() * (Geo<Sh>::lds_bytes <= 80 * 1024 ? 2 : 1) / 8 * 8;
+  return unsigned(std::min(tiles, std::max<int64_t>(8, most)));
 }
 
 // f(type, shape) of a kernel
@@ -893,8 +998,8 @@ extern "C" int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t w
     const int rc = with_kernels(io_type, q.logits, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
-      hipLaunchKernelGGL((loss_kernel<T, Sh>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)), dim3(Geo<Sh>::threads), 0,
-                         s, a);
+      hipLaunchKernelGGL((loss_kernel<T, Sh>), dim3(resident<Sh>(int64_t(a.tiles_m) * a.tiles_n)), dim3(Geo<Sh>::threads),
+                         0, s, a);
       return check_launch(what);
     });
     if (rc) return rc;
@@ -957,7 +1062,6 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   a.lse = lse, a.row_grad = row_grad;
   a.x = static_cast<const char*>(x), a.ld_x = ld_x;
   a.g = ws + q.g_at, a.ld_g = q.ld_g;
-  a.stream = rows * q.ld_g * esz >= kStreamBytes;
   a.tiles_m = int((rows + q.tm - 1) / q.tm);
   b.dx_m = dx ? int((rows + q.pm - 1) / q.pm) : 0;
   b.dx_n = b.dw_n = int((width + q.pn - 1) / q.pn);
@@ -1002,8 +1106,8 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     int rc = with_kernels(io_type, q.logits, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
-      hipLaunchKernelGGL((grad_kernel<T, Sh>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)), dim3(Geo<Sh>::threads), 0,
-                         s, a);
+      hipLaunchKernelGGL((grad_kernel<T, Sh>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)), dim3(Geo<Sh>::threads),
+                         0, s, a);
       return check_launch(what);
     });
     if (rc) return rc;
