@@ -660,44 +660,53 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   store32<Sh>(wave, lane, reinterpret_cast<float*>(p.dw) + m0 * p.ld_dw + n0, p.ld_dw, rows, cols, p.dw_vec, value);
 }
 
-// dx = the slices' sums, in order, times the factor.  A block has the 32 rows x WN
-// columns of one of a wave's accumulator rows, as they lay, and stores them in
-// rows through LDS.
-template <class T, class Sh>
-__global__ __launch_bounds__(kThreads) void dx_kernel(const float* sums, int64_t rows, int64_t width, int dx_m, int dx_n,
-                                                      int slices, const float* dyn, float unit, char* dx, int64_t ld,
-                                                      int vec) {
+// dx = the slices' sums times the factor.  A block has the 32 rows x WN columns of
+// one of a wave's accumulator rows, as they lay, and stores them in rows through
+// LDS.  Many slices are added by NG groups of threads, each every NG-th slice in
+// order, then the groups in order (64 slices by one group: 12 us of latency).
+template <class T, class Sh, int NG>
+__global__ __launch_bounds__(kThreads* NG) void dx_kernel(const float* sums, int64_t rows, int64_t width, int dx_m,
+                                                          int dx_n, int slices, const float* dyn, float unit, char* dx,
+                                                          int64_t ld, int vec) {
   using G = Geo<Sh>;
-  constexpr int kPitch = G::WN + 4;
-  __shared__ float lds[32 * kPitch];
+  constexpr int kPitch = G::WN + 4, kSize = 32 * kPitch;
+  __shared__ float lds[NG * kSize];
+  const int group = int(threadIdx.x) / kThreads, tid = int(threadIdx.x) % kThreads;
   const int64_t tiles = int64_t(dx_m) * dx_n, tile = blockIdx.x / (G::W * G::I);
   const int part = int(blockIdx.x % (G::W * G::I)), wave = part / G::I, a = part % G::I;
   const f32x4* from = reinterpret_cast<const f32x4*>(sums) + tile * (Sh::TM * Sh::TN / 4);
-  const float f = dyn ? dyn[1] : unit;
 #pragma unroll
-  for (int i = int(threadIdx.x); i < G::J * 4 * 64; i += kThreads) {
+  for (int i = tid; i < G::J * 4 * 64; i += kThreads) {
     const int lane = i & 63, br = i >> 6;  // accumulator group: b, rg
     const f32x4* p = from + (a * G::J * 4 + br) * G::threads + wave * 64 + lane;
-    f32x4 s = p[0];
+    f32x4 s = {{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 8
-    for (int q = 1; q < slices; ++q) {
+    for (int q = group; q < slices; q += NG) {
       const f32x4 v = p[q * tiles * (Sh::TM * Sh::TN / 4)];
 #pragma unroll
       for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      lds[(lane & 31) * kPitch + 32 * (br >> 2) + 8 * (br & 3) + 4 * (lane >> 5) + e] = s.v[e] * f;
+      lds[group * kSize + (lane & 31) * kPitch + 32 * (br >> 2) + 8 * (br & 3) + 4 * (lane >> 5) + e] = s.v[e];
   }
   __syncthreads();
   const int64_t m0 = tile / dx_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a;
   const int64_t n0 = tile % dx_n * Sh::TN + wave % Sh::WGN * G::WN;
+  const float f = dyn ? dyn[1] : unit;
 #pragma unroll
-  for (int i = int(threadIdx.x); i < 32 * G::WN / 4; i += kThreads) {
+  for (int i = int(threadIdx.x); i < 32 * G::WN / 4; i += kThreads * NG) {
     const int row = i / (G::WN / 4), col = i % (G::WN / 4) * 4;
     const int64_t m = m0 + row, n = n0 + col;
     if (m >= rows || n >= width) continue;
-    const float* v = lds + row * kPitch + col;
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = lds[row * kPitch + col + e];
+#pragma unroll
+      for (int q = 1; q < NG; ++q) v[e] += lds[q * kSize + row * kPitch + col + e];
+      v[e] *= f;
+    }
     char* to = dx + (m * ld + n) * T::esz;
     if (vec && n + 4 <= width) {
       if constexpr (T::esz == 2) *reinterpret_cast<uint2*>(to) = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
@@ -828,19 +837,40 @@ int64_t ends(int64_t dw, int64_t kw, int64_t dx, int64_t kx, int64_t slots) {
   return lo;
 }
 
-// Runs that dx's sums over a piece's classes are cut into: the fewest k tiles in a
-// row, against what a run costs, its tile of sums written and read again in each
-// piece and by the last launch (256 x 256: 256 KB at about 4.5 TB/s, where a k tile
-// takes 1.75 us).
-int64_t dx_slices(int64_t dx_tiles, int64_t kx, int64_t dw_tiles, int64_t kw, int64_t tile_bytes, bool big) {
-  const int64_t slots = std::max<int64_t>(1, cu_count() / 8 * (big ? 1 : 2));
-  const double step = big ? 1.75 : 1.2;
-  int64_t best = 1;
-  double best_t = 0;
+// Tile shapes: a k tile of 256 x 256 takes 1.75 us on a CU, one of 128 x 128 with
+// another beside it on the CU 1.12 us, alone 0.78 of that.  A tile's begin and end
+// count as more k tiles: fitted to both shapes' times on the cases below.
+constexpr int64_t kSizes[2][2] = {{256, 256}, {128, 128}};
+constexpr double kStep[2] = {1.75, 1.12};
+
+// Estimated us of the logits' tiles, kt k tiles each.  Measured, 256 and 128: loss of
+// 300 x 768 x 50257 46, 39, of 1000 92, 93; gradient of 1000 (with the same products)
+// 311, 304, of 1777 x 1001 x 30011 415, 423, of 8192 1911, 2034.
+double logits_time(int shape, int64_t rows, int64_t classes, int64_t kt, bool bwd) {
+  const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1];
+  const int64_t tiles = (rows + tm - 1) / tm * ((classes + tn - 1) / tn);
+  const int64_t cus = cu_count(), slots = shape == kBig ? cus : 2 * cus, rest = tiles % slots;
+  const double last = rest == 0 ? 0.0 : shape == kMid && rest <= cus ? 0.78 : 1.0;
+  return (double(tiles / slots) + last) * kStep[shape] * (double(kt) + (bwd && shape == kBig ? 3.0 : 1.5));
+}
+
+// Estimated us of dx's and dw's tiles of a piece: dw's over `rows`, and dx's over the
+// classes cut into `slices` runs, which are chosen: fewer k tiles one after the other,
+// against a tile of sums a run, written and read again in each piece and by the last
+// launch, at about 4.5 TB/s.  Measured, 256 and 128 (the whole gradient): 100 x 768 x
+// 50257 87, 73, 300 144, 129, 1000 311, 297; 2048 x 1024 x 32000 390, 428; 1777 x
+// 1001 x 30011 417, 450.
+double products_time(int shape, int64_t rows, int64_t width, int64_t classes, int64_t deep, int64_t& slices) {
+  constexpr int64_t kEndW[2] = {4, 1}, kEndX[2] = {8, 5};
+  const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1], across = (width + tn - 1) / tn;
+  const int64_t dx = (rows + tm - 1) / tm * across, dw = (classes + tm - 1) / tm * across;
+  const int64_t kx = (classes + deep - 1) / deep, kw = (rows + deep - 1) / deep;
+  const int64_t slots = std::max<int64_t>(1, cu_count() / 8 * (shape == kBig ? 1 : 2));
+  double best = 0;
   for (int64_t n = 1; n <= 64 && n <= kx; n *= 2) {
-    const double t = double(ends((dw_tiles + 7) / 8, kw, (dx_tiles * n + 7) / 8, (kx + n - 1) / n, slots)) * step +
-                     double(dx_tiles * n * tile_bytes) * 2 / 4.5e6;
-    if (n == 1 || t < best_t) best = n, best_t = t;
+    const double t = double(ends((dw + 7) / 8, kw + kEndW[shape], (dx * n + 7) / 8, (kx + n - 1) / n + kEndX[shape], slots)) *
+                         kStep[shape] + double(dx * n * tm * tn * 4) * 2 / 4.5e6;
+    if (n == 1 || t < best) best = t, slices = n;
   }
   return best;
 }
@@ -850,10 +880,10 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   Plan q{};
   q.esz = dtype_bytes(io_type);
   q.rows = rows, q.width = width, q.vocab = vocab;
-  q.logits = q.products = rows > 128 ? kBig : kMid;
-  const int64_t sizes[][2] = {{256, 256}, {128, 128}};
-  q.tm = sizes[q.logits][0], q.tn = sizes[q.logits][1];
-  q.pm = sizes[q.products][0], q.pn = sizes[q.products][1];
+  const int64_t deep = 128 / q.esz;
+  const int64_t kt = (width + deep - 1) / deep;
+  q.logits = logits_time(kMid, rows, vocab, kt, bwd) < logits_time(kBig, rows, vocab, kt, bwd) ? kMid : kBig;
+  q.tm = kSizes[q.logits][0], q.tn = kSizes[q.logits][1];
   q.pack_x = !on_grid(x, ld_x, width, q.esz) || (bwd && has_ignore);
   q.pack_w = !on_grid(w, ld_w, width, q.esz);
   q.pitch = up(width, 16 / q.esz);
@@ -878,9 +908,14 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
     const int64_t classes = std::min(vocab, q.piece);
     q.ld_g = up(classes, 64);
     q.g_at = take(rows * q.ld_g * q.esz);
-    const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn), deep = 128 / q.esz;
-    q.slices = dx_slices(tiles, (classes + deep - 1) / deep, (classes + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn),
-                         (rows + deep - 1) / deep, q.pm * q.pn * 4, q.products == kBig);
+    int64_t slices[2];
+    q.products = products_time(kMid, rows, width, classes, deep, slices[kMid]) <
+                         products_time(kBig, rows, width, classes, deep, slices[kBig])
+                     ? kMid
+                     : kBig;
+    q.slices = slices[q.products];
+    q.pm = kSizes[q.products][0], q.pn = kSizes[q.products][1];
+    const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn);
     q.sums_at = take(q.slices * tiles * q.pm * q.pn * 4);
     q.dyn_at = take(8);
   }
@@ -1126,9 +1161,14 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     using T = decltype(t);
     using Sh = decltype(sh);
     const int64_t blocks = int64_t(b.dx_m) * b.dx_n * Geo<Sh>::W * Geo<Sh>::I;
-    if (int r = check_tiles(what, blocks, kThreads)) return r;
-    hipLaunchKernelGGL((dx_kernel<T, Sh>), dim3(unsigned(blocks)), dim3(kThreads), 0, s, b.sums, rows, width, b.dx_m, b.dx_n,
-                       b.slices, b.dyn, b.unit, static_cast<char*>(dx), ld_dx, dx_vec);
+    if (int r = check_tiles(what, blocks, 4 * kThreads)) return r;
+    auto sum = [&](auto groups) {
+      constexpr int NG = decltype(groups)::value;
+      hipLaunchKernelGGL((dx_kernel<T, Sh, NG>), dim3(unsigned(blocks)), dim3(kThreads * NG), 0, s, b.sums, rows, width,
+                         b.dx_m, b.dx_n, b.slices, b.dyn, b.unit, static_cast<char*>(dx), ld_dx, dx_vec);
+    };
+    if (b.slices > 8) sum(Int<4>{});
+    else sum(Int<1>{});
     return check_launch(what);
   });
 }
