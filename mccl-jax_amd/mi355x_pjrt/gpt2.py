@@ -19,6 +19,9 @@ operation is a call through the C-ABI of include/mk_kernels.h:
             projection-bias column sums, position-embedding column sum,
             deterministic scatter-add of the token gradient into the
             embedding gradient
+  dropout   (cfg.dropout > 0) of the embeddings and of both branches of a
+            block, in the pass that adds a branch to the residual stream; its
+            backward fused with the projection-bias column sums
   update    one Adam launch over all parameters (fp32 master, m, v; bf16
             working copy rewritten), lr and bias corrections read from a
             device buffer so the whole step can be replayed as a HIP graph
@@ -61,6 +64,7 @@ _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
 _D = ctypes.c_double
+_U64 = ctypes.c_uint64
 
 BF16, F32, S32 = K.MK["BF16"], K.MK["F32"], K.MK["S32"]
 
@@ -74,6 +78,7 @@ class GPT2Config:
     batch: int = 8
     vocab: int = 50257
     ln_eps: float = 1e-5
+    dropout: float = 0.0  # of the embeddings and of both branches of a block
 
     @property
     def head_dim(self) -> int:
@@ -156,17 +161,27 @@ class GPT2TrainStep:
     # pre-activations, the column pass) costs more than the pass it replaces
     FUSE_GELU_FWD = True
     FUSE_GELU_BWD = False
+    # keep_logits=False: the loss from linear_xent and its gradient, which form the
+    # logits twice and keep none (8192 x 50264 of bf16, 824 MB): one step 0.2 ms longer
+    # dropout: sites 0 (embeddings), 1 + 2 l and 2 + 2 l (the branches of layer l) draw
+    # at site * 2^40 + the step's count, a device number the step itself raises, so
+    # that forward, backward and every replay of a captured step agree on it
+    DROP_SITE = 1 << 40
     # the hidden-state gradient through the embedding (K = vocabulary): bf16
     # out, split along K in uneven slices (measured: 8 slices 664 us, 2 693,
     # unsplit 910; rocBLAS 682-687)
     DHF_SPLITS = 8
 
     def __init__(self, cfg: GPT2Config, params: dict | None = None, seed: int = 0, lr: float = 3e-4,
-                 b1: float = 0.9, b2: float = 0.999, adam_eps: float = 1e-8, device="cuda", stream=None):
+                 b1: float = 0.9, b2: float = 0.999, adam_eps: float = 1e-8, device="cuda", stream=None,
+                 keep_logits: bool = True, dropout_seed: int = 0):
         if cfg.head_dim not in (64, 128):
             raise ValueError("head_dim must be 64 or 128 (mk_sdpa_fwd)")
         if cfg.d_model > 2048 or cfg.d_model % 8:
             raise ValueError("d_model must be a multiple of 8, at most 2048 (mk_layernorm_bwd)")
+        if not 0.0 <= cfg.dropout < 1.0:
+            raise ValueError("dropout must be in [0, 1)")
+        self.keep_logits, self.dropout_seed = keep_logits, dropout_seed
         self.cfg, self.dev = cfg, torch.device(device)
         self.lr, self.b1, self.b2, self.adam_eps = lr, b1, b2, adam_eps
         self.t = 0  # Adam step count
@@ -234,7 +249,13 @@ class GPT2TrainStep:
         # logits, then their gradient in place, rows padded to a 16-byte
         # multiple (the padding is never written)
         self.vocab_pitch = (c.vocab + 7) // 8 * 8
-        self.logits = torch.zeros(T, self.vocab_pitch, **bf)
+        if self.keep_logits:
+            self.logits = torch.zeros(T, self.vocab_pitch, **bf)
+        else:
+            self.lse_rows = torch.empty(T, dtype=torch.float32, device=dev)
+        if c.dropout > 0:
+            self.drop_step = torch.zeros(1, dtype=torch.int64, device=dev)
+            self.branch = torch.empty(T, d, **bf)  # the gradient of a dropped branch
         self.tmp = torch.empty(T, d, **bf)
         self.dx = torch.empty(T, d, **bf)
         self.dh = torch.empty(T, d, **bf)
@@ -251,7 +272,11 @@ class GPT2TrainStep:
         ws = max(*sk, lib.mk_col_sum_workspace_bytes(T, c.d_ff), lib.mk_col_sum_workspace_bytes(c.batch, c.seq * d),
                  lib.mk_layernorm_bwd_workspace_bytes(T, d), lib.mk_gemm_gelu_bwd_workspace_bytes(T, c.d_ff),
                  lib.mk_sdpa_bwd_workspace_bytes(c.batch, c.n_head, c.seq, c.seq, c.d_model // c.n_head),
-                 lib.mk_scatter_add_workspace_bytes(c.vocab, T))
+                 lib.mk_scatter_add_workspace_bytes(c.vocab, T), lib.mk_dropout_add_bwd_workspace_bytes(T, d))
+        if not self.keep_logits:
+            head = [self.hf.data_ptr(), d, self.view(self.param, "wte").data_ptr(), d]
+            ws = max(ws, lib.mk_linear_xent_workspace_bytes(BF16, T, d, c.vocab, *head),
+                     lib.mk_linear_xent_bwd_workspace_bytes(BF16, T, d, c.vocab, *head, 0))
         self.ws = torch.empty(int(ws), dtype=torch.uint8, device=dev)
 
     # ------------------------------------------------------------------ launch list
@@ -317,6 +342,28 @@ class GPT2TrainStep:
                                                       G(prefix + "_b"), colsum_out or _P(0), ws],
                                "mk_layernorm_bwd"))
 
+        def dropout(site, rows, cols, x, bias, residual, out):
+            calls.append(_Call(lib.mk_dropout_add, [st, _I(BF16), _I64(rows), _I64(cols), x, _I64(cols), bias or _P(0),
+                                                    residual or _P(0), _I64(cols), _D(c.dropout), _U64(self.dropout_seed),
+                                                    _U64(site * self.DROP_SITE), P(self.drop_step), out, _I64(cols)],
+                               "mk_dropout_add"))
+
+        def dropout_bwd(site, dy, dx, colsum_out):
+            calls.append(_Call(lib.mk_dropout_add_bwd, [st, _I(BF16), _I64(T), _I64(d), dy, _I64(d), _D(c.dropout),
+                                                        _U64(self.dropout_seed), _U64(site * self.DROP_SITE),
+                                                        P(self.drop_step), dx, _I64(d), colsum_out or _P(0), ws],
+                               "mk_dropout_add_bwd"))
+
+        drop = c.dropout > 0
+
+        def residual_ln(l, branch, x, bias, ln, sum_out, y):
+            """sum_out = x + (dropped) branch + bias and y = its LayerNorm; branch 0: attention, 1: MLP"""
+            if drop:
+                dropout(1 + 2 * l + branch, T, d, P(self.tmp), bias, x, sum_out)
+                layernorm(sum_out, ln + "_g", ln + "_b", y)
+            else:
+                add_layernorm(x, P(self.tmp), bias, ln, sum_out, y)
+
         scale = 1.0 / math.sqrt(hd)
         # the MLP's products can take the GELU in their epilogues where the
         # tiled kernel takes the shapes (16-byte aligned rows, M, N >= 128, K >= 64)
@@ -326,6 +373,9 @@ class GPT2TrainStep:
                                                 P(self.ids), P(self.x[0])], "mk_gather_rows"))
         # x0 += wpe broadcast over the batch: [B, S*d] + [S*d]
         add_rows(P(self.x[0]), B, S * d, P(self.x[0]), bias=W("wpe"), tag="pos")
+        if drop:
+            calls.insert(0, _Call(self._next_draw, [], "next draw"))
+            dropout(0, T, d, P(self.x[0]), None, None, P(self.x[0]))
         # LN1 of layer 0 stands alone; every later LayerNorm (LN1 of the next
         # layer, LN2, the final LN) is fused with the residual add before it
         layernorm(P(self.x[0]), "h0.ln1_g", "h0.ln1_b", P(self.h1[0]))
@@ -340,7 +390,7 @@ class GPT2TrainStep:
                                                  P(self.att[l]), _I64(S * d), _I64(hd), _I64(d),
                                                  _F(scale), _I(1), P(self.lse[l])], "mk_sdpa_fwd"))
             gemm(BF16, BF16, T, d, d, P(self.att[l]), d, 1, W(p + "w_o"), d, 1, P(self.tmp), d, tag="o")
-            add_layernorm(P(self.x[l]), P(self.tmp), W(p + "b_o"), p + "ln2", P(self.xm[l]), P(self.h2[l]))
+            residual_ln(l, 0, P(self.x[l]), W(p + "b_o"), p + "ln2", P(self.xm[l]), P(self.h2[l]))
             if tiled_mlp and self.FUSE_GELU_FWD:
                 # the up-projection, its bias and the GELU in one launch (the tiled
                 # kernel's shapes): f = h2 w_fc + b_fc, kept for the backward, and
@@ -355,46 +405,67 @@ class GPT2TrainStep:
                                                       P(self.f[l]), P(self.g[l])], "mk_bias_gelu"))
             gemm(BF16, BF16, T, d, F, P(self.g[l]), F, 1, W(p + "w_pr"), d, 1, P(self.tmp), d, tag="proj")
             nxt, y = (f"h{l + 1}.ln1", P(self.h1[l + 1])) if l + 1 < L else ("lnf", P(self.hf))
-            add_layernorm(P(self.xm[l]), P(self.tmp), W(p + "b_pr"), nxt, P(self.x[l + 1]), y)
-        # logits = hf @ wteᵀ, then loss rows and dlogits (over the logits)
+            residual_ln(l, 1, P(self.xm[l]), W(p + "b_pr"), nxt, P(self.x[l + 1]), y)
         Vp = self.vocab_pitch
-        gemm(BF16, BF16, T, V, d, P(self.hf), d, 1, W("wte"), 1, d, P(self.logits), Vp, tag="logits")
-        calls.append(_Call(lib.mk_softmax_xent_strided, [st, _I(BF16), _I(BF16), _I64(T), _I64(V), P(self.logits),
-                                                         _I64(Vp), _I(S32), P(self.labels), _F(1.0 / T),
-                                                         P(self.loss_rows), P(self.logits), _I64(Vp)],
-                           "mk_softmax_xent_strided"))
-        calls.append(_Call(lib.mk_row_reduce, [st, _I(F32), _I(F32), _I(0), _I64(1), _I64(T), P(self.loss_rows),
-                                               _F(0.0), P(self.loss_sum)], "mk_row_reduce"))
-        # ---- backward
-        dlog = P(self.logits)
-        gemm(BF16, BF16, T, d, V, dlog, Vp, 1, W("wte"), d, 1, P(self.dh), d, tag="dhf")
-        gemm(BF16, F32, V, d, T, dlog, 1, Vp, P(self.hf), d, 1, G("wte"), d, tag="dwte")
+        head = [_I64(T), _I64(d), _I64(V), P(self.hf), _I64(d), W("wte"), _I64(d), _I(S32), P(self.labels), _I(0), _I64(0)]
+
+        def loss_sum():
+            calls.append(_Call(lib.mk_row_reduce, [st, _I(F32), _I(F32), _I(0), _I64(1), _I64(T), P(self.loss_rows),
+                                                   _F(0.0), P(self.loss_sum)], "mk_row_reduce"))
+
+        if self.keep_logits:
+            # logits = hf @ wteᵀ, then loss rows and dlogits (over the logits)
+            gemm(BF16, BF16, T, V, d, P(self.hf), d, 1, W("wte"), 1, d, P(self.logits), Vp, tag="logits")
+            calls.append(_Call(lib.mk_softmax_xent_strided, [st, _I(BF16), _I(BF16), _I64(T), _I64(V), P(self.logits),
+                                                             _I64(Vp), _I(S32), P(self.labels), _F(1.0 / T),
+                                                             P(self.loss_rows), P(self.logits), _I64(Vp)],
+                               "mk_softmax_xent_strided"))
+            loss_sum()
+            # ---- backward
+            dlog = P(self.logits)
+            gemm(BF16, BF16, T, d, V, dlog, Vp, 1, W("wte"), d, 1, P(self.dh), d, tag="dhf")
+            gemm(BF16, F32, V, d, T, dlog, 1, Vp, P(self.hf), d, 1, G("wte"), d, tag="dwte")
+        else:
+            calls.append(_Call(lib.mk_linear_xent, [st, _I(BF16), *head, P(self.loss_rows), P(self.lse_rows), ws],
+                               "mk_linear_xent"))
+            loss_sum()
+            # ---- backward
+            calls.append(_Call(lib.mk_linear_xent_bwd, [st, _I(BF16), _I(F32), *head, P(self.lse_rows), _P(0), _F(1.0 / T),
+                                                        P(self.dh), _I64(d), G("wte"), _I64(d), ws],
+                               "mk_linear_xent_bwd"))
         # the bias gradient of each residual projection is the column sum of
         # the residual-stream gradient, produced by the LayerNorm backward
-        # that writes it
-        ln_bwd(P(self.x[L]), "lnf_g", P(self.dh), None, P(self.dx), "lnf", G(f"h{L - 1}.b_pr"))
+        # that writes it (or, of a dropped branch, by the dropout backward)
+        ln_bwd(P(self.x[L]), "lnf_g", P(self.dh), None, P(self.dx), "lnf", None if drop else G(f"h{L - 1}.b_pr"))
         for l in reversed(range(L)):
             p = f"h{l}."
             # MLP branch of x[l+1] = xm + proj(gelu(fc(ln2(xm))))
-            gemm(BF16, F32, F, d, T, P(self.g[l]), 1, F, P(self.dx), d, 1, G(p + "w_pr"), d, tag="dw_pr")
+            dbr = self.dx
+            if drop:
+                dbr = self.branch
+                dropout_bwd(2 + 2 * l, P(self.dx), P(dbr), G(p + "b_pr"))
+            gemm(BF16, F32, F, d, T, P(self.g[l]), 1, F, P(dbr), d, 1, G(p + "w_pr"), d, tag="dw_pr")
             if tiled_mlp and self.FUSE_GELU_BWD:
                 # dff = gelu'(f) * (dx w_prᵀ) and the fc bias gradient, the GELU
                 # backward in the product's epilogue
-                calls.append(_Call(lib.mk_gemm_gelu_bwd, [st, _I(BF16), _I64(T), _I64(F), _I64(d), P(self.dx), _I64(d),
+                calls.append(_Call(lib.mk_gemm_gelu_bwd, [st, _I(BF16), _I64(T), _I64(F), _I64(d), P(dbr), _I64(d),
                                                           _I64(1), W(p + "w_pr"), _I64(1), _I64(d), P(self.dff),
                                                           _I64(F), P(self.f[l]), _I64(F), G(p + "b_fc"), ws],
                                    "mk_gemm_gelu_bwd dg"))
             else:
-                gemm(BF16, BF16, T, F, d, P(self.dx), d, 1, W(p + "w_pr"), 1, d, P(self.dff), F, tag="dg")
+                gemm(BF16, BF16, T, F, d, P(dbr), d, 1, W(p + "w_pr"), 1, d, P(self.dff), F, tag="dg")
                 calls.append(_Call(lib.mk_gelu_tanh_bwd_colsum, [st, _I(BF16), _I64(T), _I64(F), P(self.f[l]),
                                                                  P(self.dff), P(self.dff), G(p + "b_fc"), ws],
                                    "mk_gelu_tanh_bwd_colsum"))
             gemm(BF16, F32, d, F, T, P(self.h2[l]), 1, d, P(self.dff), F, 1, G(p + "w_fc"), F, tag="dw_fc")
             gemm(BF16, BF16, T, d, F, P(self.dff), F, 1, W(p + "w_fc"), 1, F, P(self.dh), d, tag="dh2")
-            ln_bwd(P(self.xm[l]), p + "ln2_g", P(self.dh), P(self.dx), P(self.dx), p + "ln2", G(p + "b_o"))
+            ln_bwd(P(self.xm[l]), p + "ln2_g", P(self.dh), P(self.dx), P(self.dx), p + "ln2",
+                   None if drop else G(p + "b_o"))
             # attention branch of xm = x[l] + o(attn(ln1(x[l])))
-            gemm(BF16, F32, d, d, T, P(self.att[l]), 1, d, P(self.dx), d, 1, G(p + "w_o"), d, tag="dw_o")
-            gemm(BF16, BF16, T, d, d, P(self.dx), d, 1, W(p + "w_o"), 1, d, P(self.dh), d, tag="datt")
+            if drop:
+                dropout_bwd(1 + 2 * l, P(self.dx), P(dbr), G(p + "b_o"))
+            gemm(BF16, F32, d, d, T, P(self.att[l]), 1, d, P(dbr), d, 1, G(p + "w_o"), d, tag="dw_o")
+            gemm(BF16, BF16, T, d, d, P(dbr), d, 1, W(p + "w_o"), 1, d, P(self.dh), d, tag="datt")
             q, k, v = (P(self.qkv[l], i * d) for i in range(3))
             dq, dk, dv = (P(self.dqkv, i * d) for i in range(3))
             sq = [_I64(S * 3 * d), _I64(hd), _I64(3 * d)]
@@ -409,7 +480,9 @@ class GPT2TrainStep:
             gemm(BF16, BF16, T, d, 3 * d, P(self.dqkv), 3 * d, 1, W(p + "w_qkv"), 1, 3 * d, P(self.dh), d,
                  tag="dh1")
             ln_bwd(P(self.x[l]), p + "ln1_g", P(self.dh), P(self.dx), P(self.dx), p + "ln1",
-                   G(f"h{l - 1}.b_pr") if l > 0 else None)
+                   G(f"h{l - 1}.b_pr") if l > 0 and not drop else None)
+        if drop:
+            dropout_bwd(0, P(self.dx), P(self.dx), None)
         # embeddings: position gradient = sum over the batch; token gradient
         # scattered (in token order) into the head's embedding gradient
         colsum(P(self.dx), B, S * d, G("wpe"))
@@ -422,6 +495,12 @@ class GPT2TrainStep:
         return calls
 
     # ------------------------------------------------------------------ running
+    def _next_draw(self):
+        """The step's count of dropout draws, raised on the device before the forward pass."""
+        with torch.cuda.stream(self.stream):
+            self.drop_step.add_(1)
+        return 0
+
     def set_batch(self, ids, labels):
         self.ids.copy_(torch.as_tensor(ids, dtype=torch.int32).reshape(-1))
         self.labels.copy_(torch.as_tensor(labels, dtype=torch.int32).reshape(-1))

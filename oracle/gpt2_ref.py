@@ -18,15 +18,20 @@ import torch
 
 
 def forward_loss(params: dict, ids: np.ndarray, labels: np.ndarray, n_layer: int, n_head: int,
-                 ln_eps: float = 1e-5):
+                 ln_eps: float = 1e-5, drop=None):
     """Mean softmax cross-entropy over all tokens; params are float64 torch
-    tensors (requires_grad as the caller wants)."""
+    tensors (requires_grad as the caller wants).  drop (dropout's multipliers, 0
+    or the scale, [2 n_layer + 1, B, S, d]): of the embeddings, then of each
+    layer's attention and MLP branches."""
     B, S = ids.shape
     wte, wpe = params["wte"], params["wpe"]
     d = wte.shape[1]
     hd = d // n_head
     ids_t = torch.as_tensor(ids, dtype=torch.long)
-    x = wte[ids_t] + wpe[:S][None]
+    def dropped(site, t):
+        return t if drop is None else t * drop[site]
+
+    x = dropped(0, wte[ids_t] + wpe[:S][None])
     causal = torch.ones(S, S, dtype=torch.bool).tril()
 
     def ln(t, g, b):
@@ -40,20 +45,20 @@ def forward_loss(params: dict, ids: np.ndarray, labels: np.ndarray, n_layer: int
         s = (q @ k.transpose(-1, -2)) / math.sqrt(hd)
         s = s.masked_fill(~causal, float("-inf"))
         a = (torch.softmax(s, -1) @ v).transpose(1, 2).reshape(B, S, d)
-        x = x + a @ p("w_o") + p("b_o")
+        x = x + dropped(1 + 2 * l, a @ p("w_o") + p("b_o"))
         h2 = ln(x, p("ln2_g"), p("ln2_b"))
         f = torch.nn.functional.gelu(h2 @ p("w_fc") + p("b_fc"), approximate="tanh")
-        x = x + f @ p("w_pr") + p("b_pr")
+        x = x + dropped(2 + 2 * l, f @ p("w_pr") + p("b_pr"))
     hf = ln(x, params["lnf_g"], params["lnf_b"])
     logits = hf @ wte.T
     return torch.nn.functional.cross_entropy(logits.reshape(B * S, -1), torch.as_tensor(labels, dtype=torch.long)
                                              .reshape(-1))
 
 
-def loss_and_grads(params_np: dict, ids, labels, n_layer, n_head, ln_eps=1e-5):
+def loss_and_grads(params_np: dict, ids, labels, n_layer, n_head, ln_eps=1e-5, drop=None):
     """(loss, {name: grad}) in float64."""
     params = {n: torch.tensor(np.asarray(a, dtype=np.float64), requires_grad=True) for n, a in params_np.items()}
-    loss = forward_loss(params, ids, labels, n_layer, n_head, ln_eps)
+    loss = forward_loss(params, ids, labels, n_layer, n_head, ln_eps, drop)
     loss.backward()
     return float(loss.detach()), {n: t.grad.numpy() for n, t in params.items()}
 
