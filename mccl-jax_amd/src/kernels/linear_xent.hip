@@ -108,10 +108,9 @@ struct Operand {
       off[c] = row < rows ? uint32_t((KC ? row * ld + k : k * ld + row) * T::esz) : uint32_t(kInvalid);
     }
   }
-  // the copies of k tile kt, of which the operand has K - kDeep kt k
-  __device__ inline void issue(int kt, int64_t K, char* tile, int wave, int lane) const {
+  // the copies of k tile kt, of which the operand has `left` k
+  __device__ inline void issue(int kt, int64_t left, char* tile, int wave, int lane) const {
     const i32x4_t r = tile_desc(base + kt * step, uint32_t(kInvalid));
-    const int64_t left = K - int64_t(kDeep) * kt;
     if (left >= kDeep) {
 #pragma unroll
       for (int c = 0; c < kC; ++c) copy_to_lds_so(r, lds_addr(tile + 1024 * (wave + W * c)), int(off[c]), 0);
@@ -152,17 +151,22 @@ struct Product {
   OA oa;
   OB ob;
   int64_t K;
+  int nk;
   __device__ inline Product(const char* A, int64_t lda, int64_t a_rows, const char* B, int64_t ldb, int64_t b_rows,
                             int64_t K, int wave, int lane)
-      : oa(wave, lane, A, a_rows, lda), ob(wave, lane, B, b_rows, ldb), K(K) {}
+      : oa(wave, lane, A, a_rows, lda), ob(wave, lane, B, b_rows, ldb), K(K), nk(int((K + OA::kDeep - 1) / OA::kDeep)) {}
+  // A's second k tile, as long as the first (at most a k tile), with B's first again
+  __device__ inline void twice() { nk = 2, ob.step = 0; }
+  __device__ inline void issue(int kt, char* to, int wave, int lane, bool a, bool b) const {
+    const int64_t left = K <= OA::kDeep ? K : K - int64_t(OA::kDeep) * kt;
+    if (a) oa.issue(kt, left, to, wave, lane);
+    if (b) ob.issue(kt, left, to + kA, wave, lane);
+  }
   __device__ inline void start(char* lds, int wave, int lane) const {
-    if (K <= 0) return;
-    oa.issue(0, K, lds, wave, lane);
-    ob.issue(0, K, lds + kA, wave, lane);
+    if (nk > 0) issue(0, lds, wave, lane, true, true);
   }
   __device__ __attribute__((always_inline)) inline void run(char* lds, int wave, int lane, Acc<Sh>& acc) const {
     const int wm = wave / Sh::WGN, wn = wave % Sh::WGN;
-    const int nk = int((K + OA::kDeep - 1) / OA::kDeep);
     for (int kt = 0; kt < nk; ++kt) {
       wait_vm<0>();
       lds_barrier();
@@ -176,8 +180,7 @@ struct Product {
         for (int a = 0; a < G::I; ++a) af[a] = read_chunk<T, AKC, Sh::TM, Sh::BK>(at, wm * G::WM + 32 * a, ks, lane);
 #pragma unroll
         for (int b = 0; b < G::J; ++b) bf[b] = read_chunk<T, BKC, Sh::TN, Sh::BK>(at + kA, wn * G::WN + 32 * b, ks, lane);
-        if (more && ks == 0) oa.issue(kt + 1, K, next, wave, lane);
-        if (more && ks == 1) ob.issue(kt + 1, K, next + kA, wave, lane);
+        if (more && ks < 2) issue(kt + 1, next, wave, lane, ks == 0, ks == 1);
 #pragma unroll
         for (int a = 0; a < G::I; ++a)
 #pragma unroll
@@ -382,12 +385,16 @@ struct GradArgs {
   float unit;        // factor of g
   char* g;           // [rows][ld_g], columns past vocab up to a whole chunk are zeros
   int64_t ld_g;
+  int low;           // what g's rounding leaves goes to the rows kLow further on
 };
 
 __device__ inline uint32_t pack2(Bf16, float a, float b) {
   return uint32_t(f32_to_bf16(a)) | (uint32_t(f32_to_bf16(b)) << 16);
 }
 __device__ inline uint32_t pack2(F16, float a, float b) { return uint32_t(f32_to_f16(a)) | (uint32_t(f32_to_f16(b)) << 16); }
+
+__device__ inline float rounded(Bf16, float a) { return bf16_to_f32(f32_to_bf16(a)); }
+__device__ inline float rounded(F16, float a) { return f16_to_f32(f32_to_f16(a)); }
 
 // 16 bits: the 8 columns 32 b + 16 h + 8 g .. + 7 of a lane's row 32 a + c as one
 // chunk.  value(a, b, rg, v) gives the 4 columns 32 b + 8 rg + 4 g .. + 3; lanes l
@@ -496,6 +503,13 @@ __device__ __attribute__((always_inline)) inline void store32(int wave, int lane
   }
 }
 
+// Few rows are not averaged over: a class that one token alone has as its label gets
+// its gradient from one product, and the rounding of that one factor would be
+// the error of the whole row.  At most kLow rows have a second operand row each,
+// what the rounding of the first leaves; their tiles have the room (16 bits: half of
+// dx's 128 rows, and of dw's two k tiles the second), so that it costs nothing.
+constexpr int kLow = 64;
+
 // One tile a workgroup: its 128 KB of stores leave while the next workgroup begins
 // (a workgroup that goes on from tile to tile as loss_kernel's, with the next
 // tile's copies and rows ahead of the stores, took the same time, 1975 us for the
@@ -570,8 +584,20 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
   constexpr int kE = 16 / T::esz;
   const int64_t rows = p.rows - m0, cols = (p.vocab + kE - 1) / kE * kE - n0;
   char* out = p.g + (m0 * p.ld_g + n0) * T::esz;
-  if constexpr (T::esz == 2) store16_direct<T, Sh>(wave, lane, out, p.ld_g, rows, cols, value);
-  else store32<Sh>(wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, true, value);
+  if constexpr (T::esz == 2) {
+    store16_direct<T, Sh>(wave, lane, out, p.ld_g, rows, cols, value);
+    if constexpr (Sh::TM == 128) {
+      if (p.low)
+        store16_direct<T, Sh>(wave, lane, out + kLow * p.ld_g * T::esz, p.ld_g, rows, cols,
+                              [&](int a, int b, int rg, float (&v)[4]) __attribute__((always_inline)) {
+                                value(a, b, rg, v);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) v[q] -= rounded(T{}, v[q]);
+                              });
+    }
+  } else {
+    store32<Sh>(wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, true, value);
+  }
 }
 
 // ---------------------------------------------------------------- backward: dx and dw of a piece
@@ -584,8 +610,11 @@ struct ProductsArgs {
   int64_t run;
   int first;       // the first piece: sums start from zero
   float* sums;     // [slices][dx tile][accumulators]
-  // dw: tiles of classes x width
-  int dw_m, dw_n;
+  // dw: tiles of classes x width; where they are few their rows are cut too
+  int dw_m, dw_n, dw_slices;
+  int64_t dw_run;
+  float* dw_sums;  // as sums, of more than one slice
+  int low;         // g has its second rows
   char* dw;        // the piece's rows
   int64_t ld_dw;
   int dw_f32, dw_vec;
@@ -593,15 +622,44 @@ struct ProductsArgs {
   float unit;      // factor of dw
 };
 
+// a tile's accumulators as they lie in a slice's sums
+template <class Sh>
+__device__ __attribute__((always_inline)) inline void keep_sums(const Acc<Sh>& acc, f32x4* sums) {
+  using G = Geo<Sh>;
+#pragma unroll
+  for (int a = 0; a < G::I; ++a)
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg)
+        sums[((a * G::J + b) * 4 + rg) * G::threads + threadIdx.x] =
+            f32x4{{acc[a][b][4 * rg], acc[a][b][4 * rg + 1], acc[a][b][4 * rg + 2], acc[a][b][4 * rg + 3]}};
+}
+template <class Sh>
+__device__ __attribute__((always_inline)) inline void take_sums(Acc<Sh>& acc, const f32x4* sums) {
+  using G = Geo<Sh>;
+#pragma unroll
+  for (int a = 0; a < G::I; ++a)
+#pragma unroll
+    for (int b = 0; b < G::J; ++b)
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {
+        const f32x4 v = sums[((a * G::J + b) * 4 + rg) * G::threads + threadIdx.x];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[a][b][4 * rg + q] = v.v[q];
+      }
+}
+
 template <class T, class Sh>
 __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const ProductsArgs p) {
   using G = Geo<Sh>;
+  constexpr int64_t kTile = Sh::TM * Sh::TN / 4;  // of a slice's sums, in f32x4
   __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // dw's tiles first: they are the long ones where there are many rows, and dx's
   // runs fill the last round (8192 x 768 x 25088: 404 k steps a CU the other way
   // round, 320 so).  Both start at a multiple of 8, an XCD each.
-  const uint32_t dw_tiles = uint32_t(p.dw_m) * p.dw_n, n_dw = (dw_tiles + 7) / 8 * 8;
+  const uint32_t n_dw = (uint32_t(p.dw_m) * p.dw_n * p.dw_slices + 7) / 8 * 8;
   Acc<Sh> acc;
   uint32_t tm, tn;
   if (blockIdx.x >= n_dw) {
@@ -609,42 +667,34 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
     const uint32_t j = blockIdx.x - n_dw, slice = j % p.slices, tile = j / p.slices;
     tm = tile / p.dx_n, tn = tile % p.dx_n;
     const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN, k0 = slice * p.run;
-    f32x4* sums = reinterpret_cast<f32x4*>(p.sums) + (int64_t(slice) * p.dx_m * p.dx_n + tile) * (Sh::TM * Sh::TN / 4);
-    zero<Sh>(acc);
-    if (!p.first) {
-#pragma unroll
-      for (int a = 0; a < G::I; ++a)
-#pragma unroll
-        for (int b = 0; b < G::J; ++b)
-#pragma unroll
-          for (int rg = 0; rg < 4; ++rg) {
-            const f32x4 v = sums[((a * G::J + b) * 4 + rg) * G::threads + threadIdx.x];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) acc[a][b][4 * rg + q] = v.v[q];
-          }
-    }
-    const Product<T, Sh, true, false> dx(p.g + (m0 * p.ld_g + k0) * T::esz, p.ld_g, p.rows - m0,
+    f32x4* sums = reinterpret_cast<f32x4*>(p.sums) + (int64_t(slice) * p.dx_m * p.dx_n + tile) * kTile;
+    if (p.first) zero<Sh>(acc);
+    else take_sums<Sh>(acc, sums);
+    const Product<T, Sh, true, false> dx(p.g + (m0 * p.ld_g + k0) * T::esz, p.ld_g, p.rows + (p.low ? kLow : 0) - m0,
                                          p.w + (k0 * p.ld_w + n0) * T::esz, p.ld_w, p.width - n0,
                                          min(p.run, p.vocab - k0), wave, lane);
     dx.start(lds, wave, lane);
     dx.run(lds, wave, lane, acc);
-#pragma unroll
-    for (int a = 0; a < G::I; ++a)
-#pragma unroll
-      for (int b = 0; b < G::J; ++b)
-#pragma unroll
-        for (int rg = 0; rg < 4; ++rg)
-          sums[((a * G::J + b) * 4 + rg) * G::threads + threadIdx.x] =
-              f32x4{{acc[a][b][4 * rg], acc[a][b][4 * rg + 1], acc[a][b][4 * rg + 2], acc[a][b][4 * rg + 3]}};
+    keep_sums<Sh>(acc, sums);
     return;
   }
-  if (!tile_of(blockIdx.x, n_dw, uint32_t(p.dw_m), uint32_t(p.dw_n), tm, tn)) return;
-  const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN;
+  if (!tile_of(blockIdx.x, n_dw, uint32_t(p.dw_m), uint32_t(p.dw_n) * p.dw_slices, tm, tn)) return;
+  const uint32_t slice = tn / p.dw_n;
+  tn %= p.dw_n;
+  const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN, k0 = slice * p.dw_run;
   zero<Sh>(acc);
-  const Product<T, Sh, false, false> dw(p.g + m0 * T::esz, p.ld_g, p.vocab - m0, p.x + n0 * T::esz, p.ld_x, p.width - n0,
-                                        p.rows, wave, lane);
+  Product<T, Sh, false, false> dw(p.g + (k0 * p.ld_g + m0) * T::esz, p.ld_g, p.vocab - m0,
+                                  p.x + (k0 * p.ld_x + n0) * T::esz, p.ld_x, p.width - n0, min(p.dw_run, p.rows - k0), wave,
+                                  lane);
+  static_assert(128 / Bf16::esz == kLow, "g's second rows are the second k tile");
+  if (p.low) dw.twice();
   dw.start(lds, wave, lane);
   dw.run(lds, wave, lane, acc);
+  if (p.dw_slices > 1) {
+    keep_sums<Sh>(acc, reinterpret_cast<f32x4*>(p.dw_sums) +
+                           ((int64_t(slice) * p.dw_m + tm) * p.dw_n + tn) * kTile);
+    return;
+  }
   const float unit = p.dyn ? p.dyn[1] : p.unit;
   auto value = [&](int a, int b, int rg, float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
@@ -660,45 +710,61 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   store32<Sh>(wave, lane, reinterpret_cast<float*>(p.dw) + m0 * p.ld_dw + n0, p.ld_dw, rows, cols, p.dw_vec, value);
 }
 
-// dx = the slices' sums times the factor.  A block has the 32 rows x WN columns of
+// dx, or dw = the slices' sums times the factor.  A block has the 32 rows x WN columns of
 // one of a wave's accumulator rows, as they lay, and stores them in rows through
 // LDS.  Many slices are added by NG groups of threads, each every NG-th slice in
 // order, then the groups in order (64 slices by one group: 12 us of latency).
+struct SumsArgs {
+  const float* sums;
+  int64_t rows, width;
+  int tiles_m, tiles_n, slices;
+  int low;  // of rows kLow further on too
+  const float* dyn;
+  float unit;
+  char* out;
+  int64_t ld;
+  int vec;
+};
+
 template <class T, class Sh, int NG>
-__global__ __launch_bounds__(kThreads* NG) void dx_kernel(const float* sums, int64_t rows, int64_t width, int dx_m,
-                                                          int dx_n, int slices, const float* dyn, float unit, char* dx,
-                                                          int64_t ld, int vec) {
+__global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
   using G = Geo<Sh>;
   constexpr int kPitch = G::WN + 4, kSize = 32 * kPitch;
   __shared__ float lds[NG * kSize];
   const int group = int(threadIdx.x) / kThreads, tid = int(threadIdx.x) % kThreads;
-  const int64_t tiles = int64_t(dx_m) * dx_n, tile = blockIdx.x / (G::W * G::I);
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n, tile = blockIdx.x / (G::W * G::I);
   const int part = int(blockIdx.x % (G::W * G::I)), wave = part / G::I, a = part % G::I;
-  const f32x4* from = reinterpret_cast<const f32x4*>(sums) + tile * (Sh::TM * Sh::TN / 4);
+  const f32x4* from = reinterpret_cast<const f32x4*>(p.sums) + tile * (Sh::TM * Sh::TN / 4);
+  // the waves kLow rows further on, in the same tile (128 rows, 32 a wave)
+  const int64_t low = kLow / G::WM * Sh::WGN * 64;
 #pragma unroll
   for (int i = tid; i < G::J * 4 * 64; i += kThreads) {
     const int lane = i & 63, br = i >> 6;  // accumulator group: b, rg
-    const f32x4* p = from + (a * G::J * 4 + br) * G::threads + wave * 64 + lane;
+    const f32x4* at = from + (a * G::J * 4 + br) * G::threads + wave * 64 + lane;
     f32x4 s = {{0.f, 0.f, 0.f, 0.f}};
+    auto add = [&](const f32x4* at) __attribute__((always_inline)) {
 #pragma unroll 8
-    for (int q = group; q < slices; q += NG) {
-      const f32x4 v = p[q * tiles * (Sh::TM * Sh::TN / 4)];
+      for (int q = group; q < p.slices; q += NG) {
+        const f32x4 v = at[q * tiles * (Sh::TM * Sh::TN / 4)];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
-    }
+        for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
+      }
+    };
+    if (p.low && wave / Sh::WGN * G::WM < kLow) add(at + low);
+    add(at);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       lds[group * kSize + (lane & 31) * kPitch + 32 * (br >> 2) + 8 * (br & 3) + 4 * (lane >> 5) + e] = s.v[e];
   }
   __syncthreads();
-  const int64_t m0 = tile / dx_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a;
-  const int64_t n0 = tile % dx_n * Sh::TN + wave % Sh::WGN * G::WN;
-  const float f = dyn ? dyn[1] : unit;
+  const int64_t m0 = tile / p.tiles_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a;
+  const int64_t n0 = tile % p.tiles_n * Sh::TN + wave % Sh::WGN * G::WN;
+  const float f = p.dyn ? p.dyn[1] : p.unit;
 #pragma unroll
   for (int i = int(threadIdx.x); i < 32 * G::WN / 4; i += kThreads * NG) {
     const int row = i / (G::WN / 4), col = i % (G::WN / 4) * 4;
     const int64_t m = m0 + row, n = n0 + col;
-    if (m >= rows || n >= width) continue;
+    if (m >= p.rows || n >= p.width) continue;
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -707,14 +773,14 @@ __global__ __launch_bounds__(kThreads* NG) void dx_kernel(const float* sums, int
       for (int q = 1; q < NG; ++q) v[e] += lds[q * kSize + row * kPitch + col + e];
       v[e] *= f;
     }
-    char* to = dx + (m * ld + n) * T::esz;
-    if (vec && n + 4 <= width) {
+    char* to = p.out + (m * p.ld + n) * T::esz;
+    if (p.vec && n + 4 <= p.width) {
       if constexpr (T::esz == 2) *reinterpret_cast<uint2*>(to) = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
       else *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (n + e < width) store_from_f32(to, e, T::mk, v[e]);
+        if (n + e < p.width) store_from_f32(to, e, T::mk, v[e]);
     }
   }
 }
@@ -815,8 +881,9 @@ struct Plan {
   int64_t pitch;                  // of packed rows, elements
   int64_t piece, pieces;          // classes of a piece
   int64_t ld_g;
-  int64_t slices;
-  int64_t x_at, w_at, part_at, target_at, g_at, sums_at, dyn_at, bytes;
+  int64_t slices, dw_slices;      // runs of dx's classes and of dw's rows
+  bool low;                       // g has its second rows
+  int64_t x_at, w_at, part_at, target_at, g_at, sums_at, dw_sums_at, dyn_at, bytes;
 };
 
 // k tiles that the last of the chip's workgroups ends with, of dw's `dw` tiles of kw
@@ -838,41 +905,69 @@ int64_t ends(int64_t dw, int64_t kw, int64_t dx, int64_t kx, int64_t slots) {
 }
 
 // Tile shapes: a k tile of 256 x 256 takes 1.75 us on a CU, one of 128 x 128 with
-// another beside it on the CU 1.12 us, alone 0.78 of that.  A tile's begin and end
-// count as more k tiles: fitted to both shapes' times on the cases below.
+// another beside it on the CU 1.12 us, alone 0.78 of that; of 32 bits what the fp32
+// MFMA takes.  A tile's begin and end count as more k tiles: fitted to both shapes'
+// times on the cases below.
 constexpr int64_t kSizes[2][2] = {{256, 256}, {128, 128}};
-constexpr double kStep[2] = {1.75, 1.12};
+double step_time(int shape, int esz) {
+  return esz == 2 ? (shape == kBig ? 1.75 : 1.12) : (shape == kBig ? 6.9 : 3.5);
+}
 
 // Estimated us of the logits' tiles, kt k tiles each.  Measured, 256 and 128: loss of
 // 300 x 768 x 50257 46, 39, of 1000 92, 93; gradient of 1000 (with the same products)
 // 311, 304, of 1777 x 1001 x 30011 415, 423, of 8192 1911, 2034.
-double logits_time(int shape, int64_t rows, int64_t classes, int64_t kt, bool bwd) {
+double logits_time(int shape, int esz, int64_t rows, int64_t classes, int64_t kt, bool bwd) {
   const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1];
   const int64_t tiles = (rows + tm - 1) / tm * ((classes + tn - 1) / tn);
   const int64_t cus = cu_count(), slots = shape == kBig ? cus : 2 * cus, rest = tiles % slots;
   const double last = rest == 0 ? 0.0 : shape == kMid && rest <= cus ? 0.78 : 1.0;
-  return (double(tiles / slots) + last) * kStep[shape] * (double(kt) + (bwd && shape == kBig ? 3.0 : 1.5));
+  return (double(tiles / slots) + last) * step_time(shape, esz) * (double(kt) + (bwd && shape == kBig ? 3.0 : 1.5));
 }
 
-// Estimated us of dx's and dw's tiles of a piece: dw's over `rows`, and dx's over the
-// classes cut into `slices` runs, which are chosen: fewer k tiles one after the other,
-// against a tile of sums a run, written and read again in each piece and by the last
-// launch, at about 4.5 TB/s.  Measured, 256 and 128 (the whole gradient): 100 x 768 x
-// 50257 87, 73, 300 144, 129, 1000 311, 297; 2048 x 1024 x 32000 390, 428; 1777 x
-// 1001 x 30011 417, 450.
-double products_time(int shape, int64_t rows, int64_t width, int64_t classes, int64_t deep, int64_t& slices) {
+struct Cuts {
+  double time;
+  int shape;
+  int64_t dx, dw;  // runs
+};
+
+// The shape of dx's and dw's tiles of a piece, and the runs that dx's classes and (where
+// dw's tiles do not fill the chip) dw's rows are cut into, by estimated us: fewer k
+// tiles one after the other, against a tile of sums a run, written and read again by
+// the last launch and in each piece, at about 4.5 TB/s.  Measured, 256 and 128 (the
+// whole gradient): 100 x 768 x 50257 87, 73, 300 144, 129, 1000 311, 297; 2048 x 1024
+// x 32000 390, 428; 1777 x 1001 x 30011 417, 450.
+Cuts products_cuts(int shape, int esz, int64_t rows, int64_t width, int64_t classes) {
   constexpr int64_t kEndW[2] = {4, 1}, kEndX[2] = {8, 5};
-  const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1], across = (width + tn - 1) / tn;
+  const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1], across = (width + tn - 1) / tn, deep = 128 / esz;
   const int64_t dx = (rows + tm - 1) / tm * across, dw = (classes + tm - 1) / tm * across;
   const int64_t kx = (classes + deep - 1) / deep, kw = (rows + deep - 1) / deep;
   const int64_t slots = std::max<int64_t>(1, cu_count() / 8 * (shape == kBig ? 1 : 2));
-  double best = 0;
-  for (int64_t n = 1; n <= 64 && n <= kx; n *= 2) {
-    const double t = double(ends((dw + 7) / 8, kw + kEndW[shape], (dx * n + 7) / 8, (kx + n - 1) / n + kEndX[shape], slots)) *
-                         kStep[shape] + double(dx * n * tm * tn * 4) * 2 / 4.5e6;
-    if (n == 1 || t < best) best = t, slices = n;
-  }
+  Cuts best{};
+  for (int64_t w = 1; w == 1 || (w <= 16 && dw * w <= 16 * slots && kw >= 4 * w); w *= 2)
+    for (int64_t n = 1; n <= 64 && n <= kx; n *= 2) {
+      const double sums = double((dx * n + (w > 1 ? dw * w : 0)) * tm * tn * 4);
+      const double t = double(ends((dw * w + 7) / 8, (kw + w - 1) / w + kEndW[shape], (dx * n + 7) / 8,
+                                   (kx + n - 1) / n + kEndX[shape], slots)) *
+                           step_time(shape, esz) +
+                       sums * 2 / 4.5e6 + (w > 1 ? 4.0 : 0.0);
+      if (best.dx == 0 || t < best.time) best = {t, shape, n, w};
+    }
   return best;
+}
+
+// The better shape's, kept for the next call of the same sizes (a call asks for its
+// workspace first).
+Cuts products_cuts(int esz, int64_t rows, int64_t width, int64_t classes, bool low) {
+  struct Last { int64_t key[5]; Cuts cuts; };
+  static thread_local Last last{};
+  const int64_t key[5] = {esz + 16 * low, rows, width, classes, cu_count()};
+  if (!std::equal(key, key + 5, last.key)) {
+    const Cuts mid = products_cuts(kMid, esz, rows, width, classes);
+    const Cuts big = low ? mid : products_cuts(kBig, esz, rows, width, classes);  // low: 128 rows a tile
+    std::copy(key, key + 5, last.key);
+    last.cuts = mid.time < big.time ? mid : big;
+  }
+  return last.cuts;
 }
 
 Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x, int64_t ld_x, const void* w,
@@ -882,7 +977,9 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   q.rows = rows, q.width = width, q.vocab = vocab;
   const int64_t deep = 128 / q.esz;
   const int64_t kt = (width + deep - 1) / deep;
-  q.logits = logits_time(kMid, rows, vocab, kt, bwd) < logits_time(kBig, rows, vocab, kt, bwd) ? kMid : kBig;
+  q.low = bwd && q.esz == 2 && rows <= kLow;
+  const double mid = logits_time(kMid, q.esz, rows, vocab, kt, bwd), big = logits_time(kBig, q.esz, rows, vocab, kt, bwd);
+  q.logits = q.low || mid < big ? kMid : kBig;
   q.tm = kSizes[q.logits][0], q.tn = kSizes[q.logits][1];
   q.pack_x = !on_grid(x, ld_x, width, q.esz) || (bwd && has_ignore);
   q.pack_w = !on_grid(w, ld_w, width, q.esz);
@@ -907,16 +1004,14 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   } else {
     const int64_t classes = std::min(vocab, q.piece);
     q.ld_g = up(classes, 64);
-    q.g_at = take(rows * q.ld_g * q.esz);
-    int64_t slices[2];
-    q.products = products_time(kMid, rows, width, classes, deep, slices[kMid]) <
-                         products_time(kBig, rows, width, classes, deep, slices[kBig])
-                     ? kMid
-                     : kBig;
-    q.slices = slices[q.products];
+    q.g_at = take((rows + (q.low ? kLow : 0)) * q.ld_g * q.esz);
+    const Cuts cuts = products_cuts(q.esz, rows, width, classes, q.low);
+    q.products = cuts.shape, q.slices = cuts.dx, q.dw_slices = cuts.dw;
     q.pm = kSizes[q.products][0], q.pn = kSizes[q.products][1];
     const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn);
     q.sums_at = take(q.slices * tiles * q.pm * q.pn * 4);
+    if (q.dw_slices > 1)
+      q.dw_sums_at = take(q.dw_slices * ((classes + q.pm - 1) / q.pm) * ((width + q.pn - 1) / q.pn) * q.pm * q.pn * 4);
     q.dyn_at = take(8);
   }
   q.bytes = at;
@@ -1100,9 +1195,11 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   a.tiles_m = int((rows + q.tm - 1) / q.tm);
   b.dx_m = dx ? int((rows + q.pm - 1) / q.pm) : 0;
   b.dx_n = b.dw_n = int((width + q.pn - 1) / q.pn);
-  b.slices = int(q.slices);
+  b.slices = int(q.slices), b.dw_slices = int(q.dw_slices);
+  b.dw_run = up((rows + q.dw_slices - 1) / q.dw_slices, 128 / esz);
+  a.low = b.low = q.low;
   const int64_t most = a.tiles_m * ((q.piece + q.tn - 1) / q.tn),
-                most2 = int64_t(b.dx_m) * b.dx_n * q.slices + (q.piece + q.pm - 1) / q.pm * b.dw_n + 8;
+                most2 = int64_t(b.dx_m) * b.dx_n * q.slices + (q.piece + q.pm - 1) / q.pm * b.dw_n * q.dw_slices + 8;
   if (int rc = check_tiles(what, std::max(most, most2), 512)) return rc;
   // fp16: g out of the subnormals, by a power of two of the largest row_grad
   a.unit = io_type == MK_F16 ? 32768.f : 1.f;
@@ -1119,10 +1216,26 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   }
   b.g = a.g, b.ld_g = a.ld_g;
   b.x = a.x, b.ld_x = a.ld_x;
-  b.sums = reinterpret_cast<float*>(ws + q.sums_at);
+  b.sums = reinterpret_cast<float*>(ws + q.sums_at), b.dw_sums = reinterpret_cast<float*>(ws + q.dw_sums_at);
   b.dw_f32 = dw_type == MK_F32;
   b.ld_dw = ld_dw;
   b.dw_vec = (reinterpret_cast<uintptr_t>(dw) & 15u) == 0 && ld_dw * dwsz % 16 == 0 && width * esz % 16 == 0;
+  // the sums of slices, dx's or a piece's dw's, into rows of type `to`
+  auto join = [&](int to, const SumsArgs& c) {
+    return with_kernels(to, q.products, [&](auto t, auto sh) {
+      using T = decltype(t);
+      using Sh = decltype(sh);
+      const int64_t blocks = int64_t(c.tiles_m) * c.tiles_n * Geo<Sh>::W * Geo<Sh>::I;
+      if (int r = check_tiles(what, blocks, 4 * kThreads)) return r;
+      const dim3 g{unsigned(blocks)};
+      if (c.slices > 8) hipLaunchKernelGGL((sums_kernel<T, Sh, 4>), g, dim3(4 * kThreads), 0, s, c);
+      else hipLaunchKernelGGL((sums_kernel<T, Sh, 1>), g, dim3(kThreads), 0, s, c);
+      return check_launch(what);
+    });
+  };
+  auto vec4 = [](const void* p, int64_t ld, int bytes) {
+    return int(reinterpret_cast<uintptr_t>(p) % (4 * bytes) == 0 && ld % 4 == 0);
+  };
   for (int64_t v0 = 0; v0 < vocab; v0 += q.piece) {
     a.v0 = v0;
     a.vocab = b.vocab = std::min(q.piece, vocab - v0);
@@ -1149,26 +1262,18 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     rc = with_kernels(io_type, q.products, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
-      const unsigned tiles = unsigned(b.dx_m) * b.dx_n * b.slices + (unsigned(b.dw_m) * b.dw_n + 7) / 8 * 8;
+      const unsigned tiles = unsigned(b.dx_m) * b.dx_n * b.slices + (unsigned(b.dw_m) * b.dw_n * b.dw_slices + 7) / 8 * 8;
       hipLaunchKernelGGL((products_kernel<T, Sh>), dim3(tiles), dim3(Geo<Sh>::threads), 0, s, b);
       return check_launch(what);
     });
     if (rc) return rc;
+    if (dw && b.dw_slices > 1) {
+      const SumsArgs c{b.dw_sums, b.vocab, width, b.dw_m, b.dw_n, b.dw_slices, 0, b.dyn, b.unit, b.dw, ld_dw,
+                       vec4(b.dw, ld_dw, dwsz)};
+      if (int r = join(dw_type, c)) return r;
+    }
   }
   if (!dx) return MK_OK;
-  const int dx_vec = reinterpret_cast<uintptr_t>(dx) % (4 * esz) == 0 && ld_dx % 4 == 0;
-  return with_kernels(io_type, q.products, [&](auto t, auto sh) {
-    using T = decltype(t);
-    using Sh = decltype(sh);
-    const int64_t blocks = int64_t(b.dx_m) * b.dx_n * Geo<Sh>::W * Geo<Sh>::I;
-    if (int r = check_tiles(what, blocks, 4 * kThreads)) return r;
-    auto sum = [&](auto groups) {
-      constexpr int NG = decltype(groups)::value;
-      hipLaunchKernelGGL((dx_kernel<T, Sh, NG>), dim3(unsigned(blocks)), dim3(kThreads * NG), 0, s, b.sums, rows, width,
-                         b.dx_m, b.dx_n, b.slices, b.dyn, b.unit, static_cast<char*>(dx), ld_dx, dx_vec);
-    };
-    if (b.slices > 8) sum(Int<4>{});
-    else sum(Int<1>{});
-    return check_launch(what);
-  });
+  return join(io_type, SumsArgs{b.sums, rows, width, b.dx_m, b.dx_n, b.slices, b.low, b.dyn, b.unit,
+                                static_cast<char*>(dx), ld_dx, vec4(dx, ld_dx, esz)});
 }

@@ -151,6 +151,46 @@ def test_strides_offsets_and_outputs(K, dtype):
     assert esz in (2, 4)
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("rows,width,vocab", [(1, 64, 500), (4, 208, 5819), (33, 39, 1000), (64, 768, 5003)])
+def test_few_rows_keep_what_rounding_leaves(K, dtype, rows, width, vocab):
+    """Up to 64 rows hold the gradients of the logits in two numbers of 16 bits."""
+    print(f"case: few rows {rows} x {width} x {vocab} {dtype}", flush=True)
+    x, w, labels = _inputs(11, rows, width, vocab, dtype, torch.int64)
+    labels[rows // 2] = vocab - 1
+    row_grad = torch.rand(rows, device="cuda") + 0.5
+    for ignore in (None, int(labels[0])) if rows > 1 else (None,):
+        _, lse = K.linear_xent(x, w, labels, ignore_index=ignore)
+        dx, dw = K.linear_xent_bwd(x, w, labels, lse, row_grad=row_grad, ignore_index=ignore, dw_dtype=torch.float32)
+        wx, ww, bx, bw = xent_grad(x, w, labels, lse, 1.0, row_grad, ignore, torch.float32, twice=True)
+        _within(dx, wx, bx, "dx")
+        _within(dw, ww, bw, "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_of_few_classes(K, dtype):
+    """The weights' gradient has few tiles here: its rows are cut into runs."""
+    for rows, width, vocab in ((4571, 64, 2148), (9001, 16, 300), (3000, 130, 2)):
+        print(f"case: many rows {rows} x {width} x {vocab} {dtype}", flush=True)
+        x, w, labels = _inputs(12, rows, width, vocab, dtype)
+        labels[::3] = -100
+        sea = torch.full((vocab * (width + 3) + 5,), 77.0, device="cuda").to(dtype)
+        dw = sea[5:].view(vocab, width + 3)[:, :width]
+        _, lse, dx, alone = _check(K, x, w, labels, scale=1.0 / rows, ignore=-100)
+        K.linear_xent_bwd(x, w, labels, lse, grad_scale=1.0 / rows, ignore_index=-100, dw=dw)
+        assert torch.equal(dw, alone)
+        assert torch.all(sea[:5] == 77) and torch.all(sea[5:].view(vocab, width + 3)[:, width:] == 77)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = K.linear_xent_bwd(x, w, labels, lse, grad_scale=1.0 / rows, ignore_index=-100)
+        for _ in range(2):
+            got[0].zero_(), got[1].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], dx) and torch.equal(got[1], alone)
+            _check(K, x[:100], w, labels[:100])
+
+
 def test_one_gradient_alone_and_fp32_weights_gradient(K):
     for dtype in TYPES:
         for rows in (60, 400):

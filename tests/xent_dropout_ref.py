@@ -67,10 +67,11 @@ def xent(x, w, labels, ignore=None):
     return loss, lse, bound
 
 
-def xent_grad(x, w, labels, lse, scale=1.0, row_grad=None, ignore=None, dw_dtype=None):
+def xent_grad(x, w, labels, lse, scale=1.0, row_grad=None, ignore=None, dw_dtype=None, twice=False):
     """(dx, dw, bound of dx, bound of dw): g is rounded once to x's type (fp16: of a power of two
     times it, so that what is lost below its normal numbers is 2^-40 of the largest), sums are
-    fp32 additions in any order, results are rounded once."""
+    fp32 additions in any order, results are rounded once.  twice: what g's rounding leaves is
+    rounded to a second number of the type."""
     dtype, dw_dtype = x.dtype, dw_dtype or w.dtype
     used = _counts(labels.long(), ignore)
     x = torch.where(used[:, None], x.double(), 0.0)  # whatever an ignored row holds
@@ -84,7 +85,7 @@ def xent_grad(x, w, labels, lse, scale=1.0, row_grad=None, ignore=None, dw_dtype
     # of g: its rounding, and the exponential's error
     dz = (x.shape[1] + 1) * H32 * (x.abs() @ w.abs().t())
     e = dz + H32 * (3 * (z - lse.double()[:, None]).abs() + 4)
-    dg = half_step(dtype) * g.abs() + (p * e + 2 * H32 * (p + hot)) * r.abs()[:, None]
+    dg = half_step(dtype) ** (2 if twice else 1) * g.abs() + (p * e + 2 * H32 * (p + hot)) * r.abs()[:, None]
     if dtype == torch.float16:
         dg = dg + 2.0 ** -40 * r.abs().max()
     dx, dw = g @ w * scale, g.t() @ x * scale
