@@ -181,6 +181,8 @@ class GPT2TrainStep:
             raise ValueError("d_model must be a multiple of 8, at most 2048 (mk_layernorm_bwd)")
         if not 0.0 <= cfg.dropout < 1.0:
             raise ValueError("dropout must be in [0, 1)")
+        if not 0 <= dropout_seed < 1 << 64:
+            raise ValueError("dropout_seed is a whole number of 64 bits")
         self.keep_logits, self.dropout_seed = keep_logits, dropout_seed
         self.cfg, self.dev = cfg, torch.device(device)
         self.lr, self.b1, self.b2, self.adam_eps = lr, b1, b2, adam_eps

@@ -988,6 +988,15 @@ def _xent_operands(what, x, w):
     return t, shape[0], shape[1], w.shape[0], dev
 
 
+def _ignore(what, ignore_index):
+    """has_ignore and ignore_index as the C-ABI takes them."""
+    if ignore_index is None:
+        return 0, 0
+    if not -1 << 63 <= ignore_index < 1 << 63:
+        raise ValueError(f"{what}: ignore_index is a whole number of 64 bits")
+    return 1, int(ignore_index)
+
+
 def _bytes(what, like, nbytes, workspace, stream, dev):
     if workspace is None:
         return _new(like, stream, torch.uint8, max(int(nbytes), 1))
@@ -1008,6 +1017,7 @@ def linear_xent(x, w, labels, ignore_index=None, loss_rows=None, lse=None, works
     what = "linear_xent"
     t, rows, width, vocab, dev = _xent_operands(what, x, w)
     label_type = _labels(what, labels, rows, dev)
+    ignore = _ignore(what, ignore_index)
     if loss_rows is None:
         loss_rows = _new(x, stream, torch.float32, rows)
     else:
@@ -1020,8 +1030,7 @@ def linear_xent(x, w, labels, ignore_index=None, loss_rows=None, lse=None, works
     at = (x.data_ptr(), x.stride()[0], w.data_ptr(), w.stride()[0])
     ws = _bytes(what, x, L.mk_linear_xent_workspace_bytes(t, rows, width, vocab, *at), workspace, stream, dev)
     rc = L.mk_linear_xent(_handle(what, stream, dev), t, rows, width, vocab, *at, label_type, labels.data_ptr(),
-                          ignore_index is not None, ignore_index or 0, loss_rows.data_ptr(), lse.data_ptr(),
-                          ws.data_ptr())
+                          *ignore, loss_rows.data_ptr(), lse.data_ptr(), ws.data_ptr())
     if rc:
         _check(rc, "mk_linear_xent")
     return loss_rows, lse
@@ -1037,6 +1046,7 @@ def linear_xent_bwd(x, w, labels, lse, grad_scale=1.0, row_grad=None, ignore_ind
     what = "linear_xent_bwd"
     t, rows, width, vocab, dev = _xent_operands(what, x, w)
     label_type = _labels(what, labels, rows, dev)
+    ignore = _ignore(what, ignore_index)
     _operand(what, "lse", lse, torch.float32, (rows,), dev)
     if row_grad is not None:
         _operand(what, "row_grad", row_grad, torch.float32, (rows,), dev)
@@ -1058,13 +1068,11 @@ def linear_xent_bwd(x, w, labels, lse, grad_scale=1.0, row_grad=None, ignore_ind
             _result(what, "dw", dw, dw_dtype, (vocab, width), dev)
     L = _lib._kernels or lib()
     at = (x.data_ptr(), x.stride()[0], w.data_ptr(), w.stride()[0])
-    ws = _bytes(what, x, L.mk_linear_xent_bwd_workspace_bytes(t, rows, width, vocab, *at,
-                                                                       ignore_index is not None),
-                         workspace, stream, dev)
+    ws = _bytes(what, x, L.mk_linear_xent_bwd_workspace_bytes(t, rows, width, vocab, *at, ignore[0]), workspace, stream,
+                dev)
     rc = L.mk_linear_xent_bwd(_handle(what, stream, dev), t, t if dw is None else _TORCH_TO_MK[dw.dtype], rows, width,
-                              vocab, *at, label_type, labels.data_ptr(), ignore_index is not None, ignore_index or 0,
-                              lse.data_ptr(), _ptr(row_grad), float(grad_scale), _ptr(dx),
-                              0 if dx is None else dx.stride()[0], _ptr(dw), 0 if dw is None else dw.stride()[0],
+                              vocab, *at, label_type, labels.data_ptr(), *ignore, lse.data_ptr(), _ptr(row_grad),
+                              float(grad_scale), _ptr(dx), 0 if dx is None else dx.stride()[0], _ptr(dw), 0 if dw is None else dw.stride()[0],
                               ws.data_ptr())
     if rc:
         _check(rc, "mk_linear_xent_bwd")
@@ -1072,7 +1080,7 @@ def linear_xent_bwd(x, w, labels, lse, grad_scale=1.0, row_grad=None, ignore_ind
 
 
 def _draw(what, seed, offset, step, dev):
-    """seed, offset and the address of step as the C-ABI takes them."""
+    """Checks seed and offset; the address of step or None."""
     if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
         raise ValueError(f"{what}: seed and offset are whole numbers of 64 bits")
     if step is None:
@@ -1111,7 +1119,7 @@ def dropout_add(x, p, seed, offset=0, step=None, bias=None, residual=None, out=N
     s_ptr = _draw(what, seed, offset, step, dev)
     handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
     rc = (_lib._kernels or lib()).mk_dropout_add(handle, t, rows, cols, x.data_ptr(), strides[0], b_ptr, r_ptr, r_ld, p,
-                                                 seed, offset, s_ptr, out.data_ptr(), ld)
+                                                 int(seed), int(offset), s_ptr, out.data_ptr(), ld)
     if rc:
         _check(rc, "mk_dropout_add")
     return out
@@ -1146,8 +1154,8 @@ def dropout_add_bwd(dy, p, seed, offset=0, step=None, want_colsum=False, dx=None
         c_ptr, w_ptr = colsum.data_ptr(), workspace.data_ptr()
     s_ptr = _draw(what, seed, offset, step, dev)
     handle = _raw_stream(dev) if stream is None else _handle(what, stream, dev)
-    rc = L.mk_dropout_add_bwd(handle, t, rows, cols, dy.data_ptr(), strides[0], p, seed, offset, s_ptr, dx.data_ptr(), ld,
-                              c_ptr, w_ptr)
+    rc = L.mk_dropout_add_bwd(handle, t, rows, cols, dy.data_ptr(), strides[0], p, int(seed), int(offset), s_ptr,
+                              dx.data_ptr(), ld, c_ptr, w_ptr)
     if rc:
         _check(rc, "mk_dropout_add_bwd")
     return dx, colsum

@@ -198,19 +198,23 @@ __global__ __launch_bounds__(1024) void colsum_final_kernel(const float* part, i
                                                             float* y) {
   __shared__ float lds[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t c = int64_t(blockIdx.x) * 32 + tx;
   const int64_t run = (parts + 31) / 32, p0 = ty * run, p1 = std::min(parts, p0 + run);
-  float s = 0.f;
-  if (c < cols) {
+  for (int64_t c0 = int64_t(blockIdx.x) * 32; c0 < cols; c0 += int64_t(gridDim.x) * 32) {
+    const int64_t c = c0 + tx;
+    float s = 0.f;
+    if (c < cols) {
 #pragma unroll 8
-    for (int64_t p = p0; p < p1; ++p) s += part[p * cols + c];
-  }
-  lds[ty][tx] = s;
-  __syncthreads();
-  if (ty != 0 || c >= cols) return;
+      for (int64_t p = p0; p < p1; ++p) s += part[p * cols + c];
+    }
+    lds[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < cols) {
 #pragma unroll
-  for (int i = 1; i < 32; ++i) s += lds[i][tx];
-  y[c] = s * scale;
+      for (int i = 1; i < 32; ++i) s += lds[i][tx];
+      y[c] = s * scale;
+    }
+    __syncthreads();
+  }
 }
 
 // Chunks a block is wide: the widest power of two that pads the row least.
@@ -305,6 +309,8 @@ extern "C" int mk_dropout_add(void* stream, int io_type, int64_t rows, int64_t c
       return fail(MK_ERR_INVALID, std::string(what) + ": " + why + q.name);
   if (ld_x < 0 || ld_residual < 0 || (rows > 1 && ld_out < cols))
     return fail(MK_ERR_INVALID, std::string(what) + ": a pitch below 0, or rows of out that overlap");
+  if (rows > 1 && ((out == x && ld_out != ld_x) || (out == residual && ld_out != ld_residual)))
+    return fail(MK_ERR_INVALID, std::string(what) + ": out over x or residual at another pitch");
   DropArgs a{};
   draw_args(a, io_type, rows, cols, p, seed, offset, step);
   a.x = x, a.bias = bias, a.residual = residual, a.out = out;
@@ -343,6 +349,8 @@ extern "C" int mk_dropout_add_bwd(void* stream, int io_type, int64_t rows, int64
       return fail(MK_ERR_INVALID, std::string(what) + ": " + why + q.name);
   if (ld_dy < 0 || (rows > 1 && ld_dx < cols))
     return fail(MK_ERR_INVALID, std::string(what) + ": a pitch below 0, or rows of dx that overlap");
+  if (rows > 1 && dx == dy && ld_dx != ld_dy)
+    return fail(MK_ERR_INVALID, std::string(what) + ": dx over dy at another pitch");
   DropArgs a{};
   draw_args(a, io_type, rows, cols, p, seed, offset, step);
   a.x = dy, a.out = dx;
@@ -351,7 +359,7 @@ extern "C" int mk_dropout_add_bwd(void* stream, int io_type, int64_t rows, int64
   hipStream_t s = as_stream(stream);
   if (int rc = launch<true>(what, s, io_type, a)) return rc;
   if (!dx_colsum) return MK_OK;
-  hipLaunchKernelGGL(colsum_final_kernel, dim3(unsigned((cols + 31) / 32)), dim3(1024), 0, s, a.part, row_parts(a), cols,
+  hipLaunchKernelGGL(colsum_final_kernel, dim3(unsigned(std::min<int64_t>((cols + 31) / 32, 1 << 16))), dim3(1024), 0, s, a.part, row_parts(a), cols,
                      a.scale, dx_colsum);
   return check_launch(what);
 }

@@ -150,6 +150,27 @@ def test_no_elements(K):
     assert dx.shape == (0, 8) and torch.equal(colsum, torch.zeros(8, device="cuda"))
 
 
+def test_more_columns_than_a_grid_of_sums(K):
+    """One row of 2^27 + 40 columns: its sums are the row itself."""
+    cols = (1 << 27) + 40
+    dy = torch.randn(1, cols, device="cuda").bfloat16()
+    dx, colsum = K.dropout_add_bwd(dy, 0.25, 3, want_colsum=True)
+    kept = dx[0] != 0
+    assert abs(float(kept.double().mean()) - 0.75) < 6 * (0.1875 / cols) ** 0.5 + 2.0 ** -8  # a few values round to 0
+    want = torch.where(kept, dy[0].float(), 0.0) * float(torch.tensor(65536 / (65536 - 16384), dtype=torch.float32))
+    assert torch.equal(colsum, want)
+    keep, _ = dropout_keep(1, 4096, 0.25, 3, 0)
+    assert torch.equal(kept[:4096].cpu() | (dy[0, :4096].cpu() == 0), keep[0] | (dy[0, :4096].cpu() == 0))
+
+
+def test_numbers_of_numpy(K):
+    import numpy as np
+
+    x = _normal(11, (20, 40), torch.float32)
+    assert torch.equal(K.dropout_add(x, np.float64(0.5), np.int64(7), offset=np.uint64(2 ** 63)),
+                       K.dropout_add(x, 0.5, 7, offset=2 ** 63))
+
+
 def test_streams_and_graphs(K):
     """A captured step draws anew on every replay from its device number, forward and backward alike."""
     x, bias = _normal(9, (500, 104), torch.bfloat16), _normal(10, (104,), torch.bfloat16)

@@ -97,3 +97,5 @@ def test_replays_draw_anew(G):
 def test_refuses_a_dropout_of_one(G):
     with pytest.raises(ValueError, match="dropout"):
         G.GPT2TrainStep(_config(G, 1.0))
+    with pytest.raises(ValueError, match="dropout_seed"):
+        G.GPT2TrainStep(_config(G, 0.1), dropout_seed=-1)
