@@ -528,7 +528,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
   logits.start(lds, wave, lane);
   const float unit = p.dyn ? p.dyn[0] : p.unit;
   float lse[G::I], factor[G::I];
-  int rel[G::I];  // the label's column of this lane's, -1: none
+  int rel[G::I];  // the label's column of this lane's, -1: none, -2: the row is ignored
   bool counts = true;
 #pragma unroll
   for (int a = 0; a < G::I; ++a) {
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
       const int64_t label = p.labels.at(m), at = label - p.v0 - n0 - wn * G::WN - 4 * g;
       lse[a] = p.lse[m];
       factor[a] = unit * (p.row_grad ? p.row_grad[m] : 1.f);
-      if (p.labels.ignored(label)) factor[a] = 0.f, counts = false;
+      if (p.labels.ignored(label)) factor[a] = 0.f, rel[a] = -2, counts = false;
       else if (at >= 0 && at < G::WN) rel[a] = int(at);
     }
   }
@@ -575,7 +575,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           // selected: an ignored row's logits may be anything
-          if (factor[a] == 0.f || 32 * b + 8 * (r / 4) + r % 4 >= left) acc[a][b][r] = 0.f;
+          if (rel[a] == -2 || 32 * b + 8 * (r / 4) + r % 4 >= left) acc[a][b][r] = 0.f;
   }
   auto value = [&](int a, int b, int rg, float (&v)[4]) __attribute__((always_inline)) {
 #pragma unroll
@@ -817,19 +817,21 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const U* src, int64_t ld
 // rows x cols of zeros (words of U): the gradient of no rows
 template <typename U>
 __global__ __launch_bounds__(kThreads) void zero_kernel(U* p, int64_t ld, int64_t rows, int64_t cols) {
-  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  if (i < rows * cols) p[i / cols * ld + i % cols] = U(0);
+  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < rows * cols; i += int64_t(gridDim.x) * kThreads)
+    p[i / cols * ld + i % cols] = U(0);
 }
 
-// dyn = {factor of g, factor of the products} for fp16: |g| <= max |row_grad|, and
+// dyn = {factor of g, factor of the products} for fp16: |g| <= max |row_grad| of the rows
+// that count (an ignored row's may be anything), and
 // 2^15 times that over its power of two is below fp16's largest value, while the
 // smallest normal value is 2^-29 of it.
-__global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad, int64_t rows, float scale, float* dyn) {
+__global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad, int64_t rows, Labels labels, float scale, float* dyn) {
   __shared__ float red[kThreads / kWave];
   float top = 0.f;
+#pragma unroll 4
   for (int64_t n = threadIdx.x; n < rows; n += kThreads) {
     const float v = fabsf(row_grad[n]);
-    if (v < INFINITY) top = fmaxf(top, v);
+    if (v < INFINITY && !(labels.has_ignore && labels.ignored(labels.at(n)))) top = fmaxf(top, v);
   }
   top = wave_max(top);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
@@ -839,7 +841,7 @@ __global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad,
   for (int i = 1; i < kThreads / kWave; ++i) top = fmaxf(top, red[i]);
   int e = 0;
   if (top > 0.f) (void)frexpf(top, &e);  // top <= 2^e
-  e = max(-100, min(100, e));
+  e = max(-112, e);  // 2^127 at most
   dyn[0] = ldexpf(1.f, 15 - e);
   dyn[1] = ldexpf(scale, e - 15);
 }
@@ -955,21 +957,6 @@ Cuts products_cuts(int shape, int esz, int64_t rows, int64_t width, int64_t clas
   return best;
 }
 
-// The better shape's, kept for the next call of the same sizes (a call asks for its
-// workspace first).
-Cuts products_cuts(int esz, int64_t rows, int64_t width, int64_t classes, bool low) {
-  struct Last { int64_t key[5]; Cuts cuts; };
-  static thread_local Last last{};
-  const int64_t key[5] = {esz + 16 * low, rows, width, classes, cu_count()};
-  if (!std::equal(key, key + 5, last.key)) {
-    const Cuts mid = products_cuts(kMid, esz, rows, width, classes);
-    const Cuts big = low ? mid : products_cuts(kBig, esz, rows, width, classes);  // low: 128 rows a tile
-    std::copy(key, key + 5, last.key);
-    last.cuts = mid.time < big.time ? mid : big;
-  }
-  return last.cuts;
-}
-
 Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x, int64_t ld_x, const void* w,
           int64_t ld_w, bool has_ignore) {
   Plan q{};
@@ -1005,7 +992,9 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
     const int64_t classes = std::min(vocab, q.piece);
     q.ld_g = up(classes, 64);
     q.g_at = take((rows + (q.low ? kLow : 0)) * q.ld_g * q.esz);
-    const Cuts cuts = products_cuts(q.esz, rows, width, classes, q.low);
+    const Cuts small = products_cuts(kMid, q.esz, rows, width, classes);
+    const Cuts large = products_cuts(kBig, q.esz, rows, width, classes);
+    const Cuts& cuts = q.low || small.time < large.time ? small : large;  // low: 128 rows a tile
     q.products = cuts.shape, q.slices = cuts.dx, q.dw_slices = cuts.dw;
     q.pm = kSizes[q.products][0], q.pn = kSizes[q.products][1];
     const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn);
@@ -1109,7 +1098,7 @@ extern "C" int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t w
   a.part = reinterpret_cast<float2*>(ws + q.part_at);
   a.target = reinterpret_cast<float*>(ws + q.target_at);
   a.tiles_m = int((rows + q.tm - 1) / q.tm);
-  if (int rc = check_tiles(what, a.tiles_m * ((q.piece + q.tn - 1) / q.tn), 512)) return rc;
+  if (int rc = check_tiles(what, std::max(a.tiles_m * ((q.piece + q.tn - 1) / q.tn), (rows + 15) / 16), 512)) return rc;
   if (q.pack_x) {
     if (int rc = pack(what, s, q, x, ld_x, rows, ws + q.x_at, Labels{})) return rc;
     a.x = ws + q.x_at, a.ld_x = q.pitch;
@@ -1169,8 +1158,7 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
       {"row_grad", row_grad, 4, false}, {"dx", dx, esz, false}, {"workspace", workspace, 16, true}};
   if (rows == 0) {
     if (!dw) return MK_OK;
-    const int64_t blocks = (vocab * width + kThreads - 1) / kThreads;
-    if (int rc = check_tiles(what, blocks, kThreads)) return rc;
+    const int64_t blocks = std::min<int64_t>((vocab * width + kThreads - 1) / kThreads, 1 << 16);
     if (dwsz == 2)
       hipLaunchKernelGGL(zero_kernel<uint16_t>, dim3(unsigned(blocks)), dim3(kThreads), 0, s, static_cast<uint16_t*>(dw),
                          ld_dw, vocab, width);
@@ -1181,7 +1169,8 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   }
   for (const auto& e : ptrs)
     if (int rc = check_pointer(what, e.name, e.p, e.bytes, e.needed)) return rc;
-  if (dx == x || (dw && dw == w)) return fail(MK_ERR_INVALID, std::string(what) + ": dx over x, or dw over w");
+  if (dx == x || dx == w || dw == w || dw == x || dx == dw)
+    return fail(MK_ERR_INVALID, std::string(what) + ": dx or dw over x, over w or one over the other");
   const Plan q = plan(true, io_type, rows, width, vocab, x, ld_x, w, ld_w, has_ignore != 0);
   char* ws = static_cast<char*>(workspace);
   const Labels lab = {labels, label_type == MK_S64, has_ignore != 0, ignore_index};
@@ -1200,13 +1189,15 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   a.low = b.low = q.low;
   const int64_t most = a.tiles_m * ((q.piece + q.tn - 1) / q.tn),
                 most2 = int64_t(b.dx_m) * b.dx_n * q.slices + (q.piece + q.pm - 1) / q.pm * b.dw_n * q.dw_slices + 8;
-  if (int rc = check_tiles(what, std::max(most, most2), 512)) return rc;
+  // the sums' blocks have 32 rows and a wave's columns, and at most 1024 threads
+  const int64_t most3 = int64_t(b.dx_m) * b.dx_n * (q.products == kBig ? 32 : 8) * 2;
+  if (int rc = check_tiles(what, std::max({most, most2, most3}), 512)) return rc;
   // fp16: g out of the subnormals, by a power of two of the largest row_grad
   a.unit = io_type == MK_F16 ? 32768.f : 1.f;
   b.unit = io_type == MK_F16 ? grad_scale / 32768.f : grad_scale;
   if (io_type == MK_F16 && row_grad) {
     float* dyn = reinterpret_cast<float*>(ws + q.dyn_at);
-    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(kThreads), 0, s, row_grad, rows, grad_scale, dyn);
+    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(kThreads), 0, s, row_grad, rows, lab, grad_scale, dyn);
     if (int rc = check_launch(what)) return rc;
     a.dyn = b.dyn = dyn;
   }
@@ -1225,9 +1216,7 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     return with_kernels(to, q.products, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
-      const int64_t blocks = int64_t(c.tiles_m) * c.tiles_n * Geo<Sh>::W * Geo<Sh>::I;
-      if (int r = check_tiles(what, blocks, 4 * kThreads)) return r;
-      const dim3 g{unsigned(blocks)};
+      const dim3 g{unsigned(c.tiles_m) * unsigned(c.tiles_n) * Geo<Sh>::W * Geo<Sh>::I};
       if (c.slices > 8) hipLaunchKernelGGL((sums_kernel<T, Sh, 4>), g, dim3(4 * kThreads), 0, s, c);
       else hipLaunchKernelGGL((sums_kernel<T, Sh, 1>), g, dim3(kThreads), 0, s, c);
       return check_launch(what);

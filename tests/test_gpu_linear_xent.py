@@ -117,6 +117,49 @@ def test_large_factors_keep_fp16_in_range(K):
         assert torch.equal(dx, first[0]) and torch.equal(dw, first[1])  # powers of two change no bit
 
 
+def test_fp16_range_of_row_gradients(K):
+    """Their largest finite value sets fp16's range; an ignored row's, whatever it holds, does not."""
+    x, w, labels = _inputs(13, 140, 64, 500, torch.float16)
+    _, lse = K.linear_xent(x, w, labels)
+    want = K.linear_xent_bwd(x, w, labels, lse, row_grad=torch.full((140,), 1.5, device="cuda"))
+    for power in (-110, 110, 126):
+        row_grad = torch.full((140,), 1.5 * 2.0 ** power, device="cuda")
+        got = K.linear_xent_bwd(x, w, labels, lse, grad_scale=2.0 ** -power, row_grad=row_grad)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    row_grad = torch.rand(140, device="cuda") + 0.5
+    labels[::5] = -100
+    row_grad[::5] = 0
+    want = K.linear_xent_bwd(x, w, labels, lse, row_grad=row_grad, ignore_index=-100)
+    row_grad[::5] = torch.tensor([1e30, float("inf"), float("nan"), -3e38], device="cuda").repeat(7)
+    got = K.linear_xent_bwd(x, w, labels, lse, row_grad=row_grad, ignore_index=-100)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_row_of_nan_stays_one(K, dtype):
+    """A row that counts and holds a NaN spoils its own dx and all of dw, beside ignored rows and at the last
+    classes alike, also with a row_grad of 0; no other row's dx."""
+    x, w, labels = _inputs(14, 150, 40, 300, dtype)
+    labels[::3] = -100
+    row_grad = torch.ones(150, device="cuda")
+    row_grad[4] = 0
+    _, lse = K.linear_xent(x, w, labels, ignore_index=-100)
+    want, _ = K.linear_xent_bwd(x, w, labels, lse, row_grad=row_grad, ignore_index=-100)
+    x[4, 7] = lse[4] = float("nan")
+    dx, dw = K.linear_xent_bwd(x, w, labels, lse, row_grad=row_grad, ignore_index=-100)
+    others = torch.arange(150, device="cuda") != 4
+    assert torch.equal(dx[others], want[others])
+    assert torch.isnan(dx[4]).all() and torch.isnan(dw).all()
+
+
+def test_no_rows_of_a_large_gradient(K):
+    w = torch.zeros(1, 32768, dtype=torch.bfloat16, device="cuda").expand(140000, 32768)
+    x = torch.zeros(0, 32768, dtype=torch.bfloat16, device="cuda")
+    dw = torch.full((140000, 32768), 7.0, dtype=torch.bfloat16, device="cuda")
+    K.linear_xent_bwd(x, w, torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, device="cuda"), dw=dw)
+    assert not any(bool(dw[i:i + 20000].any()) for i in range(0, 140000, 20000))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_strides_offsets_and_outputs(K, dtype):
     """Views of any pitch and start give the same numbers; nothing is written past a row's end."""
@@ -347,7 +390,7 @@ def test_wrapper_refusals(K):
     lse = torch.zeros(8, device="cuda")
     for bad in (lambda: K.linear_xent(x.double(), w, labels), lambda: K.linear_xent(x, w.float(), labels),
                 lambda: K.linear_xent(x, w[:, :8], labels), lambda: K.linear_xent(x, w, labels[:4]),
-                lambda: K.linear_xent(x, w, labels.short()), lambda: K.linear_xent(x.t(), w, labels),
+                lambda: K.linear_xent(x, w, labels.short()), lambda: K.linear_xent(x, w, labels, ignore_index=2 ** 63), lambda: K.linear_xent(x.t(), w, labels),
                 lambda: K.linear_xent(x.cpu(), w, labels), lambda: K.linear_xent(x, w, labels.cpu()),
                 lambda: K.linear_xent(x, w, labels, workspace=torch.empty(8, dtype=torch.uint8, device="cuda")),
                 lambda: K.linear_xent_bwd(x, w, labels, lse[:4]), lambda: K.linear_xent_bwd(x, w, labels, lse.double()),

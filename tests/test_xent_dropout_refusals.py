@@ -45,12 +45,13 @@ def test_loss(lib):
     for name, off in (("x", 1), ("w", 1), ("labels", 2), ("out", 2), ("lse", 1), ("ws", 8)):
         _refused(lib, 1, "aligned", loss(**{name: P + off}))
     _refused(lib, 2, "tiles", loss(rows=(1 << 31) - 1, vocab=(1 << 31) - 1))
+    _refused(lib, 2, "tiles", loss(rows=1 << 30, vocab=2))
     assert loss(rows=0, x=None) == 0
 
 
 def test_gradient(lib):
     def grad(t=BF16, dt=BF16, rows=4, width=64, vocab=100, x=P, ldx=64, w=Q, ldw=64, lt=S64, labels=R, lse=R, rg=None,
-             dx=R, lddx=64, dw=R, lddw=64, ws=R):
+             dx=R, lddx=64, dw=2 * R, lddw=64, ws=R):
         return lib.mk_linear_xent_bwd(None, t, dt, rows, width, vocab, x, ldx, w, ldw, lt, labels, 0, 0, lse, rg, 1.0, dx,
                                       lddx, dw, lddw, ws)
 
@@ -66,6 +67,9 @@ def test_gradient(lib):
         _refused(lib, 1, "aligned", grad(**{name: P + off}))
     _refused(lib, 1, "over x", grad(dx=P))
     _refused(lib, 1, "over w", grad(dw=Q))
+    for kw in (dict(dx=Q), dict(dw=P), dict(dx=R, dw=R)):
+        _refused(lib, 1, "over", grad(**kw))
+    _refused(lib, 2, "tiles", grad(rows=(1 << 31) - 1, width=4096, vocab=2, ldx=4096, ldw=4096, lddx=4096, lddw=4096))
     assert grad(dx=None, dw=None) == 0
     assert grad(rows=0, dw=None) == 0
 
@@ -121,12 +125,15 @@ def test_dropout(lib):
         _refused(lib, 1, "aligned", fwd(**{name: P + 1}))
     _refused(lib, 1, "overlap", fwd(ldo=63))
     _refused(lib, 1, "pitch", fwd(ldx=-64))
+    _refused(lib, 1, "another pitch", fwd(out=P, ldx=72))
+    _refused(lib, 1, "another pitch", fwd(out=P, x=R, r=P, ldr=0))
     assert fwd(rows=0, x=None) == 0
     for name in ("dy", "dx", "ws"):
         _refused(lib, 1, "null", bwd(**{name: None}))
     for name, off in (("dy", 1), ("dx", 1), ("cs", 2), ("ws", 2)):
         _refused(lib, 1, "aligned", bwd(**{name: P + off}))
     _refused(lib, 1, "overlap", bwd(lddx=63))
+    _refused(lib, 1, "another pitch", bwd(dx=P, lddx=72))
     assert bwd(rows=0, cs=None) == 0
 
 
