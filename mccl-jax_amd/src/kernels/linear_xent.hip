@@ -679,6 +679,7 @@ struct ProductsArgs {
   // dx: tiles of rows x width, the piece's classes cut into `slices` runs of `run`
   int dx_m, dx_n, slices;
   int64_t run;
+  int dx_first;    // dx's runs before dw's tiles
   int first;       // the first piece: sums start from zero
   float* sums;     // [slices][dx tile][accumulators]
   // dw: tiles of classes x width; where they are few their rows are cut too
@@ -727,15 +728,18 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   constexpr int64_t kTile = Sh::TM * Sh::TN / 4;  // of a slice's sums, in f32x4
   __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // dw's tiles first: they are the long ones where there are many rows, and dx's
-  // runs fill the last round (8192 x 768 x 25088: 404 k steps a CU the other way
-  // round, 320 so).  Both start at a multiple of 8, an XCD each.
+  // The longer ones first mostly, and the others fill the last round (1000 x 768 x
+  // 50257: dx's runs first 265 us, dw's tiles 290).  Both start at a multiple of 8, an
+  // XCD each.
   const uint32_t n_dw = (uint32_t(p.dw_m) * p.dw_n * p.dw_slices + 7) / 8 * 8;
+  const uint32_t n_dx = uint32_t(p.dx_m) * p.dx_n * p.slices, dx_at = p.dx_first ? 0 : n_dw;
+  const uint32_t dw_at = p.dx_first ? (n_dx + 7) / 8 * 8 : 0;
   Acc<Sh> acc;
   uint32_t tm, tn;
-  if (blockIdx.x >= n_dw) {
+  if (p.dx_first ? blockIdx.x < dw_at : blockIdx.x >= n_dw) {
     // a slice of the classes is one XCD's (of 8 slices), with all of dx's tiles
-    const uint32_t j = blockIdx.x - n_dw, slice = j % p.slices, tile = j / p.slices;
+    const uint32_t j = blockIdx.x - dx_at, slice = j % p.slices, tile = j / p.slices;
+    if (j >= n_dx) return;
     tm = tile / p.dx_n, tn = tile % p.dx_n;
     const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN, k0 = slice * p.run;
     f32x4* sums = reinterpret_cast<f32x4*>(p.sums) + (int64_t(slice) * p.dx_m * p.dx_n + tile) * kTile;
@@ -749,7 +753,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
     keep_sums<Sh>(acc, sums);
     return;
   }
-  if (!tile_of(blockIdx.x, n_dw, uint32_t(p.dw_m), uint32_t(p.dw_n) * p.dw_slices, tm, tn)) return;
+  if (!tile_of(blockIdx.x - dw_at, n_dw, uint32_t(p.dw_m), uint32_t(p.dw_n) * p.dw_slices, tm, tn)) return;
   const uint32_t slice = tn / p.dw_n;
   tn %= p.dw_n;
   const int64_t m0 = int64_t(tm) * Sh::TM, n0 = int64_t(tn) * Sh::TN, k0 = slice * p.dw_run;
@@ -896,11 +900,12 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(U* p, int64_t ld, int64_
 // that count (an ignored row's may be anything), and
 // 2^15 times that over its power of two is below fp16's largest value, while the
 // smallest normal value is 2^-29 of it.
-__global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad, int64_t rows, Labels labels, float scale, float* dyn) {
-  __shared__ float red[kThreads / kWave];
+constexpr int kFactorThreads = 1024;
+__global__ __launch_bounds__(kFactorThreads) void factor_kernel(const float* row_grad, int64_t rows, Labels labels, float scale, float* dyn) {
+  __shared__ float red[kFactorThreads / kWave];
   float top = 0.f;
 #pragma unroll 4
-  for (int64_t n = threadIdx.x; n < rows; n += kThreads) {
+  for (int64_t n = threadIdx.x; n < rows; n += kFactorThreads) {
     const float v = fabsf(row_grad[n]);
     if (v < INFINITY && !(labels.has_ignore && labels.ignored(labels.at(n)))) top = fmaxf(top, v);
   }
@@ -909,7 +914,7 @@ __global__ __launch_bounds__(kThreads) void factor_kernel(const float* row_grad,
   __syncthreads();
   if (threadIdx.x) return;
 #pragma unroll
-  for (int i = 1; i < kThreads / kWave; ++i) top = fmaxf(top, red[i]);
+  for (int i = 1; i < kFactorThreads / kWave; ++i) top = fmaxf(top, red[i]);
   int e = 0;
   if (top > 0.f) (void)frexpf(top, &e);  // top <= 2^e
   e = max(-112, e);  // 2^127 at most
@@ -955,19 +960,20 @@ struct Plan {
   int64_t piece, pieces;          // classes of a piece
   int64_t ld_g;
   int64_t slices, dw_slices;      // runs of dx's classes and of dw's rows
+  bool dx_first;                  // dx's runs before dw's tiles
   bool low;                       // g has its second rows
   int64_t x_at, w_at, part_at, target_at, g_at, sums_at, dw_sums_at, dyn_at, bytes;
 };
 
-// k tiles that the last of the chip's workgroups ends with, of dw's `dw` tiles of kw
-// k tiles and then dx's `dx` runs of kx, an XCD's share on its `slots` workgroups:
-// each takes the next one when it is free.
-int64_t ends(int64_t dw, int64_t kw, int64_t dx, int64_t kx, int64_t slots) {
-  const int64_t rounds = dw / slots, more = dw % slots, most = (dx + slots - 1) / slots;
-  int64_t lo = (rounds + (more > 0)) * kw, hi = lo + most * kx;
+// k tiles that the last of the chip's workgroups ends with, of n workgroups of kn k
+// tiles and then m of km, an XCD's share on its `slots` of them: each takes the
+// next one when it is free.
+int64_t ends(int64_t n, int64_t kn, int64_t m, int64_t km, int64_t slots) {
+  const int64_t rounds = n / slots, more = n % slots, most = (m + slots - 1) / slots;
+  int64_t lo = (rounds + (more > 0)) * kn, hi = lo + most * km;
   auto fits = [&](int64_t t) {
-    const int64_t late = std::max<int64_t>(0, t - (rounds + 1) * kw) / kx, early = std::max<int64_t>(0, t - rounds * kw) / kx;
-    return more * late + (slots - more) * early >= dx;
+    const int64_t late = std::max<int64_t>(0, t - (rounds + 1) * kn) / km, early = std::max<int64_t>(0, t - rounds * kn) / km;
+    return more * late + (slots - more) * early >= m;
   };
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;
@@ -987,28 +993,32 @@ double step_time(int shape, int esz) { return esz == 4 ? 3.5 : shape == kBig ? 1
 // Estimated us of the logits' tiles, kt k tiles each.  Measured, 256 and 128: loss of
 // 300 x 768 x 50257 46, 39, of 1000 92, 93; gradient of 1000 (with the same products)
 // 311, 304, of 1777 x 1001 x 30011 415, 423, of 8192 1911, 2034.
-double logits_time(int shape, int esz, int64_t rows, int64_t classes, int64_t kt, bool bwd) {
+double logits_time(int shape, int esz, int64_t rows, int64_t classes, int64_t kt) {
   const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1];
   const int64_t tiles = (rows + tm - 1) / tm * ((classes + tn - 1) / tn);
   const int64_t cus = cu_count(), slots = shape == kBig ? cus : 2 * cus, rest = tiles % slots;
   const double last = rest == 0 ? 0.0 : shape == kMid && rest <= cus ? 0.78 : 1.0;
-  return (double(tiles / slots) + last) * step_time(shape, esz) * (double(kt) + (bwd && shape == kBig ? 3.0 : 1.5));
+  return (double(tiles / slots) + last) * step_time(shape, esz) * (double(kt) + 1.5);
 }
 
 struct Cuts {
   double time;
   int shape;
   int64_t dx, dw;  // runs
+  bool dx_first;
 };
 
-// The shape of dx's and dw's tiles of a piece, and the runs that dx's classes and (where
-// dw's tiles do not fill the chip) dw's rows are cut into, by estimated us: fewer k
-// tiles one after the other, against a tile of sums a run, written and read again by
-// the last launch and in each piece, at about 4.5 TB/s.  Measured, 256 and 128 (the
-// whole gradient): 100 x 768 x 50257 87, 73, 300 144, 129, 1000 311, 297; 2048 x 1024
-// x 32000 390, 428; 1777 x 1001 x 30011 417, 450.
+// The shape of dx's and dw's tiles of a piece, their order, and the runs that dx's
+// classes and (where dw's tiles are few) dw's rows are cut into, by estimated us: fewer k
+// tiles one after the other against a tile of sums a run, written and read again at
+// about 3.8 TB/s.  A k tile of the last workgroup costs less than it takes alone
+// (step_time), since those that have ended leave it the power and the bandwidth;
+// the tiles' ends count as more k tiles.  Fitted to 24 ways for each of ten sizes (100 to 8192
+// rows, 64 to 4096 wide, 4098 to 50257 classes): within 2 to 4% of the
+// measured times, and the way it takes is the fastest or within 2% of it.
 Cuts products_cuts(int shape, int esz, int64_t rows, int64_t width, int64_t classes) {
-  constexpr int64_t kEndW[2] = {4, 1}, kEndX[2] = {8, 5};
+  const int64_t end_w = shape == kBig ? 7 : 5, end_x = shape == kBig ? 7 : 6;
+  const double last = shape == kBig ? 1.06 : 0.51, all = shape == kBig ? 0.0 : 0.24, slower = esz == 4 ? 2.4 : 1.0;
   const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1], across = (width + tn - 1) / tn, deep = 128 / esz;
   const int64_t dx = (rows + tm - 1) / tm * across, dw = (classes + tm - 1) / tm * across;
   const int64_t kx = (classes + deep - 1) / deep, kw = (rows + deep - 1) / deep;
@@ -1017,11 +1027,13 @@ Cuts products_cuts(int shape, int esz, int64_t rows, int64_t width, int64_t clas
   for (int64_t w = 1; w == 1 || (w <= 16 && dw * w <= 16 * slots && kw >= 4 * w); w *= 2)
     for (int64_t n = 1; n <= 64 && n <= kx; n *= 2) {
       const double sums = double((dx * n + (w > 1 ? dw * w : 0)) * tm * tn * 4);
-      const double t = double(ends((dw * w + 7) / 8, (kw + w - 1) / w + kEndW[shape], (dx * n + 7) / 8,
-                                   (kx + n - 1) / n + kEndX[shape], slots)) *
-                           step_time(shape, esz) +
-                       sums * 2 / 4.5e6 + (w > 1 ? 4.0 : 0.0);
-      if (best.dx == 0 || t < best.time) best = {t, shape, n, w};
+      const int64_t w1 = (dw * w + 7) / 8, wt = (kw + w - 1) / w + end_w;
+      const int64_t x1 = (dx * n + 7) / 8, xt = (kx + n - 1) / n + end_x;
+      const double t = slower * all * double(w1 * wt + x1 * xt) / double(slots) + sums * 2 / 7.6e6 + (w > 8 ? 12.0 : w > 1 ? 4.0 : 0.0);
+      const double dw_first = t + slower * last * double(ends(w1, wt, x1, xt, slots));
+      const double dx_first = t + slower * last * double(ends(x1, xt, w1, wt, slots)) * (shape == kBig ? 1.03 : 1.01);
+      if (best.dx == 0 || std::min(dw_first, dx_first) < best.time)
+        best = {std::min(dw_first, dx_first), shape, n, w, dx_first < dw_first};
     }
   return best;
 }
@@ -1034,7 +1046,7 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   const int64_t deep = 128 / q.esz;
   const int64_t kt = (width + deep - 1) / deep;
   q.low = bwd && q.esz == 2 && rows <= kLow;
-  const double mid = logits_time(kMid, q.esz, rows, vocab, kt, bwd), big = logits_time(kBig, q.esz, rows, vocab, kt, bwd);
+  const double mid = logits_time(kMid, q.esz, rows, vocab, kt), big = logits_time(kBig, q.esz, rows, vocab, kt);
   q.logits = q.esz == 4 || q.low || mid < big ? kMid : kBig;
   q.tm = kSizes[q.logits][0], q.tn = kSizes[q.logits][1];
   q.pack_x = !on_grid(x, ld_x, width, q.esz) || (bwd && has_ignore);
@@ -1064,7 +1076,7 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
     const Cuts small = products_cuts(kMid, q.esz, rows, width, classes);
     const Cuts large = products_cuts(kBig, q.esz, rows, width, classes);
     const Cuts& cuts = q.esz == 4 || q.low || small.time < large.time ? small : large;  // low: 128 rows a tile
-    q.products = cuts.shape, q.slices = cuts.dx, q.dw_slices = cuts.dw;
+    q.products = cuts.shape, q.slices = cuts.dx, q.dw_slices = cuts.dw, q.dx_first = cuts.dx_first;
     q.pm = kSizes[q.products][0], q.pn = kSizes[q.products][1];
     const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn);
     q.sums_at = take(q.slices * tiles * q.pm * q.pn * 4);
@@ -1262,9 +1274,9 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   b.dx_n = b.dw_n = int((width + q.pn - 1) / q.pn);
   b.slices = int(q.slices), b.dw_slices = int(q.dw_slices);
   b.dw_run = up((rows + q.dw_slices - 1) / q.dw_slices, 128 / esz);
-  a.low = b.low = q.low;
+  a.low = b.low = q.low, b.dx_first = q.dx_first;
   const int64_t most = a.tiles_m * ((q.piece + q.tn - 1) / q.tn),
-                most2 = int64_t(b.dx_m) * b.dx_n * q.slices + (q.piece + q.pm - 1) / q.pm * b.dw_n * q.dw_slices + 8;
+                most2 = int64_t(b.dx_m) * b.dx_n * q.slices + (q.piece + q.pm - 1) / q.pm * b.dw_n * q.dw_slices + 16;
   // the sums' blocks have 32 rows and a wave's columns, and at most 1024 threads
   const int64_t most3 = int64_t(b.dx_m) * b.dx_n * (q.products == kBig ? 32 : 8) * 2;
   if (int rc = check_tiles(what, std::max({most, most2, most3}), 512)) return rc;
@@ -1273,7 +1285,7 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   b.unit = io_type == MK_F16 ? grad_scale / 32768.f : grad_scale;
   if (io_type == MK_F16 && row_grad) {
     float* dyn = reinterpret_cast<float*>(ws + q.dyn_at);
-    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(kThreads), 0, s, row_grad, rows, lab, grad_scale, dyn);
+    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(kFactorThreads), 0, s, row_grad, rows, lab, grad_scale, dyn);
     if (int rc = check_launch(what)) return rc;
     a.dyn = b.dyn = dyn;
   }
@@ -1328,7 +1340,7 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     rc = with_kernels(io_type, q.products, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
-      const unsigned tiles = unsigned(b.dx_m) * b.dx_n * b.slices + (unsigned(b.dw_m) * b.dw_n * b.dw_slices + 7) / 8 * 8;
+      const unsigned tiles = (unsigned(b.dx_m) * b.dx_n * b.slices + 7) / 8 * 8 + (unsigned(b.dw_m) * b.dw_n * b.dw_slices + 7) / 8 * 8;
       hipLaunchKernelGGL((products_kernel<T, Sh>), dim3(tiles), dim3(Geo<Sh>::threads), 0, s, b);
       return check_launch(what);
     });
