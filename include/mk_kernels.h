@@ -610,12 +610,13 @@ int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t width, int64
  * row_grad (fp32 [rows]) may be NULL (1).  grad_scale = 1 / rows gives the
  * gradient of the mean loss.  With has_ignore, rows whose label is
  * ignore_index have a gradient of 0 and add nothing to dw, whatever their x
- * holds.  g is formed in pieces of the vocabulary and rounded to io_type (before
- * grad_scale; for MK_F16 scaled by powers of two out of the subnormals), the
- * operand of the products with w and x; their sums are fp32, in a fixed order:
- * the same inputs give the same bits.  dx is of io_type, dw of dw_type (io_type
- * or MK_F32); either may be NULL, then only the other is computed.  dx may not
- * overlap x, nor dw w.  Workspace as above. */
+ * and row_grad hold.  g is formed in pieces of the vocabulary and rounded to io_type
+ * (before grad_scale; for MK_F16 scaled by powers of two out of the subnormals), the
+ * operand of the products with w and x; up to 64 rows keep what that rounding
+ * leaves as a second operand.  Sums are fp32, in a fixed order: the same inputs
+ * give the same bits.  dx is of io_type, dw of dw_type (io_type or MK_F32);
+ * either may be NULL, then only the other is computed.  dx and dw may overlap neither
+ * x, w nor each other.  Workspace as above. */
 size_t mk_linear_xent_bwd_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
                                           int64_t ld_x, const void* w, int64_t ld_w, int has_ignore);
 int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_t rows, int64_t width, int64_t vocab,

@@ -19,6 +19,11 @@
 // is CT chunks wide (a power of two that wastes little of the last tile) and 256 /
 // CT rows high.  Sums of columns go through LDS, then as one partial row a block to
 // the workspace, and a second launch adds the partial rows in order.
+//
+// Memory bounds the large ones: 20011 x 4097 fp32 116 us (5.7 TB/s of the bytes read
+// and written, some of them in the last-level cache; a copy 5.4).  8192 x 768 bf16 with
+// bias and residual 7.3 us (5.2 TB/s), its gradient 11.5 with the sums, of which 2 are
+// the second launch.  64 x 768 is a launch: 2.4 us on the GPU, 7 with the call.
 #include "mk_common.h"
 
 #include <algorithm>

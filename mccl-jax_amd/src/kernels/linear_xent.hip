@@ -11,7 +11,15 @@
 // a row's tiles.  Backward, piece by piece of the vocabulary: the same product
 // again, ending with g in the operands' type (a matrix product reads it next;
 // its rounding is as small as that of the gradients themselves, and it is formed
-// from fp32 logits), then dx and dw of the piece in one launch.
+// from fp32 logits), then dx and dw of the piece in one launch.  g is the only
+// large thing that goes through memory, 512 MB at a time.
+//
+// Many rows are bound by the matrix rate: 8192 x 768 x 50257 bf16 takes 553 us
+// forward (1.14 PFLOP/s; the library's product of the logits alone 597) and 1823
+// backward (three products, 1.04 PFLOP/s; the library's three 2008, without the
+// softmax), 8192 x 4096 x 65536 10.8 ms backward (1.22).  Twelve k tiles of 768 are short
+// beside a tile's end.  Few rows are bound by w: 16 rows of it 20 us forward (16 us
+// of products, 4.8 TB/s), 100 rows 67 backward, where w is read twice and dw written.
 // The products are tiles as in gemm_tiled.hip (copies HBM -> LDS, two stages, k
 // tiles of 128 bytes a row); fp32 operands take the same bytes and the fp32 MFMA.
 // Operand bases move along k in 64 bits, so no operand's size is limited by a
@@ -985,14 +993,13 @@ int64_t ends(int64_t n, int64_t kn, int64_t m, int64_t km, int64_t slots) {
 
 // Tile shapes: a k tile of 256 x 256 takes 1.75 us on a CU, one of 128 x 128 with
 // another beside it on the CU 1.12 us, alone 0.78 of that; of 32 bits what the fp32
-// MFMA takes.  A tile's begin and end count as more k tiles: fitted to both shapes'
-// times on the cases below.
+// MFMA takes.  A tile's begin and end count as more k tiles.
 constexpr int64_t kSizes[2][2] = {{256, 256}, {128, 128}};
 double step_time(int shape, int esz) { return esz == 4 ? 3.5 : shape == kBig ? 1.75 : 1.12; }
 
 // Estimated us of the logits' tiles, kt k tiles each.  Measured, 256 and 128: loss of
-// 300 x 768 x 50257 46, 39, of 1000 92, 93; gradient of 1000 (with the same products)
-// 311, 304, of 1777 x 1001 x 30011 415, 423, of 8192 1911, 2034.
+// 300 x 768 x 50257 46, 39, of 1000 92, 93; gradient of 300 (with the same products)
+// 136, 129, of 1000 293, 302, of 2048 x 1024 x 32000 374, 413, of 187 x 2409 x 4098 94, 69.
 double logits_time(int shape, int esz, int64_t rows, int64_t classes, int64_t kt) {
   const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1];
   const int64_t tiles = (rows + tm - 1) / tm * ((classes + tn - 1) / tn);
