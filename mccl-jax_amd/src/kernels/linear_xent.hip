@@ -8,7 +8,7 @@
 //
 // Forward: one product, tile by tile; a tile ends with each of its rows' maximum
 // and sum of exponentials (8 bytes a row for TN logits), and a second launch joins
-// a row's tiles.  Backward, piece by piece of the vocabulary: the same product
+// a row's tiles.  Up to 32 rows have kernels of their own.  Backward, piece by piece of the vocabulary: the same product
 // again, ending with g in the operands' type (a matrix product reads it next;
 // its rounding is as small as that of the gradients themselves, and it is formed
 // from fp32 logits), then dx and dw of the piece in one launch.  g is the only
@@ -18,7 +18,7 @@
 // forward (1.14 PFLOP/s; the library's product of the logits alone 597) and 1823
 // backward (three products, 1.04 PFLOP/s; the library's three 2008, without the
 // softmax), 8192 x 4096 x 65536 10.8 ms backward (1.22).  Twelve k tiles of 768 are short
-// beside a tile's end.  Few rows are bound by w: 16 rows of it 20 us forward (16 us
+// beside a tile's end.  Few rows are bound by w: 16 rows of it 20.7 us forward (16 us
 // of products, 4.8 TB/s), 100 rows 67 backward, where w is read twice and dw written.
 // The products are tiles as in gemm_tiled.hip (copies HBM -> LDS, two stages, k
 // tiles of 128 bytes a row); fp32 operands take the same bytes and the fp32 MFMA.
@@ -29,6 +29,7 @@
 #include <cmath>
 #include <numeric>
 #include <string>
+#include <type_traits>
 
 #include "gemm_tile.h"
 
@@ -345,21 +346,22 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void loss_kernel(const LossArg
   }
 }
 
-// A row's tiles joined: 16 rows a block, 16 threads a row over the tiles, 8 of
-// them loaded at a time (one after the other a row's 393 tiles took 9 us).
-__global__ __launch_bounds__(kThreads) void loss_final_kernel(const float2* part, const float* target, int64_t rows,
+// A row's tiles joined: 16 rows a block, 16 threads a row over the tiles (64 where there are
+// few rows), 8 of them loaded at a time (one after the other a row's 393 tiles took 9 us).
+template <int NT>
+__global__ __launch_bounds__(16 * NT) void loss_final_kernel(const float2* part, const float* target, int64_t rows,
                                                               int64_t vocab, int64_t tiles, Labels labels, float* loss,
                                                               float* lse) {
   constexpr int kAt = 8;
-  __shared__ float2 red[16][16];
+  __shared__ float2 red[NT / 4][16];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int64_t n = int64_t(blockIdx.x) * 16 + tx;
   float top = -INFINITY, sum = 0.f;
   if (n < rows) {
-    for (int64_t t = ty; t < tiles; t += 16 * kAt) {
+    for (int64_t t = ty; t < tiles; t += NT * kAt) {
       float2 v[kAt];
 #pragma unroll
-      for (int i = 0; i < kAt; ++i) v[i] = t + 16 * i < tiles ? part[(t + 16 * i) * rows + n] : float2{-INFINITY, 0.f};
+      for (int i = 0; i < kAt; ++i) v[i] = t + NT * i < tiles ? part[(t + NT * i) * rows + n] : float2{-INFINITY, 0.f};
       float to = top;
 #pragma unroll
       for (int i = 0; i < kAt; ++i) to = fmaxf(to, v[i].x);
@@ -370,20 +372,67 @@ __global__ __launch_bounds__(kThreads) void loss_final_kernel(const float2* part
       top = to;
     }
   }
-  red[ty][tx] = float2{top, sum};
+  // 4 of them are lanes of a wave
+#pragma unroll
+  for (int d = 16; d < 64; d *= 2) {
+    const float t = __shfl_xor(top, d), more = __shfl_xor(sum, d), to = fmaxf(top, t), from = to == -INFINITY ? 0.f : to;
+    const float mine = sum * __builtin_amdgcn_exp2f(top - from), its = more * __builtin_amdgcn_exp2f(t - from);
+    sum = mine + its;  // the same in both lanes
+    top = to;
+  }
+  if (ty % 4 == 0) red[ty / 4][tx] = float2{top, sum};
   __syncthreads();
   if (ty != 0 || n >= rows) return;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, red[i][tx].x);
+  for (int i = 1; i < NT / 4; ++i) top = fmaxf(top, red[i][tx].x);
   const float from = top == -INFINITY ? 0.f : top;
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum += red[i][tx].y * __builtin_amdgcn_exp2f(red[i][tx].x - from);
+  for (int i = 0; i < NT / 4; ++i) sum += red[i][tx].y * __builtin_amdgcn_exp2f(red[i][tx].x - from);
   const float z = (top + log2f(sum)) * kLn2;
   if (lse) lse[n] = z;
   if (!loss) return;
   const int64_t label = labels.at(n);
   loss[n] = labels.ignored(label) ? 0.f : (label >= 0 && label < vocab ? z - target[n] : z);
+}
+
+// ---------------------------------------------------------------- operands off the 16-byte boundaries
+// Rows copied to a pitch of whole 16-byte chunks with zeros past their end, and
+// (has_ignore) zeros for ignored rows, which g's zeros would not keep out of dw
+// if they held infinities.  again > 0: every `again` rows anew, zeros past `held` of them.
+struct PackArgs {
+  const void* src;
+  int64_t ld, rows, cols;
+  void* dst;
+  int64_t ld_dst;
+  Labels labels;
+  int64_t held;
+  int again;
+};
+template <typename U, int THREADS>
+__device__ inline void pack_block(const PackArgs& p, int64_t block) {
+  constexpr int kE = 16 / int(sizeof(U));
+  struct __attribute__((packed, aligned(sizeof(U)))) Any { U v[kE]; };  // 16 bytes at any element
+  struct alignas(16) Chunk { U v[kE]; };
+  const int64_t chunks = p.ld_dst / kE, first = block * THREADS;
+  const uint32_t in = uint32_t(first % chunks) + threadIdx.x;
+  const int64_t to = first / chunks + in / uint32_t(chunks), col = int64_t(in % uint32_t(chunks)) * kE;
+  const int64_t row = p.again ? to % p.again : to;
+  if (to >= p.rows) return;
+  const U* src = static_cast<const U*>(p.src) + row * p.ld + col;
+  Chunk c;
+  if (row >= p.held || (p.labels.has_ignore && p.labels.ignored(p.labels.at(row)))) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) c.v[e] = U(0);
+  } else if (col + kE <= p.cols) {
+    const Any l = *reinterpret_cast<const Any*>(src);
+#pragma unroll
+    for (int e = 0; e < kE; ++e) c.v[e] = l.v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) c.v[e] = col + e < p.cols ? src[e] : U(0);
+  }
+  *reinterpret_cast<Chunk*>(static_cast<U*>(p.dst) + to * p.ld_dst + col) = c;
 }
 
 // ---------------------------------------------------------------- backward: g
@@ -399,6 +448,7 @@ struct GradArgs {
   char* g;           // [rows][ld_g], columns past vocab up to a whole chunk are zeros
   int64_t ld_g;
   int low;           // what g's rounding leaves goes to the rows kLow further on
+  PackArgs pack;     // of few rows: dw's x, by the workgroups past the tiles
 };
 
 __device__ inline uint32_t pack2(Bf16, float a, float b) {
@@ -407,6 +457,7 @@ __device__ inline uint32_t pack2(Bf16, float a, float b) {
 __device__ inline uint32_t pack2(F16, float a, float b) { return uint32_t(f32_to_f16(a)) | (uint32_t(f32_to_f16(b)) << 16); }
 
 __device__ inline float rounded(Bf16, float a) { return bf16_to_f32(f32_to_bf16(a)); }
+__device__ inline float rounded(F32, float a) { return a; }
 __device__ inline float rounded(F16, float a) { return f16_to_f32(f32_to_f16(a)); }
 
 // 16 bits: the 8 columns 32 b + 16 h + 8 g .. + 7 of a lane's row 32 a + c as one
@@ -425,6 +476,27 @@ __device__ __attribute__((always_inline)) inline u32x4_t chunk16(int a, int b, i
   const auto s1 = __builtin_amdgcn_permlane32_swap(w[0].y, w[1].y, false, false);
   return u32x4_t{static_cast<uint32_t>(s0[0]), static_cast<uint32_t>(s1[0]), static_cast<uint32_t>(s0[1]),
                  static_cast<uint32_t>(s1[1])};
+}
+
+// 16 bytes at an element's alignment: one instruction, whatever the address
+template <class T> using Elem = std::conditional_t<T::esz == 2, uint16_t, uint32_t>;
+template <class T> struct __attribute__((packed, aligned(sizeof(Elem<T>)))) Loose { u32x4_t v; };
+template <class T>
+__device__ inline u32x4_t loose16(const char* p) {
+  return reinterpret_cast<const Loose<T>*>(p)->v;
+}
+// The same to a row's elements, of which `left` are inside.
+template <class T>
+__device__ inline void store_chunk(char* to, const u32x4_t& v, int64_t left) {
+  constexpr int kE = 16 / T::esz;
+  if (left >= kE) {
+    reinterpret_cast<Loose<T>*>(to)->v = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kE; ++e)
+    if (e < left)
+      reinterpret_cast<Elem<T>*>(to)[e] = T::esz == 2 ? Elem<T>(v[e / 2] >> 16 * (e & 1)) : Elem<T>(v[e % 4]);
 }
 
 // A tile of 16-bit results, whole chunks of rows (cols a multiple of 8), through a part of
@@ -461,11 +533,11 @@ __device__ __attribute__((always_inline)) inline void store16_wave(char* lds, in
   }
 }
 
-// The same through LDS (gemm_tiled.hip's store_staged): rows go out in runs, as whole
-// chunks or (vec false) element by element.
+// A tile of 16-bit results of any alignment through LDS (gemm_tiled.hip's
+// store_staged): rows go out in runs of 16 bytes.
 template <class T, class Sh, class V>
 __device__ __attribute__((always_inline)) inline void store16(char* lds, int wave, int lane, char* out, int64_t ld,
-                                                              int64_t rows, int64_t cols, bool vec, V&& value) {
+                                                              int64_t rows, int64_t cols, V&& value) {
   using G = Geo<Sh>;
   constexpr int kCpr = Sh::TN / 8;
   static_assert(kCpr % 16 == 0, "staging rows of whole 16-chunk groups");
@@ -483,27 +555,19 @@ __device__ __attribute__((always_inline)) inline void store16(char* lds, int wav
       }
   }
   lds_barrier();
-  if (vec) {
 #pragma unroll 4
-    for (int it = 0; it < Sh::TM * kCpr / G::threads; ++it) {
-      const int e = it * G::threads + int(threadIdx.x), row = e / kCpr, cn = e % kCpr;
-      const u32x4_t v = *reinterpret_cast<const u32x4_t*>(st + row * Sh::TN + 8 * (cn ^ (row & 15)));
-      if (row < rows && 8 * cn < cols) *reinterpret_cast<u32x4_t*>(out + (row * ld + 8 * cn) * 2) = v;
-    }
-  } else {
-    for (int it = 0; it < Sh::TM * Sh::TN / G::threads; ++it) {
-      const int e = it * G::threads + int(threadIdx.x), row = e / Sh::TN, col = e % Sh::TN;
-      const uint16_t v = st[row * Sh::TN + 8 * ((col >> 3) ^ (row & 15)) + (col & 7)];
-      if (row < rows && col < cols) reinterpret_cast<uint16_t*>(out)[row * ld + col] = v;
-    }
+  for (int it = 0; it < Sh::TM * kCpr / G::threads; ++it) {
+    const int e = it * G::threads + int(threadIdx.x), row = e / kCpr, cn = e % kCpr;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(st + row * Sh::TN + 8 * (cn ^ (row & 15)));
+    if (row < rows) store_chunk<T>(out + (row * ld + 8 * cn) * 2, v, cols - 8 * cn);
   }
 }
 
-// A tile of fp32 results straight from the accumulators: 16 bytes a lane (two
-// lanes' are neighbours), or (vec false) element by element.
+// A tile of fp32 results of any alignment straight from the accumulators: 16 bytes a
+// lane (two lanes' are neighbours).
 template <class Sh, class V>
 __device__ __attribute__((always_inline)) inline void store32(int wave, int lane, float* out, int64_t ld,
-                                                              int64_t rows, int64_t cols, bool vec, V&& value) {
+                                                              int64_t rows, int64_t cols, V&& value) {
   using G = Geo<Sh>;
   const int wm = wave / Sh::WGN, wn = wave % Sh::WGN, c = lane & 31, g = lane >> 5;
 #pragma unroll
@@ -516,15 +580,9 @@ __device__ __attribute__((always_inline)) inline void store32(int wave, int lane
         const int nl = wn * G::WN + 32 * b + 8 * rg + 4 * g;
         float v[4];
         value(a, b, rg, v);
-        float* to = out + ml * ld + nl;
-        if (ml >= rows) continue;
-        if (vec && nl + 4 <= cols) {
-          *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (nl + q < cols) to[q] = v[q];
-        }
+        if (ml < rows)
+          store_chunk<F32>(reinterpret_cast<char*>(out + ml * ld + nl),
+                           __builtin_bit_cast(u32x4_t, f32x4{{v[0], v[1], v[2], v[3]}}), cols - nl);
       }
   }
 }
@@ -673,7 +731,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
         }
       }
     } else {
-      store32<Sh>(wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, true, value);
+      store32<Sh>(wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, value);
     }
     if (!kOn || i >= nt) return;
   }
@@ -697,7 +755,7 @@ struct ProductsArgs {
   int low;         // g has its second rows
   char* dw;        // the piece's rows
   int64_t ld_dw;
-  int dw_f32, dw_vec;
+  int dw_f32;
   const float* dyn;
   float unit;      // factor of dw
 };
@@ -786,11 +844,11 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   const int64_t rows = p.vocab - m0, cols = p.width - n0;
   if constexpr (T::esz == 2) {
     if (!p.dw_f32) {
-      store16<T, Sh>(lds, wave, lane, p.dw + (m0 * p.ld_dw + n0) * 2, p.ld_dw, rows, cols, p.dw_vec, value);
+      store16<T, Sh>(lds, wave, lane, p.dw + (m0 * p.ld_dw + n0) * 2, p.ld_dw, rows, cols, value);
       return;
     }
   }
-  store32<Sh>(wave, lane, reinterpret_cast<float*>(p.dw) + m0 * p.ld_dw + n0, p.ld_dw, rows, cols, p.dw_vec, value);
+  store32<Sh>(wave, lane, reinterpret_cast<float*>(p.dw) + m0 * p.ld_dw + n0, p.ld_dw, rows, cols, value);
 }
 
 // dx, or dw = the slices' sums times the factor.  A block has the 32 rows x WN columns of
@@ -806,7 +864,6 @@ struct SumsArgs {
   float unit;
   char* out;
   int64_t ld;
-  int vec;
 };
 
 template <class T, class Sh, int NG>
@@ -857,9 +914,10 @@ __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
       v[e] *= f;
     }
     char* to = p.out + (m * p.ld + n) * T::esz;
-    if (p.vec && n + 4 <= p.width) {
-      if constexpr (T::esz == 2) *reinterpret_cast<uint2*>(to) = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
-      else *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
+    if (n + 4 <= p.width) {
+      struct __attribute__((packed, aligned(sizeof(Elem<T>)))) Half { uint2 v; };
+      if constexpr (T::esz == 2) reinterpret_cast<Half*>(to)->v = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
+      else store_chunk<T>(to, __builtin_bit_cast(u32x4_t, f32x4{{v[0], v[1], v[2], v[3]}}), 4);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -868,34 +926,286 @@ __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
   }
 }
 
-// ---------------------------------------------------------------- operands off the 16-byte boundaries
-// Rows copied to a pitch of whole 16-byte chunks with zeros past their end, and
-// (has_ignore) zeros for ignored rows, which g's zeros would not keep out of dw
-// if they held infinities.
-template <typename U>
-__global__ __launch_bounds__(kThreads) void pack_kernel(const U* src, int64_t ld, int64_t rows, int64_t cols, U* dst,
-                                                        int64_t ld_dst, Labels labels) {
-  constexpr int kE = 16 / int(sizeof(U));
-  struct __attribute__((packed, aligned(sizeof(U)))) Loose { U v[kE]; };  // 16 bytes at any element
-  struct alignas(16) Chunk { U v[kE]; };
-  const int64_t chunks = ld_dst / kE, first = int64_t(blockIdx.x) * kThreads;
-  const uint32_t in = uint32_t(first % chunks) + threadIdx.x;
-  const int64_t row = first / chunks + in / uint32_t(chunks), col = int64_t(in % uint32_t(chunks)) * kE;
-  if (row >= rows) return;
-  Chunk c;
-  if (labels.has_ignore && labels.ignored(labels.at(row))) {
+// ---------------------------------------------------------------- few rows
+// Up to 32 rows: one MFMA block of them, so that a call is the reading of w, and a tile of
+// 128 rows would have most of the matrix rate for nothing (fp32) and, of few
+// classes, few workgroups.  The waves of a workgroup share the k of their tile, each
+// with a part of LDS that no barrier guards, and w is read where it lies, whatever its
+// alignment; their accumulators are added through LDS.  Measured, tiles of 128
+// rows and here: forward 1 x 3680 x 1313 bf16 31 us, 15; 6 x 3686 x 16342 fp32 313, 59;
+// 8 x 769 x 50257 bf16 52, 30; 1 x 4096 x 65536 127, 117; 16 x 768 x 50257 20.2, 20.7;
+// backward of the second 574, 242, of the last 61, 61.
+constexpr int kThinRows = 32, kThinClasses = 64;
+
+// the same of a row of `n` elements from element `at` on, zeros past its end
+template <class T>
+__device__ inline u32x4_t row_end16(const char* row, int64_t at, int64_t n) {
+  constexpr int kE = 16 / T::esz;
+  if (at + kE <= n) return loose16<T>(row + at * T::esz);
+  struct alignas(16) { Elem<T> v[kE]; } c;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) c.v[e] = U(0);
-  } else if (col + kE <= cols) {
-    const Loose l = *reinterpret_cast<const Loose*>(src + row * ld + col);
-#pragma unroll
-    for (int e = 0; e < kE; ++e) c.v[e] = l.v[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < kE; ++e) c.v[e] = col + e < cols ? src[row * ld + col + e] : U(0);
-  }
-  *reinterpret_cast<Chunk*>(dst + row * ld_dst + col) = c;
+  for (int e = 0; e < kE; ++e) c.v[e] = at + e < n ? reinterpret_cast<const Elem<T>*>(row)[at + e] : Elem<T>(0);
+  return __builtin_bit_cast(u32x4_t, c);
 }
+
+// The accumulators of two blocks of W waves, added: wave q gets quads q, q + W .. of 8,
+// quad t the four columns 32 (t / 4) + 8 (t % 4) + 4 g .. + 3 of row lane % 32.
+template <int W>
+struct ThinSums { f32x4 v[W][8][64]; };
+template <int W>
+__device__ __attribute__((always_inline)) inline void join_waves(ThinSums<W>& red, const f32x16_t& a, const f32x16_t& b,
+                                                                 int wave, int lane, f32x4 (&s)[8 / W]) {
+#pragma unroll
+  for (int rg = 0; rg < 4; ++rg) {
+    red.v[wave][rg][lane] = f32x4{{a[4 * rg], a[4 * rg + 1], a[4 * rg + 2], a[4 * rg + 3]}};
+    red.v[wave][4 + rg][lane] = f32x4{{b[4 * rg], b[4 * rg + 1], b[4 * rg + 2], b[4 * rg + 3]}};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8 / W; ++i) {
+    s[i] = red.v[0][wave + W * i][lane];
+#pragma unroll
+    for (int q = 1; q < W; ++q) {
+      const f32x4 v = red.v[q][wave + W * i][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i].v[e] += v.v[e];
+    }
+  }
+}
+
+// The logits of 64 classes, and their end: LossArgs, each row's maximum and sum; GradArgs, g.
+template <class T, int W, class Args>
+__global__ __launch_bounds__(64 * W) void thin_logits_kernel(const Args p) {
+  constexpr int kE = 16 / T::esz, kChunk = 8 * kE;  // 128 bytes of a row
+  constexpr int kRows = kThinRows + kThinClasses;  // of a wave's part of LDS, a chunk each
+  __shared__ __attribute__((aligned(16))) char lds[W * kRows * 128];
+  static_assert(sizeof(ThinSums<W>) <= sizeof(lds), "the sums lie where the operands were");
+  if constexpr (std::is_same_v<Args, GradArgs>) {
+    if (int(blockIdx.x) >= p.tiles_n) {
+      pack_block<Elem<T>, 64 * W>(p.pack, int(blockIdx.x) - p.tiles_n);
+      return;
+    }
+  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, g = lane >> 5;
+  const int64_t v0 = int64_t(blockIdx.x) * kThinClasses;
+  // 8 lanes a row load whole lines (lanes as the MFMA has them would load 32 bytes of
+  // 32 lines: 94 us against 70 for 247 MB of w); the wave's own LDS turns them
+  const int part = lane & 7, sub = lane >> 3;
+  const char* from[kRows / 8];
+#pragma unroll
+  for (int i = 0; i < kRows / 8; ++i)
+    from[i] = i < kThinRows / 8 ? p.x + min(int64_t(8 * i + sub), p.rows - 1) * p.ld_x * T::esz
+                                : p.w + min(v0 + 8 * i - kThinRows + sub, p.vocab - 1) * p.ld_w * T::esz;
+  u32x4_t next[kRows / 8];
+  auto load = [&](int64_t k) __attribute__((always_inline)) {
+    if (k + kChunk <= p.width) {
+#pragma unroll
+      for (int i = 0; i < kRows / 8; ++i) next[i] = loose16<T>(from[i] + (k + part * kE) * T::esz);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRows / 8; ++i) next[i] = row_end16<T>(from[i], k + part * kE, p.width);
+    }
+  };
+  f32x16_t acc[2];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[0][r] = acc[1][r] = 0.f;
+  char* st = lds + wave * (kRows * 128);
+  int64_t k = int64_t(wave) * kChunk;
+  if (k < p.width) load(k);
+  while (k < p.width) {
+#pragma unroll
+    for (int i = 0; i < kRows / 8; ++i)
+      *reinterpret_cast<u32x4_t*>(st + (8 * i + sub) * 128 + 16 * (part ^ sub)) = next[i];
+    k += W * kChunk;
+    if (k < p.width) load(k);
+    asm volatile("" ::: "memory");  // what another lane of the wave wrote: LDS is in order
+    auto read = [&](int row, int s) __attribute__((always_inline)) {
+      return *reinterpret_cast<const u32x4_t*>(st + (row + c) * 128 + 16 * ((2 * s + g) ^ (c & 7)));
+    };
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const u32x4_t a = read(0, s);
+      acc[0] = T::mma(read(kThinRows, s), a, acc[0]);
+      acc[1] = T::mma(read(kThinRows + 32, s), a, acc[1]);
+    }
+    asm volatile("" ::: "memory");
+  }
+  __syncthreads();
+  ThinSums<W>& red = *reinterpret_cast<ThinSums<W>*>(lds);
+  f32x4 sums[8 / W];
+  join_waves<W>(red, acc[0], acc[1], wave, lane, sums);
+  const int64_t label = c < p.rows ? p.labels.at(c) : -1;
+  if constexpr (std::is_same_v<Args, LossArgs>) {
+    __shared__ float2 ends[8][32];
+#pragma unroll
+    for (int i = 0; i < 8 / W; ++i) {
+      const int t = wave + W * i;
+      const int64_t col = v0 + 32 * (t / 4) + 8 * (t % 4) + 4 * g, left = p.vocab - col, at = label - p.v0 - col;
+      f32x4& z = sums[i];
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e >= left) z.v[e] = -INFINITY;
+        else if (c < p.rows && at == e) p.target[c] = z.v[e];
+        top = fmaxf(top, z.v[e]);
+      }
+      float lo, hi;
+      lane_halves_sched(top, lo, hi);
+      top = fmaxf(lo, hi);
+      const float t2 = top * kLog2e, from = t2 == -INFINITY ? 0.f : t2;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(fmaf(z.v[e], kLog2e, -from));
+      lane_halves_sched(sum, lo, hi);
+      if (g == 0) ends[t][c] = float2{t2, lo + hi};
+    }
+    __syncthreads();
+    if (int(threadIdx.x) >= p.rows) return;
+    float most = -INFINITY, all = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) most = fmaxf(most, ends[q][threadIdx.x].x);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      all += ends[q][threadIdx.x].y * __builtin_amdgcn_exp2f(ends[q][threadIdx.x].x - (most == -INFINITY ? 0.f : most));
+    p.part[int64_t(blockIdx.x) * p.rows + threadIdx.x] = float2{most, all};
+  } else {
+    // 16 bits: all of the 64 rows are written, what the rounding leaves 32 rows further on:
+    // they are one k tile of dw
+    const bool here = c < p.rows;
+    if (!here && T::esz == 4) return;
+    const float lse = here ? p.lse[c] : 0.f, from = -lse * kLog2e;
+    const float factor = here ? (p.dyn ? p.dyn[0] : p.unit) * (p.row_grad ? p.row_grad[c] : 1.f) : 0.f;
+    const bool none = !here || p.labels.ignored(label);
+#pragma unroll
+    for (int i = 0; i < 8 / W; ++i) {
+      const int t = wave + W * i;
+      const int64_t col = v0 + 32 * (t / 4) + 8 * (t % 4) + 4 * g, left = p.vocab - col, at = label - p.v0 - col;
+      float v[4], rest[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float z = sums[i].v[e];
+        v[e] = __builtin_amdgcn_exp2f(T::esz == 4 ? (z - lse) * kLog2e : fmaf(z, kLog2e, from));
+        if (at == e) v[e] -= 1.f;
+        v[e] = none || e >= left ? 0.f : v[e] * factor;  // whole tiles are written, zeros past the classes
+        rest[e] = v[e] - rounded(T{}, v[e]);
+      }
+      char* to = p.g + (c * p.ld_g + col) * T::esz;
+      if constexpr (T::esz == 2) {
+        *reinterpret_cast<uint2*>(to) = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
+        *reinterpret_cast<uint2*>(to + kThinRows * p.ld_g * 2) =
+            uint2{pack2(T{}, rest[0], rest[1]), pack2(T{}, rest[2], rest[3])};
+      } else {
+        *reinterpret_cast<f32x4*>(to) = f32x4{{v[0], v[1], v[2], v[3]}};
+      }
+    }
+  }
+}
+
+// dx: a workgroup has a run of classes and 32 chunks of 16 bytes of w's rows (256 columns
+// of 16 bits, 128 of 32).  A lane takes a chunk from each of the kE classes its
+// half of an MFMA step has, and a block of the MFMA is element j of all lanes' chunks:
+// turning them by kE x kE is two bytes picked from two registers each (16 bits), or
+// nothing (32 bits).
+struct ThinDxArgs {
+  const char *g, *w;
+  int64_t rows, width, vocab;  // vocab: of this piece
+  int64_t ld_g, ld_w;
+  int slices;
+  int64_t run;
+  int first;
+  float* sums;  // [slices][groups of columns][j][4][64 lanes][4]
+};
+
+template <class T>
+__global__ __launch_bounds__(512, 2) void thin_dx_kernel(const ThinDxArgs p) {
+  constexpr int kE = 16 / T::esz, kStep = 2 * kE, W = 8;
+  __shared__ ThinSums<W> red;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, g = lane >> 5;
+  const uint32_t slice = blockIdx.x % p.slices, group = blockIdx.x / p.slices;
+  const int64_t col = (int64_t(group) * 32 + c) * kE, k0 = slice * p.run, k1 = min(k0 + p.run, p.vocab);
+  const char* ga = p.g + min(int64_t(c), p.rows - 1) * p.ld_g * T::esz;
+  f32x16_t acc[kE];
+#pragma unroll
+  for (int j = 0; j < kE; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+  for (int64_t k = k0 + wave * kStep; k < k1; k += W * kStep) {
+    const int64_t v = k + kE * g;
+    u32x4_t raw[kE];
+    const char* w = p.w + v * p.ld_w * T::esz;
+    if (k + kStep <= p.vocab && col + kE <= p.width) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) raw[e] = loose16<T>(w + (e * p.ld_w + col) * T::esz);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        raw[e] = v + e < p.vocab ? row_end16<T>(w + e * p.ld_w * T::esz, col, p.width) : u32x4_t{0, 0, 0, 0};
+    }
+    const u32x4_t a = *reinterpret_cast<const u32x4_t*>(ga + v * T::esz);
+    u32x4_t low = a;
+    if constexpr (T::esz == 2) low = *reinterpret_cast<const u32x4_t*>(ga + (kThinRows * p.ld_g + v) * 2);
+#pragma unroll
+    for (int j = 0; j < kE; ++j) {
+      u32x4_t b;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if constexpr (T::esz == 2) b[h] = __builtin_amdgcn_perm(raw[2 * h + 1][j / 2], raw[2 * h][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+        else b[h] = raw[h][j];
+      }
+      acc[j] = T::mma(b, a, acc[j]);
+      if constexpr (T::esz == 2) acc[j] = T::mma(b, low, acc[j]);
+    }
+  }
+  f32x4* to = reinterpret_cast<f32x4*>(p.sums) + (int64_t(slice) * (gridDim.x / p.slices) + group) * kE * 256;
+#pragma unroll
+  for (int j = 0; j < kE; j += 2) {
+    f32x4 sum[1];
+    join_waves<W>(red, acc[j], acc[j + 1], wave, lane, sum);
+    f32x4& s = sum[0];
+    f32x4* at = to + (4 * j + wave) * 64 + lane;
+    if (!p.first) {
+      const f32x4 v = *at;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
+    }
+    *at = s;
+    __syncthreads();
+  }
+}
+
+// The slices' sums, 16 runs of them in order, times the factor, to dx.
+template <class T>
+__global__ __launch_bounds__(1024) void thin_sums_kernel(const SumsArgs p) {
+  constexpr int kE = 16 / T::esz;
+  __shared__ f32x4 red[16][64];
+  const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const int64_t all = int64_t(p.tiles_n) * kE * 256;  // f32x4 of a slice
+  const f32x4* at = reinterpret_cast<const f32x4*>(p.sums) + int64_t(blockIdx.x) * 64 + lane;
+  f32x4 s = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 4
+  for (int i = q; i < p.slices; i += 16) {
+    const f32x4 v = at[i * all];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s.v[e] += v.v[e];
+  }
+  red[q][lane] = s;
+  __syncthreads();
+  const int row = lane & 31, g = lane >> 5, rg = blockIdx.x % 4, j = blockIdx.x / 4 % kE;
+  if (q > 0 || row >= p.rows) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s.v[e] += red[i][lane].v[e];
+  const float f = p.dyn ? p.dyn[1] : p.unit;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t col = (int64_t(blockIdx.x / (4 * kE)) * 32 + 8 * rg + 4 * g + e) * kE + j;
+    if (col < p.width) store_from_f32(p.out + row * p.ld * T::esz, col, T::mk, s.v[e] * f);
+  }
+}
+
+template <typename U>
+__global__ __launch_bounds__(kThreads) void pack_kernel(const PackArgs p) { pack_block<U, kThreads>(p, blockIdx.x); }
 
 // rows x cols of zeros (words of U): the gradient of no rows
 template <typename U>
@@ -969,6 +1279,7 @@ struct Plan {
   int64_t ld_g;
   int64_t slices, dw_slices;      // runs of dx's classes and of dw's rows
   bool dx_first;                  // dx's runs before dw's tiles
+  bool thin, twice;               // the kernels of few rows; their g and x have 64 rows
   bool low;                       // g has its second rows
   int64_t x_at, w_at, part_at, target_at, g_at, sums_at, dw_sums_at, dyn_at, bytes;
 };
@@ -1052,12 +1363,15 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   q.rows = rows, q.width = width, q.vocab = vocab;
   const int64_t deep = 128 / q.esz;
   const int64_t kt = (width + deep - 1) / deep;
-  q.low = bwd && q.esz == 2 && rows <= kLow;
+  q.thin = rows <= kThinRows;
+  q.low = bwd && q.esz == 2 && rows <= kLow && !q.thin;
   const double mid = logits_time(kMid, q.esz, rows, vocab, kt), big = logits_time(kBig, q.esz, rows, vocab, kt);
   q.logits = q.esz == 4 || q.low || mid < big ? kMid : kBig;
-  q.tm = kSizes[q.logits][0], q.tn = kSizes[q.logits][1];
-  q.pack_x = !on_grid(x, ld_x, width, q.esz) || (bwd && has_ignore);
-  q.pack_w = !on_grid(w, ld_w, width, q.esz);
+  q.tm = q.thin ? kThinRows : kSizes[q.logits][0], q.tn = q.thin ? kThinClasses : kSizes[q.logits][1];
+  // few rows are read as they lie, but by dw's tiles (16 bits: twice, beside both rows of g)
+  q.twice = q.thin && bwd && q.esz == 2;
+  q.pack_x = q.thin && !bwd ? false : q.twice || !on_grid(x, ld_x, width, q.esz) || (bwd && has_ignore);
+  q.pack_w = !q.thin && !on_grid(w, ld_w, width, q.esz);
   q.pitch = up(width, 16 / q.esz);
   int64_t most = vocab;
   if (q.pack_w) most = std::min(most, std::max<int64_t>(q.tn, kPackBytes / (q.pitch * q.esz)));
@@ -1071,7 +1385,8 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   q.pieces = (vocab + q.piece - 1) / q.piece;
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t here = at; at += align256(bytes); return here; };
-  if (q.pack_x) q.x_at = take(rows * q.pitch * q.esz);
+  const int64_t kept = q.twice ? 2 * kThinRows : rows;
+  if (q.pack_x) q.x_at = take(kept * q.pitch * q.esz);
   if (q.pack_w) q.w_at = take(std::min(vocab, q.piece) * q.pitch * q.esz);
   if (!bwd) {
     q.part_at = take(((vocab + q.tn - 1) / q.tn + q.pieces) * rows * 8);
@@ -1079,14 +1394,19 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   } else {
     const int64_t classes = std::min(vocab, q.piece);
     q.ld_g = up(classes, 64);
-    q.g_at = take((rows + (q.low ? kLow : 0)) * q.ld_g * q.esz);
+    q.g_at = take((kept + (q.low ? kLow : 0)) * q.ld_g * q.esz);
     const Cuts small = products_cuts(kMid, q.esz, rows, width, classes);
     const Cuts large = products_cuts(kBig, q.esz, rows, width, classes);
-    const Cuts& cuts = q.esz == 4 || q.low || small.time < large.time ? small : large;  // low: 128 rows a tile
+    const Cuts& cuts = q.esz == 4 || rows <= kLow || small.time < large.time ? small : large;  // low: 128 rows a tile
     q.products = cuts.shape, q.slices = cuts.dx, q.dw_slices = cuts.dw, q.dx_first = cuts.dx_first;
     q.pm = kSizes[q.products][0], q.pn = kSizes[q.products][1];
-    const int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn);
-    q.sums_at = take(q.slices * tiles * q.pm * q.pn * 4);
+    int64_t tiles = (rows + q.pm - 1) / q.pm * ((width + q.pn - 1) / q.pn) * q.pm * q.pn;
+    if (q.thin) {  // a workgroup a CU, or 8 MFMA steps of its waves
+      const int64_t columns = 512 / q.esz, groups = (width + columns - 1) / columns, step = 8 * 32 / q.esz;
+      q.slices = std::max<int64_t>(1, std::min(cu_count() / groups, (classes + step - 1) / step));
+      tiles = groups * kThinRows * columns;
+    }
+    q.sums_at = take(q.slices * tiles * 4);
     if (q.dw_slices > 1)
       q.dw_sums_at = take(q.dw_slices * ((classes + q.pm - 1) / q.pm) * ((width + q.pn - 1) / q.pn) * q.pm * q.pn * 4);
     q.dyn_at = take(8);
@@ -1118,17 +1438,12 @@ int check_tiles(const std::string& what, int64_t tiles, int threads) {
   return MK_OK;
 }
 
-int pack(const char* what, hipStream_t s, const Plan& q, const void* src, int64_t ld, int64_t rows, char* dst,
-         const Labels& labels) {
-  const int64_t blocks = (rows * (q.pitch * q.esz / 16) + kThreads - 1) / kThreads;
+int pack(const char* what, hipStream_t s, const Plan& q, const PackArgs& p) {
+  const int64_t blocks = (p.rows * (p.ld_dst * q.esz / 16) + kThreads - 1) / kThreads;
   if (int rc = check_tiles(what, blocks, kThreads)) return rc;
   const dim3 g{unsigned(blocks)}, b{kThreads};
-  if (q.esz == 2)
-    hipLaunchKernelGGL(pack_kernel<uint16_t>, g, b, 0, s, static_cast<const uint16_t*>(src), ld, rows, q.width,
-                       reinterpret_cast<uint16_t*>(dst), q.pitch, labels);
-  else
-    hipLaunchKernelGGL(pack_kernel<uint32_t>, g, b, 0, s, static_cast<const uint32_t*>(src), ld, rows, q.width,
-                       reinterpret_cast<uint32_t*>(dst), q.pitch, labels);
+  if (q.esz == 2) hipLaunchKernelGGL(pack_kernel<uint16_t>, g, b, 0, s, p);
+  else hipLaunchKernelGGL(pack_kernel<uint32_t>, g, b, 0, s, p);
   return check_launch(what);
 }
 
@@ -1157,6 +1472,19 @@ template <class F>
 int with_results(int to, int shape, F&& f) {
   if (to == MK_F32) return with_shape(F32{}, shape, f);
   return with_kernels(to, shape, f);
+}
+
+// 4 waves a tile where the tiles fill the chip, else 8
+template <class T, class Args>
+int thin_logits(const char* what, hipStream_t s, const Args& a) {
+  const int waves = a.tiles_n > 2 * cu_count() ? 4 : 8;
+  int64_t more = 0;
+  if constexpr (std::is_same_v<Args, GradArgs>)
+    if (a.v0 == 0) more = (a.pack.rows * (a.pack.ld_dst * T::esz / 16) + 64 * waves - 1) / (64 * waves);
+  const dim3 g{unsigned(a.tiles_n + more)}, b{unsigned(64 * waves)};
+  if (waves == 4) hipLaunchKernelGGL((thin_logits_kernel<T, 4, Args>), g, b, 0, s, a);
+  else hipLaunchKernelGGL((thin_logits_kernel<T, 8, Args>), g, b, 0, s, a);
+  return check_launch(what);
 }
 
 }  // namespace
@@ -1195,7 +1523,7 @@ extern "C" int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t w
   a.tiles_m = int((rows + q.tm - 1) / q.tm);
   if (int rc = check_tiles(what, std::max(a.tiles_m * ((q.piece + q.tn - 1) / q.tn), (rows + 15) / 16), 512)) return rc;
   if (q.pack_x) {
-    if (int rc = pack(what, s, q, x, ld_x, rows, ws + q.x_at, Labels{})) return rc;
+    if (int rc = pack(what, s, q, {x, ld_x, rows, width, ws + q.x_at, q.pitch, Labels{}, rows, 0})) return rc;
     a.x = ws + q.x_at, a.ld_x = q.pitch;
   }
   const float2* part = a.part;
@@ -1205,13 +1533,16 @@ extern "C" int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t w
     a.vocab = std::min(q.piece, vocab - v0);
     a.w = static_cast<const char*>(w) + v0 * ld_w * esz, a.ld_w = ld_w;
     if (q.pack_w) {
-      if (int rc = pack(what, s, q, a.w, ld_w, a.vocab, ws + q.w_at, Labels{})) return rc;
+      if (int rc = pack(what, s, q, {a.w, ld_w, a.vocab, width, ws + q.w_at, q.pitch, Labels{}, a.vocab, 0})) return rc;
       a.w = ws + q.w_at, a.ld_w = q.pitch;
     }
     a.tiles_n = int((a.vocab + q.tn - 1) / q.tn);
     const int rc = with_kernels(io_type, q.logits, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
+      if (q.thin) {
+        return thin_logits<T>(what, s, a);
+      }
       hipLaunchKernelGGL((loss_kernel<T, Sh>), dim3(resident<Sh>(int64_t(a.tiles_m) * a.tiles_n)), dim3(Geo<Sh>::threads),
                          0, s, a);
       return check_launch(what);
@@ -1220,8 +1551,13 @@ extern "C" int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t w
     a.part += a.tiles_n * rows;
     tiles += a.tiles_n;
   }
-  hipLaunchKernelGGL(loss_final_kernel, dim3(unsigned((rows + 15) / 16)), dim3(kThreads), 0, s, part, a.target, rows, vocab,
-                     tiles, a.labels, loss_rows, lse);
+  const dim3 joins{unsigned((rows + 15) / 16)};
+  if (rows <= 1024)
+    hipLaunchKernelGGL(loss_final_kernel<64>, joins, dim3(1024), 0, s, part, a.target, rows, vocab, tiles, a.labels,
+                       loss_rows, lse);
+  else
+    hipLaunchKernelGGL(loss_final_kernel<16>, joins, dim3(256), 0, s, part, a.target, rows, vocab, tiles, a.labels,
+                       loss_rows, lse);
   return check_launch(what);
 }
 
@@ -1271,16 +1607,17 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   const Labels lab = {labels, label_type == MK_S64, has_ignore != 0, ignore_index};
   GradArgs a{};
   ProductsArgs b{};
-  a.rows = b.rows = rows, a.width = b.width = width;
+  a.rows = rows, b.rows = q.twice ? 2 * kThinRows : rows, a.width = b.width = width;
   a.labels = lab;
   a.lse = lse, a.row_grad = row_grad;
   a.x = static_cast<const char*>(x), a.ld_x = ld_x;
   a.g = ws + q.g_at, a.ld_g = q.ld_g;
   a.tiles_m = int((rows + q.tm - 1) / q.tm);
-  b.dx_m = dx ? int((rows + q.pm - 1) / q.pm) : 0;
+  b.dx_m = dx && !q.thin ? int((rows + q.pm - 1) / q.pm) : 0;
   b.dx_n = b.dw_n = int((width + q.pn - 1) / q.pn);
+  const int64_t thin_groups = (width + 512 / esz - 1) / (512 / esz);
   b.slices = int(q.slices), b.dw_slices = int(q.dw_slices);
-  b.dw_run = up((rows + q.dw_slices - 1) / q.dw_slices, 128 / esz);
+  b.dw_run = up((b.rows + q.dw_slices - 1) / q.dw_slices, 128 / esz);
   a.low = b.low = q.low, b.dx_first = q.dx_first;
   const int64_t most = a.tiles_m * ((q.piece + q.tn - 1) / q.tn),
                 most2 = int64_t(b.dx_m) * b.dx_n * q.slices + (q.piece + q.pm - 1) / q.pm * b.dw_n * q.dw_slices + 16;
@@ -1296,16 +1633,21 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     if (int rc = check_launch(what)) return rc;
     a.dyn = b.dyn = dyn;
   }
-  if (q.pack_x) {
-    if (int rc = pack(what, s, q, x, ld_x, rows, ws + q.x_at, lab)) return rc;
-    a.x = ws + q.x_at, a.ld_x = q.pitch;
-  }
   b.g = a.g, b.ld_g = a.ld_g;
   b.x = a.x, b.ld_x = a.ld_x;
+  if (q.pack_x) {
+    const PackArgs c{x, ld_x, b.rows, width, ws + q.x_at, q.pitch, lab, rows, q.twice ? kThinRows : 0};
+    b.x = ws + q.x_at, b.ld_x = q.pitch;
+    if (q.thin) {
+      a.pack = c;
+    } else {
+      if (int rc = pack(what, s, q, c)) return rc;
+      a.x = b.x, a.ld_x = b.ld_x;
+    }
+  }
   b.sums = reinterpret_cast<float*>(ws + q.sums_at), b.dw_sums = reinterpret_cast<float*>(ws + q.dw_sums_at);
   b.dw_f32 = dw_type == MK_F32;
   b.ld_dw = ld_dw;
-  b.dw_vec = (reinterpret_cast<uintptr_t>(dw) & 15u) == 0 && ld_dw * dwsz % 16 == 0 && width * esz % 16 == 0;
   // the sums of slices, dx's or a piece's dw's, into rows of type `to`
   auto join = [&](int to, const SumsArgs& c) {
     return with_results(to, q.products, [&](auto t, auto sh) {
@@ -1317,15 +1659,12 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
       return check_launch(what);
     });
   };
-  auto vec4 = [](const void* p, int64_t ld, int bytes) {
-    return int(reinterpret_cast<uintptr_t>(p) % (4 * bytes) == 0 && ld % 4 == 0);
-  };
   for (int64_t v0 = 0; v0 < vocab; v0 += q.piece) {
     a.v0 = v0;
     a.vocab = b.vocab = std::min(q.piece, vocab - v0);
     a.w = static_cast<const char*>(w) + v0 * ld_w * esz, a.ld_w = ld_w;
     if (q.pack_w) {
-      if (int rc = pack(what, s, q, a.w, ld_w, a.vocab, ws + q.w_at, Labels{})) return rc;
+      if (int rc = pack(what, s, q, {a.w, ld_w, a.vocab, width, ws + q.w_at, q.pitch, Labels{}, a.vocab, 0})) return rc;
       a.w = ws + q.w_at, a.ld_w = q.pitch;
     }
     b.w = a.w, b.ld_w = a.ld_w;
@@ -1338,12 +1677,26 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     int rc = with_kernels(io_type, q.logits, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
+      if (q.thin) {
+        return thin_logits<T>(what, s, a);
+      }
       const int64_t tiles = int64_t(a.tiles_m) * a.tiles_n;
       hipLaunchKernelGGL((grad_kernel<T, Sh>), dim3(q.logits == kBig ? resident<Sh>(tiles) : unsigned(tiles)),
                          dim3(Geo<Sh>::threads), 0, s, a);
       return check_launch(what);
     });
     if (rc) return rc;
+    if (dx && q.thin) {
+      const ThinDxArgs c{b.g, b.w, rows, width, b.vocab, b.ld_g, b.ld_w, b.slices, up((a.vocab + q.slices - 1) / q.slices, 8 * 32 / esz),
+                         b.first, b.sums};
+      rc = with_kernels(io_type, q.products, [&](auto t, auto) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(thin_dx_kernel<T>, dim3(unsigned(thin_groups * q.slices)), dim3(512), 0, s, c);
+        return check_launch(what);
+      });
+      if (rc) return rc;
+    }
+    if (q.thin && !dw) continue;
     rc = with_kernels(io_type, q.products, [&](auto t, auto sh) {
       using T = decltype(t);
       using Sh = decltype(sh);
@@ -1353,12 +1706,19 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     });
     if (rc) return rc;
     if (dw && b.dw_slices > 1) {
-      const SumsArgs c{b.dw_sums, b.vocab, width, b.dw_m, b.dw_n, b.dw_slices, 0, b.dyn, b.unit, b.dw, ld_dw,
-                       vec4(b.dw, ld_dw, dwsz)};
+      const SumsArgs c{b.dw_sums, b.vocab, width, b.dw_m, b.dw_n, b.dw_slices, 0, b.dyn, b.unit, b.dw, ld_dw};
       if (int r = join(dw_type, c)) return r;
     }
   }
   if (!dx) return MK_OK;
+  if (q.thin) {
+    const SumsArgs c{b.sums, rows, width, 1, int(thin_groups), b.slices, 0, b.dyn, b.unit, static_cast<char*>(dx), ld_dx};
+    return with_kernels(io_type, q.products, [&](auto t, auto) {
+      using T = decltype(t);
+      hipLaunchKernelGGL(thin_sums_kernel<T>, dim3(unsigned(thin_groups) * (64 / T::esz)), dim3(1024), 0, s, c);
+      return check_launch(what);
+    });
+  }
   return join(io_type, SumsArgs{b.sums, rows, width, b.dx_m, b.dx_n, b.slices, b.low, b.dyn, b.unit,
-                                static_cast<char*>(dx), ld_dx, vec4(dx, ld_dx, esz)});
+                                static_cast<char*>(dx), ld_dx});
 }

@@ -211,6 +211,70 @@ def test_few_rows_keep_what_rounding_leaves(K, dtype, rows, width, vocab):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 5, 31, 32, 33])
+def test_up_to_32_rows(K, dtype, rows):
+    """The kernels of few rows: any pitch and start, ignored rows that hold anything, streams, graphs."""
+    for width, vocab in ((130, 1000), (64, 70), (520, 333)):
+        print(f"case: rows {rows} x {width} x {vocab} {dtype}", flush=True)
+        x, w, labels = _inputs(15, rows, width, vocab, dtype, torch.int64)
+        labels[-1] = vocab - 1
+        row_grad = torch.rand(rows, device="cuda") + 0.5
+        if rows > 1:
+            labels[0] = -100
+            row_grad[0] = float("nan")
+        clean = torch.where((labels != -100)[:, None], x, torch.zeros_like(x))
+        x = torch.where((labels != -100)[:, None], x, torch.full_like(x, float("inf")))
+        kept = labels != -100
+        loss, lse = K.linear_xent(x, w, labels, ignore_index=-100)
+        want, want_lse, bound = xent(clean, w, labels, -100)
+        _within(loss, want, bound, "loss")
+        _within(lse[kept], want_lse[kept], bound[kept], "lse")
+        dx, dw = K.linear_xent_bwd(x, w, labels, lse, grad_scale=0.5, row_grad=row_grad, ignore_index=-100,
+                                   dw_dtype=torch.float32)
+        wx, ww, bx, bw = xent_grad(clean, w, labels, torch.where(kept, lse, 0.0), 0.5,
+                                   torch.where(kept, row_grad, 0.0), -100, torch.float32, twice=dtype != torch.float32)
+        _within(dx, wx, bx, "dx")
+        _within(dw, ww, bw, "dw")
+        assert torch.all(dx[~kept] == 0)
+        for pitch, off in ((width + 1, 1), (width + 11, 3)):
+            def view(t):
+                sea = torch.full((t.shape[0] * pitch + off + 9,), float("nan"), dtype=t.dtype, device="cuda")
+                v = sea[off:off + t.shape[0] * pitch].view(t.shape[0], pitch)[:, :width]
+                v.copy_(t)
+                return sea, v
+
+            (_, xv), (_, wv) = view(x), view(w)
+            (sx, dxv), (sw, dwv) = view(torch.zeros_like(x)), view(torch.zeros(vocab, width, device="cuda"))
+            l2, z2 = K.linear_xent(xv, wv, labels, ignore_index=-100)
+            assert torch.equal(l2, loss) and torch.equal(z2[kept], lse[kept])
+            K.linear_xent_bwd(xv, wv, labels, lse, grad_scale=0.5, row_grad=row_grad, ignore_index=-100, dx=dxv, dw=dwv)
+            assert torch.equal(dxv, dx) and torch.equal(dwv, dw)
+            dxv.fill_(float("nan")), dwv.fill_(float("nan"))
+            assert torch.isnan(sx).all() and torch.isnan(sw).all()  # nothing past the rows' ends
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            l3, z3 = K.linear_xent(x, w, labels, ignore_index=-100)
+            d3 = K.linear_xent_bwd(x, w, labels, z3, grad_scale=0.5, row_grad=row_grad, ignore_index=-100,
+                                   dw_dtype=torch.float32)
+        for _ in range(3):
+            for t in (l3, z3, *d3):
+                t.zero_()
+            graph.replay()
+            eager = K.linear_xent(x, w, labels, ignore_index=-100, stream=torch.cuda.Stream())
+            torch.cuda.synchronize()
+            assert torch.equal(l3, loss) and torch.equal(eager[0], loss)
+            assert torch.equal(d3[0], dx) and torch.equal(d3[1], dw)
+
+
+def test_few_rows_of_more_classes_than_a_piece(K):
+    rows, width, vocab = 3, 8, (1 << 20) + 77
+    x, w, labels = _inputs(16, rows, width, vocab, torch.bfloat16)
+    labels[0], labels[1] = vocab - 1, 1 << 20
+    _check(K, x, w, labels, dw_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_many_rows_of_few_classes(K, dtype):
     """The weights' gradient has few tiles here: its rows are cut into runs."""
     for rows, width, vocab in ((4571, 64, 2148), (9001, 16, 300), (3000, 130, 2)):
