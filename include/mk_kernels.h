@@ -595,9 +595,9 @@ int mk_sdpa_bwd(void* stream, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int6
  * label is ignore_index have loss 0.  lse is each row's, ignored or not.
  * loss_rows and lse are fp32 [rows], either may be NULL.  The vocabulary is
  * gone through in tiles, of which the workspace holds each row's maximum and
- * sum.  Operands off the 16-byte boundaries (base, pitch or width) are copied
- * to them first, w piece by piece; the size of the workspace counts that, so
- * the pointers and pitches given to it are those of the call. */
+ * sum.  Operands of more than 32 rows off the 16-byte boundaries (base, pitch or
+ * width) are copied to them first, w piece by piece; the size of the workspace
+ * counts that, so the pointers and pitches given to it are those of the call. */
 size_t mk_linear_xent_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
                                       int64_t ld_x, const void* w, int64_t ld_w);
 int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x, int64_t ld_x,
