@@ -612,8 +612,9 @@ int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t width, int64
  * ignore_index have a gradient of 0 and add nothing to dw, whatever their x
  * and row_grad hold.  g is formed in pieces of the vocabulary and rounded to io_type
  * (before grad_scale; for MK_F16 scaled by powers of two out of the subnormals), the
- * operand of the products with w and x; up to 64 rows keep what that rounding
- * leaves as a second operand.  Sums are fp32, in a fixed order: the same inputs
+ * operand of the products with w and x.  What that rounding leaves of each row's label
+ * is added to both gradients; up to 64 rows keep what it leaves of every
+ * element as a second operand.  Sums are fp32, in a fixed order: the same inputs
  * give the same bits.  dx is of io_type, dw of dw_type (io_type or MK_F32);
  * either may be NULL, then only the other is computed.  dx and dw may overlap neither
  * x, w nor each other.  Workspace as above. */

@@ -8,11 +8,11 @@
 //
 // Forward: one product, tile by tile; a tile ends with each of its rows' maximum
 // and sum of exponentials (8 bytes a row for TN logits), and a second launch joins
-// a row's tiles.  Up to 32 rows have kernels of their own.  Backward, piece by piece of the vocabulary: the same product
-// again, ending with g in the operands' type (a matrix product reads it next;
-// its rounding is as small as that of the gradients themselves, and it is formed
-// from fp32 logits), then dx and dw of the piece in one launch.  g is the only
-// large thing that goes through memory, 512 MB at a time.
+// a row's tiles.  Up to 32 rows have kernels of their own.  Backward, piece by piece
+// of the vocabulary: the same product again, ending with g in the operands' type (a
+// matrix product reads it next; it is formed from fp32 logits, and what its rounding
+// leaves of the labels' elements is kept beside it), then dx and dw of the piece in
+// one launch.  g is the only large thing that goes through memory, 512 MB at a time.
 //
 // Many rows are bound by the matrix rate: 8192 x 768 x 50257 bf16 takes 553 us
 // forward (1.14 PFLOP/s; the library's product of the logits alone 597) and 1823
@@ -145,11 +145,30 @@ __device__ inline u32x4_t read_chunk(const char* t, int rb, int ks, int lane) {
   }
 }
 
+// ---------------------------------------------------------------- labels
+struct Labels {
+  const void* p;
+  int wide;  // int64
+  int has_ignore;
+  int64_t ignore;
+  __device__ inline int64_t at(int64_t n) const {
+    return wide ? static_cast<const int64_t*>(p)[n] : int64_t(static_cast<const int32_t*>(p)[n]);
+  }
+  __device__ inline bool ignored(int64_t label) const { return has_ignore && label == ignore; }
+};
+
 // acc += A B of one workgroup tile over K: the k loop of gemm_tiled.hip.  A wave
 // waits for its own copies of tile kt, the barrier publishes all and frees the
 // other stage, whose next copies are issued beside the first k-steps' MFMAs.
 // start() issues the first k tile's copies, into the first stage; run() ends with a
 // barrier: the operands' LDS is free, and start() of the next product may follow.
+// rest: what is added beside the operands' k tiles (LabelRest).
+struct NoRest {
+  __device__ inline void load(int) const {}
+  __device__ inline void take(int) const {}
+  template <class A>
+  __device__ inline void add(A&) const {}
+};
 template <class T, class Sh, bool AKC, bool BKC>
 struct Product {
   using G = Geo<Sh>;
@@ -176,14 +195,15 @@ struct Product {
   }
   // LATE: stores that may still be on their way when the first k tile is there (late: exactly
   // so many came after its copies)
-  template <int LATE = 0>
+  template <int LATE = 0, class Beside = NoRest>
   __device__ __attribute__((always_inline)) inline void run(char* lds, int wave, int lane, Acc<Sh>& acc,
-                                                            bool late = false) const {
+                                                            bool late = false, Beside&& rest = {}) const {
     const int wm = wave / Sh::WGN, wn = wave % Sh::WGN;
     for (int kt = 0; kt < nk; ++kt) {
       if (LATE > 0 && late && kt == 0) wait_vm<LATE>();
       else wait_vm<0>();
       lds_barrier();
+      rest.take(kt);
       const char* at = lds + (kt & 1) * G::stage;
       char* next = lds + ((kt + 1) & 1) * G::stage;
       const bool more = kt + 1 < nk;
@@ -195,11 +215,13 @@ struct Product {
 #pragma unroll
         for (int b = 0; b < G::J; ++b) bf[b] = read_chunk<T, BKC, Sh::TN, Sh::BK>(at + kA, wn * G::WN + 32 * b, ks, lane);
         if (more && ks < 2) issue(kt + 1, next, wave, lane, ks == 0, ks == 1);
+        if (more && ks == 1) rest.load(kt + 1);
 #pragma unroll
         for (int a = 0; a < G::I; ++a)
 #pragma unroll
           for (int b = 0; b < G::J; ++b) acc[a][b] = T::mma(bf[b], af[a], acc[a][b]);
       }
+      rest.add(acc);
     }
     lds_barrier();
   }
@@ -228,18 +250,6 @@ __device__ inline bool tile_of(uint32_t i, uint32_t nt, uint32_t tiles_m, uint32
   tn = in / gm;
   return t < tiles_m * tiles_n;
 }
-
-// ---------------------------------------------------------------- labels
-struct Labels {
-  const void* p;
-  int wide;  // int64
-  int has_ignore;
-  int64_t ignore;
-  __device__ inline int64_t at(int64_t n) const {
-    return wide ? static_cast<const int64_t*>(p)[n] : int64_t(static_cast<const int32_t*>(p)[n]);
-  }
-  __device__ inline bool ignored(int64_t label) const { return has_ignore && label == ignore; }
-};
 
 // ---------------------------------------------------------------- forward
 struct LossArgs {
@@ -436,10 +446,14 @@ __device__ inline void pack_block(const PackArgs& p, int64_t block) {
 }
 
 // ---------------------------------------------------------------- backward: g
+struct Rest {
+  int label;   // -1: outside the vocabulary, or the row is ignored
+  float left;  // what the rounding of g leaves of the label's element, in g's scale
+};
 struct GradArgs {
   const char *x, *w;
   int64_t rows, width, vocab;  // vocab: of this piece
-  int64_t ld_x, ld_w, v0;
+  int64_t ld_x, ld_w, v0, all;  // all: classes of the vocabulary
   int tiles_m, tiles_n;
   Labels labels;
   const float *lse, *row_grad;
@@ -448,6 +462,7 @@ struct GradArgs {
   char* g;           // [rows][ld_g], columns past vocab up to a whole chunk are zeros
   int64_t ld_g;
   int low;           // what g's rounding leaves goes to the rows kLow further on
+  Rest* rest;        // [rows] (16 bits without those rows), or null
   PackArgs pack;     // of few rows: dw's x, by the workgroups past the tiles
 };
 
@@ -455,6 +470,10 @@ __device__ inline uint32_t pack2(Bf16, float a, float b) {
   return uint32_t(f32_to_bf16(a)) | (uint32_t(f32_to_bf16(b)) << 16);
 }
 __device__ inline uint32_t pack2(F16, float a, float b) { return uint32_t(f32_to_f16(a)) | (uint32_t(f32_to_f16(b)) << 16); }
+
+// of the low 16 bits
+__device__ inline float widened(Bf16, uint32_t a) { return bf16_to_f32(uint16_t(a)); }
+__device__ inline float widened(F16, uint32_t a) { return f16_to_f32(uint16_t(a)); }
 
 __device__ inline float rounded(Bf16, float a) { return bf16_to_f32(f32_to_bf16(a)); }
 __device__ inline float rounded(F32, float a) { return a; }
@@ -587,11 +606,18 @@ __device__ __attribute__((always_inline)) inline void store32(int wave, int lane
   }
 }
 
-// Few rows are not averaged over: a class that one token alone has as its label gets
-// its gradient from one product, and the rounding of that one factor would be
-// the error of the whole row.  At most kLow rows have a second operand row each,
-// what the rounding of the first leaves; their tiles have the room (16 bits: half of
-// dx's 128 rows, and of dw's two k tiles the second), so that it costs nothing.
+// What the rounding of g to 16 bits leaves.  A row of g is its label's element, near
+// -1, and many small ones, and a class that one token has as its label gets its
+// gradient from that one product: the rounding of this element would be the error of
+// the whole rows of dx and dw.  So what it leaves of it is kept (Rest, fp32) and
+// added to both: to dw by its tiles (LabelRest), to dx where its sums are joined.  Errors
+// against 64 bits, without it and with it: 100 x 768 x 50257 bf16 0.00188, 0.00165; 1777
+// x 1001 x 30011 fp16 0.000279, 0.000207, both then those of fp32 products.  Times:
+// 8192 x 768 x 50257 1875 us, 1925; 1777 x 1001 x 30011 402, 416; 100 rows 69 either
+// way; of few classes, each with many labels, 2000 x 2048 x 1500 63, 72.  At most
+// kLow rows have a second operand row each, what the rounding leaves of every
+// element; their tiles have the room (16 bits: half of dx's 128 rows, and of dw's
+// two k tiles the second), so that it costs nothing.
 constexpr int kLow = 64;
 
 // 256 x 256: a workgroup has every gridDim-th tile, as in loss_kernel: the next
@@ -621,6 +647,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
   // of a tile's rows: lse, factor, the label's column of the tile or -1, or -2: the row is ignored
   __shared__ float row_lse[2][Sh::TM], row_factor[2][Sh::TM];
   __shared__ int row_rel[2][Sh::TM];
+  __shared__ float row_label[Sh::TM];  // the label's element without its factor, for the lane that had it
   static_assert(Sh::TM <= G::threads, "a thread a row");
   const int t = int(threadIdx.x);
   int64_t label;
@@ -646,6 +673,14 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
   now.start(lds, wave, lane);
   rows_load(m0);
   rows_keep(0, n0);
+  if constexpr (T::esz == 2) {
+    if (p.rest && p.v0 == 0) {
+      for (int64_t n = int64_t(blockIdx.x) * G::threads + t; n < p.rows; n += int64_t(gridDim.x) * G::threads) {
+        const int64_t l = p.labels.at(n);
+        p.rest[n].label = l >= 0 && l < p.all && !p.labels.ignored(l) ? int(l) : -1;
+      }
+    }
+  }
   bool late = false;
   int at = 0;
   for (uint32_t i = blockIdx.x;;) {
@@ -671,6 +706,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
     // by the few lanes that have one.
     const bool some = !__all(counts) || n_now + Sh::TN > p.vocab;
     const int64_t left = p.vocab - n_now - wn * G::WN - 4 * g;  // columns below it exist
+    bool found = false;  // a label's element
 #pragma unroll
     for (int a = 0; a < G::I; ++a) {
       const float lse = row_lse[at][wm * G::WM + 32 * a + c], from = -lse * kLog2e;
@@ -682,12 +718,13 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
           // 32-bit results: the difference first, which is exact where it is small
           acc[a][b][r] = __builtin_amdgcn_exp2f(T::esz == 4 ? (acc[a][b][r] - lse) * kLog2e
                                                             : fmaf(acc[a][b][r], kLog2e, from));
-      if (rel[a] >= 0 && mine >= 0 && mine < G::WN) {
+      if (rel[a] >= 0 && mine >= 0 && mine < G::WN && !(mine & 4)) {
+        found = true;
 #pragma unroll
         for (int b = 0; b < G::J; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (mine == 32 * b + 8 * (r / 4) + r % 4) acc[a][b][r] -= 1.f;
+            if (mine == 32 * b + 8 * (r / 4) + r % 4) row_label[wm * G::WM + 32 * a + c] = acc[a][b][r] -= 1.f;
       }
     }
     if (some) {
@@ -733,6 +770,17 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
     } else {
       store32<Sh>(wave, lane, reinterpret_cast<float*>(out), p.ld_g, rows, cols, value);
     }
+    if constexpr (T::esz == 2) {
+      if (p.rest && __any(found)) {  // now that the accumulators' registers are free
+#pragma unroll
+        for (int a = 0; a < G::I; ++a) {
+          const int row = wm * G::WM + 32 * a + c, rel_at = row_rel[at ^ 1][row], mine = rel_at - wn * G::WN - 4 * g;
+          if (rel_at < 0 || mine < 0 || mine >= G::WN || (mine & 4)) continue;
+          const float v = row_label[row] * row_factor[at ^ 1][row];
+          p.rest[m_now + row].left = v - rounded(T{}, v);
+        }
+      }
+    }
     if (!kOn || i >= nt) return;
   }
 }
@@ -753,6 +801,8 @@ struct ProductsArgs {
   int64_t dw_run;
   float* dw_sums;  // as sums, of more than one slice
   int low;         // g has its second rows
+  const Rest* rest;  // GradArgs' rest, or null
+  int64_t v0;        // the piece's first class
   char* dw;        // the piece's rows
   int64_t ld_dw;
   int dw_f32;
@@ -787,6 +837,85 @@ __device__ __attribute__((always_inline)) inline void take_sums(Acc<Sh>& acc, co
         for (int q = 0; q < 4; ++q) acc[a][b][4 * rg + q] = v.v[q];
       }
 }
+
+// dw's share of `rest`: row n adds left x[n] to its label's class.  A wave lists the rows
+// with a label in its classes as the k loop passes them (lane l has row l of a k tile's
+// 64), and multiplies 64 of them, or what there is at the end, as four more steps of
+// 16 rows: their x comes from memory as a lane needs it, and A holds each row's rest at
+// its label and zeros.  (Multiplied within the k tile that has them, dx's and dw's launch
+// of 8192 x 768 x 26624 took 34 us of 580 more, so 14: a wait is the whole workgroup's.)
+template <class T, class Sh>
+struct LabelRest {
+  using G = Geo<Sh>;
+  struct Entry {
+    int row;        // of the run
+    uint32_t part;  // its label's class of the wave's, and in the low half what is left, rounded to T
+  };
+  static constexpr int kMost = 128;  // 63 kept and a k tile's
+  Entry* list;       // in LDS, the wave's own
+  const Rest* rows;  // the run's first row; null: none (nor where the wave has no columns)
+  int64_t count;     // its rows
+  int first, classes;  // the wave's first class of the vocabulary, and those of its classes that are the piece's
+  const char* x;       // the run's first row of x, at the wave's first column
+  int64_t ld_x, cols;  // cols: those from there on
+  int lane;
+  Rest next;
+  int n = 0;
+  __device__ inline void load(int kt) {
+    const int64_t at = 64 * int64_t(kt) + lane;
+    next = Rest{-1, 0.f};
+    if (rows && at < count) next = rows[at];
+  }
+  __device__ inline void take(int kt) {
+    const unsigned at = unsigned(next.label) - unsigned(first);
+    const bool mine = next.label >= 0 && at < unsigned(classes);
+    const uint64_t all = __ballot(mine);
+    if (all == 0) return;
+    const int before = __builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0));
+    if (mine) list[n + before] = Entry{64 * kt + lane, at << 16 | (pack2(T{}, next.left, 0.f) & 0xFFFFu)};
+    n += __builtin_popcountll(all);
+  }
+  __device__ inline void add(Acc<Sh>& acc) {
+    if (n < 64) return;
+    multiply(64, acc);
+    list[lane] = list[64 + lane];
+    n -= 64;
+  }
+  __device__ __attribute__((always_inline)) inline void multiply(int most, Acc<Sh>& acc) const {
+    const int c = lane & 31, g = lane >> 5;
+    asm volatile("" ::: "memory");  // what other lanes listed: LDS is in order
+#pragma unroll 1
+    for (int k0 = 0; k0 < most; k0 += 16) {
+      uint32_t part[8], v[G::J][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int e = k0 + 8 * g + j;
+        const Entry at = list[min(e, most - 1)];
+        part[j] = e < most ? at.part : 0xFFFF0000u;  // no class
+        const uint16_t* row = reinterpret_cast<const uint16_t*>(x + int64_t(at.row) * ld_x * 2);
+#pragma unroll
+        for (int b = 0; b < G::J; ++b) v[b][j] = row[min(int64_t(32 * b + c), cols - 1)];
+      }
+      u32x4_t bf[G::J];
+#pragma unroll
+      for (int b = 0; b < G::J; ++b)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) bf[b][w] = v[b][2 * w] | v[b][2 * w + 1] << 16;
+#pragma unroll
+      for (int a = 0; a < G::I; ++a) {
+        u32x4_t af;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t mine = uint32_t(32 * a + c);
+          af[w] = (part[2 * w] >> 16 == mine ? part[2 * w] & 0xFFFFu : 0u) |
+                  (part[2 * w + 1] >> 16 == mine ? part[2 * w + 1] << 16 : 0u);
+        }
+#pragma unroll
+        for (int b = 0; b < G::J; ++b) acc[a][b] = T::mma(bf[b], af, acc[a][b]);
+      }
+    }
+  }
+};
 
 template <class T, class Sh>
 __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const ProductsArgs p) {
@@ -830,7 +959,18 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   static_assert(128 / Bf16::esz == kLow, "g's second rows are the second k tile");
   if (p.low) dw.twice();
   dw.start(lds, wave, lane);
-  dw.run(lds, wave, lane, acc);
+  if constexpr (T::esz == 2) {
+    using L = LabelRest<T, Sh>;
+    __shared__ typename L::Entry lists[G::W][L::kMost];
+    const int64_t c0 = m0 + wave / Sh::WGN * G::WM, d0 = n0 + wave % Sh::WGN * G::WN;
+    L rest{lists[wave], p.rest && d0 < p.width ? p.rest + k0 : nullptr, min(p.dw_run, p.rows - k0), int(p.v0 + c0),
+           int(max(int64_t(0), min(int64_t(G::WM), p.vocab - c0))), p.x + (k0 * p.ld_x + d0) * 2, p.ld_x, p.width - d0, lane};
+    rest.load(0);
+    dw.template run<0>(lds, wave, lane, acc, false, rest);
+    rest.multiply(rest.n, acc);
+  } else {
+    dw.run(lds, wave, lane, acc);
+  }
   if (p.dw_slices > 1) {
     keep_sums<Sh>(acc, reinterpret_cast<f32x4*>(p.dw_sums) +
                            ((int64_t(slice) * p.dw_m + tm) * p.dw_n + tn) * kTile);
@@ -864,6 +1004,9 @@ struct SumsArgs {
   float unit;
   char* out;
   int64_t ld;
+  const Rest* rest;  // of dx: what is left times w's row of the label is added (null: nothing)
+  const char* w;
+  int64_t ld_w;
 };
 
 template <class T, class Sh, int NG>
@@ -875,6 +1018,35 @@ __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n, tile = blockIdx.x / (G::W * G::I);
   const int part = int(blockIdx.x % (G::W * G::I)), wave = part / G::I, a = part % G::I;
   const f32x4* from = reinterpret_cast<const f32x4*>(p.sums) + tile * (Sh::TM * Sh::TN / 4);
+  const int64_t m0 = tile / p.tiles_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a;
+  const int64_t n0 = tile % p.tiles_n * Sh::TN + wave % Sh::WGN * G::WN;
+  // what a thread stores: 4 columns of a row each
+  constexpr int kItems = 32 * G::WN / 4, kMine = (kItems + kThreads * NG - 1) / (kThreads * NG);
+  struct __attribute__((packed, aligned(sizeof(Elem<T>)))) Half { uint2 v; };
+  Rest rest[kMine];
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) {
+    const int i = int(threadIdx.x) + q * kThreads * NG;
+    const int64_t m = m0 + i / (G::WN / 4);
+    rest[q] = Rest{-1, 0.f};
+    if (T::esz == 2 && p.rest && i < kItems && m < p.rows) rest[q] = p.rest[m];
+  }
+  uint32_t wrow[kMine][2];  // w's row of the label, 4 columns
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) {
+    wrow[q][0] = wrow[q][1] = 0;
+    const int64_t n = n0 + (int(threadIdx.x) + q * kThreads * NG) % (G::WN / 4) * 4;
+    if (T::esz != 2 || rest[q].label < 0 || n >= p.width) continue;
+    const char* w = p.w + (rest[q].label * p.ld_w + n) * T::esz;
+    if (n + 4 <= p.width) {
+      const uint2 v = reinterpret_cast<const Half*>(w)->v;
+      wrow[q][0] = v.x, wrow[q][1] = v.y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.width) wrow[q][e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(w)[e]) << (16 * (e & 1));
+    }
+  }
   // the waves kLow rows further on, in the same tile (128 rows, 32 a wave)
   const int64_t low = kLow / G::WM * Sh::WGN * 64;
 #pragma unroll
@@ -897,25 +1069,25 @@ __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
       lds[group * kSize + (lane & 31) * kPitch + 32 * (br >> 2) + 8 * (br & 3) + 4 * (lane >> 5) + e] = s.v[e];
   }
   __syncthreads();
-  const int64_t m0 = tile / p.tiles_n * Sh::TM + wave / Sh::WGN * G::WM + 32 * a;
-  const int64_t n0 = tile % p.tiles_n * Sh::TN + wave % Sh::WGN * G::WN;
   const float f = p.dyn ? p.dyn[1] : p.unit;
 #pragma unroll
-  for (int i = int(threadIdx.x); i < 32 * G::WN / 4; i += kThreads * NG) {
-    const int row = i / (G::WN / 4), col = i % (G::WN / 4) * 4;
+  for (int k = 0; k < kMine; ++k) {
+    const int i = int(threadIdx.x) + k * kThreads * NG, row = i / (G::WN / 4), col = i % (G::WN / 4) * 4;
     const int64_t m = m0 + row, n = n0 + col;
-    if (m >= p.rows || n >= p.width) continue;
+    if (i >= kItems || m >= p.rows || n >= p.width) continue;
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = lds[row * kPitch + col + e];
 #pragma unroll
       for (int q = 1; q < NG; ++q) v[e] += lds[q * kSize + row * kPitch + col + e];
+      if constexpr (T::esz == 2) {
+        if (rest[k].label >= 0) v[e] += rest[k].left * widened(T{}, wrow[k][e / 2] >> (16 * (e & 1)));
+      }
       v[e] *= f;
     }
     char* to = p.out + (m * p.ld + n) * T::esz;
     if (n + 4 <= p.width) {
-      struct __attribute__((packed, aligned(sizeof(Elem<T>)))) Half { uint2 v; };
       if constexpr (T::esz == 2) reinterpret_cast<Half*>(to)->v = uint2{pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3])};
       else store_chunk<T>(to, __builtin_bit_cast(u32x4_t, f32x4{{v[0], v[1], v[2], v[3]}}), 4);
     } else {
@@ -1281,7 +1453,8 @@ struct Plan {
   bool dx_first;                  // dx's runs before dw's tiles
   bool thin, twice;               // the kernels of few rows; their g and x have 64 rows
   bool low;                       // g has its second rows
-  int64_t x_at, w_at, part_at, target_at, g_at, sums_at, dw_sums_at, dyn_at, bytes;
+  bool rest;                      // what g's rounding leaves of the labels' elements is kept
+  int64_t x_at, w_at, part_at, target_at, g_at, rest_at, sums_at, dw_sums_at, dyn_at, bytes;
 };
 
 // k tiles that the last of the chip's workgroups ends with, of n workgroups of kn k
@@ -1365,6 +1538,7 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
   const int64_t kt = (width + deep - 1) / deep;
   q.thin = rows <= kThinRows;
   q.low = bwd && q.esz == 2 && rows <= kLow && !q.thin;
+  q.rest = bwd && q.esz == 2 && rows > kLow;
   const double mid = logits_time(kMid, q.esz, rows, vocab, kt), big = logits_time(kBig, q.esz, rows, vocab, kt);
   q.logits = q.esz == 4 || q.low || mid < big ? kMid : kBig;
   q.tm = q.thin ? kThinRows : kSizes[q.logits][0], q.tn = q.thin ? kThinClasses : kSizes[q.logits][1];
@@ -1395,6 +1569,7 @@ Plan plan(bool bwd, int io_type, int64_t rows, int64_t width, int64_t vocab, con
     const int64_t classes = std::min(vocab, q.piece);
     q.ld_g = up(classes, 64);
     q.g_at = take((kept + (q.low ? kLow : 0)) * q.ld_g * q.esz);
+    if (q.rest) q.rest_at = take(rows * sizeof(Rest));
     const Cuts small = products_cuts(kMid, q.esz, rows, width, classes);
     const Cuts large = products_cuts(kBig, q.esz, rows, width, classes);
     const Cuts& cuts = q.esz == 4 || rows <= kLow || small.time < large.time ? small : large;  // low: 128 rows a tile
@@ -1612,6 +1787,8 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
   a.lse = lse, a.row_grad = row_grad;
   a.x = static_cast<const char*>(x), a.ld_x = ld_x;
   a.g = ws + q.g_at, a.ld_g = q.ld_g;
+  a.all = vocab;
+  if (q.rest) b.rest = a.rest = reinterpret_cast<Rest*>(ws + q.rest_at);
   a.tiles_m = int((rows + q.tm - 1) / q.tm);
   b.dx_m = dx && !q.thin ? int((rows + q.pm - 1) / q.pm) : 0;
   b.dx_n = b.dw_n = int((width + q.pn - 1) / q.pn);
@@ -1660,7 +1837,7 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     });
   };
   for (int64_t v0 = 0; v0 < vocab; v0 += q.piece) {
-    a.v0 = v0;
+    a.v0 = b.v0 = v0;
     a.vocab = b.vocab = std::min(q.piece, vocab - v0);
     a.w = static_cast<const char*>(w) + v0 * ld_w * esz, a.ld_w = ld_w;
     if (q.pack_w) {
@@ -1720,5 +1897,5 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
     });
   }
   return join(io_type, SumsArgs{b.sums, rows, width, b.dx_m, b.dx_n, b.slices, b.low, b.dyn, b.unit,
-                                static_cast<char*>(dx), ld_dx});
+                                static_cast<char*>(dx), ld_dx, b.rest, static_cast<const char*>(w), ld_w});
 }
