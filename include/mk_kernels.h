@@ -593,6 +593,8 @@ int mk_sdpa_bwd(void* stream, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int6
  * Labels are MK_S32 or MK_S64.  A label outside [0, vocab) has no target term
  * (loss_rows[n] = lse[n], as in mk_softmax_xent); with has_ignore, rows whose
  * label is ignore_index have loss 0.  lse is each row's, ignored or not.
+ * Logits may lie anywhere in fp32's range, as weights of a type's lowest value give
+ * them; +inf or NaN among a row's makes its loss and lse NaN.
  * loss_rows and lse are fp32 [rows], either may be NULL.  The vocabulary is
  * gone through in tiles, of which the workspace holds each row's maximum and
  * sum.  Operands of more than 32 rows off the 16-byte boundaries (base, pitch or

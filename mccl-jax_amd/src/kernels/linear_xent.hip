@@ -259,12 +259,25 @@ struct LossArgs {
   int64_t v0;              // the piece's first class
   int tiles_m, tiles_n;
   Labels labels;
-  float2* part;            // [tiles_n][rows]: t and the sum of 2^(s log2(e) - t)
+  float2* part;            // [tiles_n][rows]: the maximum and the sum of e^(s - maximum)
   float* target;           // [rows]: the label's logit
 };
 
-// Exponentials are of base 2, of s log2(e) - t with t the rounded product of the
-// row's maximum and log2(e): t is what the tile's sum is relative to, exactly.
+// Exponentials are of base 2, of s log2(e) - t in one instruction, with t the rounded
+// product of the row's maximum and log2(e); the sum is then made relative to the
+// maximum itself.  t's rounding is at most 2^-15 where t is below 2^10, below that of an
+// fp32 lse's own logarithm; past that (weights of a type's lowest value give
+// logits up to the end of fp32's range, where rounding is more than an exponent can
+// hold) differences are taken first, an instruction more.
+__device__ inline float base2(float top, bool& plain) {
+  const float t = top * kLog2e;
+  plain = fabsf(t) < 1024.f;
+  return plain ? t : 0.f;
+}
+// e^(top - to), a sum's weight among sums relative to `to`; to is that of top that is finite, or 0
+__device__ inline float weight(float top, float to) { return __builtin_amdgcn_exp2f((top - to) * kLog2e); }
+__device__ inline float or_zero(float top) { return top == -INFINITY ? 0.f : top; }  // nothing but -inf: a sum of 0
+
 // A workgroup has every gridDim-th tile, and the next one's first copies in flight
 // while it ends a tile.
 template <class T, class Sh>
@@ -332,25 +345,33 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void loss_kernel(const LossArg
       float lo, hi;
       lane_halves_sched(top, lo, hi);
       top = fmaxf(lo, hi);
-      const float t = top * kLog2e, from = t == -INFINITY ? 0.f : t;  // nothing but -inf: a sum of 0
+      bool plain;
+      const float from = base2(top, plain);
+      if (!plain && top != -INFINITY) {
+#pragma unroll
+        for (int b = 0; b < G::J; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[a][b][r] -= top;
+      }
       float sum = 0.f;
 #pragma unroll
       for (int b = 0; b < G::J; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[a][b][r], kLog2e, -from));
       lane_halves_sched(sum, lo, hi);
-      if (g == 0) red[wn * Sh::TM + ml] = float2{t, lo + hi};
+      sum = lo + hi;
+      if (plain) sum *= __builtin_amdgcn_exp2f(fmaf(top, -kLog2e, from));
+      if (g == 0) red[wn * Sh::TM + ml] = float2{top, sum};
     }
     lds_barrier();
     for (int e = int(threadIdx.x); e < Sh::TM; e += G::threads) {
       if (m_now + e >= p.rows) break;
-      float t = -INFINITY, sum = 0.f;
+      float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int q = 0; q < Sh::WGN; ++q) t = fmaxf(t, red[q * Sh::TM + e].x);
+      for (int q = 0; q < Sh::WGN; ++q) top = fmaxf(top, red[q * Sh::TM + e].x);
 #pragma unroll
-      for (int q = 0; q < Sh::WGN; ++q)
-        sum += red[q * Sh::TM + e].y * __builtin_amdgcn_exp2f(red[q * Sh::TM + e].x - (t == -INFINITY ? 0.f : t));
-      p.part[n_now / Sh::TN * p.rows + m_now + e] = float2{t, sum};
+      for (int q = 0; q < Sh::WGN; ++q) sum += red[q * Sh::TM + e].y * weight(red[q * Sh::TM + e].x, or_zero(top));
+      p.part[n_now / Sh::TN * p.rows + m_now + e] = float2{top, sum};
     }
     if (i >= nt) return;
   }
@@ -375,18 +396,18 @@ __global__ __launch_bounds__(16 * NT) void loss_final_kernel(const float2* part,
       float to = top;
 #pragma unroll
       for (int i = 0; i < kAt; ++i) to = fmaxf(to, v[i].x);
-      const float from = to == -INFINITY ? 0.f : to;
-      sum *= __builtin_amdgcn_exp2f(top - from);
+      const float from = or_zero(to);
+      sum *= weight(top, from);
 #pragma unroll
-      for (int i = 0; i < kAt; ++i) sum += v[i].y * __builtin_amdgcn_exp2f(v[i].x - from);
+      for (int i = 0; i < kAt; ++i) sum += v[i].y * weight(v[i].x, from);
       top = to;
     }
   }
   // 4 of them are lanes of a wave
 #pragma unroll
   for (int d = 16; d < 64; d *= 2) {
-    const float t = __shfl_xor(top, d), more = __shfl_xor(sum, d), to = fmaxf(top, t), from = to == -INFINITY ? 0.f : to;
-    const float mine = sum * __builtin_amdgcn_exp2f(top - from), its = more * __builtin_amdgcn_exp2f(t - from);
+    const float t = __shfl_xor(top, d), more = __shfl_xor(sum, d), to = fmaxf(top, t), from = or_zero(to);
+    const float mine = sum * weight(top, from), its = more * weight(t, from);
     sum = mine + its;  // the same in both lanes
     top = to;
   }
@@ -395,11 +416,10 @@ __global__ __launch_bounds__(16 * NT) void loss_final_kernel(const float2* part,
   if (ty != 0 || n >= rows) return;
 #pragma unroll
   for (int i = 1; i < NT / 4; ++i) top = fmaxf(top, red[i][tx].x);
-  const float from = top == -INFINITY ? 0.f : top;
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < NT / 4; ++i) sum += red[i][tx].y * __builtin_amdgcn_exp2f(red[i][tx].x - from);
-  const float z = (top + log2f(sum)) * kLn2;
+  for (int i = 0; i < NT / 4; ++i) sum += red[i][tx].y * weight(red[i][tx].x, or_zero(top));
+  const float z = top + log2f(sum) * kLn2;
   if (lse) lse[n] = z;
   if (!loss) return;
   const int64_t label = labels.at(n);
@@ -685,7 +705,20 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
   int at = 0;
   for (uint32_t i = blockIdx.x;;) {
     Acc<Sh> acc;
-    zero<Sh>(acc);
+    if constexpr (T::esz == 2) {
+      // from -lse on: the difference costs no instruction, and holds where lse log2(e) would not
+      lds_barrier();
+#pragma unroll
+      for (int a = 0; a < G::I; ++a) {
+        const float from = -row_lse[at][wm * G::WM + 32 * a + c];
+#pragma unroll
+        for (int b = 0; b < G::J; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[a][b][r] = from;
+      }
+    } else {
+      zero<Sh>(acc);
+    }
     now.template run<kLate>(lds, wave, lane, acc, late);
     const int64_t m_now = m0, n_now = n0;
     i += gridDim.x;
@@ -709,15 +742,14 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void grad_kernel(const GradArg
     bool found = false;  // a label's element
 #pragma unroll
     for (int a = 0; a < G::I; ++a) {
-      const float lse = row_lse[at][wm * G::WM + 32 * a + c], from = -lse * kLog2e;
+      const float lse = T::esz == 4 ? row_lse[at][wm * G::WM + 32 * a + c] : 0.f;
       const int mine = rel[a] - wn * G::WN - 4 * g;
 #pragma unroll
       for (int b = 0; b < G::J; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          // 32-bit results: the difference first, which is exact where it is small
-          acc[a][b][r] = __builtin_amdgcn_exp2f(T::esz == 4 ? (acc[a][b][r] - lse) * kLog2e
-                                                            : fmaf(acc[a][b][r], kLog2e, from));
+          // 32-bit results: the difference of whole sums, which is exact where it is small
+          acc[a][b][r] = __builtin_amdgcn_exp2f((T::esz == 4 ? acc[a][b][r] - lse : acc[a][b][r]) * kLog2e);
       if (rel[a] >= 0 && mine >= 0 && mine < G::WN && !(mine & 4)) {
         found = true;
 #pragma unroll
@@ -1224,12 +1256,11 @@ __global__ __launch_bounds__(64 * W) void thin_logits_kernel(const Args p) {
       float lo, hi;
       lane_halves_sched(top, lo, hi);
       top = fmaxf(lo, hi);
-      const float t2 = top * kLog2e, from = t2 == -INFINITY ? 0.f : t2;
       float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(fmaf(z.v[e], kLog2e, -from));
+      for (int e = 0; e < 4; ++e) sum += weight(z.v[e], or_zero(top));
       lane_halves_sched(sum, lo, hi);
-      if (g == 0) ends[t][c] = float2{t2, lo + hi};
+      if (g == 0) ends[t][c] = float2{top, lo + hi};
     }
     __syncthreads();
     if (int(threadIdx.x) >= p.rows) return;
@@ -1237,15 +1268,14 @@ __global__ __launch_bounds__(64 * W) void thin_logits_kernel(const Args p) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) most = fmaxf(most, ends[q][threadIdx.x].x);
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      all += ends[q][threadIdx.x].y * __builtin_amdgcn_exp2f(ends[q][threadIdx.x].x - (most == -INFINITY ? 0.f : most));
+    for (int q = 0; q < 8; ++q) all += ends[q][threadIdx.x].y * weight(ends[q][threadIdx.x].x, or_zero(most));
     p.part[int64_t(blockIdx.x) * p.rows + threadIdx.x] = float2{most, all};
   } else {
     // 16 bits: all of the 64 rows are written, what the rounding leaves 32 rows further on:
     // they are one k tile of dw
     const bool here = c < p.rows;
     if (!here && T::esz == 4) return;
-    const float lse = here ? p.lse[c] : 0.f, from = -lse * kLog2e;
+    const float lse = here ? p.lse[c] : 0.f;
     const float factor = here ? (p.dyn ? p.dyn[0] : p.unit) * (p.row_grad ? p.row_grad[c] : 1.f) : 0.f;
     const bool none = !here || p.labels.ignored(label);
 #pragma unroll
@@ -1256,7 +1286,7 @@ __global__ __launch_bounds__(64 * W) void thin_logits_kernel(const Args p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float z = sums[i].v[e];
-        v[e] = __builtin_amdgcn_exp2f(T::esz == 4 ? (z - lse) * kLog2e : fmaf(z, kLog2e, from));
+        v[e] = weight(z, lse);
         if (at == e) v[e] -= 1.f;
         v[e] = none || e >= left ? 0.f : v[e] * factor;  // whole tiles are written, zeros past the classes
         rest[e] = v[e] - rounded(T{}, v[e]);
