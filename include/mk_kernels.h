@@ -597,7 +597,7 @@ int mk_sdpa_bwd(void* stream, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int6
  * them; +inf or NaN among a row's makes its loss and lse NaN.
  * loss_rows and lse are fp32 [rows], either may be NULL.  The vocabulary is
  * gone through in tiles, of which the workspace holds each row's maximum and
- * sum.  Operands of more than 32 rows off the 16-byte boundaries (base, pitch or
+ * sum.  With more than 32 rows, operands off the 16-byte boundaries (base, pitch or
  * width) are copied to them first, w piece by piece; the size of the workspace
  * counts that, so the pointers and pitches given to it are those of the call. */
 size_t mk_linear_xent_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
@@ -619,7 +619,8 @@ int mk_linear_xent(void* stream, int io_type, int64_t rows, int64_t width, int64
  * element as a second operand.  Sums are fp32, in a fixed order: the same inputs
  * give the same bits.  dx is of io_type, dw of dw_type (io_type or MK_F32);
  * either may be NULL, then only the other is computed.  dx and dw may overlap neither
- * x, w nor each other.  Workspace as above. */
+ * x, w nor each other.  Workspace as above; x, whatever its number of rows, is copied where
+ * it lies off the 16-byte boundaries, with has_ignore, and up to 32 rows of 16 bits always. */
 size_t mk_linear_xent_bwd_workspace_bytes(int io_type, int64_t rows, int64_t width, int64_t vocab, const void* x,
                                           int64_t ld_x, const void* w, int64_t ld_w, int has_ignore);
 int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_t rows, int64_t width, int64_t vocab,
