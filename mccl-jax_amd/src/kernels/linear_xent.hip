@@ -633,8 +633,9 @@ __device__ __attribute__((always_inline)) inline void store32(int wave, int lane
 // added to both: to dw by its tiles (LabelRest), to dx where its sums are joined.  Errors
 // against 64 bits, without it and with it: 100 x 768 x 50257 bf16 0.00188, 0.00165; 1777
 // x 1001 x 30011 fp16 0.000279, 0.000207, both then those of fp32 products.  Times:
-// 8192 x 768 x 50257 1875 us, 1925; 1777 x 1001 x 30011 402, 416; 100 rows 69 either
-// way; of few classes, each with many labels, 2000 x 2048 x 1500 63, 72.  At most
+// 8192 x 768 x 50257 1847 us, 1880; 1777 x 1001 x 30011 384, 394; 100 x 768 x 50257 66,
+// 69; of few classes, each with many labels, 2000 x 2048 x 1500 61, 71.  (Another
+// class with much of a row's probability is rounded with the rest of g.)  At most
 // kLow rows have a second operand row each, what the rounding leaves of every
 // element; their tiles have the room (16 bits: half of dx's 128 rows, and of dw's
 // two k tiles the second), so that it costs nothing.
@@ -833,7 +834,7 @@ struct ProductsArgs {
   int64_t dw_run;
   float* dw_sums;  // as sums, of more than one slice
   int low;         // g has its second rows
-  const Rest* rest;  // GradArgs' rest, or null
+  const Rest* rest;  // GradArgs' rest
   int64_t v0;        // the piece's first class
   char* dw;        // the piece's rows
   int64_t ld_dw;
@@ -949,7 +950,9 @@ struct LabelRest {
   }
 };
 
-template <class T, class Sh>
+// REST: of more than kLow rows of 16 bits; the others do without its lists (32 x 768 x 50257
+// 62.8 us with them, 61.8 without)
+template <class T, class Sh, bool REST>
 __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const ProductsArgs p) {
   using G = Geo<Sh>;
   constexpr int64_t kTile = Sh::TM * Sh::TN / 4;  // of a slice's sums, in f32x4
@@ -991,11 +994,11 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   static_assert(128 / Bf16::esz == kLow, "g's second rows are the second k tile");
   if (p.low) dw.twice();
   dw.start(lds, wave, lane);
-  if constexpr (T::esz == 2) {
+  if constexpr (REST) {
     using L = LabelRest<T, Sh>;
     __shared__ typename L::Entry lists[G::W][L::kMost];
     const int64_t c0 = m0 + wave / Sh::WGN * G::WM, d0 = n0 + wave % Sh::WGN * G::WN;
-    L rest{lists[wave], p.rest && d0 < p.width ? p.rest + k0 : nullptr, min(p.dw_run, p.rows - k0), int(p.v0 + c0),
+    L rest{lists[wave], d0 < p.width ? p.rest + k0 : nullptr, min(p.dw_run, p.rows - k0), int(p.v0 + c0),
            int(max(int64_t(0), min(int64_t(G::WM), p.vocab - c0))), p.x + (k0 * p.ld_x + d0) * 2, p.ld_x, p.width - d0, lane};
     rest.load(0);
     dw.template run<0>(lds, wave, lane, acc, false, rest);
@@ -1026,7 +1029,9 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
 // dx, or dw = the slices' sums times the factor.  A block has the 32 rows x WN columns of
 // one of a wave's accumulator rows, as they lay, and stores them in rows through
 // LDS.  Many slices are added by NG groups of threads, each every NG-th slice in
-// order, then the groups in order (64 slices by one group: 12 us of latency).
+// order, then the groups in order (64 slices by one group: 12 us of latency).  REST: of
+// dx with what is left of the labels; a kernel of its own, since the labels' loads beside
+// the slices' cost calls without them too (40 x 2048 x 32000 11.9 us, 5.4).
 struct SumsArgs {
   const float* sums;
   int64_t rows, width;
@@ -1036,12 +1041,12 @@ struct SumsArgs {
   float unit;
   char* out;
   int64_t ld;
-  const Rest* rest;  // of dx: what is left times w's row of the label is added (null: nothing)
+  const Rest* rest;  // of dx (REST): what is left times w's row of the label is added
   const char* w;
   int64_t ld_w;
 };
 
-template <class T, class Sh, int NG>
+template <class T, class Sh, int NG, bool REST>
 __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
   using G = Geo<Sh>;
   constexpr int kPitch = G::WN + 4, kSize = 32 * kPitch;
@@ -1055,28 +1060,32 @@ __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
   // what a thread stores: 4 columns of a row each
   constexpr int kItems = 32 * G::WN / 4, kMine = (kItems + kThreads * NG - 1) / (kThreads * NG);
   struct __attribute__((packed, aligned(sizeof(Elem<T>)))) Half { uint2 v; };
-  Rest rest[kMine];
-#pragma unroll
-  for (int q = 0; q < kMine; ++q) {
-    const int i = int(threadIdx.x) + q * kThreads * NG;
-    const int64_t m = m0 + i / (G::WN / 4);
-    rest[q] = Rest{-1, 0.f};
-    if (T::esz == 2 && p.rest && i < kItems && m < p.rows) rest[q] = p.rest[m];
-  }
+  float left[kMine];
   uint32_t wrow[kMine][2];  // w's row of the label, 4 columns
+  if constexpr (REST) {
+    Rest rest[kMine];
 #pragma unroll
-  for (int q = 0; q < kMine; ++q) {
-    wrow[q][0] = wrow[q][1] = 0;
-    const int64_t n = n0 + (int(threadIdx.x) + q * kThreads * NG) % (G::WN / 4) * 4;
-    if (T::esz != 2 || rest[q].label < 0 || n >= p.width) continue;
-    const char* w = p.w + (rest[q].label * p.ld_w + n) * T::esz;
-    if (n + 4 <= p.width) {
-      const uint2 v = reinterpret_cast<const Half*>(w)->v;
-      wrow[q][0] = v.x, wrow[q][1] = v.y;
-    } else {
+    for (int k = 0; k < kMine; ++k) {
+      const int i = int(threadIdx.x) + k * kThreads * NG;
+      rest[k] = p.rest[min(m0 + i / (G::WN / 4), p.rows - 1)];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.width) wrow[q][e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(w)[e]) << (16 * (e & 1));
+    for (int k = 0; k < kMine; ++k) {
+      const int64_t n = n0 + (int(threadIdx.x) + k * kThreads * NG) % (G::WN / 4) * 4;
+      const bool labelled = rest[k].label >= 0;
+      left[k] = labelled ? rest[k].left : 0.f;
+      wrow[k][0] = wrow[k][1] = 0;
+      if (labelled && n < p.width) {
+        const char* w = p.w + (rest[k].label * p.ld_w + n) * T::esz;
+        if (n + 4 <= p.width) {
+          const uint2 v = reinterpret_cast<const Half*>(w)->v;
+          wrow[k][0] = v.x, wrow[k][1] = v.y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < p.width) wrow[k][e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(w)[e]) << (16 * (e & 1));
+        }
+      }
     }
   }
   // the waves kLow rows further on, in the same tile (128 rows, 32 a wave)
@@ -1113,9 +1122,7 @@ __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
       v[e] = lds[row * kPitch + col + e];
 #pragma unroll
       for (int q = 1; q < NG; ++q) v[e] += lds[q * kSize + row * kPitch + col + e];
-      if constexpr (T::esz == 2) {
-        if (rest[k].label >= 0) v[e] += rest[k].left * widened(T{}, wrow[k][e / 2] >> (16 * (e & 1)));
-      }
+      if constexpr (REST) v[e] += left[k] * widened(T{}, wrow[k][e / 2] >> (16 * (e & 1)));
       v[e] *= f;
     }
     char* to = p.out + (m * p.ld + n) * T::esz;
@@ -1861,8 +1868,15 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
       using T = decltype(t);
       using Sh = decltype(sh);
       const dim3 g{unsigned(c.tiles_m) * unsigned(c.tiles_n) * Geo<Sh>::W * Geo<Sh>::I};
-      if (c.slices > 8) hipLaunchKernelGGL((sums_kernel<T, Sh, 4>), g, dim3(4 * kThreads), 0, s, c);
-      else hipLaunchKernelGGL((sums_kernel<T, Sh, 1>), g, dim3(kThreads), 0, s, c);
+      if constexpr (T::esz == 2) {
+        if (c.rest) {
+          if (c.slices > 8) hipLaunchKernelGGL((sums_kernel<T, Sh, 4, true>), g, dim3(4 * kThreads), 0, s, c);
+          else hipLaunchKernelGGL((sums_kernel<T, Sh, 1, true>), g, dim3(kThreads), 0, s, c);
+          return check_launch(what);
+        }
+      }
+      if (c.slices > 8) hipLaunchKernelGGL((sums_kernel<T, Sh, 4, false>), g, dim3(4 * kThreads), 0, s, c);
+      else hipLaunchKernelGGL((sums_kernel<T, Sh, 1, false>), g, dim3(kThreads), 0, s, c);
       return check_launch(what);
     });
   };
@@ -1908,7 +1922,15 @@ extern "C" int mk_linear_xent_bwd(void* stream, int io_type, int dw_type, int64_
       using T = decltype(t);
       using Sh = decltype(sh);
       const unsigned tiles = (unsigned(b.dx_m) * b.dx_n * b.slices + 7) / 8 * 8 + (unsigned(b.dw_m) * b.dw_n * b.dw_slices + 7) / 8 * 8;
-      hipLaunchKernelGGL((products_kernel<T, Sh>), dim3(tiles), dim3(Geo<Sh>::threads), 0, s, b);
+      const dim3 n{tiles}, threads{Geo<Sh>::threads};
+      if constexpr (T::esz == 4) {
+        hipLaunchKernelGGL((products_kernel<T, Sh, false>), n, threads, 0, s, b);
+      } else if constexpr (Sh::TM == 256) {  // never of up to kLow rows
+        hipLaunchKernelGGL((products_kernel<T, Sh, true>), n, threads, 0, s, b);
+      } else {
+        if (q.rest) hipLaunchKernelGGL((products_kernel<T, Sh, true>), n, threads, 0, s, b);
+        else hipLaunchKernelGGL((products_kernel<T, Sh, false>), n, threads, 0, s, b);
+      }
       return check_launch(what);
     });
     if (rc) return rc;

@@ -18,6 +18,9 @@ TILES = [
     (50416, 709, 389, "f16", "f32", False),
     (50416, 709, 389, "bf16", "bf16", True),
     (24000, 1500, 512, "bf16", "f32", False),
+    (24000, 1500, 512, "bf16", "bf16", True),
+    (24000, 1500, 512, "f16", "f16", False),
+    (44936, 960, 137, "f16", "f16", True),
     # g in two pieces of the vocabulary
     (9000, 200, 33000, "bf16", "f32", False),
     # 128 x 128 tiles
@@ -25,6 +28,9 @@ TILES = [
     (300, 520, 5003, "f16", "f16", False),
     (700, 264, 3001, "f32", "f32", True),
     (100, 768, 9001, "bf16", "f32", False),
+    (40, 100, 90, "bf16", "bf16", False),
+    (64, 40, 129, "f16", "f32", True),
+    (130, 40, 200, "f16", "f16", False),
 ]
 # weights past the workspace's share of them (copied piece by piece), and past 2^31 bytes where they lie
 PIECES = [
