@@ -165,9 +165,9 @@ struct Labels {
 // rest: what is added beside the operands' k tiles (LabelRest).
 struct NoRest {
   __device__ inline void load(int) const {}
-  __device__ inline void take(int) const {}
+  __device__ inline void arrived() const {}
   template <class A>
-  __device__ inline void add(A&) const {}
+  __device__ inline void add(int, A&) const {}
 };
 template <class T, class Sh, bool AKC, bool BKC>
 struct Product {
@@ -193,8 +193,8 @@ struct Product {
   __device__ inline void start(char* lds, int wave, int lane) const {
     if (nk > 0) issue(0, lds, wave, lane, true, true);
   }
-  // LATE: stores that may still be on their way when the first k tile is there (late: exactly
-  // so many came after its copies)
+  // LATE: stores that may still be on their way when the first k tile is there (late: so many
+  // or more came after its copies)
   template <int LATE = 0, class Beside = NoRest>
   __device__ __attribute__((always_inline)) inline void run(char* lds, int wave, int lane, Acc<Sh>& acc,
                                                             bool late = false, Beside&& rest = {}) const {
@@ -203,7 +203,7 @@ struct Product {
       if (LATE > 0 && late && kt == 0) wait_vm<LATE>();
       else wait_vm<0>();
       lds_barrier();
-      rest.take(kt);
+      rest.arrived();
       const char* at = lds + (kt & 1) * G::stage;
       char* next = lds + ((kt + 1) & 1) * G::stage;
       const bool more = kt + 1 < nk;
@@ -221,7 +221,7 @@ struct Product {
 #pragma unroll
           for (int b = 0; b < G::J; ++b) acc[a][b] = T::mma(bf[b], af[a], acc[a][b]);
       }
-      rest.add(acc);
+      rest.add(kt, acc);
     }
     lds_barrier();
   }
@@ -633,8 +633,8 @@ __device__ __attribute__((always_inline)) inline void store32(int wave, int lane
 // added to both: to dw by its tiles (LabelRest), to dx where its sums are joined.  Errors
 // against 64 bits, without it and with it: 100 x 768 x 50257 bf16 0.00188, 0.00165; 1777
 // x 1001 x 30011 fp16 0.000279, 0.000207, both then those of fp32 products.  Times:
-// 8192 x 768 x 50257 1847 us, 1880; 1777 x 1001 x 30011 384, 394; 100 x 768 x 50257 66,
-// 69; of few classes, each with many labels, 2000 x 2048 x 1500 61, 71.  (Another
+// 8192 x 768 x 50257 1848 us, 1880; 1777 x 1001 x 30011 393, 400; 100 x 768 x 50257 68,
+// 70; of few classes, each with many labels, 2000 x 2048 x 1500 61, 68.  (Another
 // class with much of a row's probability is rounded with the rest of g.)  At most
 // kLow rows have a second operand row each, what the rounding leaves of every
 // element; their tiles have the room (16 bits: half of dx's 128 rows, and of dw's
@@ -892,23 +892,25 @@ struct LabelRest {
   const char* x;       // the run's first row of x, at the wave's first column
   int64_t ld_x, cols;  // cols: those from there on
   int lane;
-  Rest next;
+  Rest next, now;  // of the k tile on its way, and of the one that is multiplied
   int n = 0;
   __device__ inline void load(int kt) {
     const int64_t at = 64 * int64_t(kt) + lane;
     next = Rest{-1, 0.f};
     if (rows && at < count) next = rows[at];
   }
-  __device__ inline void take(int kt) {
-    const unsigned at = unsigned(next.label) - unsigned(first);
-    const bool mine = next.label >= 0 && at < unsigned(classes);
+  __device__ inline void arrived() {
+    now = next;
+    asm volatile("" : "+v"(now.label), "+v"(now.left));  // waited for here, not past the next copies
+  }
+  __device__ inline void add(int kt, Acc<Sh>& acc) {
+    const unsigned at = unsigned(now.label) - unsigned(first);
+    const bool mine = now.label >= 0 && at < unsigned(classes);
     const uint64_t all = __ballot(mine);
     if (all == 0) return;
     const int before = __builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0));
-    if (mine) list[n + before] = Entry{64 * kt + lane, at << 16 | (pack2(T{}, next.left, 0.f) & 0xFFFFu)};
+    if (mine) list[n + before] = Entry{64 * kt + lane, at << 16 | (pack2(T{}, now.left, 0.f) & 0xFFFFu)};
     n += __builtin_popcountll(all);
-  }
-  __device__ inline void add(Acc<Sh>& acc) {
     if (n < 64) return;
     multiply(64, acc);
     list[lane] = list[64 + lane];
