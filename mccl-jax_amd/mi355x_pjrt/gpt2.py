@@ -216,6 +216,8 @@ class GPT2TrainStep:
         self._alloc()
         self.ids = torch.zeros(cfg.tokens, dtype=torch.int32, device=self.dev)
         self.labels = torch.zeros(cfg.tokens, dtype=torch.int32, device=self.dev)
+        # whichever streams the batches come on and the step runs on, its buffers are filled
+        torch.cuda.current_stream(self.dev).synchronize()
         self.calls = self._build()
 
     # ------------------------------------------------------------------ params
@@ -227,6 +229,7 @@ class GPT2TrainStep:
         for name, (off, shape) in self.offsets.items():
             a = torch.from_numpy(np.ascontiguousarray(params[name], dtype=np.float32)).reshape(shape)
             self.view(self.master, name).copy_(a.to(self.dev))
+        self.stream.wait_stream(torch.cuda.current_stream(self.dev))
         rc = self.lib.mk_convert(_P(self.stream.cuda_stream), F32, BF16, self.n_flat, _P(self.master.data_ptr()),
                                  _P(self.param.data_ptr()))
         K._check(rc, "mk_convert")
