@@ -163,11 +163,11 @@ class GPT2TrainStep:
     FUSE_GELU_BWD = False
     # keep_logits=False: the loss from linear_xent and its gradient, which form the
     # logits twice and keep none (8192 x 50264 of bf16, 824 MB), in the same time: a
-    # GPT-2-small step of 8 x 1024 tokens 11.90 ms, 11.88 with them
+    # GPT-2-small step of 8 x 1024 tokens 12.33 ms, 12.25 with them
     # dropout: sites 0 (embeddings), 1 + 2 l and 2 + 2 l (the branches of layer l) draw
     # at site * 2^40 + the step's count, a device number the step itself raises, so
     # that forward, backward and every replay of a captured step agree on it; 0.1
-    # makes that step 0.37 ms longer (its branches' LayerNorms stand alone)
+    # makes that step 0.35 to 0.45 ms longer (its branches' LayerNorms stand alone)
     DROP_SITE = 1 << 40
     # the hidden-state gradient through the embedding (K = vocabulary): bf16
     # out, split along K in uneven slices (measured: 8 slices 664 us, 2 693,

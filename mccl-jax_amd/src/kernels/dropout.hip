@@ -22,8 +22,8 @@
 //
 // Memory bounds the large ones: 20011 x 4097 fp32 116 us (5.7 TB/s of the bytes read
 // and written, some of them in the last-level cache; a copy 5.4).  8192 x 768 bf16 with
-// bias and residual 7.3 us (5.2 TB/s), its gradient 11.5 with the sums, of which 2 are
-// the second launch.  64 x 768 is a launch: 2.4 us on the GPU, 7 with the call.
+// bias and residual 7.4 us (5.1 TB/s), its gradient 11.5 with the sums, of which 2 to 4
+// are the second launch.  64 x 768 is a launch: 2.8 us on the GPU, 7 with the call.
 #include "mk_common.h"
 
 #include <algorithm>

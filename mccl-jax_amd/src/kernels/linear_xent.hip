@@ -14,12 +14,12 @@
 // leaves of the labels' elements is kept beside it), then dx and dw of the piece in
 // one launch.  g is the only large thing that goes through memory, 512 MB at a time.
 //
-// Many rows are bound by the matrix rate: 8192 x 768 x 50257 bf16 takes 553 us
-// forward (1.14 PFLOP/s; the library's product of the logits alone 597) and 1823
-// backward (three products, 1.04 PFLOP/s; the library's three 2008, without the
-// softmax), 8192 x 4096 x 65536 10.8 ms backward (1.22).  Twelve k tiles of 768 are short
-// beside a tile's end.  Few rows are bound by w: 16 rows of it 20.7 us forward (16 us
-// of products, 4.8 TB/s), 100 rows 67 backward, where w is read twice and dw written.
+// Many rows are bound by the matrix rate: 8192 x 768 x 50257 bf16 takes 570 us
+// forward (1.11 PFLOP/s; the library's product of the logits alone 597) and 1866
+// backward (three products, 1.02 PFLOP/s; the library's three 2008, without the
+// softmax), 8192 x 4096 x 65536 11.1 ms backward (1.19).  Twelve k tiles of 768 are short
+// beside a tile's end.  Few rows are bound by w: 16 rows of it 20.4 us forward (16 us
+// of products, 4.8 TB/s), 100 rows 70 backward, where w is read twice and dw written.
 // The products are tiles as in gemm_tiled.hip (copies HBM -> LDS, two stages, k
 // tiles of 128 bytes a row); fp32 operands take the same bytes and the fp32 MFMA.
 // Operand bases move along k in 64 bits, so no operand's size is limited by a
@@ -961,7 +961,7 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
   __shared__ __attribute__((aligned(1024))) char lds[G::lds_bytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // The longer ones first mostly, and the others fill the last round (1000 x 768 x
-  // 50257: dx's runs first 265 us, dw's tiles 290).  Both start at a multiple of 8, an
+  // 50257: dx's runs first 266 us, dw's tiles 305).  Both start at a multiple of 8, an
   // XCD each.
   const uint32_t n_dw = (uint32_t(p.dw_m) * p.dw_n * p.dw_slices + 7) / 8 * 8;
   const uint32_t n_dx = uint32_t(p.dx_m) * p.dx_n * p.slices, dx_at = p.dx_first ? 0 : n_dw;
@@ -1147,7 +1147,9 @@ __global__ __launch_bounds__(kThreads* NG) void sums_kernel(const SumsArgs p) {
 // alignment; their accumulators are added through LDS.  Measured, tiles of 128
 // rows and here: forward 1 x 3680 x 1313 bf16 31 us, 15; 6 x 3686 x 16342 fp32 313, 59;
 // 8 x 769 x 50257 bf16 52, 30; 1 x 4096 x 65536 127, 117; 16 x 768 x 50257 20.2, 20.7;
-// backward of the second 574, 242, of the last 61, 61.
+// backward of the second 574, 242, of the last 61, 61.  The rule looks at the rows alone:
+// where the classes fill the chip and rows lie on the 16-byte boundaries both are the
+// reading of w, and within 3%.
 constexpr int kThinRows = 32, kThinClasses = 64;
 
 // the same of a row of `n` elements from element `at` on, zeros past its end
@@ -1521,8 +1523,9 @@ constexpr int64_t kSizes[2][2] = {{256, 256}, {128, 128}};
 double step_time(int shape, int esz) { return esz == 4 ? 3.5 : shape == kBig ? 1.75 : 1.12; }
 
 // Estimated us of the logits' tiles, kt k tiles each.  Measured, 256 and 128: loss of
-// 300 x 768 x 50257 46, 39, of 1000 92, 93; gradient of 300 (with the same products)
-// 136, 129, of 1000 293, 302, of 2048 x 1024 x 32000 374, 413, of 187 x 2409 x 4098 94, 69.
+// 300 x 768 x 50257 51, 39, of 1000 94, 88 (here it is 6% off); gradient of 300 (with the
+// same products) 136, 125, of 1000 263, 266, of 2048 x 1024 x 32000 383, 417, of 187 x
+// 2409 x 4098 96, 71.
 double logits_time(int shape, int esz, int64_t rows, int64_t classes, int64_t kt) {
   const int64_t tm = kSizes[shape][0], tn = kSizes[shape][1];
   const int64_t tiles = (rows + tm - 1) / tm * ((classes + tn - 1) / tn);
@@ -1543,9 +1546,9 @@ struct Cuts {
 // tiles one after the other against a tile of sums a run, written and read again at
 // about 3.8 TB/s.  A k tile of the last workgroup costs less than it takes alone
 // (step_time), since those that have ended leave it the power and the bandwidth;
-// the tiles' ends count as more k tiles.  Fitted to 24 ways for each of ten sizes (100 to 8192
-// rows, 64 to 4096 wide, 4098 to 50257 classes): within 2 to 4% of the
-// measured times, and the way it takes is the fastest or within 2% of it.
+// the tiles' ends count as more k tiles.  Measured, up to 28 ways each of twelve sizes (100
+// to 8192 rows, 64 to 4096 wide, 2148 to 50257 classes): it takes the fastest or one
+// within 3% at ten, 4% slower at 4527 x 1328 x 7316 bf16, 8% at 560 x 284 x 28975 fp32.
 Cuts products_cuts(int shape, int esz, int64_t rows, int64_t width, int64_t classes) {
   const int64_t end_w = shape == kBig ? 7 : 5, end_x = shape == kBig ? 7 : 6;
   const double last = shape == kBig ? 1.06 : 0.51, all = shape == kBig ? 0.0 : 0.24, slower = esz == 4 ? 2.4 : 1.0;
