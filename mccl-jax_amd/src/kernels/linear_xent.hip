@@ -265,18 +265,19 @@ struct LossArgs {
 
 // Exponentials are of base 2, of s log2(e) - t in one instruction, with t the rounded
 // product of the row's maximum and log2(e); the sum is then made relative to the
-// maximum itself.  t's rounding is at most 2^-15 where t is below 2^10, below that of an
-// fp32 lse's own logarithm; past that (weights of a type's lowest value give
-// logits up to the end of fp32's range, where rounding is more than an exponent can
-// hold) differences are taken first, an instruction more.
+// maximum itself, which undoes t's rounding.  That is at most 2^-15 where t is below 2^10;
+// past that (weights of a type's lowest value give logits up to the end of fp32's
+// range, where it is more than an exponent can hold) differences are taken first, an
+// instruction more.
 __device__ inline float base2(float top, bool& plain) {
   const float t = top * kLog2e;
   plain = fabsf(t) < 1024.f;
   return plain ? t : 0.f;
 }
-// e^(top - to), a sum's weight among sums relative to `to`; to is that of top that is finite, or 0
+// e^(top - to): what a sum relative to top weighs among those relative to `to`, the largest
+// top, or 0 where that is -inf (all sums are 0 then)
 __device__ inline float weight(float top, float to) { return __builtin_amdgcn_exp2f((top - to) * kLog2e); }
-__device__ inline float or_zero(float top) { return top == -INFINITY ? 0.f : top; }  // nothing but -inf: a sum of 0
+__device__ inline float or_zero(float top) { return top == -INFINITY ? 0.f : top; }
 
 // A workgroup has every gridDim-th tile, and the next one's first copies in flight
 // while it ends a tile.
@@ -1001,7 +1002,8 @@ __global__ __launch_bounds__(Geo<Sh>::threads, 2) void products_kernel(const Pro
     __shared__ typename L::Entry lists[G::W][L::kMost];
     const int64_t c0 = m0 + wave / Sh::WGN * G::WM, d0 = n0 + wave % Sh::WGN * G::WN;
     L rest{lists[wave], d0 < p.width ? p.rest + k0 : nullptr, min(p.dw_run, p.rows - k0), int(p.v0 + c0),
-           int(max(int64_t(0), min(int64_t(G::WM), p.vocab - c0))), p.x + (k0 * p.ld_x + d0) * 2, p.ld_x, p.width - d0, lane};
+           int(max(int64_t(0), min(int64_t(G::WM), p.vocab - c0))), p.x + (k0 * p.ld_x + d0) * 2, p.ld_x,
+           p.width - d0, lane};
     rest.load(0);
     dw.template run<0>(lds, wave, lane, acc, false, rest);
     rest.multiply(rest.n, acc);
